@@ -318,4 +318,80 @@ inline void launch_rmsnorm_gemv_dual_gate_up_swiglu_w4a16(const half* input, con
                   "launch_rmsnorm_gemv_dual_gate_up_swiglu_w4a16");
 }
 
+// ---- 4-bit key/value cache and log probabilities (no counterpart in kernels.cuh) ----
+inline void launch_qkv_bias_rope_kv4_append(const half* q, half* q_out, const half* k, const half* v,
+                                            const half* q_bias, const half* k_bias, const half* v_bias,
+                                            uint8_t* layer_k_cache, uint8_t* layer_v_cache,
+                                            const DeviceControlBlock* d_control, const int32_t* d_evicted,
+                                            int num_tokens, hipStream_t stream, int num_q_heads = NUM_Q_HEADS,
+                                            int num_kv_heads = NUM_KV_HEADS, int head_dim = HEAD_DIM,
+                                            int max_seq_len = MAX_SEQ_LEN, int rotary_dim = 0,
+                                            float rope_theta = ROPE_THETA) {
+    detail::check(qe_launch_qkv_bias_rope_kv4_append(detail::h(q), detail::h(q_out), detail::h(k), detail::h(v),
+                                                     detail::h(q_bias), detail::h(k_bias), detail::h(v_bias),
+                                                     layer_k_cache, layer_v_cache, d_control, d_evicted, num_tokens,
+                                                     stream, num_q_heads, num_kv_heads, head_dim, max_seq_len,
+                                                     rotary_dim, rope_theta),
+                  "launch_qkv_bias_rope_kv4_append");
+}
+
+inline void launch_kv4_unpack(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, half* out_k, half* out_v,
+                              int first_row, int num_rows, hipStream_t stream, int num_kv_heads = NUM_KV_HEADS,
+                              int head_dim = HEAD_DIM, int max_seq_len = MAX_SEQ_LEN) {
+    detail::check(qe_launch_kv4_unpack(layer_k_cache, layer_v_cache, detail::h(out_k), detail::h(out_v), first_row,
+                                       num_rows, stream, num_kv_heads, head_dim, max_seq_len),
+                  "launch_kv4_unpack");
+}
+
+inline void launch_attention_gqa_flash_decode_kv4(const half* q, const uint8_t* layer_k_cache,
+                                                  const uint8_t* layer_v_cache, void* workspace, half* attn_out,
+                                                  const DeviceControlBlock* d_control, const int32_t* d_evicted,
+                                                  hipStream_t stream, int num_q_heads = NUM_Q_HEADS,
+                                                  int num_kv_heads = NUM_KV_HEADS, int head_dim = HEAD_DIM,
+                                                  int max_seq_len = MAX_SEQ_LEN, int8_t* out_q8 = nullptr,
+                                                  float* out_scale = nullptr, int32_t* out_sum8 = nullptr,
+                                                  const float* key_weights_in = nullptr,
+                                                  float* key_weights_out = nullptr) {
+    detail::check(qe_launch_attention_gqa_flash_decode_kv4(detail::h(q), layer_k_cache, layer_v_cache, workspace,
+                                                           detail::h(attn_out), d_control, d_evicted, stream,
+                                                           num_q_heads, num_kv_heads, head_dim, max_seq_len, out_q8,
+                                                           out_scale, out_sum8, key_weights_in, key_weights_out),
+                  "launch_attention_gqa_flash_decode_kv4");
+}
+
+inline void launch_attention_gqa_prefill_kv4(const half* q, const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
+                                             half* attn_out, const DeviceControlBlock* d_control,
+                                             const int32_t* d_evicted, int num_tokens, hipStream_t stream,
+                                             int num_q_heads = NUM_Q_HEADS, int num_kv_heads = NUM_KV_HEADS,
+                                             int head_dim = HEAD_DIM, int max_seq_len = MAX_SEQ_LEN,
+                                             int hidden_size = HIDDEN_SIZE, const float* key_weights_in = nullptr,
+                                             float* key_weights_out = nullptr, float* row_lse = nullptr) {
+    detail::check(qe_launch_attention_gqa_prefill_kv4(detail::h(q), layer_k_cache, layer_v_cache, detail::h(attn_out),
+                                                      d_control, d_evicted, num_tokens, stream, num_q_heads,
+                                                      num_kv_heads, head_dim, max_seq_len, hidden_size,
+                                                      key_weights_in, key_weights_out, row_lse),
+                  "launch_attention_gqa_prefill_kv4");
+}
+
+inline void launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, const float* key_weights,
+                             const int32_t* d_evicted, uint8_t* out_k_cache, uint8_t* out_v_cache,
+                             float* out_key_weights, int32_t* out_evicted, int32_t* kept_rows,
+                             const DeviceControlBlock* d_control, int keep, int sinks, int recent, hipStream_t stream,
+                             int num_kv_heads = NUM_KV_HEADS, int head_dim = HEAD_DIM,
+                             int max_seq_len = MAX_SEQ_LEN) {
+    detail::check(qe_launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache,
+                                      out_key_weights, out_evicted, kept_rows, d_control, keep, sinks, recent, stream,
+                                      num_kv_heads, head_dim, max_seq_len),
+                  "launch_kv4_evict");
+}
+
+inline void launch_token_logprobs(const half* logits, const int32_t* token_ids, float* out_logprob,
+                                  float* out_entropy, float* out_top_logprob, int32_t* out_top_ids, void* workspace,
+                                  int num_rows, hipStream_t stream, int vocab_size = VOCAB_SIZE,
+                                  long long row_stride = VOCAB_SIZE, int top_k = 0) {
+    detail::check(qe_launch_token_logprobs(detail::h(logits), token_ids, out_logprob, out_entropy, out_top_logprob,
+                                           out_top_ids, workspace, num_rows, vocab_size, row_stride, top_k, stream),
+                  "launch_token_logprobs");
+}
+
 }  // namespace qwen

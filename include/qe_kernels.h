@@ -426,6 +426,117 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
                                     hipStream_t stream, int num_q_heads, int num_kv_heads, int head_dim,
                                     int max_seq_len, int hidden_size);
 
+/* ---- 4-bit key/value cache ------------------------------------------------------- */
+/* No counterpart in the reference (its cache is fp16).  A layer's K and V caches
+ * are uint8 [kv_head][max_seq_len][QE_KV4_ROW_BYTES], 16-byte aligned, 5 bits a
+ * value.  A row holds one head's 128 values of one token: sixteen little-endian
+ * 32-bit words of eight nibbles, element 8w + j at bit 16 * (j % 2) + 4 * (j / 2) of
+ * word w, then four pairs (scale, low) of fp16, one for every 32 elements.  A nibble
+ * n stands for fp16(n * scale + low), rounded once.  Storing x: low = fp16(min),
+ * scale = fp16((max - low) / 15), n = clamp(rint((x - low) / scale), 0, 15), n = 0
+ * for a scale of 0.  A token whose K or V holds a value that fp16 cannot (infinite,
+ * NaN, 65520 and more) is stored with NaN pairs in its K row: every row that
+ * attends to it gives NaN, rows that do not are untouched.
+ *
+ * The row of position p is p - d_evicted[kv_head]: d_evicted (device int32
+ * [num_kv_heads], NULL = zeros) counts the positions that eviction has taken out of
+ * this layer's cache.  It is not larger than the position (a larger count is taken
+ * as the position).  d_control->seq_pos keeps counting positions, which may exceed
+ * max_seq_len; rotations use the position, not the row.  A token whose row would be
+ * max_seq_len or more is not stored, and attends to the whole cache.
+ * d_control NULL means position 0.
+ *
+ * Key weights: float [num_kv_heads][max_seq_len], what the queries have given to a
+ * cache row so far: the sum of its softmax weights over queries and over the q heads of
+ * the kv head.  Attention reads key_weights_in (NULL = zeros) and writes key_weights_out
+ * for the rows in use, in place when both are the same pointer; rows behind them keep
+ * what they hold, and the rows of the launch's own tokens start from zero.
+ *
+ * Streams and graphs: launches keep no state and allocate nothing.  Recorded into a
+ * graph they read d_control and d_evicted at replay. */
+#define QE_KV4_ROW_BYTES 80
+
+/* Bias, NeoX RoPE and append of num_tokens tokens from d_control->seq_pos on, as
+ * qe_launch_qkv_bias_rope_kv_append does for an fp16 cache: q [T][num_q_heads][128]
+ * biased, rotated and written to q_out (which may be q; no other overlap), k and v
+ * [T][num_kv_heads][128] biased, k rotated, both stored in 4 bits (k and v themselves
+ * are not written).  Biases may be NULL.  Sums and rotation in fp32, angles in 64 bits,
+ * one rounding at the end.  head_dim 128; rotary_dim 0 (= 128) or a multiple of 16 up
+ * to 128; q, k, v and the biases 16-byte aligned. */
+int qe_launch_qkv_bias_rope_kv4_append(const uint16_t* q, uint16_t* q_out, const uint16_t* k, const uint16_t* v,
+                                       const uint16_t* q_bias, const uint16_t* k_bias, const uint16_t* v_bias,
+                                       uint8_t* layer_k_cache, uint8_t* layer_v_cache,
+                                       const qe_device_control_block* d_control, const int32_t* d_evicted,
+                                       int num_tokens, hipStream_t stream, int num_q_heads, int num_kv_heads,
+                                       int head_dim, int max_seq_len, int rotary_dim, float rope_theta);
+
+/* Rows first_row .. first_row + num_rows - 1 of every head as fp16
+ * [num_kv_heads][num_rows][128] (16-byte aligned).  Either cache may be left out,
+ * together with its output. */
+int qe_launch_kv4_unpack(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, uint16_t* out_k, uint16_t* out_v,
+                         int first_row, int num_rows, hipStream_t stream, int num_kv_heads, int head_dim,
+                         int max_seq_len);
+
+/* Bytes of the workspace of qe_launch_attention_gqa_flash_decode_kv4 (host only). */
+int qe_kv4_decode_workspace_bytes(int num_q_heads, int max_seq_len, int with_key_weights, size_t* bytes);
+
+/* Attention of one token (position d_control->seq_pos, its row appended before) over
+ * the 4-bit cache: the counterpart of qe_launch_attention_gqa_flash_decode, Q8_1
+ * outputs included (out_q8 NULL = none).  `workspace` (16-byte aligned, the size
+ * above) is scratch that two launches in flight must not share.  At most 64 q heads
+ * for each kv head.  The cache is split over blocks by max_seq_len, the number of heads
+ * and the rows in use; a launch's bits depend on those alone. */
+int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const uint8_t* layer_k_cache,
+                                             const uint8_t* layer_v_cache, void* workspace, uint16_t* attn_out,
+                                             const qe_device_control_block* d_control, const int32_t* d_evicted,
+                                             hipStream_t stream, int num_q_heads, int num_kv_heads, int head_dim,
+                                             int max_seq_len, int8_t* out_q8, float* out_scale, int32_t* out_sum8,
+                                             const float* key_weights_in, float* key_weights_out);
+
+/* Causal attention of the rows of num_tokens tokens from d_control->seq_pos on
+ * (appended before) over the 4-bit cache: the counterpart of
+ * qe_launch_attention_gqa_prefill, which also says when the split workspace is used.
+ * row_lse (float [T][num_q_heads], NULL = not wanted) receives the natural logarithm
+ * of each row's softmax sum; key weights need it. */
+int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
+                                        uint16_t* attn_out, const qe_device_control_block* d_control,
+                                        const int32_t* d_evicted, int num_tokens, hipStream_t stream,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int max_seq_len,
+                                        int hidden_size, const float* key_weights_in, float* key_weights_out,
+                                        float* row_lse);
+
+/* Bounds the cache: where a head has n > keep rows in use (n = d_control->seq_pos -
+ * d_evicted, i.e. between two tokens), the first `sinks` rows, the last `recent` and, of
+ * the rest, those with the largest key weights stay, keep rows in all (equal weights:
+ * the lower row; NaN counts as the lowest), in their order; K and V rows and weights
+ * move to the front, the weights behind them become zero, and out_evicted[head] =
+ * d_control->seq_pos - keep.  Heads with n <= keep keep everything.  kept_rows
+ * (int32 [num_kv_heads][keep]) receives the old rows of the new ones, -1 behind the last.
+ * Every output may be its input (in place) or memory apart from it, not in between. */
+int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, const float* key_weights,
+                        const int32_t* d_evicted, uint8_t* out_k_cache, uint8_t* out_v_cache, float* out_key_weights,
+                        int32_t* out_evicted, int32_t* kept_rows, const qe_device_control_block* d_control, int keep,
+                        int sinks, int recent, hipStream_t stream, int num_kv_heads, int head_dim, int max_seq_len);
+
+/* ---- log probabilities ------------------------------------------------------------- */
+
+/* Bytes of the workspace of qe_launch_token_logprobs (host only). */
+int qe_token_logprobs_workspace_bytes(int num_rows, int vocab_size, int top_k, size_t* bytes);
+
+/* For each row of fp16 logits (rows row_stride elements apart, any alignment of 2
+ * bytes): out_logprob[row] = log softmax at token_ids[row] (0 for an id outside
+ * [0, vocab_size), e.g. padding; both pointers or neither), out_entropy[row] = -sum p log p
+ * (natural logarithm), and the top_k (0..32) most likely tokens, out_top_ids and
+ * out_top_logprob [num_rows][top_k], the lower index first among equals, as
+ * qe_launch_sample_and_advance settles them.  NULL outputs are skipped.  -inf logits have
+ * probability 0; a row of nothing else has log probabilities -inf and entropy 0; a
+ * row with a NaN or +inf has NaN log probabilities, and NaN logits are never among the
+ * alternatives (id -1 where there are too few).  `workspace` (4-byte aligned, the size
+ * above) is scratch that two launches in flight must not share. */
+int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* token_ids, float* out_logprob, float* out_entropy,
+                             float* out_top_logprob, int32_t* out_top_ids, void* workspace, int num_rows,
+                             int vocab_size, long long row_stride, int top_k, hipStream_t stream);
+
 /* ---- measurement ---------------------------------------------------------------- */
 
 /* Reads `bytes` from `data` with the GEMV weight-stream access pattern

@@ -1,0 +1,956 @@
+// Attention over the 4-bit key/value cache (layout: kv4_common.hpp): one token
+// (flash decode) and the rows of a chunk (causal prefill), each with the weights
+// that its rows give to the cache rows, added up per kv head, when asked for.
+//
+// Rows of the cache come from positions less those evicted (kv4_row); a token at
+// row r sees rows 0..r.  q [T][q heads][128] fp16, head dimension 128.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.hpp"
+#include "kv4_common.hpp"
+
+namespace qe {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kScoreScale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
+
+// The largest value over lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_over_quarters(float x) {
+    x = fmaxf(x, qwen::swz_xor16_f32(x));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_quarters(float x) {
+    x += qwen::swz_xor16_f32(x);
+    return x + __shfl_xor(x, 32);
+}
+
+// ---- one token -------------------------------------------------------------------
+// Split over the cache rows: a block takes a run of rows of one kv head for up to
+// 16 of its q heads, a wave 32 rows at a time, with its own running maximum,
+// sum and output; the waves meet in LDS, the blocks in the second kernel.
+// v_mfma_f32_16x16x32_f16 with the q heads as the columns:
+//   S (16 rows x 16 heads) = K . Q^T: lane l holds cache row l % 16 and, of the
+//   k order, dims 32 (l / 16) + 8 kk..: its four MFMAs take the four words of
+//   one 16-byte chunk, i.e. one quantization group;
+//   the result has lane l = head l % 16 holding rows 4 (l / 16) + i;
+//   O^T (16 dims x 16 heads) += V^T . P^T over 32 rows: P^T is the lane's own
+//   eight probabilities; V^T wants eight rows of one dim in a lane, and MFMA dt
+//   takes dim 8 (l % 16) + dt, so a lane reads word l % 16 of its eight rows.
+//   Two rows' words joined half by half (v_perm) expand to (row, row + 1)
+//   pairs of one dim with the rows' own scales: no transposition through LDS.
+// The whole group of q heads shares one expansion of K and V.
+constexpr int kKd4MaxSplits = 128;   // runs of a kv head, at most
+constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each wave
+constexpr int kKd4Waves = 4;
+constexpr int kKd4MaxGroup = 64;     // q heads of a kv head
+
+// rows of a run for `ctx` rows over at most `splits` runs
+__host__ __device__ __forceinline__ int kd4_run(int ctx, int splits) {
+    const int per = (ctx + splits - 1) / splits;
+    return per > kKd4MinRun ? (per + 31) & ~31 : kKd4MinRun;
+}
+
+struct Decode4Params {
+    const uint16_t* q;
+    const uint8_t* kc;
+    const uint8_t* vc;
+    const qe_device_control_block* ctl;
+    const int32_t* evicted;
+    float* part_o;   // [q head][split][128], relative to the run's maximum
+    float* part_ml;  // [q head][split][2] (maximum in the exp2 domain, sum)
+    float* scores;   // [q head][score_stride] in the exp2 domain, with key weights only
+    uint16_t* out;
+    int8_t* q8;
+    float* q_scale;
+    int32_t* q_sum8;
+    const float* w_in;
+    float* w_out;
+    int nq, nkv, group, head_blocks, max_seq, splits, score_stride;
+};
+
+// cache rows the token sees (one that found the cache full sees all of it)
+__device__ __forceinline__ int kd4_context(const Decode4Params& p, int kvh) {
+    return min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq - 1) + 1;
+}
+
+struct Kd4Tile {
+    u32x4 k[2];          // chunk l / 16 of rows l % 16 and 16 + l % 16
+    uint32_t kp[2];      // its (scale, low)
+    uint32_t v[8], vp[8];  // word l % 16 of the lane's eight rows, its group's (scale, low)
+};
+
+template <bool WEIGHTS>
+__global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Params p) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = lane & 15, h = lane >> 4;
+    const int kvh = blockIdx.x % p.nkv;
+    const int hb = (blockIdx.x / p.nkv) % p.head_blocks, split = blockIdx.x / (p.nkv * p.head_blocks);
+    const int ctx = kd4_context(p, kvh);
+    const int run = kd4_run(ctx, p.splits);
+    const int t0 = split * run, t1 = min(t0 + run, ctx);
+    if (t0 >= t1) return;
+    const int heads = min(16, p.group - 16 * hb), qh0 = kvh * p.group + 16 * hb;
+
+    const size_t head_base = static_cast<size_t>(kvh) * p.max_seq * kKv4Row;
+    const uint8_t* kh = p.kc + head_base;
+    const uint8_t* vh = p.vc + head_base;
+    auto load = [&](int r0, Kd4Tile& t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint8_t* row = kh + static_cast<size_t>(min(r0 + 16 * i + n, t1 - 1)) * kKv4Row;
+            t.k[i] = *reinterpret_cast<const u32x4*>(row + 16 * h);
+            t.kp[i] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * h);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 16 * (i >> 2) + 4 * h + (i & 3);
+            const uint8_t* row = vh + static_cast<size_t>(min(r, t1 - 1)) * kKv4Row;
+            t.v[i] = *reinterpret_cast<const uint32_t*>(row + 4 * n);
+            t.vp[i] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (n >> 2));
+        }
+    };
+    f16x8 qf[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        qf[kk] = f16x8{};
+        if (n < heads)
+            qf[kk] = *reinterpret_cast<const f16x8*>(p.q + static_cast<size_t>(qh0 + n) * kKv4Dim + 32 * h + 8 * kk);
+    }
+    f32x4 acc[8];
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
+    float m = -INFINITY, l = 0.0f;
+    auto use = [&](int r0, const Kd4Tile& t) __attribute__((always_inline)) {
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x4 c = {};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                const uint32_t w = t.k[i][kk];
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_expand_word(w, t.kp[i]), qf[kk], c, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = r0 + 16 * i + 4 * h + e;
+                s[4 * i + e] = r < t1 ? c[e] * kScoreScale : -INFINITY;
+            }
+            if constexpr (WEIGHTS) {
+                if (n < heads)  // the row of scores is padded to whole tiles
+                    *reinterpret_cast<float4*>(p.scores + static_cast<size_t>(qh0 + n) * p.score_stride + r0 + 16 * i +
+                                               4 * h) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(max_over_quarters(mx), m);
+        const float alpha = mx == m ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        f16x8 pf;
+        float ps = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = __builtin_amdgcn_exp2f(s[e] - ref);
+            ps += x;
+            pf[e] = static_cast<_Float16>(x);
+        }
+        l = l * alpha + ps;
+        // V^T: pairs of rows, all eight dims of the lane's word
+        uint32_t vf[8][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t a = t.v[2 * j], b = t.v[2 * j + 1], pa = t.vp[2 * j], pb = t.vp[2 * j + 1];
+            const f16x2 sc = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pb, pa, 0x05040100u));
+            const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pb, pa, 0x07060302u));
+            f16x2 even[4], odd[4];
+            kv4_expand(__builtin_amdgcn_perm(b, a, 0x05040100u), sc, lo, even);
+            kv4_expand(__builtin_amdgcn_perm(b, a, 0x07060302u), sc, lo, odd);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                vf[2 * e][j] = __builtin_bit_cast(uint32_t, even[e]);
+                vf[2 * e + 1][j] = __builtin_bit_cast(uint32_t, odd[e]);
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            const u32x4 a = {vf[dt][0], vf[dt][1], vf[dt][2], vf[dt][3]};
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), pf, acc[dt] * alpha, 0, 0, 0);
+        }
+    };
+    Kd4Tile a;
+    for (int r0 = t0 + 32 * wave; r0 < t1; r0 += 32 * kKd4Waves) {
+        load(r0, a);
+        use(r0, a);
+    }
+    l = sum_over_quarters(l);
+    // the waves meet: common maximum, then outputs
+    __shared__ float s_m[kKd4Waves][16], s_l[kKd4Waves][16];
+    __shared__ float s_o[kKd4Waves][16][kKv4Dim + 4];
+    if (h == 0) {
+        s_m[wave][n] = m;
+        s_l[wave][n] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // dims 8 (4 h + i) + dt
+        float* o = &s_o[wave][n][8 * (4 * h + i)];
+        *reinterpret_cast<float4*>(o) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+        *reinterpret_cast<float4*>(o + 4) = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < heads * 32; u += 64 * kKd4Waves) {
+        const int head = u >> 5, d = 4 * (u & 31);
+        float mg = s_m[0][head];
+#pragma unroll
+        for (int w = 1; w < kKd4Waves; ++w) mg = fmaxf(mg, s_m[w][head]);
+        float lg = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kKd4Waves; ++w) {
+            const float mw = s_m[w][head];
+            const float f = mw == mg ? 1.0f : __builtin_amdgcn_exp2f(mw - mg);
+            const float4 x = *reinterpret_cast<const float4*>(&s_o[w][head][d]);
+            lg += f * s_l[w][head];
+            o.x += f * x.x;
+            o.y += f * x.y;
+            o.z += f * x.z;
+            o.w += f * x.w;
+        }
+        const size_t at = static_cast<size_t>(qh0 + head) * p.splits + split;
+        *reinterpret_cast<float4*>(p.part_o + at * kKv4Dim + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(mg, lg);
+    }
+}
+
+// Weight of every run of one head and the head's sum, by one wave: w = exp2(m - M),
+// L = sum w l.  A NaN sum (a NaN score) makes L NaN.
+__device__ __forceinline__ void kd4_run_weights(const float* ml, int live, int lane, float (&w)[kKd4MaxSplits / 64],
+                                                float& M, float& L) {
+    float2 x[kKd4MaxSplits / 64];
+    M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kKd4MaxSplits / 64; ++i) {
+        const int s = lane + 64 * i;
+        x[i] = s < live ? *reinterpret_cast<const float2*>(ml + 2 * s) : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, x[i].x);
+    }
+    M = qwen::seg_max<64>(M);
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kKd4MaxSplits / 64; ++i) {
+        w[i] = x[i].x == M ? 1.0f : __builtin_amdgcn_exp2f(x[i].x - M);
+        if (lane + 64 * i >= live) w[i] = 0.0f;
+        L += w[i] * x[i].y;
+    }
+    L = qwen::seg_sum<64>(L);
+}
+
+// Blocks 0..nq-1: one q head each, its runs merged (32 lanes x 4 dims, 16 groups
+// of runs), rounded once to fp16, and the Q8_1 of it when asked for.  The blocks
+// behind them, with key weights: 256 rows of one kv head, the sum over its q
+// heads of exp2(score - M) / L added to the weight so far; the newest row
+// starts at its own sum.
+constexpr int kKd4MergeThreads = 512;
+template <bool WEIGHTS>
+__global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Decode4Params p) {
+    constexpr int G = kKd4MergeThreads / 32, PER = kKd4MaxSplits / G;
+    __shared__ __align__(16) float s_o[G][kKv4Dim];
+    __shared__ float s_w[kKd4MaxSplits];
+    __shared__ float s_M[kKd4MaxGroup], s_inv[kKd4MaxGroup];
+    __shared__ float s_max[kKd4MergeThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (WEIGHTS && static_cast<int>(blockIdx.x) >= p.nq) {
+        const int b = blockIdx.x - p.nq, kvh = b % p.nkv;
+        const int row = (b / p.nkv) * kKd4MergeThreads + tid;
+        const int ctx = kd4_context(p, kvh);
+        if (row - tid >= ctx) return;
+        const int run = kd4_run(ctx, p.splits), live = (ctx + run - 1) / run;
+        for (int g = wave; g < p.group; g += kKd4MergeThreads / 64) {
+            float w[kKd4MaxSplits / 64], M, L;
+            kd4_run_weights(p.part_ml + static_cast<size_t>(kvh * p.group + g) * p.splits * 2, live, lane, w, M, L);
+            if (lane == 0) {
+                s_M[g] = M == -INFINITY ? 0.0f : M;
+                s_inv[g] = 1.0f / L;
+            }
+        }
+        __syncthreads();
+        if (row >= ctx) return;
+        const size_t at = static_cast<size_t>(kvh) * p.max_seq + row;
+        float sum = 0.0f;
+        for (int g = 0; g < p.group; ++g)
+            sum += __builtin_amdgcn_exp2f(p.scores[static_cast<size_t>(kvh * p.group + g) * p.score_stride + row] -
+                                          s_M[g]) * s_inv[g];
+        p.w_out[at] = (p.w_in != nullptr && row < kv4_row(p.ctl, p.evicted, kvh) ? p.w_in[at] : 0.0f) + sum;
+        return;
+    }
+    const int qh = blockIdx.x, kvh = qh / p.group;
+    const int ctx = kd4_context(p, kvh);
+    const int run = kd4_run(ctx, p.splits), live = (ctx + run - 1) / run;
+    const int d = 4 * (tid & 31), g = tid >> 5;
+    const float* po = p.part_o + static_cast<size_t>(qh) * p.splits * kKv4Dim;
+    float4 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {  // requested before the weights are known
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (g + G * i < live) x[i] = *reinterpret_cast<const float4*>(po + static_cast<size_t>(g + G * i) * kKv4Dim + d);
+    }
+    if (wave == 0) {
+        float w[kKd4MaxSplits / 64], M, L;
+        kd4_run_weights(p.part_ml + static_cast<size_t>(qh) * p.splits * 2, live, lane, w, M, L);
+        const float inv = 1.0f / L;
+#pragma unroll
+        for (int i = 0; i < kKd4MaxSplits / 64; ++i) s_w[lane + 64 * i] = w[i] * inv;
+    }
+    __syncthreads();
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (g + G * i >= live) break;
+        const float w = s_w[g + G * i];
+        o.x += w * x[i].x;
+        o.y += w * x[i].y;
+        o.z += w * x[i].z;
+        o.w += w * x[i].w;
+    }
+    *reinterpret_cast<float4*>(&s_o[g][d]) = o;
+    __syncthreads();
+    float acc = 0.0f;
+    if (tid < kKv4Dim) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) acc += s_o[i][tid];
+        p.out[static_cast<size_t>(qh) * kKv4Dim + tid] = f2h(acc);
+    }
+    if (p.q8 == nullptr) return;
+    // Q8_1 of the head (one group of 128), as the fp16 flash decode writes it
+    const float mx = qwen::seg_max<64>(fabsf(acc));
+    if (lane == 0) s_max[wave] = mx;
+    __syncthreads();
+    if (tid >= kKv4Dim) return;
+    const float dd = flash_q8_scale(fmaxf(s_max[0], s_max[1]));
+    if (tid == 0 && p.q_scale != nullptr) p.q_scale[qh] = dd;
+    const int v = flash_q8_value(acc, dd);
+    p.q8[static_cast<size_t>(qh) * kKv4Dim + tid] = static_cast<int8_t>(v);
+    int s8 = -8 * v;
+    s8 += qwen::dpp_i32<0xB1>(s8);
+    s8 += qwen::dpp_i32<0x4E>(s8);
+    s8 += qwen::dpp_i32<0x141>(s8);
+    if ((tid & 7) == 0 && p.q_sum8 != nullptr) p.q_sum8[qh * (kKv4Dim / 8) + (tid >> 3)] = s8;
+}
+
+// ---- the rows of a chunk -------------------------------------------------------------
+// Query rows r = token r / group, head kvh * group + r % group; a block takes
+// 32 WAVES consecutive rows of one kv head, 32 a wave, and walks its run of
+// key tiles (64 cache rows).  Both products are v_mfma_f32_32x32x16_f16 with the
+// rows as columns, as in the fp16 prefill: S^T = K . Q^T, a row's maximum and sum
+// in its own lane and lane ^ 32; O^T += V^T . P^T with P^T the lane's own.
+// A tile is expanded once per block, into LDS as fp16: a thread takes 16-byte chunk
+// g (one quantization group) of one row and writes four 16-byte chunks, 4 g + i,
+// stored at chunk ^ swz(row).  Its 16 lanes that store together hold 16 rows
+// of one g, so they touch 16 different bank groups, like the readers (16 rows of one
+// chunk for K; 4 rows x 4 chunks through ds_read_b64_tr_b16 for V).
+// The raw 20 bytes of the tile after the next are in registers a whole step
+// before they are expanded.
+constexpr int kP4Keys = 64;
+constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
+constexpr float kP4Lag = 8.0f;  // how far a row's maximum grows before its reference value follows
+constexpr int kP4MinTiles = 4;
+constexpr int kP4MaxSplits = 16;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct Prefill4Params {
+    const uint16_t* q;
+    const uint8_t* kc;
+    const uint8_t* vc;
+    uint16_t* out;
+    const qe_device_control_block* ctl;
+    const int32_t* evicted;
+    float* part_o;   // [split][kv head][row][128] unnormalized
+    float* part_ml;  // [split][kv head][row][2] (reference value, sum)
+    float* lse;      // [token][q head] natural log, or NULL
+    const float* w_in;
+    float* w_out;
+    int T, nq, nkv, group, max_seq, out_stride, splits, row_blocks, block_rows;
+};
+
+__device__ __forceinline__ int p4_live_splits(int tiles, int splits) {
+    return max(1, min(splits, tiles / kP4MinTiles));
+}
+// key tiles of row block rb (the rows of the cache that its last row sees)
+__device__ __forceinline__ int p4_tiles(const Prefill4Params& p, int rb, int base) {
+    const int last = min((rb + 1) * p.block_rows, p.T * p.group) - 1;
+    const int len = min(base, p.max_seq) + last / p.group + 1;
+    return (min(len, p.max_seq) + kP4Keys - 1) / kP4Keys;
+}
+
+__device__ __forceinline__ float xor32_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x),
+                                                    false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Params p) {
+    __shared__ __align__(16) char smem[4 * kP4TileBytes];  // K buffers 0 and 1, V buffers 0 and 1
+    constexpr int UNITS = 8 / WAVES;  // (K or V) chunks a thread expands for a tile: 512 in all
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int fr = lane & 31, h = lane >> 5;
+    const int rb = p.row_blocks - 1 - static_cast<int>(blockIdx.x) % p.row_blocks;  // longest rows first
+    const int cb = static_cast<int>(blockIdx.x) / p.row_blocks;
+    const int kvh = cb % p.nkv, split = cb / p.nkv;
+    const int rows = p.T * p.group;
+    const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
+    const int nt_all = p4_tiles(p, rb, base);
+    const int live = p4_live_splits(nt_all, p.splits);
+    if (split >= live) return;
+    const int it0 = static_cast<int>((static_cast<long long>(split) * nt_all) / live);
+    const int it1 = static_cast<int>((static_cast<long long>(split + 1) * nt_all) / live);
+    const int r = rb * (32 * WAVES) + wave * 32 + fr;
+    const int rc = min(r, rows - 1);
+    const int qi = rc / p.group, qh = kvh * p.group + rc % p.group;
+    const int lim = min(min(base + qi, p.max_seq - 1), it1 * kP4Keys - 1);  // last cache row this row takes here
+    const int wave_lim = __builtin_amdgcn_readlane(lim, 0);
+    const int wave_last = __builtin_amdgcn_readlane(lim, 31);
+    const int key_max = min(base + p.T, p.max_seq) - 1;  // the last cache row that holds anything
+
+    u32x4 qf[8];
+    {
+        const uint16_t* qr = p.q + (static_cast<size_t>(qi) * p.nq + qh) * kKv4Dim + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
+    }
+    // staging: unit u = chunk g of row srow, K units first; with 8 waves, waves
+    // 0..3 expand K and 4..7 V, with 4 every thread does one of each
+    const int su = threadIdx.x & 255, srow = (su & 15) + 16 * (su >> 6), sg = (su >> 4) & 3;
+    const size_t hb = static_cast<size_t>(kvh) * p.max_seq * kKv4Row;
+    const uint8_t* src[UNITS];
+    char* dst[UNITS];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
+        src[u] = (is_v ? p.vc : p.kc) + hb;
+        dst[u] = smem + (is_v ? 2 : 0) * kP4TileBytes + srow * 256;
+    }
+    const int sswz = ((srow & 3) << 2) | ((srow >> 2) & 3);
+    u32x4 raw[UNITS];
+    uint32_t rawp[UNITS];
+    // tile tk for the K units, tv for the V units
+    auto fetch = [&](int tk, int tv) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
+            const uint8_t* row = src[u] + static_cast<size_t>(min((is_v ? tv : tk) * kP4Keys + srow, key_max)) * kKv4Row;
+            raw[u] = *reinterpret_cast<const u32x4*>(row + 16 * sg);
+            rawp[u] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * sg);
+        }
+    };
+    auto expand = [&](int kbuf, int vbuf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
+            char* d = dst[u] + (is_v ? vbuf : kbuf) * kP4TileBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = raw[u][i];
+                *reinterpret_cast<f16x8*>(d + 16 * ((4 * sg + i) ^ sswz)) = kv4_expand_word(w, rawp[u]);
+            }
+        }
+    };
+    auto tile_barrier = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) void*)smem));
+    // LDS addresses: K chunk 2 kk + h of row fr; V^T reads (dt: 32 dims, u: rows + 8)
+    uint32_t ka[8], va[4][2];
+    {
+        const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
+        const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
+        const int s16 = lane & 15, b16 = (lane >> 4) & 1;
+        const uint32_t v0 = lds0 + 2 * kP4TileBytes + (4 * h + (s16 >> 2)) * 256 +
+                            16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+            va[dt][0] = v0 ^ (64 * dt);
+            va[dt][1] = (v0 ^ (64 * dt) ^ 32) + 8 * 256;
+        }
+    }
+    // K operand of MFMA i of a tile: 32-row half i % 2, dims 16 (i / 2); V^T
+    // operand: 16-row quarter i / 4, dims 32 (i % 4)
+    auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
+        typedef const __attribute__((address_space(3))) f16x8* lptr;
+        return *reinterpret_cast<lptr>(ka[i >> 1] + buf * kP4TileBytes + (i & 1) * 32 * 256);
+    };
+    auto read_v = [&](int buf, int i) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) s16x4* lptr;
+        const uint32_t off = buf * kP4TileBytes + (i >> 2) * 16 * 256;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][0] + off));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][1] + off));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    f32x16 acc[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
+    float mref = -INFINITY, lsum = 0.0f;
+    auto mask = [&](int t, f32x16 (&sc)[2]) __attribute__((always_inline)) {
+        if ((t + 1) * kP4Keys - 1 > wave_lim) {  // wave-uniform
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int key = t * kP4Keys + 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
+                    sc[j][v] = key <= lim ? sc[j][v] : -INFINITY;
+                }
+        }
+    };
+    auto renew_ref = [&](float mx) __attribute__((always_inline)) {
+        const bool grow = mx > mref + kP4Lag;
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+            const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
+            mref = grow ? mx : mref;
+            lsum *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+        }
+    };
+    auto row_max = [&](const f32x16 (&sc)[2]) __attribute__((always_inline)) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[j][v]);
+        return xor32_max(mx) * kScoreScale;
+    };
+    // probabilities 2 i and 2 i + 1 of a tile's scores (32-row half i / 8), packed
+    auto probs = [&](const f32x16 (&sc)[2], int i, float neg, float (&ps)[2]) __attribute__((always_inline)) {
+        const int j = i >> 3, v = 2 * (i & 7);
+        const f32x2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v], kScoreScale, neg)),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v + 1], kScoreScale, neg))};
+        ps[0] += e.x;
+        ps[1] += e.y;
+        uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, f16x2));
+        asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]));  // here, not past the mask's branch
+        return w;
+    };
+    constexpr int AHEAD = 4;  // operand reads in flight before their MFMA
+    // Scores of the K tile in `buf`; beside them, when EXP, the probabilities of
+    // the scores `cur`, each MFMA fenced together with its share of the vector work.
+    auto scores = [&](auto exp_too, int buf, f32x16 (&sc)[2], const f32x16 (&cur)[2],
+                      uint32_t (&pw)[2][8]) __attribute__((always_inline)) {
+        const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
+        float ps[2] = {0.0f, 0.0f};
+        f16x8 kf[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kf[i] = read_k(buf, i);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % AHEAD], __builtin_bit_cast(f16x8, qf[i >> 1]),
+                                                               i < 2 ? f32x16{} : sc[i & 1], 0, 0, 0);
+            if (i + AHEAD < 16) kf[i % AHEAD] = read_k(buf, i + AHEAD);
+            if constexpr (decltype(exp_too)::value) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (decltype(exp_too)::value) lsum += ps[0] + ps[1];
+    };
+    // O^T += V^T . P^T; beside it, when MAX, the (scaled) row maximum of nxt
+    auto add_pv = [&](auto max_too, const uint32_t (&pw)[2][8], int buf,
+                      const f32x16 (&nxt)[2]) __attribute__((always_inline)) {
+        f16x8 vf[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) vf[i] = read_v(buf, i);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int j = i >> 3, ks = (i >> 2) & 1, dt = i & 3;
+            const u32x4 pf = {pw[j][4 * ks], pw[j][4 * ks + 1], pw[j][4 * ks + 2], pw[j][4 * ks + 3]};
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % AHEAD], __builtin_bit_cast(f16x8, pf), acc[dt], 0, 0, 0);
+            if (i + AHEAD < 16) vf[i % AHEAD] = read_v(buf, i + AHEAD);
+            if constexpr (decltype(max_too)::value)
+                mx = fmaxf(fmaxf(mx, nxt[j][2 * (i & 7)]), nxt[j][2 * (i & 7) + 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return decltype(max_too)::value ? xor32_max(mx) * kScoreScale : 0.0f;
+    };
+    typedef std::true_type yes;
+    typedef std::false_type no;
+    // what a step does for everyone: K of the tile after next and V of the next
+    // go to LDS (b: parity of tile t), the raw bytes behind them are requested
+    auto stage = [&](int t, int b) __attribute__((always_inline)) {
+        expand(b, b ^ 1);
+        fetch(t + 3, t + 2);
+    };
+    // Tile t's scores are in cur: the scores of the next tile beside the
+    // probabilities of t, then V of t beside the next tile's maximum.
+    auto step = [&](int t, int b, f32x16 (&cur)[2], f32x16 (&nxt)[2]) __attribute__((always_inline)) {
+        uint32_t pw[2][8];
+        stage(t, b);
+        scores(yes{}, b ^ 1, nxt, cur, pw);
+        mask(t + 1, nxt);
+        const float mx = add_pv(yes{}, pw, b, nxt);
+        renew_ref(mx);
+        tile_barrier();
+    };
+    auto finish = [&](int b, f32x16 (&cur)[2]) __attribute__((always_inline)) {
+        uint32_t pw[2][8];
+        const float neg = mref == -INFINITY ? 0.0f : -mref;
+        float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
+        lsum += ps[0] + ps[1];
+        add_pv(no{}, pw, b, cur);
+    };
+    if (it0 < it1) {
+        const int n = it1 - it0;
+        int t = it0;
+        fetch(t, t);
+        expand(0, 0);
+        fetch(t + 1, t + 1);
+        // K of the second tile now; V of it comes with the first step, which
+        // expands what is in registers: K of the third, V of the second
+        if constexpr (UNITS == 2) {
+            expand(1, 1);
+        } else {
+            if (wave < 4) expand(1, 1);
+        }
+        fetch(t + 2, t + 1);
+        tile_barrier();
+        f32x16 s0[2], s1[2];
+        {
+            uint32_t pw[2][8];
+            scores(no{}, 0, s0, s1, pw);
+        }
+        mask(t, s0);
+        renew_ref(row_max(s0));
+        tile_barrier();  // K buffer 0 is read
+        // tiles past the wave's last key are not multiplied
+        const int mine = wave_last < t * kP4Keys ? 0 : min(n, wave_last / kP4Keys - t + 1);
+        int left = mine;
+        for (; left > 2; left -= 2) {
+            step(t, 0, s0, s1);
+            step(t + 1, 1, s1, s0);
+            t += 2;
+        }
+        if (left == 2) {
+            step(t, 0, s0, s1);
+            finish(1, s1);
+        } else if (left == 1) {
+            finish(0, s0);
+        }
+        for (int i = max(mine - 1, 0); i < n - 1; ++i) {  // the tiles of the other waves
+            stage(it0 + i, i & 1);
+            tile_barrier();
+        }
+    }
+    lsum += __shfl_xor(lsum, 32);
+    if (r >= rows) return;
+    if (live == 1) {
+        const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+        uint16_t* o = p.out + static_cast<size_t>(qi) * p.out_stride + qh * kKv4Dim;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {  // dims 32dt + 8g + 4h .. +3
+                const uint32_t w0 = static_cast<uint32_t>(f2h(acc[dt][4 * g] * inv)) |
+                                    (static_cast<uint32_t>(f2h(acc[dt][4 * g + 1] * inv)) << 16);
+                const uint32_t w1 = static_cast<uint32_t>(f2h(acc[dt][4 * g + 2] * inv)) |
+                                    (static_cast<uint32_t>(f2h(acc[dt][4 * g + 3] * inv)) << 16);
+                *reinterpret_cast<uint2*>(o + 32 * dt + 8 * g + 4 * h) = make_uint2(w0, w1);
+            }
+        if (p.lse != nullptr && h == 0)
+            p.lse[static_cast<size_t>(qi) * p.nq + qh] = (mref == -INFINITY ? 0.0f : mref) * kLn2 + logf(lsum);
+        return;
+    }
+    const size_t prow = (static_cast<size_t>(split) * p.nkv + kvh) * rows + r;
+    if (h == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * prow) = make_float2(mref, lsum);
+    float* po = p.part_o + prow * kKv4Dim;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4*>(po + 32 * dt + 8 * g + 4 * h) =
+                make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+}
+
+// Merges the splits of every row: 32 lanes a row (4 dims each), 8 rows a block.
+// Rows whose block had one split are already written.
+__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p) {
+    const int rows = p.T * p.group;
+    const int s_lane = threadIdx.x & 31, d = 4 * s_lane;
+    const long long all = static_cast<long long>(rows) * p.nkv;
+    const long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (i >= all) return;
+    const int kvh = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<long long>(kvh) * rows);
+    const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
+    const int live = p4_live_splits(p4_tiles(p, r / p.block_rows, base), p.splits);
+    if (live == 1) return;
+    constexpr int B = 8;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (s_lane < live) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (s_lane * all + i));
+    float4 v[B];
+    auto request = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            v[b] = *reinterpret_cast<const float4*>(p.part_o + (min(s0 + b, live - 1) * all + i) * kKv4Dim + d);
+    };
+    request(0);
+    const float m = qwen::seg_max<32>(ml.x);
+    // (a split whose scores are all NaN has no maximum and a NaN sum, which the product below keeps)
+    const float w_lane = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < live; s0 += B) {
+        if (s0 > 0) request(s0);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (s0 + b >= live) break;
+            const float w = __shfl(w_lane, s0 + b, 32);
+            l += w * __shfl(ml.y, s0 + b, 32);
+            o.x += w * v[b].x;
+            o.y += w * v[b].y;
+            o.z += w * v[b].z;
+            o.w += w * v[b].w;
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int qi = r / p.group, qh = kvh * p.group + r % p.group;
+    uint16_t* dst = p.out + static_cast<size_t>(qi) * p.out_stride + qh * kKv4Dim + d;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(static_cast<uint32_t>(f2h(o.x * inv)) | (static_cast<uint32_t>(f2h(o.y * inv)) << 16),
+                   static_cast<uint32_t>(f2h(o.z * inv)) | (static_cast<uint32_t>(f2h(o.w * inv)) << 16));
+    if (p.lse != nullptr && s_lane == 0)
+        p.lse[static_cast<size_t>(qi) * p.nq + qh] = (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
+}
+
+// Column sums of the probabilities: what the rows of the chunk give to 64 cache
+// rows of one kv head.  The block's 64 K rows stay in registers, expanded once;
+// a wave takes 32 query rows at a time, S^T = K . Q^T again, p = exp(s - lse) with
+// the row's final log sum, and keeps 32 sums a lane; lanes, then waves, add up
+// at the end in one order.
+constexpr int kW4Waves = 8;
+__global__ __launch_bounds__(64 * kW4Waves, 2) void kv4_prefill_weights_kernel(Prefill4Params p) {
+    __shared__ float s_sum[kW4Waves][kP4Keys];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int fr = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x % p.nkv, t = blockIdx.x / p.nkv;
+    const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
+    const int len = min(base + p.T, p.max_seq);  // (base <= max_seq, T fits)
+    const int key0 = t * kP4Keys;
+    if (key0 >= len) return;
+    const int rows = p.T * p.group;
+    f16x8 kf[2][8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint8_t* row = p.kc + (static_cast<size_t>(kvh) * p.max_seq + min(key0 + 32 * j + fr, len - 1)) * kKv4Row;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // word 2 kk + h: dims 16 kk + 8 h..
+            kf[j][kk] = kv4_expand_word(*reinterpret_cast<const uint32_t*>(row + 4 * (2 * kk + h)),
+                                        *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (kk >> 1)));
+    }
+    f32x16 sum[2] = {f32x16{}, f32x16{}};
+    const int first = max(0, min(key0 - base, p.T - 1)) * p.group / 32 * 32;  // no row before it sees key0
+    for (int r0 = first + 32 * wave; r0 < rows; r0 += 32 * kW4Waves) {
+        const int r = r0 + fr, rc = min(r, rows - 1);
+        const int qi = rc / p.group, qh = kvh * p.group + rc % p.group;
+        const uint16_t* qr = p.q + (static_cast<size_t>(qi) * p.nq + qh) * kKv4Dim + 8 * h;
+        const float neg = -p.lse[static_cast<size_t>(qi) * p.nq + qh] * kLog2e;
+        const int lim = r < rows ? min(base + qi, p.max_seq - 1) : -1;
+        f32x16 sc[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+            const f16x8 qf = *reinterpret_cast<const f16x8*>(qr + 16 * kk);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][kk], qf, sc[j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int key = key0 + 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v], kScoreScale, neg));
+                sum[j][v] += key <= lim ? e : 0.0f;
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const float x = qwen::seg_sum<32>(sum[j][v]);
+            if (fr == 0) s_sum[wave][32 * j + 8 * (v >> 2) + 4 * h + (v & 3)] = x;
+        }
+    __syncthreads();
+    const int key = key0 + static_cast<int>(threadIdx.x);
+    if (threadIdx.x >= kP4Keys || key >= len) return;
+    float x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kW4Waves; ++w) x += s_sum[w][threadIdx.x];
+    const size_t at = static_cast<size_t>(kvh) * p.max_seq + key;
+    p.w_out[at] = (p.w_in != nullptr && key < base ? p.w_in[at] : 0.0f) + x;
+}
+
+inline bool capturing(hipStream_t stream) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &st) == hipSuccess) return st != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();
+    return true;
+}
+
+inline int check_heads(const char* what, int nq, int nkv) {
+    QE_REQUIRE(nq > 0 && nq % nkv == 0, "%s: %d q heads over %d kv heads", what, nq, nkv);
+    QE_REQUIRE(nq / nkv <= kKd4MaxGroup, "%s: %d q heads for each kv head (at most %d)", what, nq / nkv, kKd4MaxGroup);
+    return QE_OK;
+}
+
+inline int score_stride(int max_seq) { return (max_seq + 31) / 32 * 32; }
+
+}  // namespace
+}  // namespace qe
+
+using namespace qe;
+
+extern "C" int qe_kv4_decode_workspace_bytes(int num_q_heads, int max_seq_len, int with_key_weights, size_t* bytes) {
+    QE_REQUIRE(bytes != nullptr, "kv4_decode_workspace_bytes: NULL pointer");
+    QE_REQUIRE(num_q_heads > 0 && max_seq_len > 0 && max_seq_len <= INT32_MAX - 31,
+               "kv4_decode_workspace_bytes: num_q_heads=%d max_seq_len=%d", num_q_heads, max_seq_len);
+    size_t floats = static_cast<size_t>(num_q_heads) * kKd4MaxSplits * (kKv4Dim + 2);
+    if (with_key_weights) floats += static_cast<size_t>(num_q_heads) * score_stride(max_seq_len);
+    *bytes = floats * sizeof(float);
+    return QE_OK;
+}
+
+extern "C" int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const uint8_t* layer_k_cache,
+                                                        const uint8_t* layer_v_cache, void* workspace,
+                                                        uint16_t* attn_out, const qe_device_control_block* d_control,
+                                                        const int32_t* d_evicted, hipStream_t stream,
+                                                        int num_q_heads, int num_kv_heads, int head_dim,
+                                                        int max_seq_len, int8_t* out_q8, float* out_scale,
+                                                        int32_t* out_sum8, const float* key_weights_in,
+                                                        float* key_weights_out) {
+    const char* what = "attention_gqa_flash_decode_kv4";
+    QE_REQUIRE(q && workspace && attn_out, "%s: NULL pointer", what);
+    QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
+    QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
+    QE_REQUIRE(max_seq_len <= INT32_MAX - 31, "%s: max_seq_len=%d", what, max_seq_len);
+    QE_REQUIRE(aligned(q, 16) && aligned(workspace, 16), "%s: q and the workspace must be 16-byte aligned", what);
+    QE_REQUIRE(key_weights_in == nullptr || key_weights_out != nullptr, "%s: key_weights_in without key_weights_out",
+               what);
+    Decode4Params p{};
+    p.q = q;
+    p.kc = layer_k_cache;
+    p.vc = layer_v_cache;
+    p.ctl = d_control;
+    p.evicted = d_evicted;
+    p.out = attn_out;
+    p.q8 = out_q8;
+    p.q_scale = out_scale;
+    p.q_sum8 = out_sum8;
+    p.w_in = key_weights_in;
+    p.w_out = key_weights_out;
+    p.nq = num_q_heads;
+    p.nkv = num_kv_heads;
+    p.group = num_q_heads / num_kv_heads;
+    p.head_blocks = (p.group + 15) / 16;
+    p.max_seq = max_seq_len;
+    p.score_stride = score_stride(max_seq_len);
+    // two blocks per CU, and no more runs than the cache can fill
+    const long long units = static_cast<long long>(num_kv_heads) * p.head_blocks;
+    p.splits = static_cast<int>(std::max(8LL, std::min<long long>(kKd4MaxSplits, 2LL * cu_count() / units)));
+    p.splits = std::min(p.splits, (max_seq_len - 1) / kKd4MinRun + 1);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + static_cast<size_t>(num_q_heads) * kKd4MaxSplits * kKv4Dim;
+    p.scores = p.part_ml + static_cast<size_t>(num_q_heads) * kKd4MaxSplits * 2;
+    const long long blocks = units * p.splits;
+    const long long weight_blocks =
+        static_cast<long long>(num_kv_heads) * ((static_cast<long long>(max_seq_len) + kKd4MergeThreads - 1) / kKd4MergeThreads);
+    QE_REQUIRE(blocks <= INT32_MAX && weight_blocks + num_q_heads <= INT32_MAX, "%s: too many heads", what);
+    if (key_weights_out != nullptr) {
+        kv4_decode_kernel<true><<<static_cast<unsigned>(blocks), 64 * kKd4Waves, 0, stream>>>(p);
+        kv4_decode_merge_kernel<true><<<static_cast<unsigned>(num_q_heads + weight_blocks), kKd4MergeThreads, 0, stream>>>(p);
+    } else {
+        kv4_decode_kernel<false><<<static_cast<unsigned>(blocks), 64 * kKd4Waves, 0, stream>>>(p);
+        kv4_decode_merge_kernel<false><<<static_cast<unsigned>(num_q_heads), kKd4MergeThreads, 0, stream>>>(p);
+    }
+    return check_launch(what);
+}
+
+extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint8_t* layer_k_cache,
+                                                   const uint8_t* layer_v_cache, uint16_t* attn_out,
+                                                   const qe_device_control_block* d_control, const int32_t* d_evicted,
+                                                   int num_tokens, hipStream_t stream, int num_q_heads,
+                                                   int num_kv_heads, int head_dim, int max_seq_len, int hidden_size,
+                                                   const float* key_weights_in, float* key_weights_out,
+                                                   float* row_lse) {
+    const char* what = "attention_gqa_prefill_kv4";
+    QE_REQUIRE(q && attn_out, "%s: NULL pointer", what);
+    QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
+    QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
+    QE_REQUIRE(hidden_size >= num_q_heads * head_dim && hidden_size % 4 == 0, "%s: hidden_size=%d", what, hidden_size);
+    QE_REQUIRE(key_weights_in == nullptr || key_weights_out != nullptr, "%s: key_weights_in without key_weights_out",
+               what);
+    QE_REQUIRE(key_weights_out == nullptr || row_lse != nullptr, "%s: key weights need row_lse", what);
+    QE_REQUIRE(aligned(q, 16) && aligned(attn_out, 8), "%s: q must be 16-byte and attn_out 8-byte aligned", what);
+    if (num_tokens <= 0) return QE_OK;
+    Prefill4Params p{};
+    p.q = q;
+    p.kc = layer_k_cache;
+    p.vc = layer_v_cache;
+    p.out = attn_out;
+    p.ctl = d_control;
+    p.evicted = d_evicted;
+    p.lse = row_lse;
+    p.w_in = key_weights_in;
+    p.w_out = key_weights_out;
+    p.T = num_tokens;
+    p.nq = num_q_heads;
+    p.nkv = num_kv_heads;
+    p.group = num_q_heads / num_kv_heads;
+    p.max_seq = max_seq_len;
+    p.out_stride = hidden_size;
+    const long long rows = static_cast<long long>(num_tokens) * p.group;
+    QE_REQUIRE(rows <= (1 << 29) && max_seq_len <= (1 << 29), "%s: num_tokens=%d max_seq_len=%d", what, num_tokens,
+               max_seq_len);
+    const int waves = rows <= 128 ? 4 : 8;
+    p.block_rows = 32 * waves;
+    p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
+    const long long blocks = static_cast<long long>(p.row_blocks) * num_kv_heads;
+    // Key splits as far as the chip has room for their blocks, the stream's
+    // workspace for their partials, and the cache has tiles.
+    const int cus = cu_count();
+    const WorkspaceLease lease(stream);  // until every kernel is enqueued
+    const StreamWorkspace ws = lease.ws;
+    const long long part = rows * num_kv_heads * (kKv4Dim + 2);  // floats of one split
+    const long long slots = waves == 4 ? 2LL * cus : cus;
+    p.splits = 1;
+    if (ws.ptr != nullptr && max_seq_len >= 16 * kP4Keys)
+        p.splits = static_cast<int>(std::max(1LL, std::min({static_cast<long long>(kP4MaxSplits), slots / blocks,
+                                                            static_cast<long long>(ws.floats) / part,
+                                                            static_cast<long long>(max_seq_len) / (kP4Keys * kP4MinTiles)})));
+    // A graph may be replayed on any stream and after the workspace is gone: a recorded launch touches none.
+    if (p.splits > 1 && capturing(stream)) p.splits = 1;
+    QE_REQUIRE(blocks * p.splits <= INT32_MAX, "%s: num_tokens=%d", what, num_tokens);
+    p.part_o = ws.ptr;
+    p.part_ml = ws.ptr + p.splits * rows * num_kv_heads * kKv4Dim;
+    const unsigned grid = static_cast<unsigned>(blocks * p.splits);
+    if (waves == 4) kv4_prefill_kernel<4><<<grid, 256, 0, stream>>>(p);
+    else kv4_prefill_kernel<8><<<grid, 512, 0, stream>>>(p);
+    if (p.splits > 1)
+        kv4_prefill_merge_kernel<<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
+    if (key_weights_out != nullptr) {
+        const long long tiles = (static_cast<long long>(max_seq_len) + kP4Keys - 1) / kP4Keys;
+        QE_REQUIRE(tiles * num_kv_heads <= INT32_MAX, "%s: max_seq_len=%d", what, max_seq_len);
+        kv4_prefill_weights_kernel<<<static_cast<unsigned>(tiles * num_kv_heads), 64 * kW4Waves, 0, stream>>>(p);
+    }
+    return check_launch(what);
+}

@@ -1,0 +1,412 @@
+// 4-bit key/value cache (layout: kv4_common.hpp): append of new tokens, reading
+// rows back as fp16, and eviction of the rows with the least attention.
+#include <algorithm>
+#include <cmath>
+
+#include "kv4_common.hpp"
+
+namespace qe {
+namespace {
+
+// ---- append ------------------------------------------------------------------
+// x = q, k, v + bias in fp32, q and k rotated (NeoX pairs i, i + rot / 2 by
+// the angle pos * theta^(-2 i / rot)), q rounded once to fp16, k and v straight
+// to 4 bits: per 32 elements low = fp16(min), scale = fp16((max - low) / 15),
+// nibble = clamp(rint((x - low) / scale), 0, 15); a scale of 0 gives nibbles 0.
+//
+// Angles: position times frequency in 64 bits, reduced to [-pi, pi] there, then
+// sine and cosine in fp32.  In fp32 the angle of position 100000 is off by
+// up to 4e-3.
+//
+// grid (tokens, ceil((nq + nkv) / 16)), 256 threads: 16 lanes a head, 8 elements a
+// lane, so a group of 32 is a quad of lanes; the first rot / 2 threads make the
+// token's sines and cosines.  The partner of a rotation is read from memory a
+// second time (it is in the cache) instead of being exchanged.
+__global__ __launch_bounds__(256) void qkv_bias_rope_kv4_append_kernel(
+    const uint16_t* q, uint16_t* q_out, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
+    const uint16_t* __restrict__ qb, const uint16_t* __restrict__ kb, const uint16_t* __restrict__ vb,
+    uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, const qe_device_control_block* ctl, const int32_t* evicted,
+    int nq, int nkv, int max_seq, int rot, double log2_theta) {
+#pragma clang fp contract(off)
+    __shared__ float s_sin[kKv4Dim / 2], s_cos[kKv4Dim / 2];
+    const int t = blockIdx.x, j = threadIdx.x & 15;
+    const int head = blockIdx.y * 16 + (threadIdx.x >> 4);
+    const int half = rot / 2;
+    const bool live = head < nq + nkv, is_k = head >= nq;
+    const int hk = is_k ? head - nq : 0;
+    // own 8 elements, their rotation partners, and v's
+    const bool turned = 8 * j < rot;
+    const int pd = turned ? (8 * j < half ? 8 * j + half : 8 * j - half) : 8 * j;
+    float x[8], y[8], w[8];
+    if (live) {
+        const uint16_t* src = is_k ? k + (static_cast<size_t>(t) * nkv + hk) * kKv4Dim
+                                   : q + (static_cast<size_t>(t) * nq + head) * kKv4Dim;
+        const uint16_t* bias = is_k ? (kb ? kb + hk * kKv4Dim : nullptr) : (qb ? qb + head * kKv4Dim : nullptr);
+        auto load8 = [](const uint16_t* p, const uint16_t* b, int d, float (&o)[8]) {
+            const f16x8 a = *reinterpret_cast<const f16x8*>(p + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(a[e]);
+            if (b != nullptr) {
+                const f16x8 c = *reinterpret_cast<const f16x8*>(b + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += static_cast<float>(c[e]);
+            }
+        };
+        load8(src, bias, 8 * j, x);
+        load8(src, bias, pd, y);
+        if (is_k) load8(v + (static_cast<size_t>(t) * nkv + hk) * kKv4Dim, vb ? vb + hk * kKv4Dim : nullptr, 8 * j, w);
+    }
+    if (static_cast<int>(threadIdx.x) < half) {
+        const int i = threadIdx.x;
+        const double pos = static_cast<double>((ctl != nullptr ? ctl->seq_pos : 0)) + t;
+        const double a = pos * exp2(-log2_theta * i / half);
+        constexpr double kTwoPi = 6.283185307179586476925;
+        const float r = static_cast<float>(a - kTwoPi * rint(a * (1.0 / kTwoPi)));
+        float sn, cs;
+        sincosf(r, &sn, &cs);
+        s_sin[i] = sn;
+        s_cos[i] = cs;
+    }
+    // also: the partners of q are read before q_out, which may be q, is written
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (!live) return;
+    if (turned) {
+        const bool first = 8 * j < half;
+        const int i0 = first ? 8 * j : 8 * j - half;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float sn = s_sin[i0 + e], cs = s_cos[i0 + e];
+            x[e] = first ? x[e] * cs - y[e] * sn : x[e] * cs + y[e] * sn;
+        }
+    }
+    if (!is_k) {
+        f16x8 o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = static_cast<_Float16>(x[e]);
+        *reinterpret_cast<f16x8*>(q_out + (static_cast<size_t>(t) * nq + head) * kKv4Dim + 8 * j) = o;
+        return;
+    }
+    const long long row = static_cast<long long>(kv4_row(ctl, evicted, hk)) + t;
+    if (row >= max_seq) return;  // no room: not stored
+    // a value that rounds to no finite fp16, anywhere in the 16 lanes of the head
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad |= !(fabsf(x[e]) < 65520.0f) || !(fabsf(w[e]) < 65520.0f);
+    const uint64_t mine = 0xFFFFull << (threadIdx.x & 48);
+    bad = (__builtin_amdgcn_ballot_w64(bad) & mine) != 0;
+    auto store = [&](const float (&z)[8], uint8_t* cache, uint32_t bad_param) {
+        float lo = z[0], hi = z[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) {
+            lo = fminf(lo, z[e]);
+            hi = fmaxf(hi, z[e]);
+        }
+        lo = -qwen::seg_max<4>(-lo);
+        hi = qwen::seg_max<4>(hi);
+        const uint16_t lo16 = f2h(lo);
+        const float low = h2f(lo16);
+        const uint16_t sc16 = f2h((hi - low) / 15.0f);
+        const float scale = h2f(sc16);
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float n = fminf(fmaxf(rintf((z[e] - low) / scale), 0.0f), 15.0f);
+            const uint32_t u = scale > 0.0f ? static_cast<uint32_t>(n) : 0u;
+            word |= u << (16 * (e & 1) + 4 * (e >> 1));
+        }
+        uint32_t param = static_cast<uint32_t>(sc16) | (static_cast<uint32_t>(lo16) << 16);
+        if (bad) {
+            word = 0;
+            param = bad_param;
+        }
+        uint8_t* dst = cache + (static_cast<size_t>(hk) * max_seq + row) * kKv4Row;
+        *reinterpret_cast<uint32_t*>(dst + 4 * j) = word;
+        if ((j & 3) == 0) *reinterpret_cast<uint32_t*>(dst + kKv4Params + j) = param;
+    };
+    store(x, kc, 0x7E007E00u);
+    store(w, vc, 0u);
+}
+
+// ---- rows as fp16 --------------------------------------------------------------
+// A lane per word: 4 bytes and the group's pair in, 16 bytes out.  blockIdx.z: K, V.
+__global__ __launch_bounds__(256) void kv4_unpack_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                         uint16_t* __restrict__ ok, uint16_t* __restrict__ ov,
+                                                         int row0, int rows, int max_seq) {
+    const uint8_t* cache = blockIdx.z == 0 ? kc : vc;
+    uint16_t* out = blockIdx.z == 0 ? ok : ov;
+    if (cache == nullptr) return;
+    const int h = blockIdx.y, w = threadIdx.x & 15;
+    const long long r = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+    if (r >= rows) return;
+    const uint8_t* src = cache + (static_cast<size_t>(h) * max_seq + row0 + r) * kKv4Row;
+    const f16x8 x = kv4_expand_word(*reinterpret_cast<const uint32_t*>(src + 4 * w),
+                                    *reinterpret_cast<const uint32_t*>(src + kKv4Params + (w & ~3)));
+    *reinterpret_cast<f16x8*>(out + (static_cast<size_t>(h) * rows + r) * kKv4Dim + 8 * w) = x;
+}
+
+// ---- eviction ------------------------------------------------------------------
+// Weights as whole numbers of the same order: NaN below everything, -0 as +0.
+__device__ __forceinline__ uint32_t evict_key(float w) {
+    if (w != w) return 0;
+    const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Rows kept of one kv head, a block each.  Of the rows between the first
+// `sinks` and the last `recent` the c with the largest weights stay, equal
+// weights by the lowest index: radix selection of the c-th largest key, 8 bits a
+// round from the top, then one ordered pass that writes the kept indices.
+constexpr int kEvictThreads = 1024;
+__global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const float* __restrict__ weights,
+                                                                         const int32_t* evicted,
+                                                                         const qe_device_control_block* ctl,
+                                                                         int32_t* __restrict__ kept, int keep,
+                                                                         int sinks, int recent, int max_seq) {
+    constexpr int W = kEvictThreads / 64;
+    __shared__ uint32_t s_hist[256];
+    __shared__ uint32_t s_pick[2];  // digit, keys above it
+    __shared__ int s_cnt[W][2];
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = min(kv4_row(ctl, evicted, h), max_seq);
+    int32_t* out = kept + static_cast<size_t>(h) * keep;
+    const int m = min(n, keep);
+    for (int i = m + tid; i < keep; i += kEvictThreads) out[i] = -1;
+    if (n <= keep) {
+        for (int i = tid; i < n; i += kEvictThreads) out[i] = i;
+        return;
+    }
+    const float* w = weights + static_cast<size_t>(h) * max_seq;
+    const int lo = sinks, hi = n - recent;  // candidates
+    const int c = keep - sinks - recent;    // 0 <= c < hi - lo
+    uint32_t prefix = 0, need = c;          // digits found so far, keys still to take at or below them
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) s_hist[tid] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += kEvictThreads) {
+            const uint32_t key = evict_key(w[i]);
+            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // lane l holds bins 255 - 4 l .. 252 - 4 l; the digit where the count from above reaches `need`
+            uint32_t b[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                b[e] = s_hist[255 - 4 * lane - e];
+                sum += b[e];
+            }
+            uint32_t incl = sum;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = __shfl_up(incl, d);
+                if (lane >= d) incl += o;
+            }
+            uint32_t above = incl - sum;
+            if (need > 0 && above < need && incl >= need) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (above < need && above + b[e] >= need) {
+                        s_pick[0] = 255 - 4 * lane - e;
+                        s_pick[1] = above;
+                    }
+                    above += b[e];
+                }
+            }
+            if (need == 0 && lane == 0) {  // nothing to take: a threshold above every key
+                s_pick[0] = 255;
+                s_pick[1] = 0;
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | s_pick[0];
+        need -= s_pick[1];
+    }
+    const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
+    // a wave takes a run of rows: its rows above the cut and at it, then its place
+    const int per = (n + W - 1) / W;
+    const int r0 = min(wave * per, n), r1 = min(r0 + per, n);
+    auto flags = [&](int i, bool& sure, bool& tie) {
+        sure = tie = false;
+        if (i >= r1) return;
+        if (i < lo || i >= hi) {
+            sure = true;
+            return;
+        }
+        const uint32_t key = evict_key(w[i]);
+        sure = c > 0 && key > cut;
+        tie = c > 0 && key == cut;
+    };
+    int sure_n = 0, tie_n = 0;
+    for (int i = r0; i < r1; i += 64) {
+        bool sure, tie;
+        flags(i + lane, sure, tie);
+        sure_n += __popcll(__builtin_amdgcn_ballot_w64(sure));
+        tie_n += __popcll(__builtin_amdgcn_ballot_w64(tie));
+    }
+    if (lane == 0) {
+        s_cnt[wave][0] = sure_n;
+        s_cnt[wave][1] = tie_n;
+    }
+    __syncthreads();
+    int at = 0, ties = 0;
+    for (int v = 0; v < wave; ++v) {
+        at += s_cnt[v][0];
+        ties += s_cnt[v][1];
+    }
+    at += min(ties, static_cast<int>(need));
+    const uint64_t below = (1ull << lane) - 1;
+    for (int i = r0; i < r1; i += 64) {
+        bool sure, tie;
+        flags(i + lane, sure, tie);
+        const uint64_t tb = __builtin_amdgcn_ballot_w64(tie);
+        const bool take = sure || (tie && ties + __popcll(tb & below) < static_cast<int>(need));
+        const uint64_t kb = __builtin_amdgcn_ballot_w64(take);
+        if (take) out[at + __popcll(kb & below)] = i + lane;
+        at += __popcll(kb);
+        ties += __popcll(tb);
+    }
+}
+
+// Moves the kept rows to the front, in their order.  grid (11, kv heads): the
+// 16-byte pieces 0..4 of the K rows, of the V rows, and the weights.  In place
+// too: row i comes from kept[i] >= i, a block takes its rows in runs from the
+// front, and within a run every load is done before the first store; later runs
+// read behind everything stored so far.  Pieces are a block's own, so nobody else
+// reads what it writes.
+constexpr int kMoveRows = 4;  // rows a thread moves in a run
+template <class T>
+__device__ __forceinline__ void move_rows(const char* src, char* dst, size_t stride, const int32_t* kept, int keep) {
+    for (int i0 = 0; i0 < keep; i0 += kEvictThreads * kMoveRows) {
+        T v[kMoveRows];
+        int from[kMoveRows];
+#pragma unroll
+        for (int u = 0; u < kMoveRows; ++u) {
+            const int i = i0 + u * kEvictThreads + static_cast<int>(threadIdx.x);
+            from[u] = i < keep ? kept[i] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kMoveRows; ++u)
+            if (from[u] >= 0) v[u] = *reinterpret_cast<const T*>(src + from[u] * stride);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kMoveRows; ++u) {
+            const size_t i = i0 + u * kEvictThreads + threadIdx.x;
+            if (from[u] >= 0) *reinterpret_cast<T*>(dst + i * stride) = v[u];
+        }
+    }
+}
+
+__global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(
+    const uint8_t* kc, const uint8_t* vc, const float* weights, const int32_t* evicted, uint8_t* out_k, uint8_t* out_v,
+    float* out_weights, int32_t* out_evicted, const int32_t* __restrict__ kept, const qe_device_control_block* ctl,
+    int keep, int max_seq) {
+    const int slice = blockIdx.x, h = blockIdx.y;
+    const int32_t* list = kept + static_cast<size_t>(h) * keep;
+    const size_t base = static_cast<size_t>(h) * max_seq;
+    if (slice < 10) {
+        const size_t at = base * kKv4Row + 16 * (slice % 5);
+        move_rows<u32x4>(reinterpret_cast<const char*>(slice < 5 ? kc : vc) + at,
+                         reinterpret_cast<char*>(slice < 5 ? out_k : out_v) + at, kKv4Row, list, keep);
+        return;
+    }
+    move_rows<float>(reinterpret_cast<const char*>(weights + base), reinterpret_cast<char*>(out_weights + base),
+                     sizeof(float), list, keep);
+    // the weights behind the kept rows start over
+    const int pos = ctl != nullptr ? ctl->seq_pos : 0;
+    const int row = kv4_row(ctl, evicted, h), n = min(row, max_seq), m = min(n, keep);
+    for (int i = m + threadIdx.x; i < n; i += kEvictThreads) out_weights[base + i] = 0.0f;
+    __syncthreads();  // evicted may be out_evicted
+    // the next position's row is m: positions that found the cache full count as gone too
+    if (threadIdx.x == 0) out_evicted[h] = row == 0 ? (evicted != nullptr ? evicted[h] : 0) : pos - m;
+}
+
+// two buffers are one and the same, or share no byte
+inline bool same_or_apart(const void* a, const void* b, size_t bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x == y || x + bytes <= y || y + bytes <= x;
+}
+
+}  // namespace
+}  // namespace qe
+
+using namespace qe;
+
+extern "C" int qe_launch_qkv_bias_rope_kv4_append(const uint16_t* q, uint16_t* q_out, const uint16_t* k,
+                                                  const uint16_t* v, const uint16_t* q_bias, const uint16_t* k_bias,
+                                                  const uint16_t* v_bias, uint8_t* layer_k_cache,
+                                                  uint8_t* layer_v_cache, const qe_device_control_block* d_control,
+                                                  const int32_t* d_evicted, int num_tokens, hipStream_t stream,
+                                                  int num_q_heads, int num_kv_heads, int head_dim, int max_seq_len,
+                                                  int rotary_dim, float rope_theta) {
+    const char* what = "qkv_bias_rope_kv4_append";
+    QE_REQUIRE(q && q_out && k && v, "%s: NULL pointer", what);
+    QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
+    QE_REQUIRE(num_q_heads > 0, "%s: num_q_heads=%d", what, num_q_heads);
+    const int rot = rotary_dim == 0 ? head_dim : rotary_dim;
+    QE_REQUIRE(rot > 0 && rot <= head_dim && rot % 16 == 0, "%s: rotary_dim=%d (a multiple of 16 up to 128)", what,
+               rotary_dim);
+    QE_REQUIRE(rope_theta > 0.0f && std::isfinite(rope_theta), "%s: rope_theta=%g", what, rope_theta);
+    QE_REQUIRE(aligned(q, 16) && aligned(q_out, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_bias, 16) &&
+                   aligned(k_bias, 16) && aligned(v_bias, 16),
+               "%s: q, k, v and the biases must be 16-byte aligned", what);
+    if (num_tokens <= 0) return QE_OK;
+    QE_REQUIRE(same_or_apart(q, q_out, static_cast<size_t>(num_tokens) * num_q_heads * kKv4Dim * 2),
+               "%s: q_out overlaps q", what);
+    const long long heads = static_cast<long long>(num_q_heads) + num_kv_heads;
+    QE_REQUIRE(heads <= 65535 * 16, "%s: %lld heads", what, heads);
+    const dim3 grid(num_tokens, static_cast<unsigned>((heads + 15) / 16));
+    qkv_bias_rope_kv4_append_kernel<<<grid, 256, 0, stream>>>(
+        q, q_out, k, v, q_bias, k_bias, v_bias, layer_k_cache, layer_v_cache, d_control, d_evicted, num_q_heads,
+        num_kv_heads, max_seq_len, rot, std::log2(static_cast<double>(rope_theta)));
+    return check_launch(what);
+}
+
+extern "C" int qe_launch_kv4_unpack(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, uint16_t* out_k,
+                                    uint16_t* out_v, int first_row, int num_rows, hipStream_t stream,
+                                    int num_kv_heads, int head_dim, int max_seq_len) {
+    const char* what = "kv4_unpack";
+    QE_REQUIRE((layer_k_cache == nullptr) == (out_k == nullptr) && (layer_v_cache == nullptr) == (out_v == nullptr) &&
+                   (out_k || out_v),
+               "%s: a cache and its output are given together", what);
+    const uint8_t* any = layer_k_cache ? layer_k_cache : layer_v_cache;
+    QE_TRY(kv4_check(what, layer_k_cache ? layer_k_cache : any, layer_v_cache ? layer_v_cache : any, num_kv_heads,
+                     head_dim, max_seq_len));
+    QE_REQUIRE(aligned(out_k, 16) && aligned(out_v, 16), "%s: the outputs must be 16-byte aligned", what);
+    QE_REQUIRE(num_kv_heads <= 65535, "%s: num_kv_heads=%d", what, num_kv_heads);
+    if (num_rows <= 0) return QE_OK;
+    QE_REQUIRE(first_row >= 0 && first_row <= max_seq_len - num_rows, "%s: rows %d..%lld of %d", what, first_row,
+               static_cast<long long>(first_row) + num_rows - 1, max_seq_len);
+    const dim3 grid((static_cast<unsigned>(num_rows) + 15) / 16, num_kv_heads, 2);
+    kv4_unpack_kernel<<<grid, 256, 0, stream>>>(layer_k_cache, layer_v_cache, out_k, out_v, first_row, num_rows,
+                                                max_seq_len);
+    return check_launch(what);
+}
+
+extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
+                                   const float* key_weights, const int32_t* d_evicted, uint8_t* out_k_cache,
+                                   uint8_t* out_v_cache, float* out_key_weights, int32_t* out_evicted,
+                                   int32_t* kept_rows, const qe_device_control_block* d_control, int keep, int sinks,
+                                   int recent, hipStream_t stream, int num_kv_heads, int head_dim, int max_seq_len) {
+    const char* what = "kv4_evict";
+    QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
+    QE_TRY(kv4_check(what, out_k_cache, out_v_cache, num_kv_heads, head_dim, max_seq_len));
+    QE_REQUIRE(key_weights && out_key_weights && out_evicted && kept_rows && d_control, "%s: NULL pointer", what);
+    QE_REQUIRE(keep > 0 && keep <= max_seq_len, "%s: keep=%d of %d rows", what, keep, max_seq_len);
+    QE_REQUIRE(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
+               "%s: sinks=%d and recent=%d do not fit in keep=%d", what, sinks, recent, keep);
+    QE_REQUIRE(num_kv_heads <= 65535, "%s: num_kv_heads=%d", what, num_kv_heads);
+    QE_REQUIRE(aligned(key_weights, 4) && aligned(out_key_weights, 4) && aligned(kept_rows, 4), "%s: alignment", what);
+    const size_t rows = static_cast<size_t>(num_kv_heads) * max_seq_len;
+    QE_REQUIRE(same_or_apart(layer_k_cache, out_k_cache, rows * kKv4Row) &&
+                   same_or_apart(layer_v_cache, out_v_cache, rows * kKv4Row) &&
+                   same_or_apart(key_weights, out_key_weights, rows * sizeof(float)),
+               "%s: an output overlaps its input without being it", what);
+    kv4_evict_select_kernel<<<num_kv_heads, kEvictThreads, 0, stream>>>(key_weights, d_evicted, d_control, kept_rows,
+                                                                        keep, sinks, recent, max_seq_len);
+    kv4_evict_move_kernel<<<dim3(11, num_kv_heads), kEvictThreads, 0, stream>>>(
+        layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights, out_evicted,
+        kept_rows, d_control, keep, max_seq_len);
+    return check_launch(what);
+}

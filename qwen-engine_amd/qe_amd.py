@@ -56,6 +56,13 @@ SIGNATURES = {
     "qe_launch_attention_gqa_flash_decode_partials": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I],
     "qe_launch_attention_combine_gemv_o_w4a8": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "qe_launch_attention_gqa_prefill": [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I],
+    "qe_launch_qkv_bias_rope_kv4_append": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I,
+                                           ctypes.c_float],
+    "qe_launch_kv4_unpack": [_P, _P, _P, _P, _I, _I, _P, _I, _I, _I],
+    "qe_launch_attention_gqa_flash_decode_kv4": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
+    "qe_launch_attention_gqa_prefill_kv4": [_P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P],
+    "qe_launch_kv4_evict": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _I],
+    "qe_launch_token_logprobs": [_P, _P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, _I, _P],
 }
 
 OTHER_SIGNATURES = {
@@ -68,6 +75,8 @@ OTHER_SIGNATURES = {
     "qe_repack_w4_tiled": [_P, _P, _I, _I, _P, _P, _P],
     "qe_gemm_prefill_plan": [_I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)],
     "qe_gemm_prefill_launch_plan": [_I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)],
+    "qe_kv4_decode_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "qe_token_logprobs_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
 }
 
 ENGINE_SIGNATURES = {
@@ -384,6 +393,80 @@ def launch_attention_gqa_prefill(q, layer_k_cache, layer_v_cache, attn_out, d_co
     _call("qe_launch_attention_gqa_prefill", _ptr(q), _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(attn_out),
           _ptr(d_control), num_tokens, _stream(stream), num_q_heads, num_kv_heads, head_dim, max_seq_len,
           hidden_size)
+
+
+# ---- 4-bit key/value cache ---------------------------------------------------------
+KV4_ROW_BYTES = 80  # QE_KV4_ROW_BYTES
+
+
+def kv4_cache(num_kv_heads=2, max_seq_len=4096, device="cuda"):
+    """An empty 4-bit K or V cache of one layer: uint8 [num_kv_heads][max_seq_len][KV4_ROW_BYTES]."""
+    import torch
+    return torch.zeros((num_kv_heads, max_seq_len, KV4_ROW_BYTES), dtype=torch.uint8, device=device)
+
+
+def launch_qkv_bias_rope_kv4_append(q, q_out, k, v, q_bias, k_bias, v_bias, layer_k_cache, layer_v_cache, d_control,
+                                    d_evicted, num_tokens, stream=None, num_q_heads=12, num_kv_heads=2, head_dim=128,
+                                    max_seq_len=4096, rotary_dim=0, rope_theta=1000000.0):
+    _call("qe_launch_qkv_bias_rope_kv4_append", _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_bias), _ptr(k_bias),
+          _ptr(v_bias), _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(d_control), _ptr(d_evicted), num_tokens,
+          _stream(stream), num_q_heads, num_kv_heads, head_dim, max_seq_len, rotary_dim, rope_theta)
+
+
+def launch_kv4_unpack(layer_k_cache, layer_v_cache, out_k, out_v, first_row, num_rows, stream=None, num_kv_heads=2,
+                      head_dim=128, max_seq_len=4096):
+    _call("qe_launch_kv4_unpack", _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(out_k), _ptr(out_v), first_row,
+          num_rows, _stream(stream), num_kv_heads, head_dim, max_seq_len)
+
+
+def kv4_decode_workspace_bytes(num_q_heads=12, max_seq_len=4096, key_weights=False) -> int:
+    """Bytes of launch_attention_gqa_flash_decode_kv4's workspace (qe_kv4_decode_workspace_bytes)."""
+    n = ctypes.c_size_t()
+    _check(lib().qe_kv4_decode_workspace_bytes(num_q_heads, max_seq_len, int(key_weights), ctypes.byref(n)),
+           "qe_kv4_decode_workspace_bytes")
+    return n.value
+
+
+def launch_attention_gqa_flash_decode_kv4(q, layer_k_cache, layer_v_cache, workspace, attn_out, d_control, d_evicted,
+                                          stream=None, num_q_heads=12, num_kv_heads=2, head_dim=128, max_seq_len=4096,
+                                          out_q8=None, out_scale=None, out_sum8=None, key_weights_in=None,
+                                          key_weights_out=None):
+    _call("qe_launch_attention_gqa_flash_decode_kv4", _ptr(q), _ptr(layer_k_cache), _ptr(layer_v_cache),
+          _ptr(workspace), _ptr(attn_out), _ptr(d_control), _ptr(d_evicted), _stream(stream), num_q_heads, num_kv_heads,
+          head_dim, max_seq_len, _ptr(out_q8), _ptr(out_scale), _ptr(out_sum8), _ptr(key_weights_in),
+          _ptr(key_weights_out))
+
+
+def launch_attention_gqa_prefill_kv4(q, layer_k_cache, layer_v_cache, attn_out, d_control, d_evicted, num_tokens,
+                                     stream=None, num_q_heads=12, num_kv_heads=2, head_dim=128, max_seq_len=4096,
+                                     hidden_size=1536, key_weights_in=None, key_weights_out=None, row_lse=None):
+    _call("qe_launch_attention_gqa_prefill_kv4", _ptr(q), _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(attn_out),
+          _ptr(d_control), _ptr(d_evicted), num_tokens, _stream(stream), num_q_heads, num_kv_heads, head_dim,
+          max_seq_len, hidden_size, _ptr(key_weights_in), _ptr(key_weights_out), _ptr(row_lse))
+
+
+def launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
+                     out_evicted, kept_rows, d_control, keep, sinks=4, recent=128, stream=None, num_kv_heads=2,
+                     head_dim=128, max_seq_len=4096):
+    _call("qe_launch_kv4_evict", _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(key_weights), _ptr(d_evicted),
+          _ptr(out_k_cache), _ptr(out_v_cache), _ptr(out_key_weights), _ptr(out_evicted), _ptr(kept_rows),
+          _ptr(d_control), keep, sinks, recent, _stream(stream), num_kv_heads, head_dim, max_seq_len)
+
+
+# ---- log probabilities ---------------------------------------------------------------
+def token_logprobs_workspace_bytes(num_rows, vocab_size=151936, top_k=0) -> int:
+    """Bytes of launch_token_logprobs's workspace (qe_token_logprobs_workspace_bytes)."""
+    n = ctypes.c_size_t()
+    _check(lib().qe_token_logprobs_workspace_bytes(num_rows, vocab_size, top_k, ctypes.byref(n)),
+           "qe_token_logprobs_workspace_bytes")
+    return n.value
+
+
+def launch_token_logprobs(logits, token_ids, out_logprob, out_entropy, out_top_logprob, out_top_ids, workspace,
+                          num_rows, vocab_size=151936, row_stride=None, top_k=0, stream=None):
+    _call("qe_launch_token_logprobs", _ptr(logits), _ptr(token_ids), _ptr(out_logprob), _ptr(out_entropy),
+          _ptr(out_top_logprob), _ptr(out_top_ids), _ptr(workspace), num_rows, vocab_size,
+          vocab_size if row_stride is None else row_stride, top_k, _stream(stream))
 
 
 # ---- engine ------------------------------------------------------------------------

@@ -2,6 +2,7 @@
 // rows back as fp16, and eviction of the rows with the least attention.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv4_common.hpp"
 
@@ -146,28 +147,58 @@ __global__ __launch_bounds__(256) void kv4_unpack_kernel(const uint8_t* __restri
 }
 
 // ---- eviction ------------------------------------------------------------------
-// Weights as whole numbers of the same order: NaN below everything, -0 as +0.
+// Weights as whole numbers of the same order: NaN (1) below everything, -0 as +0.
+// 0 and kEvictSafe are left over: no row, and a row that stays whatever its weight.
+constexpr uint32_t kEvictSafe = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t evict_key(float w) {
-    if (w != w) return 0;
+    if (w != w) return 1;
     const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Rows kept of one kv head, a block each.  Of the rows between the first
-// `sinks` and the last `recent` the c with the largest weights stay, equal
-// weights by the lowest index: radix selection of the c-th largest key, 8 bits a
-// round from the top, then one ordered pass that writes the kept indices.
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value,
+                                                               decltype(rows)::value, 0xF, false));
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr 1, 2, 4, 8
+    add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // lane 15 of a row to the next row
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // lane 31 to rows 2 and 3
+    return x;
+}
+
+// Rows kept of one kv head, a block each.  The first `sinks` and the last
+// `recent` rows count as larger than every weight, so what stays are the `keep`
+// largest keys, equal ones by the lowest index: radix selection of the keep-th
+// largest, then one ordered pass that writes the kept indices.
+// The keys of the first 32768 rows stay in LDS (they are read from memory once), the
+// others are read again where they are needed; a wave owns a run of rows and takes
+// 4 times 64 of them at a time.  Loops, not keys in registers: unrolled for 32
+// keys a lane the five passes are 34 KB of code, and fetching it costs more than it
+// saves (4096 rows 8.5 us).  Digits of 11, 11 and 10 bits: the first holds the sign, the
+// exponent and two bits of the mantissa, so that weights of like size still spread
+// over the bins and lanes seldom meet in one.
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictCached = 32768;  // keys in LDS
+constexpr int kEvictBins = 2048;
 __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const float* __restrict__ weights,
                                                                          const int32_t* evicted,
                                                                          const qe_device_control_block* ctl,
                                                                          int32_t* __restrict__ kept, int keep,
                                                                          int sinks, int recent, int max_seq) {
-    constexpr int W = kEvictThreads / 64;
-    __shared__ uint32_t s_hist[256];
+    constexpr int W = kEvictThreads / 64, U = 4;
+    extern __shared__ uint32_t s_key[];  // min(max_seq, kEvictCached)
+    __shared__ uint32_t s_hist[3][kEvictBins];
+    __shared__ uint32_t s_wave[W];
     __shared__ uint32_t s_pick[2];  // digit, keys above it
-    __shared__ int s_cnt[W][2];
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int2 s_cnt[W];
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = min(kv4_row(ctl, evicted, h), max_seq);
     int32_t* out = kept + static_cast<size_t>(h) * keep;
     const int m = min(n, keep);
@@ -177,149 +208,196 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
         return;
     }
     const float* w = weights + static_cast<size_t>(h) * max_seq;
-    const int lo = sinks, hi = n - recent;  // candidates
-    const int c = keep - sinks - recent;    // 0 <= c < hi - lo
-    uint32_t prefix = 0, need = c;          // digits found so far, keys still to take at or below them
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kEvictThreads) {
-            const uint32_t key = evict_key(w[i]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
+    const int lo = sinks, hi = n - recent;
+    const int cached = min(n, kEvictCached);
+    auto key_of = [&](int i, float x) { return i >= n ? 0u : i < lo || i >= hi ? kEvictSafe : evict_key(x); };
+    for (int i0 = tid; i0 < cached; i0 += 8 * kEvictThreads) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = w[min(i0 + u * kEvictThreads, n - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u * kEvictThreads;
+            if (i < cached) s_key[i] = key_of(i, x[u]);
         }
-        __syncthreads();
-        if (wave == 0) {
-            // lane l holds bins 255 - 4 l .. 252 - 4 l; the digit where the count from above reaches `need`
-            uint32_t b[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                b[e] = s_hist[255 - 4 * lane - e];
-                sum += b[e];
-            }
-            uint32_t incl = sum;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t o = __shfl_up(incl, d);
-                if (lane >= d) incl += o;
-            }
-            uint32_t above = incl - sum;
-            if (need > 0 && above < need && incl >= need) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (above < need && above + b[e] >= need) {
-                        s_pick[0] = 255 - 4 * lane - e;
-                        s_pick[1] = above;
-                    }
-                    above += b[e];
-                }
-            }
-            if (need == 0 && lane == 0) {  // nothing to take: a threshold above every key
-                s_pick[0] = 255;
-                s_pick[1] = 0;
-            }
-        }
-        __syncthreads();
-        prefix = (prefix << 8) | s_pick[0];
-        need -= s_pick[1];
     }
-    const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
-    // a wave takes a run of rows: its rows above the cut and at it, then its place
+    for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) s_hist[0][i] = 0;
+    __syncthreads();
     const int per = (n + W - 1) / W;
     const int r0 = min(wave * per, n), r1 = min(r0 + per, n);
-    auto flags = [&](int i, bool& sure, bool& tie) {
-        sure = tie = false;
-        if (i >= r1) return;
-        if (i < lo || i >= hi) {
-            sure = true;
-            return;
+    // f(row, key) for the rows of the wave in order, 64 neighbours at a time; key 0 past the last
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        for (int i0 = r0; i0 < r1; i0 += 64 * U) {
+            uint32_t k[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 64 * u + lane;
+                if (i0 + 64 * U <= kEvictCached) k[u] = s_key[min(i, cached - 1)];
+                else k[u] = key_of(i, w[min(i, n - 1)]);
+                if (i >= r1) k[u] = 0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) f(i0 + 64 * u + lane, k[u]);
         }
-        const uint32_t key = evict_key(w[i]);
-        sure = c > 0 && key > cut;
-        tie = c > 0 && key == cut;
     };
+    uint32_t prefix = 0, need = keep;  // digits found so far, keys still to take at or below them
+    auto round = [&](auto number) __attribute__((always_inline)) {
+        constexpr int R = decltype(number)::value, shift = R == 0 ? 21 : R == 1 ? 10 : 0, bits = R == 2 ? 10 : 11;
+        each([&](int, uint32_t k) {
+            // (rows that stay anyway are many and in one place: counted below, not one by one)
+            if (R == 0 ? k + 1u > 1u : (k >> ((shift + bits) & 31)) == prefix)
+                atomicAdd(&s_hist[R][(k >> shift) & ((1u << bits) - 1u)], 1u);
+        });
+        if (R == 0 && tid == 0) atomicAdd(&s_hist[R][kEvictBins - 1], static_cast<uint32_t>(sinks + recent));
+        __syncthreads();
+        // thread t holds bins 2047 - 2 t and 2046 - 2 t; the digit where the count from above reaches `need`
+        const uint2 b = *reinterpret_cast<const uint2*>(&s_hist[R][kEvictBins - 2 - 2 * tid]);
+        const uint32_t incl = wave_scan(b.x + b.y);
+        if (lane == 63) s_wave[wave] = incl;
+        __syncthreads();
+        uint32_t above = incl - b.x - b.y;
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            const uint32_t x = s_wave[v];
+            above += v < wave ? x : 0u;
+        }
+        if (above < need && above + b.x + b.y >= need) {
+            const bool first = above + b.y >= need;
+            s_pick[0] = kEvictBins - 1 - 2 * tid - (first ? 0 : 1);
+            s_pick[1] = above + (first ? 0 : b.y);
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | s_pick[0];
+        need -= s_pick[1];
+    };
+    round(std::integral_constant<int, 0>{});
+    round(std::integral_constant<int, 1>{});
+    round(std::integral_constant<int, 2>{});
+    const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
     int sure_n = 0, tie_n = 0;
-    for (int i = r0; i < r1; i += 64) {
-        bool sure, tie;
-        flags(i + lane, sure, tie);
-        sure_n += __popcll(__builtin_amdgcn_ballot_w64(sure));
-        tie_n += __popcll(__builtin_amdgcn_ballot_w64(tie));
-    }
-    if (lane == 0) {
-        s_cnt[wave][0] = sure_n;
-        s_cnt[wave][1] = tie_n;
-    }
+    each([&](int, uint32_t k) {
+        sure_n += __popcll(__builtin_amdgcn_ballot_w64(k > cut));
+        tie_n += __popcll(__builtin_amdgcn_ballot_w64(k == cut));
+    });
+    if (lane == 0) s_cnt[wave] = make_int2(sure_n, tie_n);
     __syncthreads();
     int at = 0, ties = 0;
-    for (int v = 0; v < wave; ++v) {
-        at += s_cnt[v][0];
-        ties += s_cnt[v][1];
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+        const int2 x = s_cnt[v];
+        at += v < wave ? x.x : 0;
+        ties += v < wave ? x.y : 0;
     }
-    at += min(ties, static_cast<int>(need));
-    const uint64_t below = (1ull << lane) - 1;
-    for (int i = r0; i < r1; i += 64) {
-        bool sure, tie;
-        flags(i + lane, sure, tie);
-        const uint64_t tb = __builtin_amdgcn_ballot_w64(tie);
-        const bool take = sure || (tie && ties + __popcll(tb & below) < static_cast<int>(need));
-        const uint64_t kb = __builtin_amdgcn_ballot_w64(take);
-        if (take) out[at + __popcll(kb & below)] = i + lane;
-        at += __popcll(kb);
-        ties += __popcll(tb);
-    }
+    const int wanted = static_cast<int>(need);
+    at = __builtin_amdgcn_readfirstlane(at + min(ties, wanted));
+    ties = __builtin_amdgcn_readfirstlane(ties);
+    each([&](int i, uint32_t k) {
+        uint64_t take = __builtin_amdgcn_ballot_w64(k > cut);
+        const uint64_t tb = __builtin_amdgcn_ballot_w64(k == cut);
+        if (tb != 0) {
+            const bool t = k == cut && ties + __popcll(tb & ((1ull << lane) - 1)) < wanted;
+            take |= __builtin_amdgcn_ballot_w64(t);
+            ties += __popcll(tb);
+        }
+        if ((take >> lane) & 1)
+            out[at + static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(take >> 32),
+                                          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(take), 0u)))] = i;
+        at += __popcll(take);
+    });
 }
 
-// Moves the kept rows to the front, in their order.  grid (11, kv heads): the
-// 16-byte pieces 0..4 of the K rows, of the V rows, and the weights.  In place
-// too: row i comes from kept[i] >= i, a block takes its rows in runs from the
-// front, and within a run every load is done before the first store; later runs
-// read behind everything stored so far.  Pieces are a block's own, so nobody else
-// reads what it writes.
-constexpr int kMoveRows = 4;  // rows a thread moves in a run
-template <class T>
-__device__ __forceinline__ void move_rows(const char* src, char* dst, size_t stride, const int32_t* kept, int keep) {
-    for (int i0 = 0; i0 < keep; i0 += kEvictThreads * kMoveRows) {
-        T v[kMoveRows];
-        int from[kMoveRows];
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u) {
-            const int i = i0 + u * kEvictThreads + static_cast<int>(threadIdx.x);
-            from[u] = i < keep ? kept[i] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u)
-            if (from[u] >= 0) v[u] = *reinterpret_cast<const T*>(src + from[u] * stride);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u) {
-            const size_t i = i0 + u * kEvictThreads + threadIdx.x;
-            if (from[u] >= 0) *reinterpret_cast<T*>(dst + i * stride) = v[u];
-        }
-    }
-}
-
-__global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(
-    const uint8_t* kc, const uint8_t* vc, const float* weights, const int32_t* evicted, uint8_t* out_k, uint8_t* out_v,
-    float* out_weights, int32_t* out_evicted, const int32_t* __restrict__ kept, const qe_device_control_block* ctl,
-    int keep, int max_seq) {
-    const int slice = blockIdx.x, h = blockIdx.y;
-    const int32_t* list = kept + static_cast<size_t>(h) * keep;
-    const size_t base = static_cast<size_t>(h) * max_seq;
-    if (slice < 10) {
-        const size_t at = base * kKv4Row + 16 * (slice % 5);
-        move_rows<u32x4>(reinterpret_cast<const char*>(slice < 5 ? kc : vc) + at,
-                         reinterpret_cast<char*>(slice < 5 ? out_k : out_v) + at, kKv4Row, list, keep);
-        return;
-    }
-    move_rows<float>(reinterpret_cast<const char*>(weights + base), reinterpret_cast<char*>(out_weights + base),
-                     sizeof(float), list, keep);
-    // the weights behind the kept rows start over
+// The weights of the kept rows move up too, and those behind them start over.
+__device__ __forceinline__ void evict_finish(float* out_weights, const int32_t* evicted, int32_t* out_evicted,
+                                             const qe_device_control_block* ctl, int h, int keep, int max_seq) {
     const int pos = ctl != nullptr ? ctl->seq_pos : 0;
     const int row = kv4_row(ctl, evicted, h), n = min(row, max_seq), m = min(n, keep);
-    for (int i = m + threadIdx.x; i < n; i += kEvictThreads) out_weights[base + i] = 0.0f;
+    const size_t base = static_cast<size_t>(h) * max_seq;
+    for (int i = m + threadIdx.x; i < n; i += blockDim.x) out_weights[base + i] = 0.0f;
     __syncthreads();  // evicted may be out_evicted
     // the next position's row is m: positions that found the cache full count as gone too
     if (threadIdx.x == 0) out_evicted[h] = row == 0 ? (evicted != nullptr ? evicted[h] : 0) : pos - m;
+}
+
+struct EvictMove {
+    const uint8_t* kc;
+    const uint8_t* vc;
+    const float* weights;
+    const int32_t* evicted;
+    uint8_t* out_k;
+    uint8_t* out_v;
+    float* out_weights;
+    int32_t* out_evicted;
+    const int32_t* kept;
+    const qe_device_control_block* ctl;
+    int keep, max_seq;
+};
+
+// The kept rows to the front, in their order, into memory apart from the caches:
+// a lane per 16-byte piece, 5 pieces a row, K (blockIdx.z 0) and V (1); the
+// blocks of K move the weights as well, the first of them ends the head.
+constexpr int kCopyRows = 51;  // rows of a block of 256 threads
+__global__ __launch_bounds__(256) void kv4_evict_copy_kernel(EvictMove p) {
+    const int h = blockIdx.y, tid = threadIdx.x;
+    const int32_t* list = p.kept + static_cast<size_t>(h) * p.keep;
+    const size_t base = static_cast<size_t>(h) * p.max_seq;
+    const int r0 = blockIdx.x * kCopyRows, r = r0 + tid / 5, piece = tid % 5;
+    if (tid < 5 * kCopyRows && r < p.keep) {
+        const int from = list[r];
+        if (from >= 0) {
+            const uint8_t* src = (blockIdx.z == 0 ? p.kc : p.vc) + (base + from) * kKv4Row + 16 * piece;
+            uint8_t* dst = (blockIdx.z == 0 ? p.out_k : p.out_v) + (base + r) * kKv4Row + 16 * piece;
+            *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
+        }
+    }
+    if (blockIdx.z != 0) return;
+    if (tid < kCopyRows && r0 + tid < p.keep) {
+        const int from = list[r0 + tid];
+        if (from >= 0) p.out_weights[base + r0 + tid] = p.weights[base + from];
+    }
+    if (blockIdx.x == 0) evict_finish(p.out_weights, p.evicted, p.out_evicted, p.ctl, h, p.keep, p.max_seq);
+}
+
+// The same in place: row i comes from kept[i] >= i, a block takes all rows of a
+// head's K or V pieces 0..2 or 3..4, or its weights, in runs from the front, and
+// within a run every load is done before the first store; later runs read behind
+// everything stored so far, and nobody else touches the block's pieces.  Rows in front of
+// the first one that left stay where they are.  PIECES of STRIDE values T a row, U
+// a thread and run: few runs, since each waits for memory twice.
+template <class T, int PIECES, int STRIDE, int U>
+__device__ __forceinline__ void move_rows(T* data, const int32_t* kept, int keep) {
+    const uint32_t all = static_cast<uint32_t>(keep) * PIECES;
+    for (uint32_t i0 = 0; i0 < all; i0 += kEvictThreads * U) {
+        T v[U];
+        bool moves[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = i0 + u * kEvictThreads + threadIdx.x, row = i / PIECES, piece = i - row * PIECES;
+            const int from = i < all ? kept[row] : -1;
+            moves[u] = from > static_cast<int>(row);
+            if (moves[u]) v[u] = data[static_cast<size_t>(from) * STRIDE + piece];
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = i0 + u * kEvictThreads + threadIdx.x, row = i / PIECES, piece = i - row * PIECES;
+            if (moves[u]) data[static_cast<size_t>(row) * STRIDE + piece] = v[u];
+        }
+    }
+}
+
+__global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(EvictMove p) {
+    const int h = blockIdx.y;
+    const int32_t* list = p.kept + static_cast<size_t>(h) * p.keep;
+    const size_t base = static_cast<size_t>(h) * p.max_seq;
+    u32x4* rows = reinterpret_cast<u32x4*>((blockIdx.x < 2 ? p.out_k : p.out_v) + base * kKv4Row);
+    if (blockIdx.x < 4) {
+        if (blockIdx.x % 2 == 0) move_rows<u32x4, 3, 5, 12>(rows, list, p.keep);
+        else move_rows<u32x4, 2, 5, 12>(rows + 3, list, p.keep);
+        return;
+    }
+    move_rows<float, 1, 1, 8>(p.out_weights + base, list, p.keep);
+    evict_finish(p.out_weights, p.evicted, p.out_evicted, p.ctl, h, p.keep, p.max_seq);
 }
 
 // two buffers are one and the same, or share no byte
@@ -393,20 +471,28 @@ extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* 
     QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
     QE_TRY(kv4_check(what, out_k_cache, out_v_cache, num_kv_heads, head_dim, max_seq_len));
     QE_REQUIRE(key_weights && out_key_weights && out_evicted && kept_rows && d_control, "%s: NULL pointer", what);
+    QE_REQUIRE(max_seq_len <= (1 << 28), "%s: max_seq_len=%d", what, max_seq_len);
     QE_REQUIRE(keep > 0 && keep <= max_seq_len, "%s: keep=%d of %d rows", what, keep, max_seq_len);
     QE_REQUIRE(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
                "%s: sinks=%d and recent=%d do not fit in keep=%d", what, sinks, recent, keep);
     QE_REQUIRE(num_kv_heads <= 65535, "%s: num_kv_heads=%d", what, num_kv_heads);
     QE_REQUIRE(aligned(key_weights, 4) && aligned(out_key_weights, 4) && aligned(kept_rows, 4), "%s: alignment", what);
     const size_t rows = static_cast<size_t>(num_kv_heads) * max_seq_len;
+    const bool in_place = layer_k_cache == out_k_cache;
+    QE_REQUIRE(in_place == (layer_v_cache == out_v_cache) && in_place == (key_weights == out_key_weights),
+               "%s: K, V and weights are all in place or all apart", what);
     QE_REQUIRE(same_or_apart(layer_k_cache, out_k_cache, rows * kKv4Row) &&
                    same_or_apart(layer_v_cache, out_v_cache, rows * kKv4Row) &&
                    same_or_apart(key_weights, out_key_weights, rows * sizeof(float)),
                "%s: an output overlaps its input without being it", what);
-    kv4_evict_select_kernel<<<num_kv_heads, kEvictThreads, 0, stream>>>(key_weights, d_evicted, d_control, kept_rows,
-                                                                        keep, sinks, recent, max_seq_len);
-    kv4_evict_move_kernel<<<dim3(11, num_kv_heads), kEvictThreads, 0, stream>>>(
-        layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights, out_evicted,
-        kept_rows, d_control, keep, max_seq_len);
+    const size_t lds = std::min(max_seq_len, kEvictCached) * sizeof(uint32_t);
+    kv4_evict_select_kernel<<<num_kv_heads, kEvictThreads, lds, stream>>>(key_weights, d_evicted, d_control, kept_rows,
+                                                                          keep, sinks, recent, max_seq_len);
+    const EvictMove p{layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
+                      out_evicted, kept_rows, d_control, keep, max_seq_len};
+    if (in_place)
+        kv4_evict_move_kernel<<<dim3(5, num_kv_heads), kEvictThreads, 0, stream>>>(p);
+    else
+        kv4_evict_copy_kernel<<<dim3((keep + kCopyRows - 1) / kCopyRows, num_kv_heads, 2), 256, 0, stream>>>(p);
     return check_launch(what);
 }

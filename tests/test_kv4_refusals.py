@@ -86,7 +86,10 @@ def test_evict(L):
         _says(L, evict(**bad), "NULL")
     for bad, text in (({"keep": 0}, "keep"), ({"keep": 65}, "keep"), ({"sinks": -1}, "sinks"), ({"recent": -1}, "recent"),
                       ({"sinks": 20, "recent": 13}, "do not fit"), ({"sinks": 2**31 - 1}, "do not fit"),
-                      ({"ok": P + 16}, "overlaps"), ({"ov": 2 * P + 80 * 64}, "overlaps"), ({"ow": 3 * P + 4}, "overlaps"),
+                      ({"ok": big}, "all in place"), ({"ov": big}, "all in place"), ({"ow": big}, "all in place"),
+                      ({"ok": P + 16, "ov": big, "ow": 2 * big}, "overlaps"),
+                      ({"ok": big, "ov": 2 * P + 80 * 64, "ow": 2 * big}, "overlaps"),
+                      ({"ok": big, "ov": 2 * big, "ow": 3 * P + 4}, "overlaps"),
                       ({"ok": big + 8}, "aligned"), ({"hd": 96}, "head_dim"), ({"nkv": 65536}, "num_kv_heads")):
         _says(L, evict(**bad), text)
 

@@ -172,28 +172,51 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x;
 }
 
+// The weights behind the kept rows start over, and so does the count of evicted rows.
+// By all threads of the one block that does it.
+__device__ __forceinline__ void evict_finish(float* out_weights, const int32_t* evicted, int32_t* out_evicted,
+                                             const qe_device_control_block* ctl, int h, int keep, int max_seq) {
+    const int pos = ctl != nullptr ? ctl->seq_pos : 0;
+    const int row = kv4_row(ctl, evicted, h), n = min(row, max_seq), m = min(n, keep);
+    const size_t base = static_cast<size_t>(h) * max_seq;
+    for (int i = m + threadIdx.x; i < n; i += blockDim.x) out_weights[base + i] = 0.0f;
+    __syncthreads();  // evicted may be out_evicted
+    // the next position's row is m: positions that found the cache full count as gone too
+    if (threadIdx.x == 0) out_evicted[h] = row == 0 ? (evicted != nullptr ? evicted[h] : 0) : pos - m;
+}
+
 // Rows kept of one kv head, a block each.  The first `sinks` and the last
 // `recent` rows count as larger than every weight, so what stays are the `keep`
 // largest keys, equal ones by the lowest index: radix selection of the keep-th
 // largest, then one ordered pass that writes the kept indices.
-// The keys of the first 32768 rows stay in LDS (they are read from memory once), the
-// others are read again where they are needed; a wave owns a run of rows and takes
-// 4 times 64 of them at a time.  Loops, not keys in registers: unrolled for 32
-// keys a lane the five passes are 34 KB of code, and fetching it costs more than it
-// saves (4096 rows 8.5 us).  Digits of 11, 11 and 10 bits: the first holds the sign, the
-// exponent and two bits of the mantissa, so that weights of like size still spread
-// over the bins and lanes seldom meet in one.
+// Up to 32768 rows the keys are read from memory once and stay in LDS (more rows: read
+// again in every pass).  A wave owns a run of rows, a multiple of 256 so that a lane
+// can take four keys with one LDS read wherever their order does not matter.  Digits
+// of 11, 11 and 10 bits: the first holds the sign, the exponent and two bits of the
+// mantissa, so that weights of like size still spread over the bins and lanes seldom
+// meet in one.  One CU a head, so instructions count: 4096 rows take 7.4 us (2 heads),
+// 32000 21 (8 heads); with digits of 8 bits, four rounds over memory and a branch for
+// every key 10.3 and 53, with the keys in registers (passes unrolled 32 times, 34 KB
+// of code) 8.5 and 20.
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictCached = 32768;  // keys in LDS
 constexpr int kEvictBins = 2048;
+
+// Rows of a wave's run for n rows.
+__host__ __device__ __forceinline__ int evict_run(int n) {
+    return ((n + kEvictWaves - 1) / kEvictWaves + 255) & ~255;
+}
+
 __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const float* __restrict__ weights,
                                                                          const int32_t* evicted,
                                                                          const qe_device_control_block* ctl,
                                                                          int32_t* __restrict__ kept, int keep,
-                                                                         int sinks, int recent, int max_seq) {
-    constexpr int W = kEvictThreads / 64, U = 4;
-    extern __shared__ uint32_t s_key[];  // min(max_seq, kEvictCached)
-    __shared__ uint32_t s_hist[3][kEvictBins];
+                                                                         int sinks, int recent, int max_seq,
+                                                                         float* apart_weights, int32_t* apart_evicted) {
+    constexpr int W = kEvictWaves;
+    extern __shared__ uint32_t s_key[];  // W evict_run(max_seq), at most kEvictCached
+    __shared__ __align__(16) uint32_t s_hist[3 * kEvictBins];  // the first digit counts in the first two
     __shared__ uint32_t s_wave[W];
     __shared__ uint32_t s_pick[2];  // digit, keys above it
     __shared__ int2 s_cnt[W];
@@ -203,55 +226,86 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     int32_t* out = kept + static_cast<size_t>(h) * keep;
     const int m = min(n, keep);
     for (int i = m + tid; i < keep; i += kEvictThreads) out[i] = -1;
+    // moved apart, nothing here is read again: the head's end is written now
+    if (apart_weights != nullptr) evict_finish(apart_weights, evicted, apart_evicted, ctl, h, keep, max_seq);
     if (n <= keep) {
         for (int i = tid; i < n; i += kEvictThreads) out[i] = i;
         return;
     }
     const float* w = weights + static_cast<size_t>(h) * max_seq;
     const int lo = sinks, hi = n - recent;
-    const int cached = min(n, kEvictCached);
     auto key_of = [&](int i, float x) { return i >= n ? 0u : i < lo || i >= hi ? kEvictSafe : evict_key(x); };
-    for (int i0 = tid; i0 < cached; i0 += 8 * kEvictThreads) {
-        float x[8];
+    const int per = evict_run(n);
+    const bool cached = W * per <= kEvictCached;
+    constexpr int J = kEvictCached / kEvictThreads;
+    float x[J];  // requested together
+    if (cached) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = w[min(i0 + u * kEvictThreads, n - 1)];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = i0 + u * kEvictThreads;
-            if (i < cached) s_key[i] = key_of(i, x[u]);
-        }
+        for (int j = 0; j < J; ++j)
+            if (j * kEvictThreads < n) x[j] = w[min(j * kEvictThreads + tid, n - 1)];
     }
-    for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) s_hist[0][i] = 0;
+    for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) s_hist[i] = 0;
     __syncthreads();
-    const int per = (n + W - 1) / W;
-    const int r0 = min(wave * per, n), r1 = min(r0 + per, n);
-    // f(row, key) for the rows of the wave in order, 64 neighbours at a time; key 0 past the last
-    auto each = [&](auto f) __attribute__((always_inline)) {
-        for (int i0 = r0; i0 < r1; i0 += 64 * U) {
-            uint32_t k[U];
+    // The first digit, lanes of odd and even number apart; rows that stay anyway are
+    // many and in one place: counted together, not one by one.
+    auto count_first = [&](uint32_t k) __attribute__((always_inline)) {
+        if (k + 1u > 1u) atomicAdd(&s_hist[(lane & 1) * kEvictBins + (k >> 21)], 1u);
+    };
+    if (tid == 0) atomicAdd(&s_hist[kEvictBins - 1], static_cast<uint32_t>(sinks + recent));
+    if (cached) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + 64 * u + lane;
-                if (i0 + 64 * U <= kEvictCached) k[u] = s_key[min(i, cached - 1)];
-                else k[u] = key_of(i, w[min(i, n - 1)]);
-                if (i >= r1) k[u] = 0;
+        for (int j = 0; j < J; ++j)
+            if (j * kEvictThreads < W * per) {
+                const uint32_t k = key_of(j * kEvictThreads + tid, x[j]);
+                s_key[j * kEvictThreads + tid] = k;
+                count_first(k);
             }
+    }
+    const int r0 = wave * per, r1 = min(r0 + per, n);
+    // f(four keys) for all of the wave's, in any order
+    auto each = [&](auto f) __attribute__((always_inline)) {
+        for (int i0 = r0; i0 < r1; i0 += 256) {
+            u32x4 k;
+            if (cached) {
+                k = *reinterpret_cast<const u32x4*>(s_key + i0 + 4 * lane);
+            } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) f(i0 + 64 * u + lane, k[u]);
+                for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + 64 * u + lane, w[min(i0 + 64 * u + lane, n - 1)]);
+            }
+            const uint32_t k4[4] = {k[0], k[1], k[2], k[3]};
+            f(k4);
         }
     };
+    if (!cached)
+        each([&](const uint32_t(&k)[4]) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) count_first(k[u]);
+        });
     uint32_t prefix = 0, need = keep;  // digits found so far, keys still to take at or below them
     auto round = [&](auto number) __attribute__((always_inline)) {
         constexpr int R = decltype(number)::value, shift = R == 0 ? 21 : R == 1 ? 10 : 0, bits = R == 2 ? 10 : 11;
-        each([&](int, uint32_t k) {
-            // (rows that stay anyway are many and in one place: counted below, not one by one)
-            if (R == 0 ? k + 1u > 1u : (k >> ((shift + bits) & 31)) == prefix)
-                atomicAdd(&s_hist[R][(k >> shift) & ((1u << bits) - 1u)], 1u);
-        });
-        if (R == 0 && tid == 0) atomicAdd(&s_hist[R][kEvictBins - 1], static_cast<uint32_t>(sinks + recent));
+        if constexpr (R > 0)
+            each([&](const uint32_t(&k)[4]) {
+                bool is[4], any = false;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    is[u] = (k[u] >> ((shift + bits) & 31)) == prefix;
+                    any |= is[u];
+                }
+                if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (is[u]) atomicAdd(&s_hist[R * kEvictBins + ((k[u] >> shift) & ((1u << bits) - 1u))], 1u);
+            });
         __syncthreads();
         // thread t holds bins 2047 - 2 t and 2046 - 2 t; the digit where the count from above reaches `need`
-        const uint2 b = *reinterpret_cast<const uint2*>(&s_hist[R][kEvictBins - 2 - 2 * tid]);
+        uint2* bins = reinterpret_cast<uint2*>(&s_hist[R * kEvictBins + kEvictBins - 2 - 2 * tid]);
+        uint2 b = *bins;
+        if (R == 0) {
+            const uint2 odd = bins[kEvictBins / 2];
+            b = make_uint2(b.x + odd.x, b.y + odd.y);
+            bins[kEvictBins / 2] = make_uint2(0, 0);  // the next digit's
+        }
         const uint32_t incl = wave_scan(b.x + b.y);
         if (lane == 63) s_wave[wave] = incl;
         __syncthreads();
@@ -275,9 +329,12 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     round(std::integral_constant<int, 2>{});
     const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
     int sure_n = 0, tie_n = 0;
-    each([&](int, uint32_t k) {
-        sure_n += __popcll(__builtin_amdgcn_ballot_w64(k > cut));
-        tie_n += __popcll(__builtin_amdgcn_ballot_w64(k == cut));
+    each([&](const uint32_t(&k)[4]) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            sure_n += __popcll(__builtin_amdgcn_ballot_w64(k[u] > cut));
+            tie_n += __popcll(__builtin_amdgcn_ballot_w64(k[u] == cut));
+        }
     });
     if (lane == 0) s_cnt[wave] = make_int2(sure_n, tie_n);
     __syncthreads();
@@ -291,31 +348,29 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     const int wanted = static_cast<int>(need);
     at = __builtin_amdgcn_readfirstlane(at + min(ties, wanted));
     ties = __builtin_amdgcn_readfirstlane(ties);
-    each([&](int i, uint32_t k) {
-        uint64_t take = __builtin_amdgcn_ballot_w64(k > cut);
-        const uint64_t tb = __builtin_amdgcn_ballot_w64(k == cut);
-        if (tb != 0) {
-            const bool t = k == cut && ties + __popcll(tb & ((1ull << lane) - 1)) < wanted;
-            take |= __builtin_amdgcn_ballot_w64(t);
-            ties += __popcll(tb);
+    for (int i0 = r0; i0 < r1; i0 += 256) {
+        uint32_t k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 64 * u + lane;
+            k[u] = cached ? s_key[i] : key_of(i, w[min(i, n - 1)]);
         }
-        if ((take >> lane) & 1)
-            out[at + static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(take >> 32),
-                                          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(take), 0u)))] = i;
-        at += __popcll(take);
-    });
-}
-
-// The weights of the kept rows move up too, and those behind them start over.
-__device__ __forceinline__ void evict_finish(float* out_weights, const int32_t* evicted, int32_t* out_evicted,
-                                             const qe_device_control_block* ctl, int h, int keep, int max_seq) {
-    const int pos = ctl != nullptr ? ctl->seq_pos : 0;
-    const int row = kv4_row(ctl, evicted, h), n = min(row, max_seq), m = min(n, keep);
-    const size_t base = static_cast<size_t>(h) * max_seq;
-    for (int i = m + threadIdx.x; i < n; i += blockDim.x) out_weights[base + i] = 0.0f;
-    __syncthreads();  // evicted may be out_evicted
-    // the next position's row is m: positions that found the cache full count as gone too
-    if (threadIdx.x == 0) out_evicted[h] = row == 0 ? (evicted != nullptr ? evicted[h] : 0) : pos - m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint64_t take = __builtin_amdgcn_ballot_w64(k[u] > cut);
+            const uint64_t tb = __builtin_amdgcn_ballot_w64(k[u] == cut);
+            if (tb != 0) {
+                const bool t = k[u] == cut && ties + __popcll(tb & ((1ull << lane) - 1)) < wanted;
+                take |= __builtin_amdgcn_ballot_w64(t);
+                ties += __popcll(tb);
+            }
+            if ((take >> lane) & 1)
+                out[at + static_cast<int>(__builtin_amdgcn_mbcnt_hi(
+                             static_cast<uint32_t>(take >> 32),
+                             __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(take), 0u)))] = i0 + 64 * u + lane;
+            at += __popcll(take);
+        }
+    }
 }
 
 struct EvictMove {
@@ -333,8 +388,7 @@ struct EvictMove {
 };
 
 // The kept rows to the front, in their order, into memory apart from the caches:
-// a lane per 16-byte piece, 5 pieces a row, K (blockIdx.z 0) and V (1); the
-// blocks of K move the weights as well, the first of them ends the head.
+// a lane per 16-byte piece, 5 pieces a row, K (blockIdx.z 0, with the weights) and V (1).
 constexpr int kCopyRows = 51;  // rows of a block of 256 threads
 __global__ __launch_bounds__(256) void kv4_evict_copy_kernel(EvictMove p) {
     const int h = blockIdx.y, tid = threadIdx.x;
@@ -349,12 +403,10 @@ __global__ __launch_bounds__(256) void kv4_evict_copy_kernel(EvictMove p) {
             *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
         }
     }
-    if (blockIdx.z != 0) return;
-    if (tid < kCopyRows && r0 + tid < p.keep) {
+    if (blockIdx.z == 0 && tid < kCopyRows && r0 + tid < p.keep) {
         const int from = list[r0 + tid];
         if (from >= 0) p.out_weights[base + r0 + tid] = p.weights[base + from];
     }
-    if (blockIdx.x == 0) evict_finish(p.out_weights, p.evicted, p.out_evicted, p.ctl, h, p.keep, p.max_seq);
 }
 
 // The same in place: row i comes from kept[i] >= i, a block takes all rows of a
@@ -485,9 +537,10 @@ extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* 
                    same_or_apart(layer_v_cache, out_v_cache, rows * kKv4Row) &&
                    same_or_apart(key_weights, out_key_weights, rows * sizeof(float)),
                "%s: an output overlaps its input without being it", what);
-    const size_t lds = std::min(max_seq_len, kEvictCached) * sizeof(uint32_t);
+    const size_t lds = std::min(kEvictWaves * evict_run(max_seq_len), kEvictCached) * sizeof(uint32_t);
     kv4_evict_select_kernel<<<num_kv_heads, kEvictThreads, lds, stream>>>(key_weights, d_evicted, d_control, kept_rows,
-                                                                          keep, sinks, recent, max_seq_len);
+                                                                          keep, sinks, recent, max_seq_len,
+                                                                          in_place ? nullptr : out_key_weights, out_evicted);
     const EvictMove p{layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
                       out_evicted, kept_rows, d_control, keep, max_seq_len};
     if (in_place)

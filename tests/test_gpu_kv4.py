@@ -481,7 +481,8 @@ def _check_evict(kv, w, pos, gone, keep, sinks, recent, ms, got):
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("n,keep,sinks,recent", [
     (1, 1, 0, 0), (2, 1, 0, 0), (2, 1, 1, 0), (2, 1, 0, 1), (10, 20, 4, 8), (20, 20, 4, 8), (21, 20, 4, 8), (100, 7, 3, 4),
-    (100, 99, 0, 0), (1000, 500, 4, 100), (1025, 64, 0, 64), (4097, 4096, 1, 1), (5000, 4300, 4, 512), (9000, 100, 4, 3)])
+    (100, 99, 0, 0), (1000, 500, 4, 100), (1025, 64, 0, 64), (4097, 4096, 1, 1), (5000, 4300, 4, 512), (9000, 100, 4, 3),
+    (32768, 20000, 4, 10000), (40000, 9000, 4, 700)])
 def test_evict(qe, n, keep, sinks, recent, in_place):
     rng = np.random.default_rng(n + keep)
     nkv, ms = 3, n + 6

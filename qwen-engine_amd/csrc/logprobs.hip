@@ -18,13 +18,21 @@ namespace qe {
 namespace {
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
-constexpr int kLpSegment = 8192;                      // logits of a block: 32 a thread
-constexpr int kLpChunks = kLpSegment / (8 * kLpThreads);  // 16-byte chunks of a thread
 constexpr int kLpMaxTop = 32;
-constexpr float kLpLog2e = 1.4426950408889634f;
+constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
+// 16-byte chunks of a thread of the segment kernel: with many rows 16 (segments of
+// 32768 logits), so that the selection of the alternatives, the same work for a
+// segment of any length, is seldom; with few 4 (8192), so that a row is spread over the chip.
+constexpr int kLpFew = 4, kLpMany = 16;
+constexpr int lp_segment(int chunks) { return 8 * kLpThreads * chunks; }
+
+// Candidates of a wave in LDS.
+constexpr int kLpCandidates = 1024;
 
 // Segments of a row: the first starts at a 16-byte boundary, up to 7 logits before the row.
-__host__ __device__ __forceinline__ int lp_segments(int vocab) { return (vocab + 7 + kLpSegment - 1) / kLpSegment; }
+__host__ __device__ __forceinline__ int lp_segments(int vocab, int chunks) {
+    return (vocab + 7 + lp_segment(chunks) - 1) / lp_segment(chunks);
+}
 // Words that one segment leaves: m, S, T, and its keys.
 __host__ __device__ __forceinline__ int lp_words(int top) { return 3 + top; }
 
@@ -38,114 +46,202 @@ __device__ __forceinline__ float lp_logit(uint32_t order) {
     return h2f(static_cast<uint16_t>(order & 0x8000u ? order & 0x7FFFu : ~order));
 }
 
+// The value of lane ^ J, by DPP within 16 lanes and lane swaps above.
+template <int J>
+__device__ __forceinline__ uint32_t lp_partner(uint32_t v) {
+    const int x = static_cast<int>(v);
+    if constexpr (J == 1) return static_cast<uint32_t>(qwen::dpp_i32<0xB1>(x));
+    if constexpr (J == 2) return static_cast<uint32_t>(qwen::dpp_i32<0x4E>(x));
+    if constexpr (J == 4) return static_cast<uint32_t>(qwen::dpp_i32<0x1B>(qwen::dpp_i32<0x141>(x)));  // ^7, ^3
+    if constexpr (J == 8) return static_cast<uint32_t>(qwen::dpp_i32<0x128>(x));                       // row_ror 8
+    if constexpr (J == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        const uint32_t a = r[0], b = r[1];
+        return (threadIdx.x & 16) ? a : b;
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return (threadIdx.x & 32) ? a : b;
+}
+template <int J>
+__device__ __forceinline__ unsigned long long lp_partner(unsigned long long v) {
+    return static_cast<unsigned long long>(lp_partner<J>(static_cast<uint32_t>(v))) |
+           (static_cast<unsigned long long>(lp_partner<J>(static_cast<uint32_t>(v >> 32))) << 32);
+}
+
 // Bitonic network over the 64 lanes: lane 0 ends with the largest.
-template <class T>
-__device__ __forceinline__ T lp_exchange(T v, int lane, int j, bool down) {
-    const T o = __shfl_xor(v, j);
-    const bool larger = ((lane & j) == 0) == down;
+template <int J, class T>
+__device__ __forceinline__ T lp_exchange(T v, bool larger) {
+    const T o = lp_partner<J>(v);
     return larger ? (o > v ? o : v) : (o < v ? o : v);
+}
+// The steps from J down, where `down` says whether the block of lanes sorts downwards.
+template <int J, class T>
+__device__ __forceinline__ T lp_steps(T v, int lane, bool down) {
+    v = lp_exchange<J>(v, ((lane & J) == 0) == down);
+    if constexpr (J > 1) return lp_steps<J / 2>(v, lane, down);
+    else return v;
 }
 template <class T>
 __device__ __forceinline__ T lp_sort(T v, int lane) {
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) v = lp_exchange(v, lane, j, (lane & k) == 0);
-    return v;
+    v = lp_steps<1>(v, lane, (lane & 2) == 0);
+    v = lp_steps<2>(v, lane, (lane & 4) == 0);
+    v = lp_steps<4>(v, lane, (lane & 8) == 0);
+    v = lp_steps<8>(v, lane, (lane & 16) == 0);
+    v = lp_steps<16>(v, lane, (lane & 32) == 0);
+    return lp_steps<32>(v, lane, true);
 }
 // The 64 largest of two sorted sets.
 template <class T>
 __device__ __forceinline__ T lp_merge(T a, T b, int lane) {
     const T o = __shfl_xor(b, 63);
-    T v = a > o ? a : o;
-#pragma unroll
-    for (int j = 32; j > 0; j >>= 1) v = lp_exchange(v, lane, j, true);
-    return v;
+    return lp_steps<32>(a > o ? a : o, lane, true);
 }
 
-__global__ __launch_bounds__(kLpThreads) void token_logprobs_segment_kernel(const uint16_t* __restrict__ logits,
+// One segment.  exp(x - m) is 2^(x L - m L), L = log2 e, in one fused multiply-add
+// with c = m L rounded; what the rounding leaves, r = m L - c, is the same for every
+// logit of the wave and comes off at the end: S = 2^-r S', T = ln 2 (T' - r S') 2^-r.
+// Per logit that is a conversion, the multiply-add, the exponential, two sums, a clamp
+// (-inf times 0) and a comparison: bound by these beside the memory.
+template <int CHUNKS>
+__global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_segment_kernel(const uint16_t* __restrict__ logits,
                                                                             uint32_t* __restrict__ parts, int vocab,
                                                                             long long row_stride, int segments,
                                                                             int top) {
-    __shared__ uint32_t s_key[kLpWaves][kLpSegment / kLpWaves];
+    constexpr int kSegment = lp_segment(CHUNKS);
+    static_assert(kSegment <= 0x10000, "an index is 16 bits of a key");
+    __shared__ uint32_t s_key[kLpWaves][kLpCandidates];
     __shared__ float s_st[kLpWaves][3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long long row = blockIdx.x / segments;
     const int seg = static_cast<int>(blockIdx.x % segments);
     const uint16_t* x = logits + row * row_stride;
     const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) >> 1);  // logits past a 16-byte boundary
-    const int seg0 = seg * kLpSegment - skew;
-    uint16_t v[kLpChunks][8];
-    uint32_t in = 0;  // which of the thread's logits belong to the row
+    const int seg0 = seg * kSegment - skew;
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    uint32_t v[CHUNKS][4];
+    uint32_t part = 0;  // chunks that lie only partly in the row, or behind it
 #pragma unroll
-    for (int c = 0; c < kLpChunks; ++c) {
+    for (int c = 0; c < CHUNKS; ++c) {
         const int i0 = seg0 + (c * kLpThreads + tid) * 8;
         if (i0 >= 0 && i0 + 8 <= vocab) {
-            const u32x4 raw = *reinterpret_cast<const u32x4*>(x + i0);
+            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + i0));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = raw[e];
-                v[c][2 * e] = static_cast<uint16_t>(w);
-                v[c][2 * e + 1] = static_cast<uint16_t>(w >> 16);
-            }
-            in |= 0xFFu << (8 * c);
+            for (int e = 0; e < 4; ++e) v[c][e] = raw[e];
         } else {
+            part |= 1u << c;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool ok = i0 + e >= 0 && i0 + e < vocab;
-                v[c][e] = ok ? x[i0 + e] : 0xFC00u;  // -inf
-                in |= static_cast<uint32_t>(ok) << (8 * c + e);
-            }
+            for (int e = 0; e < 4; ++e) v[c][e] = 0xFC00FC00u;  // -inf
         }
     }
-    float mine = -INFINITY;
+    if (__builtin_amdgcn_ballot_w64(part != 0) != 0) {
 #pragma unroll
-    for (int c = 0; c < kLpChunks; ++c)
+        for (int c = 0; c < CHUNKS; ++c) {
+            const int i0 = seg0 + (c * kLpThreads + tid) * 8;
+            if (!((part >> c) & 1) || i0 + 8 <= 0 || i0 >= vocab) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine = fmaxf(mine, h2f(v[c][e]));
+            for (int e = 0; e < 8; ++e)
+                if (i0 + e >= 0 && i0 + e < vocab)
+                    v[c][e >> 1] = e & 1 ? (v[c][e >> 1] & 0xFFFFu) | (static_cast<uint32_t>(x[i0 + e]) << 16)
+                                         : (v[c][e >> 1] & 0xFFFF0000u) | x[i0 + e];
+        }
+    }
+    auto at = [&](int c, int e) { return h2f(static_cast<uint16_t>(e & 1 ? v[c][e >> 1] >> 16 : v[c][e >> 1])); };
+    f16x2 most = {(_Float16)-INFINITY, (_Float16)-INFINITY};
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t w = v[c][e];
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(f16x2, w));  // a NaN is passed over
+        }
+    const float mine = fmaxf(static_cast<float>(most.x), static_cast<float>(most.y));
     const float m = qwen::seg_max<64>(mine);
     const float ref = m == -INFINITY ? 0.0f : m;
-    float S = 0.0f, T = 0.0f;
+    const float c0 = ref * kLpLog2e, rest = __builtin_fmaf(ref, kLpLog2e, -c0);
+    float S = 0.0f, T = 0.0f, S1 = 0.0f, T1 = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kLpChunks; ++c)
+    for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = h2f(v[c][e]) - ref;
-            const float p = __builtin_amdgcn_exp2f(d * kLpLog2e);
-            S += p;
-            T = __builtin_fmaf(p, fmaxf(d, -1e4f), T);  // p is 0 there, and d may be -inf
+        for (int e = 0; e < 8; e += 2) {
+            const float t0 = __builtin_fmaf(at(c, e), kLpLog2e, -c0), t1 = __builtin_fmaf(at(c, e + 1), kLpLog2e, -c0);
+            const float p0 = __builtin_amdgcn_exp2f(t0), p1 = __builtin_amdgcn_exp2f(t1);
+            S += p0;
+            S1 += p1;
+            T = __builtin_fmaf(p0, fmaxf(t0, -1e4f), T);  // p is 0 there, and t may be -inf
+            T1 = __builtin_fmaf(p1, fmaxf(t1, -1e4f), T1);
         }
-    S = qwen::seg_sum<64>(S);
-    T = qwen::seg_sum<64>(T);
+    S = qwen::seg_sum<64>(S + S1);
+    T = qwen::seg_sum<64>(T + T1);
     if (lane == 0) {
+        const float f = __builtin_amdgcn_exp2f(-rest);
         s_st[wave][0] = m;
-        s_st[wave][1] = S;
-        s_st[wave][2] = T;
+        s_st[wave][1] = f * S;
+        s_st[wave][2] = f * kLpLn2 * (T - rest * S);
     }
     uint32_t* out = parts + (row * segments + seg) * lp_words(top);
     if (top > 0) {
-        // the top-th largest of the lanes' maxima: at least `top` logits reach it, few do
-        const float cut = __shfl(lp_sort(mine, lane), top - 1);
+        // The top-th largest of the lanes' maxima: at least `top` logits reach it, few
+        // do.  They are collected as bits and index, and sorted 64 at a time.
+        float cut = lp_logit(__shfl(lp_sort(lp_order(__builtin_bit_cast(uint16_t, static_cast<_Float16>(mine))), lane), top - 1));
         int n = 0;
-#pragma unroll
-        for (int c = 0; c < kLpChunks; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool take = h2f(v[c][e]) >= cut && ((in >> (8 * c + e)) & 1u);
-                const uint64_t b = __builtin_amdgcn_ballot_w64(take);
-                if (b == 0) continue;
-                // index within the segment, the lower the larger
-                if (take)
-                    s_key[wave][n + __popcll(b & ((1ull << lane) - 1))] =
-                        (lp_order(v[c][e]) << 16) | (0xFFFFu - ((c * kLpThreads + tid) * 8 + e));
-                n += __popcll(b);
-            }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave reads what its lanes wrote
         uint32_t best = 0;
-        for (int i = 0; i < n; i += 64) {
-            const uint32_t k = lp_sort(i + lane < n ? s_key[wave][i + lane] : 0u, lane);
-            best = i == 0 ? k : lp_merge(best, k, lane);
+        // Index within the segment, the lower the larger.
+        auto collect = [&](bool take, uint32_t bits, int i) __attribute__((always_inline)) {
+            const uint64_t b = __builtin_amdgcn_ballot_w64(take);
+            if (b == 0) return;
+            const int slot = n + static_cast<int>(__builtin_amdgcn_mbcnt_hi(
+                                     static_cast<uint32_t>(b >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(b), 0u)));
+            if (take) s_key[wave][slot] = (bits << 16) | (0xFFFFu - i);
+            n += __popcll(b);
+        };
+        // The last n - from of them, at most 64, into the best so far.
+        auto sort_last = [&](int from) __attribute__((always_inline)) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave reads what its lanes wrote
+            uint32_t k = 0;
+            if (from + lane < n) {
+                k = s_key[wave][from + lane];
+                const int i = seg0 + static_cast<int>(0xFFFFu - (k & 0xFFFFu));
+                // what stands for logits outside the row is -inf, and reaches a cut of -inf
+                k = i >= 0 && i < vocab ? (lp_order(static_cast<uint16_t>(k >> 16)) << 16) | (k & 0xFFFFu) : 0u;
+            }
+            best = lp_merge(best, lp_sort(k, lane), lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            n = from;
+        };
+        bool fits = true;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) any |= at(c, e) >= cut;
+            if (!fits || __builtin_amdgcn_ballot_w64(any) == 0) continue;
+            fits = n <= kLpCandidates - 8 * 64;
+            if (!fits) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                collect(at(c, e) >= cut, e & 1 ? v[c][e >> 1] >> 16 : v[c][e >> 1] & 0xFFFFu, (c * kLpThreads + tid) * 8 + e);
         }
+        if (!fits) {
+            // Hundreds of equal logits: again, from memory, sorting on the way.  What
+            // comes after a sort has to beat the top-th of it, being later in the row.
+            n = 0;
+            for (int c = 0; c < CHUNKS; ++c) {
+                const int i = (c * kLpThreads + tid) * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = seg0 + i + e;
+                    const bool in = j >= 0 && j < vocab;
+                    const uint16_t bits = in ? x[j] : 0x7E00u;
+                    collect(in && h2f(bits) >= cut, bits, i + e);
+                }
+                if (n >= 64) {
+                    while (n >= 64) sort_last(n - 64);
+                    cut = lp_logit((__shfl(best, top - 1) >> 16) + 1);
+                }
+            }
+        }
+        while (n > 0) sort_last(max(n - 64, 0));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (lane < top) s_key[wave][lane] = best;
     }
@@ -177,7 +273,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_segment_kernel(cons
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
     const uint16_t* __restrict__ logits, const uint32_t* __restrict__ parts, const int32_t* __restrict__ ids,
     float* __restrict__ out_logprob, float* __restrict__ out_entropy, float* __restrict__ top_logprob,
-    int32_t* __restrict__ top_ids, int vocab, long long row_stride, int segments, int top) {
+    int32_t* __restrict__ top_ids, int vocab, long long row_stride, int segments, int segment, int top) {
     __shared__ float s_st[kLpWaves][3];
     __shared__ unsigned long long s_key[kLpWaves][kLpMaxTop];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -217,7 +313,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
             if (i < n) {
                 const int s = i / top;
                 const uint32_t key = part[s * words + 3 + (i - s * top)];
-                const uint32_t at = s * kLpSegment - skew + (0xFFFFu - (key & 0xFFFFu));
+                const uint32_t at = s * segment - skew + (0xFFFFu - (key & 0xFFFFu));
                 if (key != 0) k = (static_cast<unsigned long long>(key >> 16) << 32) | (0xFFFFFFFFu - at);
             }
             best = lp_merge(best, lp_sort(k, lane), lane);
@@ -269,9 +365,9 @@ using namespace qe;
 extern "C" int qe_token_logprobs_workspace_bytes(int num_rows, int vocab_size, int top_k, size_t* bytes) {
     const char* what = "token_logprobs_workspace_bytes";
     QE_REQUIRE(bytes != nullptr, "%s: NULL pointer", what);
-    QE_REQUIRE(num_rows >= 0 && vocab_size > 0 && vocab_size <= INT32_MAX - kLpSegment && top_k >= 0 && top_k <= kLpMaxTop,
+    QE_REQUIRE(num_rows >= 0 && vocab_size > 0 && vocab_size <= INT32_MAX - lp_segment(kLpMany) && top_k >= 0 && top_k <= kLpMaxTop,
                "%s: num_rows=%d vocab_size=%d top_k=%d", what, num_rows, vocab_size, top_k);
-    *bytes = static_cast<size_t>(num_rows) * lp_segments(vocab_size) * lp_words(top_k) * sizeof(uint32_t);
+    *bytes = static_cast<size_t>(num_rows) * lp_segments(vocab_size, kLpFew) * lp_words(top_k) * sizeof(uint32_t);
     return QE_OK;
 }
 
@@ -283,7 +379,7 @@ extern "C" int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* t
     QE_REQUIRE(logits && workspace, "%s: NULL pointer", what);
     QE_REQUIRE((token_ids == nullptr) == (out_logprob == nullptr), "%s: token_ids and out_logprob are given together",
                what);
-    QE_REQUIRE(vocab_size > 0 && vocab_size <= INT32_MAX - kLpSegment, "%s: vocab_size=%d", what, vocab_size);
+    QE_REQUIRE(vocab_size > 0 && vocab_size <= INT32_MAX - lp_segment(kLpMany), "%s: vocab_size=%d", what, vocab_size);
     QE_REQUIRE(row_stride >= vocab_size || num_rows <= 1, "%s: row_stride=%lld < vocab_size=%d", what, row_stride,
                vocab_size);
     QE_REQUIRE(top_k >= 0 && top_k <= kLpMaxTop && top_k <= vocab_size, "%s: top_k=%d (0..%d, at most vocab_size)", what,
@@ -292,13 +388,19 @@ extern "C" int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* t
     QE_REQUIRE(top_k == 0 || out_top_logprob || out_top_ids, "%s: top_k=%d without an output", what, top_k);
     QE_REQUIRE(aligned(logits, 2) && aligned(workspace, 4), "%s: alignment", what);
     if (num_rows <= 0) return QE_OK;
-    const int segments = lp_segments(vocab_size);
+    // many: enough rows for two blocks of long segments on every CU
+    const bool many = static_cast<long long>(num_rows) * lp_segments(vocab_size, kLpMany) >= 2LL * cu_count();
+    const int chunks = many ? kLpMany : kLpFew, segments = lp_segments(vocab_size, chunks);
     QE_REQUIRE(static_cast<long long>(num_rows) * segments <= INT32_MAX, "%s: num_rows=%d", what, num_rows);
     uint32_t* parts = static_cast<uint32_t*>(workspace);
-    token_logprobs_segment_kernel<<<num_rows * segments, kLpThreads, 0, stream>>>(logits, parts, vocab_size, row_stride,
-                                                                                  segments, top_k);
+    if (many)
+        token_logprobs_segment_kernel<kLpMany><<<num_rows * segments, kLpThreads, 0, stream>>>(
+            logits, parts, vocab_size, row_stride, segments, top_k);
+    else
+        token_logprobs_segment_kernel<kLpFew><<<num_rows * segments, kLpThreads, 0, stream>>>(
+            logits, parts, vocab_size, row_stride, segments, top_k);
     token_logprobs_row_kernel<<<num_rows, kLpThreads, 0, stream>>>(logits, parts, token_ids, out_logprob, out_entropy,
                                                                    out_top_logprob, out_top_ids, vocab_size, row_stride,
-                                                                   segments, top_k);
+                                                                   segments, lp_segment(chunks), top_k);
     return check_launch(what);
 }

@@ -105,9 +105,10 @@ __device__ __forceinline__ T lp_merge(T a, T b, int lane) {
 // (-inf times 0) and a comparison: bound by these beside the memory.
 template <int CHUNKS>
 __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_segment_kernel(const uint16_t* __restrict__ logits,
-                                                                            uint32_t* __restrict__ parts, int vocab,
-                                                                            long long row_stride, int segments,
-                                                                            int top) {
+                                                                               float* __restrict__ stats,
+                                                                               uint32_t* __restrict__ keys, int vocab,
+                                                                               long long row_stride, int segments,
+                                                                               int top) {
     constexpr int kSegment = lp_segment(CHUNKS);
     static_assert(kSegment <= 0x10000, "an index is 16 bits of a key");
     __shared__ uint32_t s_key[kLpWaves][kLpCandidates];
@@ -179,7 +180,6 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_segment_kernel(c
         s_st[wave][1] = f * S;
         s_st[wave][2] = f * kLpLn2 * (T - rest * S);
     }
-    uint32_t* out = parts + (row * segments + seg) * lp_words(top);
     if (top > 0) {
         // The top-th largest of the lanes' maxima: at least `top` logits reach it, few
         // do.  They are collected as bits and index, and sorted 64 at a time.
@@ -259,32 +259,63 @@ __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_segment_kernel(c
         Tg += f * (s_st[w][2] + d * s_st[w][1]);
     }
     if (lane == 0) {
-        out[0] = __builtin_bit_cast(uint32_t, mg);
-        out[1] = __builtin_bit_cast(uint32_t, Sg);
-        out[2] = __builtin_bit_cast(uint32_t, Tg);
+        float* out = stats + (row * segments + seg) * 3;
+        out[0] = mg;
+        out[1] = Sg;
+        out[2] = Tg;
     }
     if (top > 0) {
         uint32_t best = lane < top ? s_key[0][lane] : 0u;
         for (int w = 1; w < kLpWaves; ++w) best = lp_merge(best, lane < top ? s_key[w][lane] : 0u, lane);
-        if (lane < top) out[3 + lane] = best;
+        if (lane < top) keys[(row * segments + seg) * top + lane] = best;
     }
 }
 
+// A row's segments together.  Of 64 keys, the segments' best, the top-th largest
+// is a bound for the alternatives; the keys that reach it, usually few more than asked
+// for, are ordered at once.  Latency only.
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
-    const uint16_t* __restrict__ logits, const uint32_t* __restrict__ parts, const int32_t* __restrict__ ids,
+    const uint16_t* __restrict__ logits, const float* __restrict__ stats, const uint32_t* __restrict__ keys,
+    const int32_t* __restrict__ ids,
     float* __restrict__ out_logprob, float* __restrict__ out_entropy, float* __restrict__ top_logprob,
     int32_t* __restrict__ top_ids, int vocab, long long row_stride, int segments, int segment, int top) {
     __shared__ float s_st[kLpWaves][3];
     __shared__ unsigned long long s_key[kLpWaves][kLpMaxTop];
+    __shared__ unsigned long long s_list[64];
+    __shared__ int s_n;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long long row = blockIdx.x;
     const uint16_t* x = logits + row * row_stride;
-    const int words = lp_words(top);
-    const uint32_t* part = parts + row * segments * words;
+    const float* part = stats + row * segments * 3;
+    const int n = segments * top;
+    const uint32_t* row_keys = keys + row * n;
+    const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) >> 1);
+    // key i of the row as (order, index)
+    auto whole = [&](uint32_t k, int i) {
+        const uint32_t at = (i / top) * segment - skew + (0xFFFFu - (k & 0xFFFFu));
+        return k != 0 ? (static_cast<unsigned long long>(k >> 16) << 32) | (0xFFFFFFFFu - at) : 0ull;
+    };
+    constexpr int EARLY = 4;  // keys of a thread, requested with the sums
+    uint32_t early[EARLY];
+    if (top > 0) {
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) early[i] = row_keys[min(tid + kLpThreads * i, n - 1)];
+    }
+    const int id = out_logprob != nullptr ? ids[row] : -1;
+    if (tid == 0) s_n = 0;
     float m = -INFINITY, S = 0.0f, T = 0.0f;
+    // the best keys of every segment, best first, 64 in all (with more segments: of 64 groups)
+    uint32_t front = 0;
+    if (top > 0) {
+        if (segments <= 64) {
+            const int rank = lane / segments;
+            if (rank < top) front = row_keys[(lane - rank * segments) * top + rank];
+        } else {
+            for (int s = lane; s < segments; s += 64) front = max(front, row_keys[s * top]);
+        }
+    }
     for (int s = tid; s < segments; s += kLpThreads) {
-        const float ms = __builtin_bit_cast(float, part[s * words]), Ss = __builtin_bit_cast(float, part[s * words + 1]),
-                    Ts = __builtin_bit_cast(float, part[s * words + 2]);
+        const float ms = part[3 * s], Ss = part[3 * s + 1], Ts = part[3 * s + 2];
         const float mn = fmaxf(m, ms);
         const float da = m == mn ? 0.0f : fmaxf(m - mn, -1e4f), db = ms == mn ? 0.0f : fmaxf(ms - mn, -1e4f);
         const float fa = __builtin_amdgcn_exp2f(da * kLpLog2e), fb = __builtin_amdgcn_exp2f(db * kLpLog2e);
@@ -292,6 +323,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
         S = fa * S + fb * Ss;
         m = mn;
     }
+    const bool has_id = id >= 0 && id < vocab;
+    const uint16_t x_id = x[has_id ? id : 0];  // not waited for until the end
     const float mw = qwen::seg_max<64>(m);
     {
         const float d = m == mw ? 0.0f : fmaxf(m - mw, -1e4f), f = __builtin_amdgcn_exp2f(d * kLpLog2e);
@@ -303,22 +336,26 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
         s_st[wave][1] = S;
         s_st[wave][2] = T;
     }
+    bool few = true;
     if (top > 0) {
-        const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) >> 1);
-        unsigned long long best = 0;
-        const int n = segments * top;
-        for (int i0 = 64 * wave; i0 < n; i0 += kLpThreads) {
-            const int i = i0 + lane;
-            unsigned long long k = 0;
-            if (i < n) {
-                const int s = i / top;
-                const uint32_t key = part[s * words + 3 + (i - s * top)];
-                const uint32_t at = s * segment - skew + (0xFFFFu - (key & 0xFFFFu));
-                if (key != 0) k = (static_cast<unsigned long long>(key >> 16) << 32) | (0xFFFFFFFFu - at);
+        const uint32_t cut = __shfl(lp_sort(front, lane), top - 1) >> 16;
+        __syncthreads();  // s_n
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i)
+            if (tid + kLpThreads * i < n && early[i] != 0 && (early[i] >> 16) >= cut) {
+                const int slot = atomicAdd(&s_n, 1);
+                if (slot < 64) s_list[slot] = whole(early[i], tid + kLpThreads * i);
             }
-            best = lp_merge(best, lp_sort(k, lane), lane);
+        __syncthreads();
+        few = s_n <= 64 && n <= EARLY * kLpThreads;
+        if (!few) {  // long rows, or many equal logits: every key, 64 at a time
+            unsigned long long best = 0;
+            for (int i0 = 64 * wave; i0 < n; i0 += kLpThreads) {
+                const int i = i0 + lane;
+                best = lp_merge(best, lp_sort(i < n ? whole(row_keys[i], i) : 0ull, lane), lane);
+            }
+            if (lane < top) s_key[wave][lane] = best;
         }
-        if (lane < top) s_key[wave][lane] = best;
     }
     __syncthreads();
     if (wave != 0) return;
@@ -337,21 +374,34 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_row_kernel(
     const float log_s = logf(S);
     auto logprob = [&](float logit) { return nothing ? -INFINITY : logit - mg - log_s; };
     if (lane == 0) {
-        if (out_logprob != nullptr) {
-            const int id = ids[row];
-            out_logprob[row] = id >= 0 && id < vocab ? logprob(h2f(x[id])) : 0.0f;
-        }
+        if (out_logprob != nullptr) out_logprob[row] = has_id ? logprob(h2f(x_id)) : 0.0f;
         if (out_entropy != nullptr) out_entropy[row] = nothing ? 0.0f : log_s - T / S;
     }
     if (top > 0) {
-        unsigned long long best = lane < top ? s_key[0][lane] : 0ull;
-        for (int w = 1; w < kLpWaves; ++w) best = lp_merge(best, lane < top ? s_key[w][lane] : 0ull, lane);
-        if (lane < top) {
+        unsigned long long best = 0;
+        int rank = lane;
+        if (few) {
+            // a lane's place is the number of larger keys: a short loop, where a sort
+            // is 21 steps of straight code that has to be fetched first
+            best = lane < s_n ? s_list[lane] : 0ull;
+            const int count = __builtin_amdgcn_readfirstlane(s_n);
+            if (lane < count) rank = 0;
+            for (int j = 0; j < count; ++j) {
+                const unsigned long long o =
+                    (static_cast<unsigned long long>(__builtin_amdgcn_readlane(static_cast<int>(best >> 32), j)) << 32) |
+                    static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(best), j));
+                rank += lane < count && o > best;
+            }
+        } else {
+            best = lane < top ? s_key[0][lane] : 0ull;
+            for (int w = 1; w < kLpWaves; ++w) best = lp_merge(best, lane < top ? s_key[w][lane] : 0ull, lane);
+        }
+        if (rank < top) {
             const bool none = best == 0;
             if (top_ids != nullptr)
-                top_ids[row * top + lane] = none ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
+                top_ids[row * top + rank] = none ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
             if (top_logprob != nullptr)
-                top_logprob[row * top + lane] =
+                top_logprob[row * top + rank] =
                     none ? __builtin_nanf("") : logprob(lp_logit(static_cast<uint32_t>(best >> 32)));
         }
     }
@@ -392,15 +442,17 @@ extern "C" int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* t
     const bool many = static_cast<long long>(num_rows) * lp_segments(vocab_size, kLpMany) >= 2LL * cu_count();
     const int chunks = many ? kLpMany : kLpFew, segments = lp_segments(vocab_size, chunks);
     QE_REQUIRE(static_cast<long long>(num_rows) * segments <= INT32_MAX, "%s: num_rows=%d", what, num_rows);
-    uint32_t* parts = static_cast<uint32_t*>(workspace);
+    float* stats = static_cast<float*>(workspace);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(stats + static_cast<size_t>(num_rows) * segments * 3);
     if (many)
         token_logprobs_segment_kernel<kLpMany><<<num_rows * segments, kLpThreads, 0, stream>>>(
-            logits, parts, vocab_size, row_stride, segments, top_k);
+            logits, stats, keys, vocab_size, row_stride, segments, top_k);
     else
         token_logprobs_segment_kernel<kLpFew><<<num_rows * segments, kLpThreads, 0, stream>>>(
-            logits, parts, vocab_size, row_stride, segments, top_k);
-    token_logprobs_row_kernel<<<num_rows, kLpThreads, 0, stream>>>(logits, parts, token_ids, out_logprob, out_entropy,
-                                                                   out_top_logprob, out_top_ids, vocab_size, row_stride,
-                                                                   segments, lp_segment(chunks), top_k);
+            logits, stats, keys, vocab_size, row_stride, segments, top_k);
+    token_logprobs_row_kernel<<<num_rows, kLpThreads, 0, stream>>>(logits, stats, keys, token_ids, out_logprob,
+                                                                   out_entropy, out_top_logprob, out_top_ids,
+                                                                   vocab_size, row_stride, segments,
+                                                                   lp_segment(chunks), top_k);
     return check_launch(what);
 }

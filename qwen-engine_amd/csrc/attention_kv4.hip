@@ -9,6 +9,7 @@
 
 #include "attn_common.hpp"
 #include "kv4_common.hpp"
+#include "lds_dma.hpp"
 
 namespace qe {
 namespace {
@@ -733,66 +734,119 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p
         p.lse[static_cast<size_t>(qi) * p.nq + qh] = (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
 }
 
-// Column sums of the probabilities: what the rows of the chunk give to 64 cache
-// rows of one kv head.  The block's 64 K rows stay in registers, expanded once;
+// Column sums of the probabilities: what the rows of the chunk give to 32 cache
+// rows of one kv head.  The block's 32 K rows stay in registers, expanded once;
 // a wave takes 32 query rows at a time, S^T = K . Q^T again, p = exp(s - lse) with
-// the row's final log sum, and keeps 32 sums a lane; lanes, then waves, add up
-// at the end in one order.
-constexpr int kW4Waves = 8;
+// the row's final log sum, and keeps 16 sums a lane; lanes, then waves, add up at
+// the end in one order.  Every block reads the q rows that see its cache rows: the
+// wave copies its 32 rows to LDS by DMA, whole rows of 256 bytes, while it uses the 32
+// before, and takes its operands from there.  (Read as operands, 32 bytes of
+// 32 rows at a time, the addresses alone made 1000 rows on 3900 positions 50 us.)
+constexpr int kW4Waves = 8, kW4Keys = 32;
+constexpr int kW4Buffer = 32 * 256 + 256;  // 32 q rows, their log sums
 __global__ __launch_bounds__(64 * kW4Waves, 2) void kv4_prefill_weights_kernel(Prefill4Params p) {
-    __shared__ float s_sum[kW4Waves][kP4Keys];
+    __shared__ __align__(16) char smem[kW4Waves * 2 * kW4Buffer];
+    __shared__ float s_sum[kW4Waves][kW4Keys];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int fr = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x % p.nkv, t = blockIdx.x / p.nkv;
     const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
-    const int len = min(base + p.T, p.max_seq);  // (base <= max_seq, T fits)
-    const int key0 = t * kP4Keys;
+    const int len = min(base + p.T, p.max_seq);
+    const int key0 = t * kW4Keys;
     if (key0 >= len) return;
     const int rows = p.T * p.group;
-    f16x8 kf[2][8];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint8_t* row = p.kc + (static_cast<size_t>(kvh) * p.max_seq + min(key0 + 32 * j + fr, len - 1)) * kKv4Row;
+    f16x8 kf[8];
+    {
+        const uint8_t* row = p.kc + (static_cast<size_t>(kvh) * p.max_seq + min(key0 + fr, len - 1)) * kKv4Row;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)  // word 2 kk + h: dims 16 kk + 8 h..
-            kf[j][kk] = kv4_expand_word(*reinterpret_cast<const uint32_t*>(row + 4 * (2 * kk + h)),
-                                        *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (kk >> 1)));
+            kf[kk] = kv4_expand_word(*reinterpret_cast<const uint32_t*>(row + 4 * (2 * kk + h)),
+                                     *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (kk >> 1)));
     }
-    f32x16 sum[2] = {f32x16{}, f32x16{}};
+    f32x16 sum = {};
     const int first = max(0, min(key0 - base, p.T - 1)) * p.group / 32 * 32;  // no row before it sees key0
-    for (int r0 = first + 32 * wave; r0 < rows; r0 += 32 * kW4Waves) {
-        const int r = r0 + fr, rc = min(r, rows - 1);
-        const int qi = rc / p.group, qh = kvh * p.group + rc % p.group;
-        const uint16_t* qr = p.q + (static_cast<size_t>(qi) * p.nq + qh) * kKv4Dim + 8 * h;
-        const float neg = -p.lse[static_cast<size_t>(qi) * p.nq + qh] * kLog2e;
-        const int lim = r < rows ? min(base + qi, p.max_seq - 1) : -1;
-        f32x16 sc[2] = {f32x16{}, f32x16{}};
+    constexpr int kStep = 32 * kW4Waves;
+    int r0 = first + 32 * wave;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                              (__attribute__((address_space(3))) void*)smem)) + wave * 2 * kW4Buffer;
+    // x / group for x < 128: group <= 64, so x (inverse group - 2^16) < 2^13 stays below 2^16
+    const uint32_t inverse = 65536u / p.group + 1u;
+    const uint16_t* q_head = p.q + static_cast<size_t>(kvh) * p.group * kKv4Dim;
+    const float* lse_head = p.lse + static_cast<size_t>(kvh) * p.group;
+    // Row r = token qi, head qg of the group, both uniform and kept up by addition.
+    // Tile load i: rows r + 4 i + lane / 16, stored chunk lane % 16, i.e. chunk
+    // (lane % 16) ^ swz(row) of memory.
+    const int step_q = kStep / p.group, step_g = kStep - step_q * p.group;
+    int qi_n = r0 / p.group, qg_n = r0 - qi_n * p.group;
+    auto request = [&](int r, int buf) __attribute__((always_inline)) {
+        const uint32_t dst = lds0 + buf * kW4Buffer;
+        // heads of the group past row r's, counted through the tokens: x = qg + rows further
+        const int most = min(32, rows - r) - 1 + qg_n;  // rows past the last are read as the last
+        const size_t token = static_cast<size_t>(qi_n) * p.nq;
+        auto place = [&](int x) __attribute__((always_inline)) {
+            x = min(x, most);
+            return static_cast<uint32_t>(x + static_cast<int>((static_cast<uint32_t>(x) * inverse) >> 16) * (p.nq - p.group));
+        };
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-            const f16x8 qf = *reinterpret_cast<const f16x8*>(qr + 16 * kk);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[j][kk], qf, sc[j], 0, 0, 0);
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t chunk = (lane & 15) ^ (((lane >> 4) << 2) | (i & 3));
+            lds_load_x4(dst + 1024 * i, q_head + token * kKv4Dim, place(qg_n + 4 * i + (lane >> 4)) * (2 * kKv4Dim) + 16 * chunk);
         }
+        lds_load_dword(dst + 8192, lse_head + token + place(qg_n + fr));
+        qi_n += step_q;
+        qg_n += step_g;
+        if (qg_n >= p.group) {
+            qg_n -= p.group;
+            ++qi_n;
+        }
+    };
+    uint32_t qa = lds0 + fr * 256 + 16 * (h ^ (((fr & 3) << 2) | ((fr >> 2) & 3)));
+    int qi_first = qi_n;
+    if (r0 < rows) request(r0, 0);
+    for (int buf = 0; r0 < rows; r0 += kStep, buf ^= 1) {
+        const int qi0 = qi_first;  // the token of row r0
+        qi_first = qi_n;
+        typedef const __attribute__((address_space(3))) f16x8* lptr;
+        typedef const __attribute__((address_space(3))) float* lfptr;
+        if (r0 + kStep < rows) {
+            request(r0 + kStep, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(9)" ::: "memory");  // all but the nine just requested
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 sc = {};
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int kk = 0; kk < 8; ++kk)
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                kf[kk], *reinterpret_cast<lptr>((qa ^ (32 * kk)) + buf * kW4Buffer), sc, 0, 0, 0);
+        const float neg = -*reinterpret_cast<lfptr>(lds0 + buf * kW4Buffer + 8192 + 4 * fr) * kLog2e;
+        // there are 32 rows, and all see every key (limits grow with the rows)
+        if (min(base + qi0, p.max_seq - 1) >= key0 + kW4Keys - 1 && r0 + 32 <= rows) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sum[v] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], kScoreScale, neg));
+        } else {
+            const int qi = (r0 + fr) / p.group;
+            const int lim = qi < p.T ? min(base + qi, p.max_seq - 1) : -1;
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                const int key = key0 + 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v], kScoreScale, neg));
-                sum[j][v] += key <= lim ? e : 0.0f;
+                const int key = key0 + 8 * (v >> 2) + 4 * h + (v & 3);
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], kScoreScale, neg));
+                sum[v] += key <= lim ? e : 0.0f;
             }
+        }
+        // the buffer is read before the next turn asks for it to be filled
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const float x = qwen::seg_sum<32>(sum[j][v]);
-            if (fr == 0) s_sum[wave][32 * j + 8 * (v >> 2) + 4 * h + (v & 3)] = x;
-        }
+    for (int v = 0; v < 16; ++v) {
+        const float x = qwen::seg_sum<32>(sum[v]);
+        if (fr == 0) s_sum[wave][8 * (v >> 2) + 4 * h + (v & 3)] = x;
+    }
     __syncthreads();
     const int key = key0 + static_cast<int>(threadIdx.x);
-    if (threadIdx.x >= kP4Keys || key >= len) return;
+    if (threadIdx.x >= kW4Keys || key >= len) return;
     float x = 0.0f;
 #pragma unroll
     for (int w = 0; w < kW4Waves; ++w) x += s_sum[w][threadIdx.x];
@@ -948,7 +1002,7 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     if (p.splits > 1)
         kv4_prefill_merge_kernel<<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
     if (key_weights_out != nullptr) {
-        const long long tiles = (static_cast<long long>(max_seq_len) + kP4Keys - 1) / kP4Keys;
+        const long long tiles = (static_cast<long long>(max_seq_len) + kW4Keys - 1) / kW4Keys;
         QE_REQUIRE(tiles * num_kv_heads <= INT32_MAX, "%s: max_seq_len=%d", what, max_seq_len);
         kv4_prefill_weights_kernel<<<static_cast<unsigned>(tiles * num_kv_heads), 64 * kW4Waves, 0, stream>>>(p);
     }

@@ -16,6 +16,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kScoreScale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
+// How far a row's maximum grows before its reference value follows: the
+// probabilities then reach 2^8, and their relative precision in fp16 is the same.
+constexpr float kReferenceLag = 8.0f;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // The largest value over lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float max_over_quarters(float x) {
@@ -43,9 +47,9 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 //   pairs of one dim with the rows' own scales: no transposition through LDS.
 // The whole group of q heads shares one expansion of K and V.
 constexpr int kKd4MaxSplits = 128;   // runs of a kv head, at most
-constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each wave
-constexpr int kKd4Waves = 4;
+constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each of four waves
 constexpr int kKd4MaxGroup = 64;     // q heads of a kv head
+constexpr int kKd4ManyWaves = 16;    // of a block where runs may be longer (waves without rows do nothing)
 
 // rows of a run for `ctx` rows over at most `splits` runs
 __host__ __device__ __forceinline__ int kd4_run(int ctx, int splits) {
@@ -59,16 +63,16 @@ struct Decode4Params {
     const uint8_t* vc;
     const qe_device_control_block* ctl;
     const int32_t* evicted;
-    float* part_o;   // [q head][split][128], relative to the run's maximum
-    float* part_ml;  // [q head][split][2] (maximum in the exp2 domain, sum)
-    float* scores;   // [q head][score_stride] in the exp2 domain, with key weights only
+    float* part_o;   // [q head][split][128], relative to the run's reference value
+    float* part_ml;  // [q head][split][2] (reference value in the exp2 domain, sum)
+    float* scores;   // [q head][score_stride] before the scale, with key weights only
     uint16_t* out;
     int8_t* q8;
     float* q_scale;
     int32_t* q_sum8;
     const float* w_in;
     float* w_out;
-    int nq, nkv, group, head_blocks, max_seq, splits, score_stride;
+    int nq, nkv, group, head_blocks, max_seq, splits, waves, score_stride;
 };
 
 // cache rows the token sees (one that found the cache full sees all of it)
@@ -82,36 +86,40 @@ struct Kd4Tile {
     uint32_t v[8], vp[8];  // word l % 16 of the lane's eight rows, its group's (scale, low)
 };
 
-template <bool WEIGHTS>
-__global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Params p) {
+template <bool WEIGHTS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 4) void kv4_decode_kernel(Decode4Params p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int n = lane & 15, h = lane >> 4;
     const int kvh = blockIdx.x % p.nkv;
     const int hb = (blockIdx.x / p.nkv) % p.head_blocks, split = blockIdx.x / (p.nkv * p.head_blocks);
-    const int ctx = kd4_context(p, kvh);
-    const int run = kd4_run(ctx, p.splits);
-    const int t0 = split * run, t1 = min(t0 + run, ctx);
-    if (t0 >= t1) return;
     const int heads = min(16, p.group - 16 * hb), qh0 = kvh * p.group + 16 * hb;
 
     const size_t head_base = static_cast<size_t>(kvh) * p.max_seq * kKv4Row;
     const uint8_t* kh = p.kc + head_base;
     const uint8_t* vh = p.vc + head_base;
-    auto load = [&](int r0, Kd4Tile& t) __attribute__((always_inline)) {
+    // Rows r0.. of the wave up to `end`; the lane's places in a tile are four
+    // offsets, and rows from `end` on read as zeros.
+    const uint32_t ko = n * kKv4Row + 16 * h, kpo = n * kKv4Row + kKv4Params + 4 * h;
+    const uint32_t vo = 4 * h * kKv4Row + 4 * n, vpo = 4 * h * kKv4Row + kKv4Params + 4 * (n >> 2);
+    auto load = [&](int r0, int end, Kd4Tile& t) __attribute__((always_inline)) {
+        const auto k = kv4_rows(kh + static_cast<size_t>(r0) * kKv4Row, min(end - r0, 32));
+        const auto v = kv4_rows(vh + static_cast<size_t>(r0) * kKv4Row, min(end - r0, 32));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint8_t* row = kh + static_cast<size_t>(min(r0 + 16 * i + n, t1 - 1)) * kKv4Row;
-            t.k[i] = *reinterpret_cast<const u32x4*>(row + 16 * h);
-            t.kp[i] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * h);
+            t.k[i] = kv4_load4(k, ko + 16 * i * kKv4Row);
+            t.kp[i] = kv4_load(k, kpo + 16 * i * kKv4Row);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int r = r0 + 16 * (i >> 2) + 4 * h + (i & 3);
-            const uint8_t* row = vh + static_cast<size_t>(min(r, t1 - 1)) * kKv4Row;
-            t.v[i] = *reinterpret_cast<const uint32_t*>(row + 4 * n);
-            t.vp[i] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (n >> 2));
+            t.v[i] = kv4_load(v, vo + (16 * (i >> 2) + (i & 3)) * kKv4Row);
+            t.vp[i] = kv4_load(v, vpo + (16 * (i >> 2) + (i & 3)) * kKv4Row);
         }
     };
+    // The first rows are requested before the position is known: with the shortest
+    // runs they are these.  What lies behind the context is masked, as K by its
+    // scores, as V by zeros.
+    Kd4Tile a;
+    if (WAVES == 4 || wave < 4) load(split * kKd4MinRun + 32 * wave, p.max_seq, a);
     f16x8 qf[4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -119,12 +127,17 @@ __global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Param
         if (n < heads)
             qf[kk] = *reinterpret_cast<const f16x8*>(p.q + static_cast<size_t>(qh0 + n) * kKv4Dim + 32 * h + 8 * kk);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    const int ctx = kd4_context(p, kvh);
+    const int run = kd4_run(ctx, p.splits);
+    const int t0 = split * run, t1 = min(t0 + run, ctx);
+    if (t0 >= t1) return;
     f32x4 acc[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
     float m = -INFINITY, l = 0.0f;
     auto use = [&](int r0, const Kd4Tile& t) __attribute__((always_inline)) {
-        float s[8];
+        float s[8];  // before the scale, which the exponent's multiply-add brings in
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             f32x4 c = {};
@@ -134,32 +147,43 @@ __global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Param
                 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_expand_word(w, t.kp[i]), qf[kk], c, 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = r0 + 16 * i + 4 * h + e;
-                s[4 * i + e] = r < t1 ? c[e] * kScoreScale : -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e) s[4 * i + e] = c[e];
             if constexpr (WEIGHTS) {
                 if (n < heads)  // the row of scores is padded to whole tiles
                     *reinterpret_cast<float4*>(p.scores + static_cast<size_t>(qh0 + n) * p.score_stride + r0 + 16 * i +
-                                               4 * h) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                                               4 * h) = make_float4(c[0], c[1], c[2], c[3]);
             }
+        }
+        if (r0 + 31 >= t1) {  // uniform
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = r0 + 16 * (e >> 2) + 4 * h + (e & 3) < t1 ? s[e] : -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
-        mx = fmaxf(max_over_quarters(mx), m);
-        const float alpha = mx == m ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
-        m = mx;
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        f16x8 pf;
-        float ps = 0.0f;
+        mx = max_over_quarters(mx) * kScoreScale;
+        // the reference value follows the maximum once it has grown by more than 8
+        const bool grow = mx > m + kReferenceLag;
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+            m = grow ? mx : m;
+            l *= alpha;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = __builtin_amdgcn_exp2f(s[e] - ref);
-            ps += x;
-            pf[e] = static_cast<_Float16>(x);
+            for (int dt = 0; dt < 8; ++dt) acc[dt] *= alpha;
         }
-        l = l * alpha + ps;
+        const float neg = m == -INFINITY ? 0.0f : -m;
+        u32x4 pw;
+        float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const f32x2 x = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], kScoreScale, neg)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], kScoreScale, neg))};
+            ps[0] += x.x;
+            ps[1] += x.y;
+            pw[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+        }
+        l += ps[0] + ps[1];
+        const f16x8 pf = __builtin_bit_cast(f16x8, pw);
         // V^T: pairs of rows, all eight dims of the lane's word
         uint32_t vf[8][4];
 #pragma unroll
@@ -179,41 +203,58 @@ __global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Param
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             const u32x4 a = {vf[dt][0], vf[dt][1], vf[dt][2], vf[dt][3]};
-            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), pf, acc[dt] * alpha, 0, 0, 0);
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), pf, acc[dt], 0, 0, 0);
         }
     };
-    Kd4Tile a;
-    for (int r0 = t0 + 32 * wave; r0 < t1; r0 += 32 * kKd4Waves) {
-        load(r0, a);
+    // One copy of the code in a loop, and the other waves to cover its loads: with the
+    // next rows in flight from a second copy it was no faster (a launch runs it a
+    // few times, and has to fetch it first).
+    int r0 = t0 + 32 * wave;
+    if (run != kKd4MinRun && r0 < t1) load(r0, t1, a);
+    while (r0 < t1) {
+        if (r0 + 31 >= t1) {  // uniform; what was requested early may be anything
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = r0 + 16 * (i >> 2) + 4 * h + (i & 3) < t1;
+                a.v[i] = in ? a.v[i] : 0u;
+                a.vp[i] = in ? a.vp[i] : 0u;
+            }
+        }
         use(r0, a);
+        r0 += 32 * WAVES;
+        if (r0 < t1) load(r0, t1, a);
     }
     l = sum_over_quarters(l);
     // the waves meet: common maximum, then outputs
-    __shared__ float s_m[kKd4Waves][16], s_l[kKd4Waves][16];
-    __shared__ float s_o[kKd4Waves][16][kKv4Dim + 4];
-    if (h == 0) {
-        s_m[wave][n] = m;
-        s_l[wave][n] = l;
-    }
+    __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+    extern __shared__ __align__(16) float s_o[];  // [wave][head][128 + 4]
+    constexpr int kRow = kKv4Dim + 4;
+    const int active = min(WAVES, (t1 - t0 + 31) / 32);  // waves that have rows
+    if (wave < active) {
+        if (h == 0) {
+            s_m[wave][n] = m;
+            s_l[wave][n] = l;
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // dims 8 (4 h + i) + dt
-        float* o = &s_o[wave][n][8 * (4 * h + i)];
-        *reinterpret_cast<float4*>(o) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
-        *reinterpret_cast<float4*>(o + 4) = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
+        for (int i = 0; i < 4; ++i) {  // dims 8 (4 h + i) + dt
+            if (n >= heads) break;
+            float* o = &s_o[(wave * heads + n) * kRow + 8 * (4 * h + i)];
+            *reinterpret_cast<float4*>(o) = make_float4(acc[0][i], acc[1][i], acc[2][i], acc[3][i]);
+            *reinterpret_cast<float4*>(o + 4) = make_float4(acc[4][i], acc[5][i], acc[6][i], acc[7][i]);
+        }
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < heads * 32; u += 64 * kKd4Waves) {
+    for (int u = threadIdx.x; u < heads * 32; u += 64 * WAVES) {
         const int head = u >> 5, d = 4 * (u & 31);
         float mg = s_m[0][head];
-#pragma unroll
-        for (int w = 1; w < kKd4Waves; ++w) mg = fmaxf(mg, s_m[w][head]);
+        for (int w = 1; w < active; ++w) mg = fmaxf(mg, s_m[w][head]);
         float lg = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kKd4Waves; ++w) {
+#pragma unroll 4
+        for (int w = 0; w < active; ++w) {
             const float mw = s_m[w][head];
             const float f = mw == mg ? 1.0f : __builtin_amdgcn_exp2f(mw - mg);
-            const float4 x = *reinterpret_cast<const float4*>(&s_o[w][head][d]);
+            const float4 x = *reinterpret_cast<const float4*>(&s_o[(w * heads + head) * kRow + d]);
             lg += f * s_l[w][head];
             o.x += f * x.x;
             o.y += f * x.y;
@@ -228,14 +269,23 @@ __global__ __launch_bounds__(64 * kKd4Waves) void kv4_decode_kernel(Decode4Param
 
 // Weight of every run of one head and the head's sum, by one wave: w = exp2(m - M),
 // L = sum w l.  A NaN sum (a NaN score) makes L NaN.
-__device__ __forceinline__ void kd4_run_weights(const float* ml, int live, int lane, float (&w)[kKd4MaxSplits / 64],
-                                                float& M, float& L) {
+struct Kd4RunSums {
     float2 x[kKd4MaxSplits / 64];
+};
+__device__ __forceinline__ Kd4RunSums kd4_run_sums(const float* ml, int splits, int lane) {
+    Kd4RunSums r;
+#pragma unroll
+    for (int i = 0; i < kKd4MaxSplits / 64; ++i)
+        r.x[i] = *reinterpret_cast<const float2*>(ml + 2 * min(lane + 64 * i, splits - 1));
+    return r;
+}
+__device__ __forceinline__ void kd4_run_weights(Kd4RunSums& r, int live, int lane, float (&w)[kKd4MaxSplits / 64],
+                                                float& M, float& L) {
+    float2(&x)[kKd4MaxSplits / 64] = r.x;
     M = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kKd4MaxSplits / 64; ++i) {
-        const int s = lane + 64 * i;
-        x[i] = s < live ? *reinterpret_cast<const float2*>(ml + 2 * s) : make_float2(-INFINITY, 0.0f);
+        if (lane + 64 * i >= live) x[i] = make_float2(-INFINITY, 0.0f);
         M = fmaxf(M, x[i].x);
     }
     M = qwen::seg_max<64>(M);
@@ -271,7 +321,8 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
         const int run = kd4_run(ctx, p.splits), live = (ctx + run - 1) / run;
         for (int g = wave; g < p.group; g += kKd4MergeThreads / 64) {
             float w[kKd4MaxSplits / 64], M, L;
-            kd4_run_weights(p.part_ml + static_cast<size_t>(kvh * p.group + g) * p.splits * 2, live, lane, w, M, L);
+            Kd4RunSums sums = kd4_run_sums(p.part_ml + static_cast<size_t>(kvh * p.group + g) * p.splits * 2, p.splits, lane);
+            kd4_run_weights(sums, live, lane, w, M, L);
             if (lane == 0) {
                 s_M[g] = M == -INFINITY ? 0.0f : M;
                 s_inv[g] = 1.0f / L;
@@ -282,25 +333,25 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
         const size_t at = static_cast<size_t>(kvh) * p.max_seq + row;
         float sum = 0.0f;
         for (int g = 0; g < p.group; ++g)
-            sum += __builtin_amdgcn_exp2f(p.scores[static_cast<size_t>(kvh * p.group + g) * p.score_stride + row] -
-                                          s_M[g]) * s_inv[g];
+            sum += __builtin_amdgcn_exp2f(__builtin_fmaf(p.scores[static_cast<size_t>(kvh * p.group + g) * p.score_stride + row],
+                                                         kScoreScale, -s_M[g])) * s_inv[g];
         p.w_out[at] = (p.w_in != nullptr && row < kv4_row(p.ctl, p.evicted, kvh) ? p.w_in[at] : 0.0f) + sum;
         return;
     }
     const int qh = blockIdx.x, kvh = qh / p.group;
-    const int ctx = kd4_context(p, kvh);
-    const int run = kd4_run(ctx, p.splits), live = (ctx + run - 1) / run;
     const int d = 4 * (tid & 31), g = tid >> 5;
     const float* po = p.part_o + static_cast<size_t>(qh) * p.splits * kKv4Dim;
     float4 x[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {  // requested before the weights are known
-        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (g + G * i < live) x[i] = *reinterpret_cast<const float4*>(po + static_cast<size_t>(g + G * i) * kKv4Dim + d);
-    }
+    for (int i = 0; i < PER; ++i)  // requested before the context is known; runs without rows are never used
+        if (g + G * i < p.splits) x[i] = *reinterpret_cast<const float4*>(po + static_cast<size_t>(g + G * i) * kKv4Dim + d);
+    Kd4RunSums sums;
+    if (wave == 0) sums = kd4_run_sums(p.part_ml + static_cast<size_t>(qh) * p.splits * 2, p.splits, lane);
+    const int ctx = kd4_context(p, kvh);
+    const int run = kd4_run(ctx, p.splits), live = (ctx + run - 1) / run;
     if (wave == 0) {
         float w[kKd4MaxSplits / 64], M, L;
-        kd4_run_weights(p.part_ml + static_cast<size_t>(qh) * p.splits * 2, live, lane, w, M, L);
+        kd4_run_weights(sums, live, lane, w, M, L);
         const float inv = 1.0f / L;
 #pragma unroll
         for (int i = 0; i < kKd4MaxSplits / 64; ++i) s_w[lane + 64 * i] = w[i] * inv;
@@ -356,10 +407,12 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // before they are expanded.
 constexpr int kP4Keys = 64;
 constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
-constexpr float kP4Lag = 8.0f;  // how far a row's maximum grows before its reference value follows
-constexpr int kP4MinTiles = 4;
-constexpr int kP4MaxSplits = 16;
-typedef float f32x2 __attribute__((ext_vector_type(2)));
+// Tiles of a split, at least, and of the splits beyond the eighth, whose merge costs
+// more: still 2 where a row is merged by 8 groups of lanes, else 8.  (us, 12 q heads, 2 kv
+// heads: 17 tokens at 1200 12.0 with 2 and 14.2 with 4, 509 at 0 16.0 and 18.9; 300
+// at 2000 27.6 with 2 for all, 24.4 with 4.)
+constexpr int kP4MinTiles = 2, kP4FarTiles = 8, kP4FarTilesMany = 2;
+constexpr int kP4MaxSplits = 64;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 struct Prefill4Params {
@@ -374,11 +427,11 @@ struct Prefill4Params {
     float* lse;      // [token][q head] natural log, or NULL
     const float* w_in;
     float* w_out;
-    int T, nq, nkv, group, max_seq, out_stride, splits, row_blocks, block_rows;
+    int T, nq, nkv, group, max_seq, out_stride, splits, row_blocks, block_rows, far_tiles;
 };
 
-__device__ __forceinline__ int p4_live_splits(int tiles, int splits) {
-    return max(1, min(splits, tiles / kP4MinTiles));
+__device__ __forceinline__ int p4_live_splits(const Prefill4Params& p, int tiles) {
+    return max(1, min(p.splits, max(min(tiles / kP4MinTiles, 8), tiles / p.far_tiles)));
 }
 // key tiles of row block rb (the rows of the cache that its last row sees)
 __device__ __forceinline__ int p4_tiles(const Prefill4Params& p, int rb, int base) {
@@ -406,7 +459,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     const int rows = p.T * p.group;
     const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
     const int nt_all = p4_tiles(p, rb, base);
-    const int live = p4_live_splits(nt_all, p.splits);
+    const int live = p4_live_splits(p, nt_all);
     if (split >= live) return;
     const int it0 = static_cast<int>((static_cast<long long>(split) * nt_all) / live);
     const int it1 = static_cast<int>((static_cast<long long>(split + 1) * nt_all) / live);
@@ -449,17 +502,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
             rawp[u] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * sg);
         }
     };
+    // word i of a unit
+    auto expand_word = [&](int u, int i, int kbuf, int vbuf) __attribute__((always_inline)) {
+        const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
+        const uint32_t w = raw[u][i];
+        *reinterpret_cast<f16x8*>(dst[u] + (is_v ? vbuf : kbuf) * kP4TileBytes + 16 * ((4 * sg + i) ^ sswz)) =
+            kv4_expand_word(w, rawp[u]);
+    };
     auto expand = [&](int kbuf, int vbuf) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
-            char* d = dst[u] + (is_v ? vbuf : kbuf) * kP4TileBytes;
+        for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t w = raw[u][i];
-                *reinterpret_cast<f16x8*>(d + 16 * ((4 * sg + i) ^ sswz)) = kv4_expand_word(w, rawp[u]);
-            }
-        }
+            for (int i = 0; i < 4; ++i) expand_word(u, i, kbuf, vbuf);
     };
     auto tile_barrier = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -470,15 +524,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) void*)smem));
     // LDS addresses: K chunk 2 kk + h of row fr; V^T reads (dt: 32 dims, u: rows + 8)
-    uint32_t ka[8], va[4][2];
+    const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ (((fr & 3) << 2) | ((fr >> 2) & 3)));
+    uint32_t va[4][2];
     {
-        const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
-        const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
         const int s16 = lane & 15, b16 = (lane >> 4) & 1;
         const uint32_t v0 = lds0 + 2 * kP4TileBytes + (4 * h + (s16 >> 2)) * 256 +
                             16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
             va[dt][0] = v0 ^ (64 * dt);
@@ -489,7 +540,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     // operand: 16-row quarter i / 4, dims 32 (i % 4)
     auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
         typedef const __attribute__((address_space(3))) f16x8* lptr;
-        return *reinterpret_cast<lptr>(ka[i >> 1] + buf * kP4TileBytes + (i & 1) * 32 * 256);
+        return *reinterpret_cast<lptr>((k0 ^ (32 * (i >> 1))) + buf * kP4TileBytes + (i & 1) * 32 * 256);
     };
     auto read_v = [&](int buf, int i) __attribute__((always_inline)) {
         typedef __attribute__((address_space(3))) s16x4* lptr;
@@ -515,7 +566,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         }
     };
     auto renew_ref = [&](float mx) __attribute__((always_inline)) {
-        const bool grow = mx > mref + kP4Lag;
+        const bool grow = mx > mref + kReferenceLag;
         if (__builtin_amdgcn_ballot_w64(grow) != 0) {
             const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
             mref = grow ? mx : mref;
@@ -545,7 +596,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]));  // here, not past the mask's branch
         return w;
     };
-    constexpr int AHEAD = 4;  // operand reads in flight before their MFMA
+    constexpr int AHEAD = 3;  // operand reads in flight before their MFMA
     // Scores of the K tile in `buf`; beside them, when EXP, the probabilities of
     // the scores `cur`, each MFMA fenced together with its share of the vector work.
     auto scores = [&](auto exp_too, int buf, f32x16 (&sc)[2], const f32x16 (&cur)[2],
@@ -565,8 +616,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         }
         if constexpr (decltype(exp_too)::value) lsum += ps[0] + ps[1];
     };
-    // O^T += V^T . P^T; beside it, when MAX, the (scaled) row maximum of nxt
-    auto add_pv = [&](auto max_too, const uint32_t (&pw)[2][8], int buf,
+    // O^T += V^T . P^T; beside it, when MORE, the (scaled) row maximum of nxt, and
+    // the tiles in registers go to LDS, K to buffer buf and V to the other
+    auto add_pv = [&](auto more, const uint32_t (&pw)[2][8], int buf,
                       const f32x16 (&nxt)[2]) __attribute__((always_inline)) {
         f16x8 vf[AHEAD];
 #pragma unroll
@@ -578,16 +630,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
             const u32x4 pf = {pw[j][4 * ks], pw[j][4 * ks + 1], pw[j][4 * ks + 2], pw[j][4 * ks + 3]};
             acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % AHEAD], __builtin_bit_cast(f16x8, pf), acc[dt], 0, 0, 0);
             if (i + AHEAD < 16) vf[i % AHEAD] = read_v(buf, i + AHEAD);
-            if constexpr (decltype(max_too)::value)
+            if constexpr (decltype(more)::value) {
                 mx = fmaxf(fmaxf(mx, nxt[j][2 * (i & 7)]), nxt[j][2 * (i & 7) + 1]);
+                if (UNITS == 2 && (i & 1) == 0) expand_word(i >> 3, (i >> 1) & 3, buf, buf ^ 1);
+                if (UNITS == 1 && (i & 3) == 0) expand_word(0, i >> 2, buf, buf ^ 1);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        return decltype(max_too)::value ? xor32_max(mx) * kScoreScale : 0.0f;
+        return decltype(more)::value ? xor32_max(mx) * kScoreScale : 0.0f;
     };
     typedef std::true_type yes;
     typedef std::false_type no;
-    // what a step does for everyone: K of the tile after next and V of the next
-    // go to LDS (b: parity of tile t), the raw bytes behind them are requested
+    // What a step does for everyone: K of the tile after next and V of the next
+    // go to LDS (b: parity of tile t), the raw bytes behind them are requested.
     auto stage = [&](int t, int b) __attribute__((always_inline)) {
         expand(b, b ^ 1);
         fetch(t + 3, t + 2);
@@ -596,10 +651,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     // probabilities of t, then V of t beside the next tile's maximum.
     auto step = [&](int t, int b, f32x16 (&cur)[2], f32x16 (&nxt)[2]) __attribute__((always_inline)) {
         uint32_t pw[2][8];
-        stage(t, b);
         scores(yes{}, b ^ 1, nxt, cur, pw);
         mask(t + 1, nxt);
         const float mx = add_pv(yes{}, pw, b, nxt);
+        fetch(t + 3, t + 2);
         renew_ref(mx);
         tile_barrier();
     };
@@ -684,44 +739,72 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
                 make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
 }
 
-// Merges the splits of every row: 32 lanes a row (4 dims each), 8 rows a block.
-// Rows whose block had one split are already written.
+// Merges the splits of every row: GROUPS groups of 32 lanes (4 dims each) a row, a
+// group takes every GROUPS-th split.  One group, eight rows a block; 8 groups and a
+// sum through LDS for few rows with more than 8 splits, where what counts is how many
+// rounds of loads a row waits for (17 rows at 20000, 64 splits: 23.0 -> 19.0 us in
+// all; with 6000 rows they cost more).  Rows whose block had one split are already
+// written.
+constexpr int kP4MergeMany = 8;
+template <int GROUPS>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p) {
+    static_assert(kP4MaxSplits <= 64, "two splits a lane");
+    __shared__ __align__(16) float s_o[GROUPS == 1 ? 1 : GROUPS][kKv4Dim];
     const int rows = p.T * p.group;
-    const int s_lane = threadIdx.x & 31, d = 4 * s_lane;
+    const int lane = threadIdx.x & 31, g32 = threadIdx.x >> 5, d = 4 * lane;
+    const int g = GROUPS == 1 ? 0 : g32;
     const long long all = static_cast<long long>(rows) * p.nkv;
-    const long long i = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const long long i = GROUPS == 1 ? static_cast<long long>(blockIdx.x) * 8 + g32 : static_cast<long long>(blockIdx.x);
     if (i >= all) return;
     const int kvh = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<long long>(kvh) * rows);
     const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
-    const int live = p4_live_splits(p4_tiles(p, r / p.block_rows, base), p.splits);
-    if (live == 1) return;
+    const int live = p4_live_splits(p, p4_tiles(p, r / p.block_rows, base));
+    if (live == 1) return;  // (with several groups the block has one row: all of it)
     constexpr int B = 8;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (s_lane < live) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (s_lane * all + i));
     float4 v[B];
     auto request = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < B; ++b)
-            v[b] = *reinterpret_cast<const float4*>(p.part_o + (min(s0 + b, live - 1) * all + i) * kKv4Dim + d);
+            v[b] = *reinterpret_cast<const float4*>(p.part_o + (min(s0 + GROUPS * b, live - 1) * all + i) * kKv4Dim + d);
     };
-    request(0);
-    const float m = qwen::seg_max<32>(ml.x);
-    // (a split whose scores are all NaN has no maximum and a NaN sum, which the product below keeps)
-    const float w_lane = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
-    float l = 0.0f;
+    request(g);
+    float2 ml[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        if (lane + 32 * k < live) ml[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((lane + 32 * k) * all + i));
+    }
+    const float m = qwen::seg_max<32>(fmaxf(ml[0].x, ml[1].x));
+    // (a split whose scores are all NaN has no maximum and a NaN sum, which the products below keep)
+    float w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) w[k] = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
+    const float l = qwen::seg_sum<32>(w[0] * ml[0].y + w[1] * ml[1].y);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < live; s0 += B) {
-        if (s0 > 0) request(s0);
+    for (int s0 = g; s0 < live; s0 += GROUPS * B) {
+        if (s0 > g) request(s0);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            if (s0 + b >= live) break;
-            const float w = __shfl(w_lane, s0 + b, 32);
-            l += w * __shfl(ml.y, s0 + b, 32);
-            o.x += w * v[b].x;
-            o.y += w * v[b].y;
-            o.z += w * v[b].z;
-            o.w += w * v[b].w;
+            const int s = s0 + GROUPS * b;
+            const float ws = __shfl(s < 32 ? w[0] : w[1], s & 31, 32);
+            if (s >= live) continue;
+            o.x += ws * v[b].x;
+            o.y += ws * v[b].y;
+            o.z += ws * v[b].z;
+            o.w += ws * v[b].w;
+        }
+    }
+    if constexpr (GROUPS > 1) {
+        *reinterpret_cast<float4*>(&s_o[g][d]) = o;
+        __syncthreads();
+        if (g != 0) return;
+#pragma unroll
+        for (int k = 1; k < GROUPS; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(&s_o[k][d]);
+            o.x += x.x;
+            o.y += x.y;
+            o.z += x.z;
+            o.w += x.w;
         }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -730,7 +813,7 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p
     *reinterpret_cast<uint2*>(dst) =
         make_uint2(static_cast<uint32_t>(f2h(o.x * inv)) | (static_cast<uint32_t>(f2h(o.y * inv)) << 16),
                    static_cast<uint32_t>(f2h(o.z * inv)) | (static_cast<uint32_t>(f2h(o.w * inv)) << 16));
-    if (p.lse != nullptr && s_lane == 0)
+    if (p.lse != nullptr && lane == 0)
         p.lse[static_cast<size_t>(qi) * p.nq + qh] = (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
 }
 
@@ -918,9 +1001,10 @@ extern "C" int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const
     p.head_blocks = (p.group + 15) / 16;
     p.max_seq = max_seq_len;
     p.score_stride = score_stride(max_seq_len);
-    // two blocks per CU, and no more runs than the cache can fill
+    // Two blocks per CU, and no more runs than the cache can fill.
     const long long units = static_cast<long long>(num_kv_heads) * p.head_blocks;
     p.splits = static_cast<int>(std::max(8LL, std::min<long long>(kKd4MaxSplits, 2LL * cu_count() / units)));
+    p.waves = max_seq_len > static_cast<long long>(kKd4MinRun) * p.splits ? kKd4ManyWaves : 4;
     p.splits = std::min(p.splits, (max_seq_len - 1) / kKd4MinRun + 1);
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + static_cast<size_t>(num_q_heads) * kKd4MaxSplits * kKv4Dim;
@@ -929,11 +1013,15 @@ extern "C" int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const
     const long long weight_blocks =
         static_cast<long long>(num_kv_heads) * ((static_cast<long long>(max_seq_len) + kKd4MergeThreads - 1) / kKd4MergeThreads);
     QE_REQUIRE(blocks <= INT32_MAX && weight_blocks + num_q_heads <= INT32_MAX, "%s: too many heads", what);
+    const unsigned grid = static_cast<unsigned>(blocks), threads = 64 * p.waves;
+    const size_t lds = static_cast<size_t>(p.waves) * std::min(16, p.group) * (kKv4Dim + 4) * sizeof(float);
     if (key_weights_out != nullptr) {
-        kv4_decode_kernel<true><<<static_cast<unsigned>(blocks), 64 * kKd4Waves, 0, stream>>>(p);
+        if (p.waves == 4) kv4_decode_kernel<true, 4><<<grid, threads, lds, stream>>>(p);
+        else kv4_decode_kernel<true, kKd4ManyWaves><<<grid, threads, lds, stream>>>(p);
         kv4_decode_merge_kernel<true><<<static_cast<unsigned>(num_q_heads + weight_blocks), kKd4MergeThreads, 0, stream>>>(p);
     } else {
-        kv4_decode_kernel<false><<<static_cast<unsigned>(blocks), 64 * kKd4Waves, 0, stream>>>(p);
+        if (p.waves == 4) kv4_decode_kernel<false, 4><<<grid, threads, lds, stream>>>(p);
+        else kv4_decode_kernel<false, kKd4ManyWaves><<<grid, threads, lds, stream>>>(p);
         kv4_decode_merge_kernel<false><<<static_cast<unsigned>(num_q_heads), kKd4MergeThreads, 0, stream>>>(p);
     }
     return check_launch(what);
@@ -975,7 +1063,12 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     const long long rows = static_cast<long long>(num_tokens) * p.group;
     QE_REQUIRE(rows <= (1 << 29) && max_seq_len <= (1 << 29), "%s: num_tokens=%d max_seq_len=%d", what, num_tokens,
                max_seq_len);
-    const int waves = rows <= 128 ? 4 : 8;
+    // Eight waves and one block per CU expand a tile for 256 rows; four waves for
+    // 128, two blocks per CU, where there are few row blocks: their splits are shorter and
+    // fewer rows idle.  (12 q heads, 2 kv heads, all in us: 40 tokens at 1200 19.0 against
+    // 15.2, 509 at 0 24.2 against 18.8; 1000 at 2900 43.8 against 46.0, 1024 at 15000 122
+    // against 132.)
+    const int waves = (rows + 255) / 256 * num_kv_heads >= 32 ? 8 : 4;
     p.block_rows = 32 * waves;
     p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
     const long long blocks = static_cast<long long>(p.row_blocks) * num_kv_heads;
@@ -986,6 +1079,8 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     const StreamWorkspace ws = lease.ws;
     const long long part = rows * num_kv_heads * (kKv4Dim + 2);  // floats of one split
     const long long slots = waves == 4 ? 2LL * cus : cus;
+    const bool few_rows = rows * num_kv_heads <= 2048;
+    p.far_tiles = few_rows ? kP4FarTilesMany : kP4FarTiles;
     p.splits = 1;
     if (ws.ptr != nullptr && max_seq_len >= 16 * kP4Keys)
         p.splits = static_cast<int>(std::max(1LL, std::min({static_cast<long long>(kP4MaxSplits), slots / blocks,
@@ -999,8 +1094,10 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     const unsigned grid = static_cast<unsigned>(blocks * p.splits);
     if (waves == 4) kv4_prefill_kernel<4><<<grid, 256, 0, stream>>>(p);
     else kv4_prefill_kernel<8><<<grid, 512, 0, stream>>>(p);
-    if (p.splits > 1)
-        kv4_prefill_merge_kernel<<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
+    if (p.splits > 8 && few_rows)
+        kv4_prefill_merge_kernel<kP4MergeMany><<<static_cast<unsigned>(rows * num_kv_heads), 256, 0, stream>>>(p);
+    else if (p.splits > 1)
+        kv4_prefill_merge_kernel<1><<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
     if (key_weights_out != nullptr) {
         const long long tiles = (static_cast<long long>(max_seq_len) + kW4Keys - 1) / kW4Keys;
         QE_REQUIRE(tiles * num_kv_heads <= INT32_MAX, "%s: max_seq_len=%d", what, max_seq_len);

@@ -39,9 +39,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ void kv4_expand(uint32_t t, f16x2 scale, f16x2 low, f16x2 (&out)[4]) {
     const f16x2 b1 = {(_Float16)-1024.0f, (_Float16)-1024.0f};
     const f16x2 r16 = {(_Float16)0.0625f, (_Float16)0.0625f}, b16 = {(_Float16)-64.0f, (_Float16)-64.0f};
+    // masks and bias in registers: as literals they would make the and and the or two instructions
+    uint32_t even = 0x000F000Fu, odd = 0x00F000F0u, bias = 0x64006400u;
+    asm("" : "+s"(even));
+    asm("" : "+s"(odd));
+    asm("" : "+v"(bias));
     const uint32_t t8 = t >> 8;
-    const uint32_t u[4] = {(t & 0x000F000Fu) | 0x64006400u, (t & 0x00F000F0u) | 0x64006400u,
-                           (t8 & 0x000F000Fu) | 0x64006400u, (t8 & 0x00F000F0u) | 0x64006400u};
+    const uint32_t u[4] = {(t & even) | bias, (t & odd) | bias, (t8 & even) | bias, (t8 & odd) | bias};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const f16x2 x = __builtin_bit_cast(f16x2, u[i]);
@@ -57,6 +61,23 @@ __device__ __forceinline__ f16x8 kv4_expand_word(uint32_t w, uint32_t param) {
     f16x2 o[4];
     kv4_expand(w, __builtin_bit_cast(f16x2, s), __builtin_bit_cast(f16x2, l), o);
     return f16x8{o[0].x, o[0].y, o[1].x, o[1].y, o[2].x, o[2].y, o[3].x, o[3].y};
+}
+
+// `rows` rows of a cache from `first` on, for loads by byte offset: what lies
+// behind them reads as zeros, whose value is 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv4_rows(const uint8_t* first, int rows) {
+    // (both are the same in every lane; said again, or each load becomes a loop over lanes)
+    const uintptr_t at = reinterpret_cast<uintptr_t>(first);
+    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32)));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<uint8_t*>(lo | (hi << 32)), 0,
+                                             __builtin_amdgcn_readfirstlane(max(rows, 0) * kKv4Row), 0x00027000);
+}
+__device__ __forceinline__ uint32_t kv4_load(__amdgpu_buffer_rsrc_t rows, uint32_t offset) {
+    return __builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, 0);
+}
+__device__ __forceinline__ u32x4 kv4_load4(__amdgpu_buffer_rsrc_t rows, uint32_t offset) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
 }
 
 // Cache row of position seq_pos for kv head h: the positions before it, less

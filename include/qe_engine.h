@@ -11,7 +11,9 @@
  * qe_set_tuning("engine_tiled_prefill", 0) was set before create, a tiled
  * copy of every layer matrix for the prefill GEMMs (+0.75 GB at
  * Qwen2.5-1.5B: about 0.8x the layer weights).  The switch is read once at
- * create.  qe_engine_arena_spans reports the arena's size.  Prefill in chunks
+ * create, and so is "engine_kv4": set to 1 before create, the engine's K and V
+ * caches hold 4-bit rows (QE_KV4_ROW_BYTES, include/qe_kernels.h) and every layer
+ * appends to and attends over them.  qe_engine_arena_spans reports the arena's size.  Prefill in chunks
  * of another size, and with qe_set_tuning("gemm_split_k", 0) (neither GEMMs nor
  * attention split), may differ in the order of fp32 sums.
  *
@@ -99,7 +101,9 @@ int qe_engine_read_hidden(qe_engine* e, uint16_t* host, int n);
 
 /* Synchronize and copy the first `bytes` of a named engine buffer to host
  * memory: "logits", "hidden", "q8", "q8_scale", "q8_sum8", "embed_w",
- * "embed_s", "lm_head_w", "lm_head_s", "final_norm", "control", or a layer
+ * "embed_s", "lm_head_w", "lm_head_s", "final_norm", "control", "kcache", "vcache"
+ * ([layer][kv head][max_seq_len] rows of 128 fp16 or, with engine_kv4,
+ * QE_KV4_ROW_BYTES bytes), or a layer
  * tensor "layer<l>.<t>" with t one of ln1 ln2 q_w q_s k_w k_s v_w v_s o_w o_s
  * gate_up_w gate_up_s down_w down_s q_bias k_bias v_bias. */
 int qe_engine_read_buffer(qe_engine* e, const char* name, void* host, size_t bytes);

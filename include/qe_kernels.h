@@ -568,7 +568,9 @@ int qe_stream_read(const void* data, size_t bytes, uint32_t* sink, hipStream_t s
  *   largest decode GEMV grid; larger row counts loop over row sets;
  *   "engine_tiled_prefill" 0/1 (default 1) - engines created afterwards keep
  *   a tiled copy of every layer matrix (qe_repack_w4_tiled) for their prefill
- *   GEMMs (about 0.75 GB more for Qwen2.5-1.5B; same results).
+ *   GEMMs (about 0.75 GB more for Qwen2.5-1.5B; same results);
+ *   "engine_kv4" 0/1 (default 0) - engines created afterwards hold their K and V
+ *   caches in 4 bits (the format above), 3.2 times smaller.
  *   Returns QE_ERR_INVALID_ARGUMENT for an unknown key or value. */
 int qe_set_tuning(const char* key, int value);
 

@@ -72,6 +72,11 @@ struct Layer {
     Mat tq, tk, tv, to, tgate_up, tdown;  // tiled copies for the prefill GEMMs (qe_repack_w4_tiled)
 };
 
+// bytes of a K or V row of one head
+inline size_t kv_row_bytes(const qe_engine_config& c, bool kv4) {
+    return kv4 ? static_cast<size_t>(QE_KV4_ROW_BYTES) : static_cast<size_t>(c.head_dim) * 2;
+}
+
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 }  // namespace
@@ -95,7 +100,7 @@ struct qe_engine {
     int32_t* q8_sum8 = nullptr;
     float *part_o = nullptr, *part_lse = nullptr, *sample_val = nullptr;
     int32_t *sample_idx = nullptr, *tokens = nullptr;
-    uint16_t *kcache = nullptr, *vcache = nullptr;
+    uint8_t *kcache = nullptr, *vcache = nullptr;
     qe_device_control_block* ctl = nullptr;
     int32_t* h_token = nullptr;  // mapped pinned
     int32_t* d_token = nullptr;
@@ -104,6 +109,8 @@ struct qe_engine {
     int seq_pos = 0;
     bool tiled = false;        // prefill GEMMs read the tiled copies
     bool want_tiled = false;   // engine_tiled_prefill, read once at create
+    bool kv4 = false;          // engine_kv4, read once at create: the caches hold 4-bit rows
+    void* kv4_ws = nullptr;    // decode workspace of the 4-bit cache
     float* gemm_ws = nullptr;  // split workspace of the engine's stream (in the arena)
 
     std::vector<std::pair<size_t, size_t>> spans;  // (offset, bytes) of every buffer taken
@@ -114,7 +121,10 @@ struct qe_engine {
         spans.emplace_back(off, bytes);
         return reinterpret_cast<T*>(arena + off);
     }
-    size_t kv_stride() const { return static_cast<size_t>(cfg.num_kv_heads) * cfg.max_seq_len * cfg.head_dim; }
+    // bytes of one layer's K or V cache
+    size_t kv_stride() const {
+        return static_cast<size_t>(cfg.num_kv_heads) * cfg.max_seq_len * qe::kv_row_bytes(cfg, kv4);
+    }
 };
 
 namespace qe {
@@ -188,10 +198,12 @@ int decode_pass(qe_engine* e, Timer* t) {
     QE_TRY(mark(e, t, 2));
     for (int l = 0; l < c.num_layers; ++l) {
         const Layer& L = e->layers[l];
-        uint16_t* kc = e->kcache + l * e->kv_stride();
-        uint16_t* vc = e->vcache + l * e->kv_stride();
+        uint8_t* const kc4 = e->kcache + l * e->kv_stride();
+        uint8_t* const vc4 = e->vcache + l * e->kv_stride();
+        uint16_t* const kc = reinterpret_cast<uint16_t*>(kc4);
+        uint16_t* const vc = reinterpret_cast<uint16_t*>(vc4);
         const qe_qkv_view view = view_of(e, L, e->dq, e->dk, e->dv);
-        if (c.fused_decode && H <= 3072) {  // RMSNorm + QKV + bias + RoPE + KV append in one launch
+        if (c.fused_decode && H <= 3072 && !e->kv4) {  // RMSNorm + QKV + bias + RoPE + KV append in one launch
             QE_TRY(qe_launch_rmsnorm_gemv_qkv_rope_kv_append_w4a16(e->act0, L.ln1, nullptr, &view, L.q_bias, L.k_bias,
                                                                    L.v_bias, kc, vc, e->ctl, s, H, c.num_q_heads,
                                                                    c.num_kv_heads, c.head_dim, c.max_seq_len,
@@ -207,12 +219,24 @@ int decode_pass(qe_engine* e, Timer* t) {
                                                c.num_kv_heads, c.head_dim));
             }
             QE_TRY(mark(e, t, 0));
-            QE_TRY(qe_launch_qkv_bias_rope_kv_append(e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc, vc, e->ctl,
-                                                     1, s, c.num_q_heads, c.num_kv_heads, c.head_dim, c.max_seq_len,
-                                                     c.head_dim, c.rope_theta));
+            if (e->kv4)
+                QE_TRY(qe_launch_qkv_bias_rope_kv4_append(e->dq, e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc4,
+                                                          vc4, e->ctl, nullptr, 1, s, c.num_q_heads, c.num_kv_heads,
+                                                          c.head_dim, c.max_seq_len, c.head_dim, c.rope_theta));
+            else
+                QE_TRY(qe_launch_qkv_bias_rope_kv_append(e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc, vc,
+                                                         e->ctl, 1, s, c.num_q_heads, c.num_kv_heads, c.head_dim,
+                                                         c.max_seq_len, c.head_dim, c.rope_theta));
             QE_TRY(mark(e, t, 2));
         }
-        if (c.fused_decode && c.num_q_heads * c.head_dim <= 2048) {  // split partials, then combine + O
+        if (e->kv4) {
+            QE_TRY(qe_launch_attention_gqa_flash_decode_kv4(e->dq, kc4, vc4, e->kv4_ws, e->attn, e->ctl, nullptr, s,
+                                                            c.num_q_heads, c.num_kv_heads, c.head_dim, c.max_seq_len,
+                                                            e->q8, e->q8_scale, e->q8_sum8, nullptr, nullptr));
+            QE_TRY(mark(e, t, 1));
+            QE_TRY(qe_launch_gemv_w4a8(L.o.w, L.o.s, e->q8, e->q8_scale, e->q8_sum8, e->act0, e->act0, H,
+                                       c.num_q_heads * c.head_dim, s));
+        } else if (c.fused_decode && c.num_q_heads * c.head_dim <= 2048) {  // split partials, then combine + O
             QE_TRY(qe_launch_attention_gqa_flash_decode_partials(e->dq, kc, vc, e->part_o, e->part_lse, e->ctl, s,
                                                                  c.num_q_heads, c.num_kv_heads, c.head_dim,
                                                                  c.max_seq_len));
@@ -269,8 +293,10 @@ int prefill_chunk(qe_engine* e, int start, int len) {
     QE_TRY(qe_launch_embed_lookup_w4a16(e->embed.w, e->embed.s, e->tokens + start, e->act0, nullptr, len, s, H));
     for (int l = 0; l < c.num_layers; ++l) {
         const Layer& L = e->layers[l];
-        uint16_t* kc = e->kcache + l * e->kv_stride();
-        uint16_t* vc = e->vcache + l * e->kv_stride();
+        uint8_t* const kc4 = e->kcache + l * e->kv_stride();
+        uint8_t* const vc4 = e->vcache + l * e->kv_stride();
+        uint16_t* const kc = reinterpret_cast<uint16_t*>(kc4);
+        uint16_t* const vc = reinterpret_cast<uint16_t*>(vc4);
         QE_TRY(qe_launch_rmsnorm_fp16(e->act0, L.ln1, e->act1, len, s, H));
         if (e->tiled) {
             const qe_qkv_view tv{L.tq.w, L.tq.s, e->dq, L.tk.w, L.tk.s, e->dk, L.tv.w, L.tv.s, e->dv};
@@ -281,11 +307,20 @@ int prefill_chunk(qe_engine* e, int start, int len) {
             QE_TRY(qe_launch_gemm_prefill_qkv_w4a16(&view, e->act1, len, s, H, c.num_q_heads, c.num_kv_heads,
                                                     c.head_dim, 0));
         }
-        QE_TRY(qe_launch_qkv_bias_rope_kv_append(e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc, vc, e->ctl,
-                                                 len, s, c.num_q_heads, c.num_kv_heads, c.head_dim, c.max_seq_len,
-                                                 c.head_dim, c.rope_theta));
-        QE_TRY(launch_prefill_attention(e->dq, kc, vc, e->attn, e->ctl, len, s, c.num_q_heads, c.num_kv_heads,
-                                        c.head_dim, c.max_seq_len, c.num_q_heads * c.head_dim, start + len));
+        if (e->kv4) {
+            QE_TRY(qe_launch_qkv_bias_rope_kv4_append(e->dq, e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc4, vc4,
+                                                      e->ctl, nullptr, len, s, c.num_q_heads, c.num_kv_heads,
+                                                      c.head_dim, c.max_seq_len, c.head_dim, c.rope_theta));
+            QE_TRY(qe_launch_attention_gqa_prefill_kv4(e->dq, kc4, vc4, e->attn, e->ctl, nullptr, len, s, c.num_q_heads,
+                                                       c.num_kv_heads, c.head_dim, c.max_seq_len,
+                                                       c.num_q_heads * c.head_dim, nullptr, nullptr, nullptr));
+        } else {
+            QE_TRY(qe_launch_qkv_bias_rope_kv_append(e->dq, e->dk, e->dv, L.q_bias, L.k_bias, L.v_bias, kc, vc, e->ctl,
+                                                     len, s, c.num_q_heads, c.num_kv_heads, c.head_dim, c.max_seq_len,
+                                                     c.head_dim, c.rope_theta));
+            QE_TRY(launch_prefill_attention(e->dq, kc, vc, e->attn, e->ctl, len, s, c.num_q_heads, c.num_kv_heads,
+                                            c.head_dim, c.max_seq_len, c.num_q_heads * c.head_dim, start + len));
+        }
         const int qd = c.num_q_heads * c.head_dim;
         if (e->tiled) {
             QE_TRY(qe_launch_gemm_prefill_w4a16_tiled(L.to.w, L.to.s, e->attn, e->act0, e->act0, len, H, qd, s));
@@ -428,10 +463,18 @@ int q8_len(const qe_engine_config& c) {
 // engine's stream with qe_gemm_attach_workspace, released at destroy).
 constexpr size_t kEngineGemmWsBytes = size_t(32) << 20;
 
-size_t workspace_bytes(const qe_engine_config& c, bool want_tiled) {
+// Bytes of the decode workspace on a 4-bit cache (0 on an fp16 one).
+size_t kv4_workspace_bytes(const qe_engine_config& c, bool kv4) {
+    size_t bytes = 0;
+    if (kv4 && qe_kv4_decode_workspace_bytes(c.num_q_heads, c.max_seq_len, 0, &bytes) != QE_OK) return 0;
+    return bytes;
+}
+
+size_t workspace_bytes(const qe_engine_config& c, bool want_tiled, bool kv4) {
     const int H = c.hidden_size, I = c.intermediate_size, qd = c.num_q_heads * c.head_dim,
               kvd = c.num_kv_heads * c.head_dim, T = c.prefill_chunk, QN = q8_len(c);
-    size_t bytes = 2 * align256(static_cast<size_t>(c.num_layers) * c.num_kv_heads * c.max_seq_len * c.head_dim * 2);
+    size_t bytes = 2 * align256(static_cast<size_t>(c.num_layers) * c.num_kv_heads * c.max_seq_len * kv_row_bytes(c, kv4)) +
+                   align256(kv4_workspace_bytes(c, kv4));
     bytes += 2 * align256(static_cast<size_t>(T) * H * 2) + align256(static_cast<size_t>(T) * qd * 2) +
              2 * align256(static_cast<size_t>(T) * kvd * 2) + align256(static_cast<size_t>(T) * qd * 2) +
              align256(static_cast<size_t>(T) * I * 2) + align256(static_cast<size_t>(c.vocab_size) * 2);
@@ -442,9 +485,10 @@ size_t workspace_bytes(const qe_engine_config& c, bool want_tiled) {
     return bytes + tiled_bytes(c, want_tiled);
 }
 
-int begin_engine(qe_engine* e, const qe_engine_config& c, bool want_tiled, size_t arena_bytes) {
+int begin_engine(qe_engine* e, const qe_engine_config& c, bool want_tiled, bool kv4, size_t arena_bytes) {
     e->cfg = c;
     e->want_tiled = want_tiled;
+    e->kv4 = kv4;
     QE_HIP(hipStreamCreate(&e->stream));
     QE_HIP(hipMalloc(&e->arena, arena_bytes));
     e->arena_size = arena_bytes;
@@ -457,9 +501,10 @@ void layout_workspace(qe_engine* e) {
     const qe_engine_config& c = e->cfg;
     const int H = c.hidden_size, I = c.intermediate_size, qd = c.num_q_heads * c.head_dim,
               kvd = c.num_kv_heads * c.head_dim, T = c.prefill_chunk, QN = q8_len(c);
-    const size_t kvb = static_cast<size_t>(c.num_layers) * e->kv_stride() * 2;
-    e->kcache = e->take<uint16_t>(kvb);
-    e->vcache = e->take<uint16_t>(kvb);
+    const size_t kvb = static_cast<size_t>(c.num_layers) * e->kv_stride();
+    e->kcache = e->take<uint8_t>(kvb);
+    e->vcache = e->take<uint8_t>(kvb);
+    if (e->kv4) e->kv4_ws = e->take<char>(kv4_workspace_bytes(c, true));
     e->act0 = e->take<uint16_t>(static_cast<size_t>(T) * H * 2);
     e->act1 = e->take<uint16_t>(static_cast<size_t>(T) * H * 2);
     e->dq = e->take<uint16_t>(static_cast<size_t>(T) * qd * 2);
@@ -487,7 +532,7 @@ int finish_engine(qe_engine* e) {
                e->arena_size);
     QE_TRY(qe_gemm_attach_workspace(e->stream, e->gemm_ws, kEngineGemmWsBytes));
     (void)cu_count();  // cache the device fact before graph capture
-    const size_t kvb = static_cast<size_t>(e->cfg.num_layers) * e->kv_stride() * 2;
+    const size_t kvb = static_cast<size_t>(e->cfg.num_layers) * e->kv_stride();
     QE_HIP(hipMemsetAsync(e->kcache, 0, kvb, e->stream));
     QE_HIP(hipMemsetAsync(e->vcache, 0, kvb, e->stream));
     const qe_device_control_block init = {0, 0, 0.0f, 0, 1337ull};
@@ -505,8 +550,8 @@ extern "C" int qe_engine_create(const qe_engine_config* cfg, uint64_t seed, qe_e
     const qe_engine_config& c = *cfg;
     QE_REQUIRE(config_ok(c), "engine_create: unsupported configuration");
     std::unique_ptr<qe_engine, void (*)(qe_engine*)> e(new qe_engine(), qe_engine_destroy);
-    const bool want_tiled = engine_tiled_prefill() != 0;
-    QE_TRY(begin_engine(e.get(), c, want_tiled, weight_bytes(c) + workspace_bytes(c, want_tiled)));
+    const bool want_tiled = engine_tiled_prefill() != 0, kv4 = engine_kv4() != 0;
+    QE_TRY(begin_engine(e.get(), c, want_tiled, kv4, weight_bytes(c) + workspace_bytes(c, want_tiled, kv4)));
     const int H = c.hidden_size, I = c.intermediate_size, qd = c.num_q_heads * c.head_dim,
               kvd = c.num_kv_heads * c.head_dim;
     // layout first, then check, then initialize
@@ -575,8 +620,8 @@ extern "C" int qe_engine_create_from_qwenbin(const char* path, int max_seq_len, 
     c.fused_decode = fused_decode;
     QE_REQUIRE(config_ok(c), "engine_create_from_qwenbin: unsupported configuration");
     std::unique_ptr<qe_engine, void (*)(qe_engine*)> e(new qe_engine(), qe_engine_destroy);
-    const bool want_tiled = engine_tiled_prefill() != 0;
-    QE_TRY(begin_engine(e.get(), c, want_tiled, workspace_bytes(c, want_tiled)));
+    const bool want_tiled = engine_tiled_prefill() != 0, kv4 = engine_kv4() != 0;
+    QE_TRY(begin_engine(e.get(), c, want_tiled, kv4, workspace_bytes(c, want_tiled, kv4)));
     // one device copy of the payload [weights_offset, end of file) (src/engine.cu:271-272)
     QE_HIP(hipMalloc(&e->payload, std::max<uint64_t>(in.weights_bytes, 256)));
     QE_HIP(hipMemcpy(e->payload, file.data() + in.weights_offset, in.weights_bytes, hipMemcpyHostToDevice));
@@ -836,6 +881,8 @@ extern "C" int qe_engine_read_buffer(qe_engine* e, const char* name, void* host,
         {"lm_head_s", e->lm.s, static_cast<size_t>(c.vocab_size) * (c.hidden_size / 128) * 2},
         {"final_norm", e->final_norm, static_cast<size_t>(c.hidden_size) * 2},
         {"control", e->ctl, sizeof(qe_device_control_block)},
+        {"kcache", e->kcache, static_cast<size_t>(c.num_layers) * e->kv_stride()},
+        {"vcache", e->vcache, static_cast<size_t>(c.num_layers) * e->kv_stride()},
     };
     // "layer<l>.<tensor>" and the LM head
     int l = -1;

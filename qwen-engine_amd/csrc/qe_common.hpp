@@ -32,6 +32,7 @@ int gemm_staged_only();    // automatic plans keep to the register-staged tiles 
 int gemm_ks2_mode();       // 0 auto, 1 never, 2 always (K % 256 == 0): the two-group k split
 int gemv_forced_bt();      // 0 auto, else GEMV block size (256, 512, 1024)
 int gemv_forced_cap();     // 0 auto, else the largest GEMV grid (larger grids loop over row sets)
+int engine_kv4();            // engines created from now on hold their K and V caches in 4 bits (default 0)
 int engine_tiled_prefill();  // engines created from now on keep tiled copies for the prefill GEMMs (default 1)
 
 // The split workspace registered for a stream (qe_gemm_reserve_workspace /

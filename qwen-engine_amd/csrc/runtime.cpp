@@ -22,6 +22,7 @@ int g_gemm_ks2 = 0;
 int g_gemv_bt = 0;
 int g_gemv_cap = 0;
 int g_engine_tiled = 1;
+int g_engine_kv4 = 0;
 }  // namespace
 
 int gemm_split_k_enabled() { return g_gemm_split_k; }
@@ -32,6 +33,7 @@ int gemm_ks2_mode() { return g_gemm_ks2; }
 int gemv_forced_bt() { return g_gemv_bt; }
 int gemv_forced_cap() { return g_gemv_cap; }
 int engine_tiled_prefill() { return g_engine_tiled; }
+int engine_kv4() { return g_engine_kv4; }
 
 void set_error(const char* fmt, ...) {
     va_list ap;
@@ -93,6 +95,10 @@ extern "C" int qe_set_tuning(const char* key, int value) {
     }
     if (std::strcmp(key, "engine_tiled_prefill") == 0) {
         qe::g_engine_tiled = value != 0;
+        return QE_OK;
+    }
+    if (std::strcmp(key, "engine_kv4") == 0) {
+        qe::g_engine_kv4 = value != 0;
         return QE_OK;
     }
     if (std::strcmp(key, "gemm_slices") == 0) {

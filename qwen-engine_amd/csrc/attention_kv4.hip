@@ -93,6 +93,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void kv4_decode_kernel(Decode4Params
     const int kvh = blockIdx.x % p.nkv;
     const int hb = (blockIdx.x / p.nkv) % p.head_blocks, split = blockIdx.x / (p.nkv * p.head_blocks);
     const int heads = min(16, p.group - 16 * hb), qh0 = kvh * p.group + 16 * hb;
+    const int ctx = kd4_context(p, kvh);
+    const int run = kd4_run(ctx, p.splits);
+    const int t0 = split * run, t1 = min(t0 + run, ctx);
+    if (t0 >= t1) return;
 
     const size_t head_base = static_cast<size_t>(kvh) * p.max_seq * kKv4Row;
     const uint8_t* kh = p.kc + head_base;
@@ -115,11 +119,6 @@ __global__ __launch_bounds__(64 * WAVES, 4) void kv4_decode_kernel(Decode4Params
             t.vp[i] = kv4_load(v, vpo + (16 * (i >> 2) + (i & 3)) * kKv4Row);
         }
     };
-    // The first rows are requested before the position is known: with the shortest
-    // runs they are these.  What lies behind the context is masked, as K by its
-    // scores, as V by zeros.
-    Kd4Tile a;
-    if (WAVES == 4 || wave < 4) load(split * kKd4MinRun + 32 * wave, p.max_seq, a);
     f16x8 qf[4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -127,11 +126,6 @@ __global__ __launch_bounds__(64 * WAVES, 4) void kv4_decode_kernel(Decode4Params
         if (n < heads)
             qf[kk] = *reinterpret_cast<const f16x8*>(p.q + static_cast<size_t>(qh0 + n) * kKv4Dim + 32 * h + 8 * kk);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    const int ctx = kd4_context(p, kvh);
-    const int run = kd4_run(ctx, p.splits);
-    const int t0 = split * run, t1 = min(t0 + run, ctx);
-    if (t0 >= t1) return;
     f32x4 acc[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
@@ -209,20 +203,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void kv4_decode_kernel(Decode4Params
     // One copy of the code in a loop, and the other waves to cover its loads: with the
     // next rows in flight from a second copy it was no faster (a launch runs it a
     // few times, and has to fetch it first).
-    int r0 = t0 + 32 * wave;
-    if (run != kKd4MinRun && r0 < t1) load(r0, t1, a);
-    while (r0 < t1) {
-        if (r0 + 31 >= t1) {  // uniform; what was requested early may be anything
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool in = r0 + 16 * (i >> 2) + 4 * h + (i & 3) < t1;
-                a.v[i] = in ? a.v[i] : 0u;
-                a.vp[i] = in ? a.vp[i] : 0u;
-            }
-        }
-        use(r0, a);
-        r0 += 32 * WAVES;
-        if (r0 < t1) load(r0, t1, a);
+    Kd4Tile tile;
+    for (int r0 = t0 + 32 * wave; r0 < t1; r0 += 32 * WAVES) {
+        load(r0, t1, tile);
+        use(r0, tile);
     }
     l = sum_over_quarters(l);
     // the waves meet: common maximum, then outputs

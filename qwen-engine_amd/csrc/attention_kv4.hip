@@ -411,7 +411,8 @@ struct Prefill4Params {
     float* lse;      // [token][q head] natural log, or NULL
     const float* w_in;
     float* w_out;
-    int T, nq, nkv, group, max_seq, out_stride, splits, row_blocks, block_rows, far_tiles;
+    float* part_w;   // [split of the q rows][kv head][max_seq]
+    int T, nq, nkv, group, max_seq, out_stride, splits, row_blocks, block_rows, far_tiles, weight_splits;
 };
 
 __device__ __forceinline__ int p4_live_splits(const Prefill4Params& p, int tiles) {
@@ -801,100 +802,110 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p
         p.lse[static_cast<size_t>(qi) * p.nq + qh] = (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
 }
 
-// Column sums of the probabilities: what the rows of the chunk give to 32 cache
-// rows of one kv head.  The block's 32 K rows stay in registers, expanded once;
-// a wave takes 32 query rows at a time, S^T = K . Q^T again, p = exp(s - lse) with
-// the row's final log sum, and keeps 16 sums a lane; lanes, then waves, add up at
-// the end in one order.  Every block reads the q rows that see its cache rows: the
-// wave copies its 32 rows to LDS by DMA, whole rows of 256 bytes, while it uses the 32
-// before, and takes its operands from there.  (Read as operands, 32 bytes of
-// 32 rows at a time, the addresses alone made 1000 rows on 3900 positions 50 us.)
-constexpr int kW4Waves = 8, kW4Keys = 32;
-constexpr int kW4Buffer = 32 * 256 + 256;  // 32 q rows, their log sums
-__global__ __launch_bounds__(64 * kW4Waves, 2) void kv4_prefill_weights_kernel(Prefill4Params p) {
-    __shared__ __align__(16) char smem[kW4Waves * 2 * kW4Buffer];
-    __shared__ float s_sum[kW4Waves][kW4Keys];
+// Column sums of the probabilities: what the rows of the chunk give to 64 cache
+// rows of one kv head.  S^T = K . Q^T again, p = exp(s - lse) with the row's final log
+// sum.  Four waves hold the first 32 K rows in registers, expanded once, four the
+// other 32; a tile of q rows, the whole tokens that 128 rows hold (so that a lane's
+// places in a tile are always the same), comes to LDS by DMA, whole rows of 256 bytes,
+// while the one before is used, and wave w takes its rows 32 (w % 4).. for its K
+// rows.  A lane keeps 16 sums; lanes, then waves, then the splits of the q rows add
+// up in one order.  Bound by the exponentials and what little is around them.  1000 rows on 2900..3900 positions (12 q heads, 2 kv heads): 50 us with
+// operands read from memory, 32 bytes of 32 rows at a time (their addresses alone), 29
+// with 32 K rows a block and a q tile for each wave, 22 and 5 for the splits' merge now.
+constexpr int kW4Keys = 64, kW4Rows = 128;
+constexpr int kW4Buffer = kW4Rows * 256 + kW4Rows * 4;  // q rows, their log sums
+constexpr int kW4MaxSplits = 4;
+__global__ __launch_bounds__(512, 4) void kv4_prefill_weights_kernel(Prefill4Params p) {
+    __shared__ __align__(16) char smem[2 * kW4Buffer];
+    __shared__ float s_sum[8][32];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int fr = lane & 31, h = lane >> 5;
-    const int kvh = blockIdx.x % p.nkv, t = blockIdx.x / p.nkv;
+    const int fr = lane & 31, h = lane >> 5, rw = wave & 3, kg = wave >> 2;
+    const int kvh = blockIdx.x % p.nkv, rest = blockIdx.x / p.nkv;
+    const int split = rest % p.weight_splits, t = rest / p.weight_splits;
     const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
     const int len = min(base + p.T, p.max_seq);
-    const int key0 = t * kW4Keys;
-    if (key0 >= len) return;
-    const int rows = p.T * p.group;
+    if (t * kW4Keys >= len) return;
+    const int key0 = t * kW4Keys + 32 * kg;
+    f32x16 sum = {};
+    // this split's share of the q tiles from the first token that sees a key of the block
+    const int per = kW4Rows / p.group, held = per * p.group;  // tokens and rows of a tile
+    const int first = max(0, min(t * kW4Keys - base, p.T - 1)) / per;
+    const int tiles = (p.T + per - 1) / per - first;
+    int u = first + tiles * split / p.weight_splits;
+    const int u1 = first + tiles * (split + 1) / p.weight_splits;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) void*)smem));
+    const uint16_t* q_head = p.q + static_cast<size_t>(kvh) * p.group * kKv4Dim;
+    const float* lse_head = p.lse + static_cast<size_t>(kvh) * p.group;
+    // x / group for x < 128: group <= 64, so x (group inverse - 2^16) <= 2^13 stays below 2^16
+    const uint32_t inverse = 65536u / p.group + 1u;
+    auto over_group = [&](int x) { return static_cast<int>((static_cast<uint32_t>(x) * inverse) >> 16); };
+    // Row x of a tile: token x / group of it, q head x % group; rows past the last are
+    // read as the last.  Its place counted from the tile's first q row; `tokens` are there.
+    auto place = [&](int x, int tokens) __attribute__((always_inline)) {
+        x = min(x, tokens * p.group - 1);
+        const int token = over_group(x);
+        return static_cast<uint32_t>(token * p.nq + x - token * p.group);
+    };
+    // Tile load i: rows 16 wave + 4 i + lane / 16, stored chunk lane % 16, i.e.
+    // chunk (lane % 16) ^ swz(row) of memory.
+    uint32_t q_at[4], lse_at;
+    auto places = [&](int tokens) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            q_at[i] = place(16 * wave + 4 * i + (lane >> 4), tokens) * (2 * kKv4Dim) +
+                      16 * ((lane & 15) ^ (((lane >> 4) << 2) | i));
+        lse_at = place(64 * (wave & 1) + lane, tokens);
+    };
+    places(per);
+    auto request = [&](int tile, int buf) __attribute__((always_inline)) {
+        if (p.T - tile * per < per) places(p.T - tile * per);  // the last tile, not whole
+        const uint32_t dst = lds0 + buf * kW4Buffer;
+        const size_t q0 = static_cast<size_t>(tile) * per * p.nq;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_load_x4(dst + 4096 * wave + 1024 * i, q_head + q0 * kKv4Dim, q_at[i]);
+        if (wave < kW4Rows / 64) lds_load_dword(dst + kW4Rows * 256 + 256 * wave, lse_head + q0 + lse_at);
+    };
+    const int mine = 32 * rw + fr, my_token = over_group(min(mine, held - 1));  // the lane's row of a tile
+    const uint32_t qa = lds0 + mine * 256 + 16 * (h ^ (((fr & 3) << 2) | ((fr >> 2) & 3)));
+    if (u < u1) request(u, 0);
     f16x8 kf[8];
     {
         const uint8_t* row = p.kc + (static_cast<size_t>(kvh) * p.max_seq + min(key0 + fr, len - 1)) * kKv4Row;
+        u32x4 w[4];
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)  // word 2 kk + h: dims 16 kk + 8 h..
-            kf[kk] = kv4_expand_word(*reinterpret_cast<const uint32_t*>(row + 4 * (2 * kk + h)),
-                                     *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * (kk >> 1)));
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(row + 16 * i);
+        const u32x4 par = *reinterpret_cast<const u32x4*>(row + kKv4Params);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {  // word 2 kk + h: dims 16 kk + 8 h..
+            const uint32_t even = w[kk >> 1][2 * (kk & 1)], odd = w[kk >> 1][2 * (kk & 1) + 1], pr = par[kk >> 1];
+            kf[kk] = kv4_expand_word(h ? odd : even, pr);
+        }
     }
-    f32x16 sum = {};
-    const int first = max(0, min(key0 - base, p.T - 1)) * p.group / 32 * 32;  // no row before it sees key0
-    constexpr int kStep = 32 * kW4Waves;
-    int r0 = first + 32 * wave;
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-                              (__attribute__((address_space(3))) void*)smem)) + wave * 2 * kW4Buffer;
-    // x / group for x < 128: group <= 64, so x (inverse group - 2^16) < 2^13 stays below 2^16
-    const uint32_t inverse = 65536u / p.group + 1u;
-    const uint16_t* q_head = p.q + static_cast<size_t>(kvh) * p.group * kKv4Dim;
-    const float* lse_head = p.lse + static_cast<size_t>(kvh) * p.group;
-    // Row r = token qi, head qg of the group, both uniform and kept up by addition.
-    // Tile load i: rows r + 4 i + lane / 16, stored chunk lane % 16, i.e. chunk
-    // (lane % 16) ^ swz(row) of memory.
-    const int step_q = kStep / p.group, step_g = kStep - step_q * p.group;
-    int qi_n = r0 / p.group, qg_n = r0 - qi_n * p.group;
-    auto request = [&](int r, int buf) __attribute__((always_inline)) {
-        const uint32_t dst = lds0 + buf * kW4Buffer;
-        // heads of the group past row r's, counted through the tokens: x = qg + rows further
-        const int most = min(32, rows - r) - 1 + qg_n;  // rows past the last are read as the last
-        const size_t token = static_cast<size_t>(qi_n) * p.nq;
-        auto place = [&](int x) __attribute__((always_inline)) {
-            x = min(x, most);
-            return static_cast<uint32_t>(x + static_cast<int>((static_cast<uint32_t>(x) * inverse) >> 16) * (p.nq - p.group));
-        };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t chunk = (lane & 15) ^ (((lane >> 4) << 2) | (i & 3));
-            lds_load_x4(dst + 1024 * i, q_head + token * kKv4Dim, place(qg_n + 4 * i + (lane >> 4)) * (2 * kKv4Dim) + 16 * chunk);
-        }
-        lds_load_dword(dst + 8192, lse_head + token + place(qg_n + fr));
-        qi_n += step_q;
-        qg_n += step_g;
-        if (qg_n >= p.group) {
-            qg_n -= p.group;
-            ++qi_n;
-        }
-    };
-    uint32_t qa = lds0 + fr * 256 + 16 * (h ^ (((fr & 3) << 2) | ((fr >> 2) & 3)));
-    int qi_first = qi_n;
-    if (r0 < rows) request(r0, 0);
-    for (int buf = 0; r0 < rows; r0 += kStep, buf ^= 1) {
-        const int qi0 = qi_first;  // the token of row r0
-        qi_first = qi_n;
+    for (int buf = 0; u < u1; ++u, buf ^= 1) {
         typedef const __attribute__((address_space(3))) f16x8* lptr;
         typedef const __attribute__((address_space(3))) float* lfptr;
-        if (r0 + kStep < rows) {
-            request(r0 + kStep, buf ^ 1);
-            asm volatile("s_waitcnt vmcnt(9)" ::: "memory");  // all but the nine just requested
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+        // the tile is there for every wave, and the other buffer is read by all
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
+        if (u + 1 < u1) request(u + 1, buf ^ 1);
         f32x16 sc = {};
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
                 kf[kk], *reinterpret_cast<lptr>((qa ^ (32 * kk)) + buf * kW4Buffer), sc, 0, 0, 0);
-        const float neg = -*reinterpret_cast<lfptr>(lds0 + buf * kW4Buffer + 8192 + 4 * fr) * kLog2e;
-        // there are 32 rows, and all see every key (limits grow with the rows)
-        if (min(base + qi0, p.max_seq - 1) >= key0 + kW4Keys - 1 && r0 + 32 <= rows) {
+        const float lse = *reinterpret_cast<lfptr>(lds0 + buf * kW4Buffer + kW4Rows * 256 + 4 * mine);
+        const int token = u * per + my_token;
+        // a row that is not there counts nothing (it stands for another, whose score is as finite)
+        const float neg = mine < held && token < p.T ? -lse * kLog2e : -INFINITY;
+        // every row of the tile sees every key (limits grow with the rows)
+        if (min(base + u * per, p.max_seq - 1) >= key0 + 31) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) sum[v] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[v], kScoreScale, neg));
         } else {
-            const int qi = (r0 + fr) / p.group;
-            const int lim = qi < p.T ? min(base + qi, p.max_seq - 1) : -1;
+            const int lim = min(base + token, p.max_seq - 1);
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int key = key0 + 8 * (v >> 2) + 4 * h + (v & 3);
@@ -902,9 +913,6 @@ __global__ __launch_bounds__(64 * kW4Waves, 2) void kv4_prefill_weights_kernel(P
                 sum[v] += key <= lim ? e : 0.0f;
             }
         }
-        // the buffer is read before the next turn asks for it to be filled
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
@@ -912,13 +920,33 @@ __global__ __launch_bounds__(64 * kW4Waves, 2) void kv4_prefill_weights_kernel(P
         if (fr == 0) s_sum[wave][8 * (v >> 2) + 4 * h + (v & 3)] = x;
     }
     __syncthreads();
-    const int key = key0 + static_cast<int>(threadIdx.x);
-    if (threadIdx.x >= kW4Keys || key >= len) return;
+    const int k = threadIdx.x, key = t * kW4Keys + k;
+    if (k >= kW4Keys || key >= len) return;
     float x = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kW4Waves; ++w) x += s_sum[w][threadIdx.x];
+    for (int w = 0; w < 4; ++w) x += s_sum[4 * (k >> 5) + w][k & 31];
     const size_t at = static_cast<size_t>(kvh) * p.max_seq + key;
-    p.w_out[at] = (p.w_in != nullptr && key < base ? p.w_in[at] : 0.0f) + x;
+    if (p.weight_splits > 1)
+        p.part_w[static_cast<size_t>(split) * p.nkv * p.max_seq + at] = x;
+    else
+        p.w_out[at] = (p.w_in != nullptr && key < base ? p.w_in[at] : 0.0f) + x;
+}
+
+// The splits of the q rows together.
+__global__ __launch_bounds__(256) void kv4_prefill_weights_merge_kernel(Prefill4Params p) {
+    const int kvh = blockIdx.x % p.nkv, key = (blockIdx.x / p.nkv) * 256 + threadIdx.x;
+    if (key >= p.max_seq) return;
+    const size_t at = static_cast<size_t>(kvh) * p.max_seq + key, stride = static_cast<size_t>(p.nkv) * p.max_seq;
+    float part[kW4MaxSplits];  // requested before the position is known
+#pragma unroll
+    for (int s = 0; s < kW4MaxSplits; ++s) part[s] = p.part_w[min(s, p.weight_splits - 1) * stride + at];
+    const float was = p.w_in != nullptr ? p.w_in[at] : 0.0f;
+    const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
+    if (key >= min(base + p.T, p.max_seq)) return;
+    float x = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kW4MaxSplits; ++s) x += s < p.weight_splits ? part[s] : 0.0f;
+    p.w_out[at] = (key < base ? was : 0.0f) + x;
 }
 
 inline bool capturing(hipStream_t stream) {
@@ -1083,9 +1111,22 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     else if (p.splits > 1)
         kv4_prefill_merge_kernel<1><<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
     if (key_weights_out != nullptr) {
-        const long long tiles = (static_cast<long long>(max_seq_len) + kW4Keys - 1) / kW4Keys;
-        QE_REQUIRE(tiles * num_kv_heads <= INT32_MAX, "%s: max_seq_len=%d", what, max_seq_len);
-        kv4_prefill_weights_kernel<<<static_cast<unsigned>(tiles * num_kv_heads), 64 * kW4Waves, 0, stream>>>(p);
+        // The q rows are shared by several blocks where there are many, if their sums find
+        // room in the workspace (the attention's partials there are merged by now).  (300
+        // tokens at 2000 33.0 against 37.8 us in all with two or three; at 16000 in a cache
+        // of 32768, where there are blocks enough, 84 against 78.)
+        const long long sums = static_cast<long long>(num_kv_heads) * max_seq_len;
+        const long long key_blocks = (static_cast<long long>(max_seq_len) + kW4Keys - 1) / kW4Keys * num_kv_heads;
+        p.weight_splits = static_cast<int>(
+            std::max(1LL, std::min<long long>(kW4MaxSplits, rows / (key_blocks > 2LL * cus ? 1024 : 512))));
+        if (p.weight_splits > 1 && (ws.ptr == nullptr || static_cast<long long>(ws.floats) < sums * p.weight_splits || capturing(stream)))
+            p.weight_splits = 1;
+        p.part_w = ws.ptr;
+        QE_REQUIRE(key_blocks * p.weight_splits <= INT32_MAX, "%s: max_seq_len=%d", what, max_seq_len);
+        kv4_prefill_weights_kernel<<<static_cast<unsigned>(key_blocks * p.weight_splits), 512, 0, stream>>>(p);
+        if (p.weight_splits > 1)
+            kv4_prefill_weights_merge_kernel<<<static_cast<unsigned>((static_cast<long long>(max_seq_len) + 255) / 256 * num_kv_heads),
+                                               256, 0, stream>>>(p);
     }
     return check_launch(what);
 }

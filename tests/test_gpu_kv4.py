@@ -263,6 +263,70 @@ def test_decode_heads(qe, nq, nkv, ctx, ms):
     _check(qe, kv, q, 1, nq, ctx - 1, [0] * nkv, ms, got, w_out=host(w))
 
 
+@pytest.mark.parametrize("nq,nkv,ctx,ms", [(64, 1, 18000, 20000), (17, 1, 30001, 70000), (12, 2, 40000, 40000), (64, 4, 5000, 33000),
+                                           (1, 1, 100, 1000000), (256, 32, 3000, 30000)])
+def test_decode_long_caches(qe, nq, nkv, ctx, ms):
+    """Blocks of sixteen waves, of which those without rows do nothing."""
+    rng = np.random.default_rng(ctx)
+    kv = np.full((2, nkv, ms, 80), 0xFF, np.uint8)
+    kv[0, :, :ctx] = ref.random_rows(rng, nkv, ctx)
+    kv[1, :, :ctx] = ref.random_rows(rng, nkv, ctx, offset=0.2)
+    q = rng.standard_normal(nq * 128).astype(np.float16)
+    w = dev(np.zeros((nkv, ms), np.float32))
+    got = _decode(qe, kv, q, nq, ctx - 1, None, ms, weights=w, w_in=w)
+    _check(qe, kv, q, 1, nq, ctx - 1, [0] * nkv, ms, got, w_out=host(w))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_query_that_is_not_finite_spoils_its_own_head_only(qe, workspace, bad):
+    rng = np.random.default_rng(13)
+    nq, nkv, ms, T = 12, 2, 1500, 40
+    kv = _cache(rng, nkv, ms, 1400)
+    q = rng.standard_normal((T, nq * 128)).astype(np.float16)
+    q[7, 3 * 128 + 5] = bad
+    clean = q.copy()
+    clean[7, 3 * 128 + 5] = 0
+    for rows, run in ((q[7:8], lambda x: _decode(qe, kv, x[0], nq, 1300, None, ms).reshape(1, -1)),
+                      (q, lambda x: _prefill(qe, kv, x, T, nq, 1300, None, ms)[0])):
+        at = 0 if len(rows) == 1 else 7
+        got, want = run(rows), run(clean[7:8] if len(rows) == 1 else clean)
+        assert np.all(np.isnan(got[at, 3 * 128:4 * 128]))
+        got[at, 3 * 128:4 * 128] = want[at, 3 * 128:4 * 128]
+        assert np.array_equal(got, want)
+
+
+def test_two_streams_at_once(qe):
+    """Launches with workspaces of their own do not disturb each other."""
+    rng = np.random.default_rng(14)
+    nq, nkv, ms = 12, 2, 30000
+    kv = _cache(rng, nkv, ms, 20000)
+    dk, dv = dev(kv[0]), dev(kv[1])
+    qs = [dev(rng.standard_normal(nq * 128).astype(np.float16)) for _ in range(2)]
+    ctls = [_ctl(19000), _ctl(700)]
+    n = qe.kv4_decode_workspace_bytes(nq, ms, True)
+    ws = [empty(n, torch.uint8) for _ in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def run(i, stream, out, w):
+        qe.launch_attention_gqa_flash_decode_kv4(qs[i], dk, dv, ws[i], out, ctls[i], None, stream, nq, nkv, max_seq_len=ms,
+                                                 key_weights_out=w)
+
+    alone = []
+    for i in range(2):
+        out, w = empty(nq * 128, torch.float16), torch.zeros((nkv, ms), device="cuda")
+        run(i, None, out, w)
+        alone.append((host(out), host(w)))
+    outs = [[(empty(nq * 128, torch.float16), torch.zeros((nkv, ms), device="cuda")) for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for k in range(20):
+        for i in range(2):
+            run(i, streams[i], *outs[i][k])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, w in outs[i]:
+            assert np.array_equal(host(out), alone[i][0]) and np.array_equal(host(w), alone[i][1])
+
+
 def test_decode_heads_of_different_lengths_and_a_full_cache(qe):
     rng = np.random.default_rng(8)
     nq, nkv, ms, pos = 8, 4, 300, 310

@@ -63,10 +63,12 @@ def test_prefill_splits_only_with_a_workspace_and_not_when_recorded(recorder):
         near(names(), "kv4_prefill_kernel", "kv4_prefill_merge")
         prefill(100, s, weights=True)
         near(names(), "kv4_prefill_kernel", "kv4_prefill_merge", "kv4_prefill_weights")
+        prefill(1000, s, weights=True)  # the q rows' sums are split too
+        near(names(), "kv4_prefill_kernel", "kv4_prefill_merge", "weights_kernel", "weights_merge")
         prefill(100, s, ms=512)  # too short to split
         near(names(), "kv4_prefill_kernel")
         R.recorder_set_capturing(V(s), I(1))
-        prefill(100, s, weights=True)
+        prefill(1000, s, weights=True)
         near(names(), "kv4_prefill_kernel", "kv4_prefill_weights")
         R.recorder_set_capturing(V(s), I(0))
         tune("gemm_split_k", 0)
@@ -123,3 +125,16 @@ def test_evict_and_logprobs(recorder):
         logprobs(1024, top=0)
         assert events()[0].grid[0] == 1024 * 5, events()
     """)
+
+
+def test_cpp_mirror_compiles():
+    import os
+    import shutil
+    import subprocess
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not available")
+    root = launch_recorder.ROOT
+    r = subprocess.run([hipcc, "-std=c++20", "-fsyntax-only", "-x", "hip", "--offload-arch=gfx950", f"-I{root}/include",
+                        os.path.join(root, "tests", "cpp", "kv4_call_shapes.cpp")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

@@ -384,9 +384,11 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // in its own lane and lane ^ 32; O^T += V^T . P^T with P^T the lane's own.
 // A tile is expanded once per block, into LDS as fp16: a thread takes 16-byte chunk
 // g (one quantization group) of one row and writes four 16-byte chunks, 4 g + i,
-// stored at chunk ^ swz(row).  Its 16 lanes that store together hold 16 rows
-// of one g, so they touch 16 different bank groups, like the readers (16 rows of one
-// chunk for K; 4 rows x 4 chunks through ds_read_b64_tr_b16 for V).
+// stored at chunk ^ swz(row).  16 lanes hold 16 rows of one g, so they touch 16
+// different bank groups, like the readers (16 rows of one chunk for K; 4 rows x 4
+// chunks through ds_read_b64_tr_b16 for V); a store moves 128 bytes a cycle, so the
+// rows are numbered for 8 lanes to touch 8 groups that differ mod 8 as well (rows in
+// order: 8 more cycles a store, 1 % of the kernel).
 // The raw 20 bytes of the tile after the next are in registers a whole step
 // before they are expanded.
 constexpr int kP4Keys = 64;
@@ -464,7 +466,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     }
     // staging: unit u = chunk g of row srow, K units first; with 8 waves, waves
     // 0..3 expand K and 4..7 V, with 4 every thread does one of each
-    const int su = threadIdx.x & 255, srow = (su & 15) + 16 * (su >> 6), sg = (su >> 4) & 3;
+    const int su = threadIdx.x & 255, sg = (su >> 4) & 3;
+    const int srow = ((su & 1) | ((su & 6) << 1) | ((su & 8) >> 2)) + 16 * (su >> 6);
     const size_t hb = static_cast<size_t>(kvh) * p.max_seq * kKv4Row;
     const uint8_t* src[UNITS];
     char* dst[UNITS];

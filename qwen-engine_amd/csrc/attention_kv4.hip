@@ -46,6 +46,13 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 //   Two rows' words joined half by half (v_perm) expand to (row, row + 1)
 //   pairs of one dim with the rows' own scales: no transposition through LDS.
 // The whole group of q heads shares one expansion of K and V.
+// A run is short where the cache is short (a block's start and end cost 2 us, a tile
+// of 32 rows 0.15), and there are at most 128: the merge reads them all.  12 q heads
+// on 2 kv heads, with the merge's 3 to 4 us behind it: 300 rows 4.3 us, 16001 with the
+// scores kept 5.1, 131000 12.3 (42 MB, 3.4 TB/s; a plain read of as much takes 7.6).
+// Short caches wait for the launch and one round of loads; long ones issue vector
+// instructions (24 for a word of eight nibbles, the matrix cores busy 9 %): neither more
+// rows in flight nor 8 waves for 16 changes them.
 constexpr int kKd4MaxSplits = 128;   // runs of a kv head, at most
 constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each of four waves
 constexpr int kKd4MaxGroup = 64;     // q heads of a kv head
@@ -287,7 +294,8 @@ __device__ __forceinline__ void kd4_run_weights(Kd4RunSums& r, int live, int lan
 // of runs), rounded once to fp16, and the Q8_1 of it when asked for.  The blocks
 // behind them, with key weights: 256 rows of one kv head, the sum over its q
 // heads of exp2(score - M) / L added to the weight so far; the newest row
-// starts at its own sum.
+// starts at its own sum.  A launch and two rounds of loads: 3.0 us with 3 runs,
+// 3.8 with 128, 4.2 with the weights of 16001 rows.
 constexpr int kKd4MergeThreads = 512;
 template <bool WEIGHTS>
 __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Decode4Params p) {
@@ -391,6 +399,13 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // order: 8 more cycles a store, 1 % of the kernel).
 // The raw 20 bytes of the tile after the next are in registers a whole step
 // before they are expanded.
+// Bound by the vector instructions between the products (6.5 for each MFMA, one of them
+// an exponential at a quarter of the rate), which overlap the MFMAs in part: 2048 tokens
+// at 14000 (12 q heads, 2 kv heads) take 236 us with the merge, 0.80 PFLOP/s of the 1.25
+// that a large fp16 product reaches, MFMAs busy 53 %; without the exponentials they would
+// take 210, without the expansion 210.  Slower: 64 rows a wave (269 us: the scores move
+// through the accumulation registers), the block's halves half a step apart (286: the
+// probabilities that cross the barrier do not fit the registers).
 constexpr int kP4Keys = 64;
 constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
 // Tiles of a split, at least, and of the splits beyond the eighth, whose merge costs
@@ -732,7 +747,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
 // sum through LDS for few rows with more than 8 splits, where what counts is how many
 // rounds of loads a row waits for (17 rows at 20000, 64 splits: 23.0 -> 19.0 us in
 // all; with 6000 rows they cost more).  Rows whose block had one split are already
-// written.
+// written.  Bound by the partials: 12000 rows in 4 splits 8 us.
 constexpr int kP4MergeMany = 8;
 template <int GROUPS>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p) {
@@ -812,7 +827,8 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p
 // places in a tile are always the same), comes to LDS by DMA, whole rows of 256 bytes,
 // while the one before is used, and wave w takes its rows 32 (w % 4).. for its K
 // rows.  A lane keeps 16 sums; lanes, then waves, then the splits of the q rows add
-// up in one order.  Bound by the exponentials and what little is around them.  1000 rows on 2900..3900 positions (12 q heads, 2 kv heads): 50 us with
+// up in one order.  Bound by the exponentials and what little is around them (MFMAs
+// busy 29 %).  1000 rows on 2900..3900 positions (12 q heads, 2 kv heads): 50 us with
 // operands read from memory, 32 bytes of 32 rows at a time (their addresses alone), 29
 // with 32 K rows a block and a q tile for each wave, 22 and 5 for the splits' merge now.
 constexpr int kW4Keys = 64, kW4Rows = 128;
@@ -935,7 +951,7 @@ __global__ __launch_bounds__(512, 4) void kv4_prefill_weights_kernel(Prefill4Par
         p.w_out[at] = (p.w_in != nullptr && key < base ? p.w_in[at] : 0.0f) + x;
 }
 
-// The splits of the q rows together.
+// The splits of the q rows together: a launch and a round of loads, 5 us for 2 x 4096 rows.
 __global__ __launch_bounds__(256) void kv4_prefill_weights_merge_kernel(Prefill4Params p) {
     const int kvh = blockIdx.x % p.nkv, key = (blockIdx.x / p.nkv) * 256 + threadIdx.x;
     if (key >= p.max_seq) return;

@@ -23,6 +23,8 @@ namespace {
 // lane, so a group of 32 is a quad of lanes; the first rot / 2 threads make the
 // token's sines and cosines.  The partner of a rotation is read from memory a
 // second time (it is in the cache) instead of being exchanged.
+// Latency: one token 3.5 us (a launch alone 1.7, then the loads, the sines and the
+// divisions behind each other), 1000 tokens 5.5 (12 q heads, 2 kv heads: 7.5 MB).
 __global__ __launch_bounds__(256) void qkv_bias_rope_kv4_append_kernel(
     const uint16_t* q, uint16_t* q_out, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
     const uint16_t* __restrict__ qb, const uint16_t* __restrict__ kb, const uint16_t* __restrict__ vb,
@@ -131,6 +133,7 @@ __global__ __launch_bounds__(256) void qkv_bias_rope_kv4_append_kernel(
 
 // ---- rows as fp16 --------------------------------------------------------------
 // A lane per word: 4 bytes and the group's pair in, 16 bytes out.  blockIdx.z: K, V.
+// Bound by its stores: 8000 rows x 8 heads of K and V, 43 MB, 7.9 us, 5.4 TB/s.
 __global__ __launch_bounds__(256) void kv4_unpack_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                          uint16_t* __restrict__ ok, uint16_t* __restrict__ ov,
                                                          int row0, int rows, int max_seq) {
@@ -389,6 +392,7 @@ struct EvictMove {
 
 // The kept rows to the front, in their order, into memory apart from the caches:
 // a lane per 16-byte piece, 5 pieces a row, K (blockIdx.z 0, with the weights) and V (1).
+// One round of loads behind the list: 8000 rows x 8 heads (21 MB both ways) 6.9 us, 3.0 TB/s.
 constexpr int kCopyRows = 51;  // rows of a block of 256 threads
 __global__ __launch_bounds__(256) void kv4_evict_copy_kernel(EvictMove p) {
     const int h = blockIdx.y, tid = threadIdx.x;
@@ -414,7 +418,9 @@ __global__ __launch_bounds__(256) void kv4_evict_copy_kernel(EvictMove p) {
 // within a run every load is done before the first store; later runs read behind
 // everything stored so far, and nobody else touches the block's pieces.  Rows in front of
 // the first one that left stay where they are.  PIECES of STRIDE values T a row, U
-// a thread and run: few runs, since each waits for memory twice.
+// a thread and run: few runs, since each waits for memory twice.  Five blocks a head, so
+// bound by a CU's loads: 8000 rows x 8 heads 20 us, three times the copy apart, which needs
+// a second cache.
 template <class T, int PIECES, int STRIDE, int U>
 __device__ __forceinline__ void move_rows(T* data, const int32_t* kept, int keep) {
     const uint32_t all = static_cast<uint32_t>(keep) * PIECES;

@@ -433,8 +433,8 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
  * 32-bit words of eight nibbles, element 8w + j at bit 16 * (j % 2) + 4 * (j / 2) of
  * word w, then four pairs (scale, low) of fp16, one for every 32 elements.  A nibble
  * n stands for fp16(n * scale + low), rounded once.  Storing x: low = fp16(min),
- * scale = fp16((max - low) / 15), n = clamp(rint((x - low) / scale), 0, 15), n = 0
- * for a scale of 0.  A token whose K or V holds a value that fp16 cannot (infinite,
+ * scale = fp16((max - low) / 15), or the fp16 below where 15 * scale + low would be
+ * infinite, n = clamp(rint((x - low) / scale), 0, 15), n = 0 for a scale of 0.  A token whose K or V holds a value that fp16 cannot (infinite,
  * NaN, 65520 and more) is stored with NaN pairs in its K row: every row that
  * attends to it gives NaN, rows that do not are untouched.
  *

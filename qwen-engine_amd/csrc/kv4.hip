@@ -12,8 +12,9 @@ namespace {
 // ---- append ------------------------------------------------------------------
 // x = q, k, v + bias in fp32, q and k rotated (NeoX pairs i, i + rot / 2 by
 // the angle pos * theta^(-2 i / rot)), q rounded once to fp16, k and v straight
-// to 4 bits: per 32 elements low = fp16(min), scale = fp16((max - low) / 15),
-// nibble = clamp(rint((x - low) / scale), 0, 15); a scale of 0 gives nibbles 0.
+// to 4 bits: per 32 elements low = fp16(min), scale = fp16((max - low) / 15) (one
+// fp16 less where 15 scale + low would round to infinity), nibble =
+// clamp(rint((x - low) / scale), 0, 15); a scale of 0 gives nibbles 0.
 //
 // Angles: position times frequency in 64 bits, reduced to [-pi, pi] there, then
 // sine and cosine in fp32.  In fp32 the angle of position 100000 is off by
@@ -109,7 +110,10 @@ __global__ __launch_bounds__(256) void qkv_bias_rope_kv4_append_kernel(
         hi = qwen::seg_max<4>(hi);
         const uint16_t lo16 = f2h(lo);
         const float low = h2f(lo16);
-        const uint16_t sc16 = f2h((hi - low) / 15.0f);
+        uint16_t sc16 = f2h((hi - low) / 15.0f);
+        // a scale rounded up must not take the largest value past 65504: one step less
+        // takes 15 of its units off, more than the at most 7.5 that it rounded up
+        if (__builtin_fmaf(15.0f, h2f(sc16), low) >= 65520.0f) --sc16;
         const float scale = h2f(sc16);
         uint32_t word = 0;
 #pragma unroll

@@ -170,6 +170,33 @@ def test_append_flat_and_tiny_groups(qe):
     assert np.all(np.abs(got[96:] - want[96:]) <= 0.001)
 
 
+def test_append_near_the_largest_fp16(qe):
+    """What is finite is stored finite, also where the scale rounds up and a nibble of 15 would pass 65504."""
+    top = 65504.0
+    pairs = [(-top, top), (0, top), (top, top), (-top, -top), (top - 32, top), (-top, top - 32), (-32768, top),
+             (-1.5, top), (-top, 0), (-61440, top), (8192, top), (-40000, 65472), (30000, top), (-50016, top),
+             (-12345, top), (60000, top)]
+    rng = np.random.default_rng(20)
+    x = np.zeros((len(pairs) // 4, 128))
+    for i, (lo, hi) in enumerate(pairs):
+        g = x[i // 4, 32 * (i % 4):32 * (i % 4) + 32]
+        g[:] = rng.uniform(lo, hi, 32)
+        g[5], g[17] = lo, hi
+    x = x.astype(np.float16)
+    for token in x:
+        kc, vc = qe.kv4_cache(1, 4), qe.kv4_cache(1, 4)
+        row = token[None]
+        _append(qe, np.zeros_like(row), row, row, [None] * 3, (kc, vc), 0, None, 4, 0)  # position 0: no rotation
+        for cache in (kc, vc):
+            got, want = host(cache)[0, 0], token.astype(np.float64)
+            _, scale, low = ref.parts(got)
+            with np.errstate(over="ignore"):
+                off = np.abs(ref.values(got) - want).reshape(4, 32)
+            # the scale: rounded by 2^-11, then up to 2^-10 less; 15 of it leave 45 * 2^-11 of a step. low and the
+            # value itself are rounded by 2^-11 of 65504 each.
+            assert np.all(off <= scale[:, None] * (0.5 + 45 * 2.0 ** -11) + 2 * 32), (off.max(-1), scale, low)
+
+
 # ---- unpack ----------------------------------------------------------------------------
 @pytest.mark.parametrize("nkv,ms,row0,n", [(1, 1, 0, 1), (2, 40, 3, 17), (5, 100, 0, 100), (3, 33, 32, 1)])
 def test_unpack_is_exact(qe, nkv, ms, row0, n):

@@ -497,7 +497,7 @@ int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const uint8_t* l
  * (appended before) over the 4-bit cache: the counterpart of
  * qe_launch_attention_gqa_prefill, which also says when the split workspace is used.
  * row_lse (float [T][num_q_heads], NULL = not wanted) receives the natural logarithm
- * of each row's softmax sum; key weights need it. */
+ * of each row's softmax sum; key weights need it, and an attn_out apart from q. */
 int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
                                         uint16_t* attn_out, const qe_device_control_block* d_control,
                                         const int32_t* d_evicted, int num_tokens, hipStream_t stream,

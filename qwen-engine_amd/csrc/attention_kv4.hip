@@ -1075,6 +1075,11 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     QE_REQUIRE(key_weights_out == nullptr || row_lse != nullptr, "%s: key weights need row_lse", what);
     QE_REQUIRE(aligned(q, 16) && aligned(attn_out, 8), "%s: q must be 16-byte and attn_out 8-byte aligned", what);
     if (num_tokens <= 0) return QE_OK;
+    // the weights' kernel reads q after the outputs are written
+    const size_t q_row = static_cast<size_t>(num_q_heads) * kKv4Dim * 2;
+    QE_REQUIRE(key_weights_out == nullptr ||
+                   apart(q, num_tokens * q_row, attn_out, (num_tokens - 1) * static_cast<size_t>(hidden_size) * 2 + q_row),
+               "%s: attn_out overlaps q", what);
     Prefill4Params p{};
     p.q = q;
     p.kc = layer_k_cache;

@@ -463,10 +463,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(EvictMove
 }
 
 // two buffers are one and the same, or share no byte
-inline bool same_or_apart(const void* a, const void* b, size_t bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x == y || x + bytes <= y || y + bytes <= x;
-}
+inline bool same_or_apart(const void* a, const void* b, size_t bytes) { return a == b || apart(a, bytes, b, bytes); }
 
 }  // namespace
 }  // namespace qe

@@ -88,6 +88,12 @@ __device__ __forceinline__ int kv4_row(const qe_device_control_block* ctl, const
     return max(pos - gone, 0);
 }
 
+// two buffers share no byte
+inline bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x + a_bytes <= y || y + b_bytes <= x;
+}
+
 // Checks that every entry point on the caches makes.
 inline int kv4_check(const char* what, const void* kc, const void* vc, int num_kv_heads, int head_dim,
                      int max_seq_len) {

@@ -69,7 +69,10 @@ def test_prefill(L):
         _says(L, prefill(**bad), "NULL")
     for bad, text in (({"nq": 13}, "13 q heads"), ({"nq": 130, "hs": 130 * 128}, "at most 64"), ({"hd": 64}, "head_dim"),
                       ({"hs": 1535}, "hidden_size"), ({"hs": 1538}, "hidden_size"), ({"w_in": P}, "without"),
-                      ({"w_out": P}, "row_lse"), ({"out": P + 4}, "aligned"), ({"q": P + 8}, "aligned"),
+                      ({"w_out": P}, "row_lse"), ({"w_out": P, "lse": P}, "attn_out overlaps q"),
+                      ({"w_out": P, "lse": P, "out": P + 4 * 1536 - 8, "T": 2}, "attn_out overlaps q"),
+                      ({"w_out": P, "lse": P, "q": P + 7056, "T": 2, "hs": 2000}, "attn_out overlaps q"),
+                      ({"out": P + 4}, "aligned"), ({"q": P + 8}, "aligned"),
                       ({"T": 2**31 - 1}, "num_tokens"), ({"ms": 2**30}, "max_seq_len")):
         _says(L, prefill(**bad), text)
     assert prefill(T=0) == 0

@@ -10,7 +10,7 @@ def decode(stream=0, nq=12, nkv=2, ms=4096, weights=False):
                                                   I(ms), V(0), V(0), V(0), V(0), V(P if weights else 0)))
 def prefill(T, stream=0, nq=12, nkv=2, ms=4096, weights=False):
     w = V(P if weights else 0)
-    ok(L.qe_launch_attention_gqa_prefill_kv4(V(P), V(P), V(P), V(P), V(0), V(0), I(T), V(stream), I(nq), I(nkv), I(128), I(ms),
+    ok(L.qe_launch_attention_gqa_prefill_kv4(V(P), V(P), V(P), V(P << 20), V(0), V(0), I(T), V(stream), I(nq), I(nkv), I(128), I(ms),
                                              I(nq * 128), w, w, w))
 def evict(in_place, nkv=2, ms=4096, keep=1000):
     a, b, c, d = (V(P * k) for k in (1, 100, 200, 300))

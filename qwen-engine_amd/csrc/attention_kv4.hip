@@ -398,7 +398,9 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // rows are numbered for 8 lanes to touch 8 groups that differ mod 8 as well (rows in
 // order: 8 more cycles a store, 1 % of the kernel).
 // The raw 20 bytes of the tile after the next are in registers a whole step
-// before they are expanded.
+// before they are expanded; a split's first two tiles are requested at once, and four
+// waves with no more than two take them from there (17 tokens at 1200: 12.9 -> 10.4 us in
+// all, a third of it the coalesced partials below).
 // Bound by the vector instructions between the products (6.5 for each MFMA, one of them
 // an exponential at a quarter of the rate), which overlap the MFMAs in part: 2048 tokens
 // at 14000 (12 q heads, 2 kv heads) take 236 us with the merge, 0.80 PFLOP/s of the 1.25
@@ -409,9 +411,9 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 constexpr int kP4Keys = 64;
 constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
 // Tiles of a split, at least, and of the splits beyond the eighth, whose merge costs
-// more: still 2 where a row is merged by 8 groups of lanes, else 8.  (us, 12 q heads, 2 kv
-// heads: 17 tokens at 1200 12.0 with 2 and 14.2 with 4, 509 at 0 16.0 and 18.9; 300
-// at 2000 27.6 with 2 for all, 24.4 with 4.)
+// more: still 2 where a row is merged by several groups, else 8.  (us, 12 q heads, 2 kv
+// heads: 17 tokens at 1200 10.7 with 2, 12.5 with 3 or 4; 509 at 0 14.9 with 2, 17.5 with
+// 3; 300 at 2000 22.5 with 2 and then 8, 25.3 with 2 and then 4.)
 constexpr int kP4MinTiles = 2, kP4FarTiles = 8, kP4FarTilesMany = 2;
 constexpr int kP4MaxSplits = 64;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -423,7 +425,7 @@ struct Prefill4Params {
     uint16_t* out;
     const qe_device_control_block* ctl;
     const int32_t* evicted;
-    float* part_o;   // [split][kv head][row][128] unnormalized
+    float* part_o;   // [split][kv head][32 rows] unnormalized, 16 bytes of [4 dt + g][h][row]: dims 32 dt + 8 g + 4 h
     float* part_ml;  // [split][kv head][row][2] (reference value, sum)
     float* lse;      // [token][q head] natural log, or NULL
     const float* w_in;
@@ -440,6 +442,12 @@ __device__ __forceinline__ int p4_tiles(const Prefill4Params& p, int rb, int bas
     const int last = min((rb + 1) * p.block_rows, p.T * p.group) - 1;
     const int len = min(base, p.max_seq) + last / p.group + 1;
     return (min(len, p.max_seq) + kP4Keys - 1) / kP4Keys;
+}
+
+// Where the partials of row r's 32 rows begin, in float4: a wave's stores of them are
+// 1 KB each, and the readers take 8 rows of a piece, 128 bytes.
+__device__ __forceinline__ size_t p4_part(const Prefill4Params& p, int split, int kvh, int r) {
+    return ((static_cast<size_t>(split) * p.nkv + kvh) * ((p.T * p.group + 31) / 32) + (r >> 5)) * 1024;
 }
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -493,30 +501,32 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         dst[u] = smem + (is_v ? 2 : 0) * kP4TileBytes + srow * 256;
     }
     const int sswz = ((srow & 3) << 2) | ((srow >> 2) & 3);
-    u32x4 raw[UNITS];
-    uint32_t rawp[UNITS];
+    struct Raw {
+        u32x4 w[UNITS];
+        uint32_t p[UNITS];
+    } raw;
     // tile tk for the K units, tv for the V units
-    auto fetch = [&](int tk, int tv) __attribute__((always_inline)) {
+    auto fetch = [&](Raw& raw, int tk, int tv) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
             const uint8_t* row = src[u] + static_cast<size_t>(min((is_v ? tv : tk) * kP4Keys + srow, key_max)) * kKv4Row;
-            raw[u] = *reinterpret_cast<const u32x4*>(row + 16 * sg);
-            rawp[u] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * sg);
+            raw.w[u] = *reinterpret_cast<const u32x4*>(row + 16 * sg);
+            raw.p[u] = *reinterpret_cast<const uint32_t*>(row + kKv4Params + 4 * sg);
         }
     };
     // word i of a unit
-    auto expand_word = [&](int u, int i, int kbuf, int vbuf) __attribute__((always_inline)) {
+    auto expand_word = [&](const Raw& raw, int u, int i, int kbuf, int vbuf) __attribute__((always_inline)) {
         const bool is_v = UNITS == 2 ? u == 1 : wave >= 4;
-        const uint32_t w = raw[u][i];
+        const uint32_t w = raw.w[u][i];
         *reinterpret_cast<f16x8*>(dst[u] + (is_v ? vbuf : kbuf) * kP4TileBytes + 16 * ((4 * sg + i) ^ sswz)) =
-            kv4_expand_word(w, rawp[u]);
+            kv4_expand_word(w, raw.p[u]);
     };
-    auto expand = [&](int kbuf, int vbuf) __attribute__((always_inline)) {
+    auto expand = [&](const Raw& raw, int kbuf, int vbuf) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) expand_word(u, i, kbuf, vbuf);
+            for (int i = 0; i < 4; ++i) expand_word(raw, u, i, kbuf, vbuf);
     };
     auto tile_barrier = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -635,8 +645,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
             if (i + AHEAD < 16) vf[i % AHEAD] = read_v(buf, i + AHEAD);
             if constexpr (decltype(more)::value) {
                 mx = fmaxf(fmaxf(mx, nxt[j][2 * (i & 7)]), nxt[j][2 * (i & 7) + 1]);
-                if (UNITS == 2 && (i & 1) == 0) expand_word(i >> 3, (i >> 1) & 3, buf, buf ^ 1);
-                if (UNITS == 1 && (i & 3) == 0) expand_word(0, i >> 2, buf, buf ^ 1);
+                if (UNITS == 2 && (i & 1) == 0) expand_word(raw, i >> 3, (i >> 1) & 3, buf, buf ^ 1);
+                if (UNITS == 1 && (i & 3) == 0) expand_word(raw, 0, i >> 2, buf, buf ^ 1);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -647,8 +657,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     // What a step does for everyone: K of the tile after next and V of the next
     // go to LDS (b: parity of tile t), the raw bytes behind them are requested.
     auto stage = [&](int t, int b) __attribute__((always_inline)) {
-        expand(b, b ^ 1);
-        fetch(t + 3, t + 2);
+        expand(raw, b, b ^ 1);
+        fetch(raw, t + 3, t + 2);
     };
     // Tile t's scores are in cur: the scores of the next tile beside the
     // probabilities of t, then V of t beside the next tile's maximum.
@@ -657,7 +667,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         scores(yes{}, b ^ 1, nxt, cur, pw);
         mask(t + 1, nxt);
         const float mx = add_pv(yes{}, pw, b, nxt);
-        fetch(t + 3, t + 2);
+        fetch(raw, t + 3, t + 2);
         renew_ref(mx);
         tile_barrier();
     };
@@ -670,31 +680,42 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
         lsum += ps[0] + ps[1];
         add_pv(no{}, pw, b, cur);
     };
-    if (it0 < it1) {
+    auto run = [&]() __attribute__((always_inline)) {
         const int n = it1 - it0;
         int t = it0;
-        fetch(t, t);
-        expand(0, 0);
-        fetch(t + 1, t + 1);
+        // two tiles are requested before the first is waited for
+        Raw first;
+        fetch(first, t, t);
+        fetch(raw, t + 1, t + 1);
+        expand(first, 0, 0);
         // K of the second tile now; V of it comes with the first step, which
         // expands what is in registers: K of the third, V of the second
         if constexpr (UNITS == 2) {
-            expand(1, 1);
+            expand(raw, 1, 1);
         } else {
-            if (wave < 4) expand(1, 1);
+            if (wave < 4) expand(raw, 1, 1);
         }
-        fetch(t + 2, t + 1);
-        tile_barrier();
+        // tiles past the wave's last key are not multiplied
+        const int mine = wave_last < t * kP4Keys ? 0 : min(n, wave_last / kP4Keys - t + 1);
         f32x16 s0[2], s1[2];
-        {
-            uint32_t pw[2][8];
-            scores(no{}, 0, s0, s1, pw);
+        uint32_t none[2][8];
+        if (UNITS == 2 && n <= 2) {  // all there: nothing left to overlap with
+            tile_barrier();
+#pragma unroll 1
+            for (int i = 0; i < mine; ++i) {
+                scores(no{}, i, s0, s1, none);
+                mask(t + i, s0);
+                renew_ref(row_max(s0));
+                finish(i, s0);
+            }
+            return;
         }
+        fetch(raw, t + 2, t + 1);
+        tile_barrier();
+        scores(no{}, 0, s0, s1, none);
         mask(t, s0);
         renew_ref(row_max(s0));
         tile_barrier();  // K buffer 0 is read
-        // tiles past the wave's last key are not multiplied
-        const int mine = wave_last < t * kP4Keys ? 0 : min(n, wave_last / kP4Keys - t + 1);
         int left = mine;
         for (; left > 2; left -= 2) {
             step(t, 0, s0, s1);
@@ -702,7 +723,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
             t += 2;
         }
         if (left == 2) {
-            step(t, 0, s0, s1);
+            // (one after the other: a step here costs registers that the loop needs)
+            scores(no{}, 1, s1, s0, none);
+            mask(t + 1, s1);
+            finish(0, s0);
+            stage(t, 0);
+            tile_barrier();
+            renew_ref(row_max(s1));
             finish(1, s1);
         } else if (left == 1) {
             finish(0, s0);
@@ -711,7 +738,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
             stage(it0 + i, i & 1);
             tile_barrier();
         }
-    }
+    };
+    if (it0 < it1) run();
     lsum += __shfl_xor(lsum, 32);
     if (r >= rows) return;
     if (live == 1) {
@@ -733,64 +761,80 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     }
     const size_t prow = (static_cast<size_t>(split) * p.nkv + kvh) * rows + r;
     if (h == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * prow) = make_float2(mref, lsum);
-    float* po = p.part_o + prow * kKv4Dim;
+    float4* po = reinterpret_cast<float4*>(p.part_o) + p4_part(p, split, kvh, r) + lane;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(po + 32 * dt + 8 * g + 4 * h) =
-                make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+            po[64 * (4 * dt + g)] = make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
 }
 
-// Merges the splits of every row: GROUPS groups of 32 lanes (4 dims each) a row, a
-// group takes every GROUPS-th split.  One group, eight rows a block; 8 groups and a
-// sum through LDS for few rows with more than 8 splits, where what counts is how many
-// rounds of loads a row waits for (17 rows at 20000, 64 splits: 23.0 -> 19.0 us in
-// all; with 6000 rows they cost more).  Rows whose block had one split are already
-// written.  Bound by the partials: 12000 rows in 4 splits 8 us.
-constexpr int kP4MergeMany = 8;
+// Merges the splits of eight rows of one kv head: a thread per row and 4 dims, rows
+// first, so that 8 lanes read 128 bytes; GROUPS groups of 256 threads, a group takes
+// every GROUPS-th split and LDS adds the groups up in their order.  One group; four
+// for few rows with more than 8 splits, where what counts is how many rounds of loads
+// a row waits for.  The rows' weights of the splits come first, a half wave a row.
+// Rows whose block had one split are already written.  Bound by the partials: 12000
+// rows in 5 splits 7.7 us (31 MB), 204 rows in 9 splits 3.3 (a launch alone 1.7).
+constexpr int kP4MergeMany = 4;
 template <int GROUPS>
-__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p) {
+__global__ __launch_bounds__(256 * GROUPS) void kv4_prefill_merge_kernel(Prefill4Params p) {
     static_assert(kP4MaxSplits <= 64, "two splits a lane");
-    __shared__ __align__(16) float s_o[GROUPS == 1 ? 1 : GROUPS][kKv4Dim];
-    const int rows = p.T * p.group;
-    const int lane = threadIdx.x & 31, g32 = threadIdx.x >> 5, d = 4 * lane;
-    const int g = GROUPS == 1 ? 0 : g32;
-    const long long all = static_cast<long long>(rows) * p.nkv;
-    const long long i = GROUPS == 1 ? static_cast<long long>(blockIdx.x) * 8 + g32 : static_cast<long long>(blockIdx.x);
-    if (i >= all) return;
-    const int kvh = static_cast<int>(i / rows), r = static_cast<int>(i - static_cast<long long>(kvh) * rows);
+    __shared__ __align__(16) float4 s_o[GROUPS][256];
+    __shared__ float s_w[8][kP4MaxSplits], s_inv[8];
+    const int rows = p.T * p.group, blocks = (rows + 7) / 8;
+    const int kvh = static_cast<int>(blockIdx.x) / blocks, r0 = 8 * (static_cast<int>(blockIdx.x) % blocks);
     const int base = min(kv4_row(p.ctl, p.evicted, kvh), p.max_seq);
-    const int live = p4_live_splits(p, p4_tiles(p, r / p.block_rows, base));
-    if (live == 1) return;  // (with several groups the block has one row: all of it)
+    const int live = p4_live_splits(p, p4_tiles(p, r0 / p.block_rows, base));
+    if (live == 1) return;
+    const int tid = threadIdx.x & 255, g = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int c = tid >> 3, r = min(r0 + (tid & 7), rows - 1);
     constexpr int B = 8;
+    const float4* po = reinterpret_cast<const float4*>(p.part_o) + p4_part(p, 0, kvh, r) + 32 * c + (r & 31);
+    const size_t stride = p4_part(p, 1, 0, 0);
     float4 v[B];
     auto request = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < B; ++b)
-            v[b] = *reinterpret_cast<const float4*>(p.part_o + (min(s0 + GROUPS * b, live - 1) * all + i) * kKv4Dim + d);
+            if (s0 + GROUPS * b < live) v[b] = po[(s0 + GROUPS * b) * stride];  // wave-uniform
     };
     request(g);
-    float2 ml[2];
+    if (g == 0) {
+        const int row = tid >> 5, lane = tid & 31;
+        const int rr = min(r0 + row, rows - 1);
+        float2 ml[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        ml[k] = make_float2(-INFINITY, 0.0f);
-        if (lane + 32 * k < live) ml[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((lane + 32 * k) * all + i));
+        for (int k = 0; k < 2; ++k) {
+            const int s = lane + 32 * k;
+            ml[k] = make_float2(-INFINITY, 0.0f);
+            if (s < live)
+                ml[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((static_cast<size_t>(s) * p.nkv + kvh) * rows + rr));
+        }
+        const float m = qwen::seg_max<32>(fmaxf(ml[0].x, ml[1].x));
+        // (a split whose scores are all NaN has no maximum and a NaN sum, which the products below keep)
+        float w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            w[k] = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
+            s_w[row][lane + 32 * k] = w[k];
+        }
+        const float l = qwen::seg_sum<32>(w[0] * ml[0].y + w[1] * ml[1].y);
+        if (lane == 0) {
+            s_inv[row] = l > 0.0f ? 1.0f / l : 0.0f;
+            if (p.lse != nullptr && r0 + row < rows)
+                p.lse[static_cast<size_t>(rr / p.group) * p.nq + kvh * p.group + rr % p.group] =
+                    (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
+        }
     }
-    const float m = qwen::seg_max<32>(fmaxf(ml[0].x, ml[1].x));
-    // (a split whose scores are all NaN has no maximum and a NaN sum, which the products below keep)
-    float w[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) w[k] = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - m);
-    const float l = qwen::seg_sum<32>(w[0] * ml[0].y + w[1] * ml[1].y);
+    __syncthreads();
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int s0 = g; s0 < live; s0 += GROUPS * B) {
         if (s0 > g) request(s0);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int s = s0 + GROUPS * b;
-            const float ws = __shfl(s < 32 ? w[0] : w[1], s & 31, 32);
-            if (s >= live) continue;
+            if (s >= live) break;
+            const float ws = s_w[tid & 7][s];
             o.x += ws * v[b].x;
             o.y += ws * v[b].y;
             o.z += ws * v[b].z;
@@ -798,26 +842,25 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(Prefill4Params p
         }
     }
     if constexpr (GROUPS > 1) {
-        *reinterpret_cast<float4*>(&s_o[g][d]) = o;
+        s_o[g][tid] = o;
         __syncthreads();
         if (g != 0) return;
 #pragma unroll
         for (int k = 1; k < GROUPS; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(&s_o[k][d]);
+            const float4 x = s_o[k][tid];
             o.x += x.x;
             o.y += x.y;
             o.z += x.z;
             o.w += x.w;
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (r0 + (tid & 7) >= rows) return;
+    const float inv = s_inv[tid & 7];
     const int qi = r / p.group, qh = kvh * p.group + r % p.group;
-    uint16_t* dst = p.out + static_cast<size_t>(qi) * p.out_stride + qh * kKv4Dim + d;
+    uint16_t* dst = p.out + static_cast<size_t>(qi) * p.out_stride + qh * kKv4Dim + 4 * c;
     *reinterpret_cast<uint2*>(dst) =
         make_uint2(static_cast<uint32_t>(f2h(o.x * inv)) | (static_cast<uint32_t>(f2h(o.y * inv)) << 16),
                    static_cast<uint32_t>(f2h(o.z * inv)) | (static_cast<uint32_t>(f2h(o.w * inv)) << 16));
-    if (p.lse != nullptr && lane == 0)
-        p.lse[static_cast<size_t>(qi) * p.nq + qh] = (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);
 }
 
 // Column sums of the probabilities: what the rows of the chunk give to 64 cache
@@ -1101,10 +1144,10 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
                max_seq_len);
     // Eight waves and one block per CU expand a tile for 256 rows; four waves for
     // 128, two blocks per CU, where there are few row blocks: their splits are shorter and
-    // fewer rows idle.  (12 q heads, 2 kv heads, all in us: 40 tokens at 1200 19.0 against
-    // 15.2, 509 at 0 24.2 against 18.8; 1000 at 2900 43.8 against 46.0, 1024 at 15000 122
-    // against 132.)
-    const int waves = (rows + 255) / 256 * num_kv_heads >= 32 ? 8 : 4;
+    // fewer rows idle.  (12 q heads, 2 kv heads, all in us: 40 tokens at 1200 13.1 against
+    // 11.1, 509 at 0 17.4 against 14.0; 600 at 1000 25.7 against 27.0, 1000 at 2900 41.5
+    // against 45.1, 1024 at 15000 117 against 129.)
+    const int waves = (rows + 255) / 256 * num_kv_heads >= 28 ? 8 : 4;
     p.block_rows = 32 * waves;
     p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
     const long long blocks = static_cast<long long>(p.row_blocks) * num_kv_heads;
@@ -1113,9 +1156,12 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     const int cus = cu_count();
     const WorkspaceLease lease(stream);  // until every kernel is enqueued
     const StreamWorkspace ws = lease.ws;
-    const long long part = rows * num_kv_heads * (kKv4Dim + 2);  // floats of one split
-    const long long slots = waves == 4 ? 2LL * cus : cus;
+    const long long part_rows = (rows + 31) / 32 * 32 * num_kv_heads;  // outputs of one split, whole waves
+    const long long part = part_rows * kKv4Dim + rows * num_kv_heads * 2;  // floats of one split
+    // (few rows: a block for every CU; twice as many cost more in the merge, us in all: 60
+    // tokens at 8000 24.0 against 21.2, at 30000 35.0 against 32.0, 17 at 1200 10.5 both)
     const bool few_rows = rows * num_kv_heads <= 2048;
+    const long long slots = waves == 4 && !few_rows ? 2LL * cus : cus;
     p.far_tiles = few_rows ? kP4FarTilesMany : kP4FarTiles;
     p.splits = 1;
     if (ws.ptr != nullptr && max_seq_len >= 16 * kP4Keys)
@@ -1126,14 +1172,13 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     if (p.splits > 1 && capturing(stream)) p.splits = 1;
     QE_REQUIRE(blocks * p.splits <= INT32_MAX, "%s: num_tokens=%d", what, num_tokens);
     p.part_o = ws.ptr;
-    p.part_ml = ws.ptr + p.splits * rows * num_kv_heads * kKv4Dim;
+    p.part_ml = ws.ptr + p.splits * part_rows * kKv4Dim;
     const unsigned grid = static_cast<unsigned>(blocks * p.splits);
     if (waves == 4) kv4_prefill_kernel<4><<<grid, 256, 0, stream>>>(p);
     else kv4_prefill_kernel<8><<<grid, 512, 0, stream>>>(p);
-    if (p.splits > 8 && few_rows)
-        kv4_prefill_merge_kernel<kP4MergeMany><<<static_cast<unsigned>(rows * num_kv_heads), 256, 0, stream>>>(p);
-    else if (p.splits > 1)
-        kv4_prefill_merge_kernel<1><<<static_cast<unsigned>((rows * num_kv_heads + 7) / 8), 256, 0, stream>>>(p);
+    const unsigned merge_grid = static_cast<unsigned>((rows + 7) / 8 * num_kv_heads);
+    if (p.splits > 8 && few_rows) kv4_prefill_merge_kernel<kP4MergeMany><<<merge_grid, 256 * kP4MergeMany, 0, stream>>>(p);
+    else if (p.splits > 1) kv4_prefill_merge_kernel<1><<<merge_grid, 256, 0, stream>>>(p);
     if (key_weights_out != nullptr) {
         // The q rows are shared by several blocks where there are many, if their sums find
         // room in the workspace (the attention's partials there are merged by now).  (300

@@ -403,11 +403,12 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // all, a third of it the coalesced partials below).
 // Bound by the vector instructions between the products (6.5 for each MFMA, one of them
 // an exponential at a quarter of the rate), which overlap the MFMAs in part: 2048 tokens
-// at 14000 (12 q heads, 2 kv heads) take 236 us with the merge, 0.80 PFLOP/s of the 1.25
-// that a large fp16 product reaches, MFMAs busy 53 %; without the exponentials they would
-// take 210, without the expansion 210.  Slower: 64 rows a wave (269 us: the scores move
-// through the accumulation registers), the block's halves half a step apart (286: the
-// probabilities that cross the barrier do not fit the registers).
+// at 14000 (12 q heads, 2 kv heads) take 222 us with the merge, 0.85 PFLOP/s of the 1.25
+// that a large fp16 product reaches, MFMAs busy 54 %; without the exponentials or without
+// the expansion they would take a tenth less, without the barrier 3 %.  Slower: 64 rows a
+// wave (by 15 %: the scores move through the accumulation registers), the block's halves
+// half a step apart (by 24 %: the probabilities that cross the barrier do not fit the
+// registers).
 constexpr int kP4Keys = 64;
 constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
 // Tiles of a split, at least, and of the splits beyond the eighth, whose merge costs

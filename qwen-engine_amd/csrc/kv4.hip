@@ -162,9 +162,8 @@ __global__ __launch_bounds__(256) void kv4_unpack_kernel(const uint8_t* __restri
 // 0 and kEvictSafe are left over: no row, and a row that stays whatever its weight.
 constexpr uint32_t kEvictSafe = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t evict_key(float w) {
-    if (w != w) return 1;
-    const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
+    return w != w ? 1u : u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 
 // Sum over the lanes up to and with this one.
@@ -201,7 +200,8 @@ __device__ __forceinline__ void evict_finish(float* out_weights, const int32_t* 
 // largest keys, equal ones by the lowest index: radix selection of the keep-th
 // largest, then one ordered pass that writes the kept indices.
 // Up to 32768 rows the keys are read from memory once and stay in LDS (more rows: read
-// again in every pass).  A wave owns a run of rows, a multiple of 256 so that a lane
+// again in every pass, 16 loads ahead of their use; with 32000 that takes 4 us more, and with
+// 4 loads and their wait at a time 60000 rows took 81 us in all, now 48).  A wave owns a run of rows, a multiple of 256 so that a lane
 // can take four keys with one LDS read wherever their order does not matter.  Digits
 // of 11, 11 and 10 bits: the first holds the sign, the exponent and two bits of the
 // mantissa, so that weights of like size still spread over the bins and lanes seldom
@@ -273,22 +273,48 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
             }
     }
     const int r0 = wave * per, r1 = min(r0 + per, n);
+    // f(keys of rows i0 + 64 u + lane, i0) for all of the wave's, from memory: 16 loads at once,
+    // the next 16 while these are used
+    auto each_read = [&](auto f) __attribute__((always_inline)) {
+        float now[16], next[16] = {};
+        auto fetch = [&](int i0, float (&x)[16]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) x[u] = w[min(i0 + 64 * u + lane, n - 1)];
+        };
+        if (r0 < r1) fetch(r0, now);
+        for (int b0 = r0; b0 < r1; b0 += 1024) {
+            if (b0 + 1024 < r1) fetch(b0 + 1024, next);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int i0 = b0 + 256 * v;
+                if (i0 >= r1) break;  // the next wave's
+                uint32_t k[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) k[u] = evict_key(now[4 * v + u]);
+                if (i0 < lo || i0 + 256 > hi) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + 64 * u + lane, now[4 * v + u]);
+                }
+                f(k, i0);
+            }
+#pragma unroll
+            for (int u = 0; u < 16; ++u) now[u] = next[u];
+        }
+    };
     // f(four keys) for all of the wave's, in any order
     auto each = [&](auto f) __attribute__((always_inline)) {
+        if (!cached) {
+            each_read(f);
+            return;
+        }
         for (int i0 = r0; i0 < r1; i0 += 256) {
-            u32x4 k;
-            if (cached) {
-                k = *reinterpret_cast<const u32x4*>(s_key + i0 + 4 * lane);
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + 64 * u + lane, w[min(i0 + 64 * u + lane, n - 1)]);
-            }
+            const u32x4 k = *reinterpret_cast<const u32x4*>(s_key + i0 + 4 * lane);
             const uint32_t k4[4] = {k[0], k[1], k[2], k[3]};
-            f(k4);
+            f(k4, i0);
         }
     };
     if (!cached)
-        each([&](const uint32_t(&k)[4]) {
+        each_read([&](const uint32_t(&k)[4], int) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) count_first(k[u]);
         });
@@ -296,7 +322,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     auto round = [&](auto number) __attribute__((always_inline)) {
         constexpr int R = decltype(number)::value, shift = R == 0 ? 21 : R == 1 ? 10 : 0, bits = R == 2 ? 10 : 11;
         if constexpr (R > 0)
-            each([&](const uint32_t(&k)[4]) {
+            each([&](const uint32_t(&k)[4], int) {
                 bool is[4], any = false;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -340,7 +366,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     round(std::integral_constant<int, 2>{});
     const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
     int sure_n = 0, tie_n = 0;
-    each([&](const uint32_t(&k)[4]) {
+    each([&](const uint32_t(&k)[4], int) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             sure_n += __popcll(__builtin_amdgcn_ballot_w64(k[u] > cut));
@@ -359,13 +385,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     const int wanted = static_cast<int>(need);
     at = __builtin_amdgcn_readfirstlane(at + min(ties, wanted));
     ties = __builtin_amdgcn_readfirstlane(ties);
-    for (int i0 = r0; i0 < r1; i0 += 256) {
-        uint32_t k[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 64 * u + lane;
-            k[u] = cached ? s_key[i] : key_of(i, w[min(i, n - 1)]);
-        }
+    auto write = [&](const uint32_t(&k)[4], int i0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             uint64_t take = __builtin_amdgcn_ballot_w64(k[u] > cut);
@@ -381,6 +401,16 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(take), 0u)))] = i0 + 64 * u + lane;
             at += __popcll(take);
         }
+    };
+    if (!cached) {
+        each_read(write);
+        return;
+    }
+    for (int i0 = r0; i0 < r1; i0 += 256) {
+        uint32_t k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = s_key[i0 + 64 * u + lane];
+        write(k, i0);
     }
 }
 

@@ -586,6 +586,13 @@ def test_evict(qe, n, keep, sinks, recent, in_place):
     _check_evict(kv, w, n + 11, [11] * nkv, keep, sinks, recent, ms, got)
 
 
+@pytest.mark.parametrize("n,keep,sinks,recent", [(32769, 32768, 0, 0), (33793, 1, 1, 0), (49153, 20000, 300, 1500),
+                                                 (70001, 123, 4, 100), (131000, 65000, 4, 40000)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_more_rows_than_lds_holds(qe, n, keep, sinks, recent, in_place):
+    test_evict(qe, n, keep, sinks, recent, in_place)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 def test_evict_odd_weights_and_heads_of_their_own(qe, in_place):
     """NaN, infinities, negative weights, zeros of both signs, subnormals; heads with other lengths, none, and full ones."""

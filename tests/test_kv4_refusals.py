@@ -120,3 +120,20 @@ def test_workspace_sizes(L):
     _says(L, L.qe_kv4_decode_workspace_bytes(12, 64, 0, None), "NULL")
     _says(L, L.qe_token_logprobs_workspace_bytes(1, 0, 0, ctypes.byref(n)), "vocab_size")
     _says(L, L.qe_token_logprobs_workspace_bytes(1, 100, 33, ctypes.byref(n)), "top_k")
+
+
+def test_tensors_in_host_memory():
+    """The Python launchers, before the library is called."""
+    import torch
+
+    import qe_amd
+    x = torch.zeros(4096, dtype=torch.uint8)
+    calls = [lambda: qe_amd.launch_qkv_bias_rope_kv4_append(x, x, x, x, None, None, None, x, x, None, None, 1),
+             lambda: qe_amd.launch_kv4_unpack(x, x, x, x, 0, 1), lambda: qe_amd.launch_kv4_unpack(None, x, None, x, 0, 1),
+             lambda: qe_amd.launch_attention_gqa_flash_decode_kv4(x, x, x, x, x, None, None),
+             lambda: qe_amd.launch_attention_gqa_prefill_kv4(x, x, x, x, None, None, 1),
+             lambda: qe_amd.launch_kv4_evict(x, x, x, None, x, x, x, x, x, x, 1),
+             lambda: qe_amd.launch_token_logprobs(x, None, None, x, None, None, x, 1, vocab_size=8)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="must be on a GPU"):
+            call()

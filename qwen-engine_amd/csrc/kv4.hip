@@ -182,33 +182,46 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x;
 }
 
+// What a head has before an eviction.
+struct EvictHead {
+    int pos, gone, row, n, m;  // position, rows gone, row of the position, rows in use, rows that stay
+};
+__device__ __forceinline__ EvictHead evict_head(const int32_t* evicted, const qe_device_control_block* ctl, int h, int keep,
+                                                int max_seq) {
+    EvictHead e;
+    e.pos = ctl != nullptr ? ctl->seq_pos : 0;
+    e.gone = evicted != nullptr ? evicted[h] : 0;
+    e.row = max(e.pos - e.gone, 0);
+    e.n = min(e.row, max_seq);
+    e.m = min(e.n, keep);
+    return e;
+}
 // The weights behind the kept rows start over, and so does the count of evicted rows.
-// By all threads of the one block that does it.
-__device__ __forceinline__ void evict_finish(float* out_weights, const int32_t* evicted, int32_t* out_evicted,
-                                             const qe_device_control_block* ctl, int h, int keep, int max_seq) {
-    const int pos = ctl != nullptr ? ctl->seq_pos : 0;
-    const int row = kv4_row(ctl, evicted, h), n = min(row, max_seq), m = min(n, keep);
+// By all threads of the one block that does it, behind a barrier that all have
+// passed since they read `evicted` (it may be out_evicted).
+__device__ __forceinline__ void evict_finish(float* out_weights, int32_t* out_evicted, const EvictHead& e, int h,
+                                             int max_seq) {
     const size_t base = static_cast<size_t>(h) * max_seq;
-    for (int i = m + threadIdx.x; i < n; i += blockDim.x) out_weights[base + i] = 0.0f;
-    __syncthreads();  // evicted may be out_evicted
+    for (int i = e.m + threadIdx.x; i < e.n; i += blockDim.x) out_weights[base + i] = 0.0f;
     // the next position's row is m: positions that found the cache full count as gone too
-    if (threadIdx.x == 0) out_evicted[h] = row == 0 ? (evicted != nullptr ? evicted[h] : 0) : pos - m;
+    if (threadIdx.x == 0) out_evicted[h] = e.row == 0 ? e.gone : e.pos - e.m;
 }
 
 // Rows kept of one kv head, a block each.  The first `sinks` and the last
 // `recent` rows count as larger than every weight, so what stays are the `keep`
 // largest keys, equal ones by the lowest index: radix selection of the keep-th
 // largest, then one ordered pass that writes the kept indices.
-// Up to 32768 rows the keys are read from memory once and stay in LDS (more rows: read
-// again in every pass, 16 loads ahead of their use; with 32000 that takes 4 us more, and with
-// 4 loads and their wait at a time 60000 rows took 81 us in all, now 48).  A wave owns a run of rows, a multiple of 256 so that a lane
-// can take four keys with one LDS read wherever their order does not matter.  Digits
-// of 11, 11 and 10 bits: the first holds the sign, the exponent and two bits of the
-// mantissa, so that weights of like size still spread over the bins and lanes seldom
-// meet in one.  One CU a head, so instructions count: 4096 rows take 7.4 us (2 heads),
-// 32000 21 (8 heads); with digits of 8 bits, four rounds over memory and a branch for
-// every key 10.3 and 53, with the keys in registers (passes unrolled 32 times, 34 KB
-// of code) 8.5 and 20.
+// Up to 32768 rows the keys are read from memory once and stay in LDS; more rows are
+// read again in every pass, eight loads a lane ahead (60000 rows, copy included, 48 us; with
+// four loads and their wait at a time 81).  A wave owns a run of rows, a multiple of 256
+// so that a lane can take four keys with one LDS read wherever their order does not
+// matter.  Digits of 11, 11 and 10 bits: the first holds the sign, the exponent and two
+// bits of the mantissa, so that weights of like size still spread over the bins and
+// lanes seldom meet in one; the third is looked at only where some, not all, of
+// the keys with the same first 22 bits stay.  One CU a head, so instructions count: 4096
+// rows take 6.0 us (2 heads), 32000 17.7 (8 heads); with the loads waited for before
+// the first count and always three digits 7.3 and 21, with digits of 8 bits, four rounds over
+// memory and a branch for every key 10.3 and 53.
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictCached = 32768;  // keys in LDS
@@ -229,18 +242,21 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     extern __shared__ uint32_t s_key[];  // W evict_run(max_seq), at most kEvictCached
     __shared__ __align__(16) uint32_t s_hist[3 * kEvictBins];  // the first digit counts in the first two
     __shared__ uint32_t s_wave[W];
-    __shared__ uint32_t s_pick[2];  // digit, keys above it
+    __shared__ uint32_t s_pick[3];  // digit, keys above it, keys of it
     __shared__ int2 s_cnt[W];
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = min(kv4_row(ctl, evicted, h), max_seq);
+    const EvictHead head = evict_head(evicted, ctl, h, keep, max_seq);
+    const int n = head.n;
     int32_t* out = kept + static_cast<size_t>(h) * keep;
-    const int m = min(n, keep);
-    for (int i = m + tid; i < keep; i += kEvictThreads) out[i] = -1;
-    // moved apart, nothing here is read again: the head's end is written now
-    if (apart_weights != nullptr) evict_finish(apart_weights, evicted, apart_evicted, ctl, h, keep, max_seq);
+    // moved apart, nothing here is read again, and the head's end can be written here
+    auto finish = [&]() __attribute__((always_inline)) {
+        if (apart_weights != nullptr) evict_finish(apart_weights, apart_evicted, head, h, max_seq);
+    };
     if (n <= keep) {
-        for (int i = tid; i < n; i += kEvictThreads) out[i] = i;
+        for (int i = tid; i < keep; i += kEvictThreads) out[i] = i < n ? i : -1;
+        __syncthreads();
+        finish();
         return;
     }
     const float* w = weights + static_cast<size_t>(h) * max_seq;
@@ -248,62 +264,65 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     auto key_of = [&](int i, float x) { return i >= n ? 0u : i < lo || i >= hi ? kEvictSafe : evict_key(x); };
     const int per = evict_run(n);
     const bool cached = W * per <= kEvictCached;
-    constexpr int J = kEvictCached / kEvictThreads;
-    float x[J];  // requested together
-    if (cached) {
+    const int r0 = wave * per, r1 = min(r0 + per, n);
+    // f(keys of rows i0 + 64 u + lane, i0) for all of the wave's, from memory: eight loads
+    // at a time, the next eight requested before these are used.  No load is behind a branch
+    // of its own, and none is copied: the compiler would wait for all at the first use.
+    float even[8], odd[8];
+    auto fetch = [&](int b0, float (&x)[8]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (j * kEvictThreads < n) x[j] = w[min(j * kEvictThreads + tid, n - 1)];
-    }
+        for (int u = 0; u < 8; ++u) x[u] = w[min(b0 + 64 * u + lane, n - 1)];
+    };
+    auto each_read = [&](auto f) __attribute__((always_inline)) {
+        auto use = [&](int b0, const float (&x)[8]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int i0 = b0 + 256 * v;
+                if (i0 >= r1) break;  // the next wave's
+                uint32_t k[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) k[u] = evict_key(x[4 * v + u]);
+                if (i0 < lo || i0 + 256 > hi) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + 64 * u + lane, x[4 * v + u]);
+                }
+                f(k, i0);
+            }
+        };
+        for (int b0 = r0; b0 < r1; b0 += 1024) {  // `even` is requested
+            if (b0 + 512 < r1) {
+                fetch(b0 + 512, odd);
+                use(b0, even);
+                fetch(b0 + 1024, even);
+                use(b0 + 512, odd);
+            } else {
+                use(b0, even);
+            }
+        }
+    };
+    fetch(r0, even);
     for (int i = tid; i < 3 * kEvictBins; i += kEvictThreads) s_hist[i] = 0;
-    __syncthreads();
+    // a barrier for LDS alone: the loads stay in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     // The first digit, lanes of odd and even number apart; rows that stay anyway are
     // many and in one place: counted together, not one by one.
     auto count_first = [&](uint32_t k) __attribute__((always_inline)) {
         if (k + 1u > 1u) atomicAdd(&s_hist[(lane & 1) * kEvictBins + (k >> 21)], 1u);
     };
     if (tid == 0) atomicAdd(&s_hist[kEvictBins - 1], static_cast<uint32_t>(sinks + recent));
-    if (cached) {
+    each_read([&](const uint32_t(&k)[4], int i0) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (j * kEvictThreads < W * per) {
-                const uint32_t k = key_of(j * kEvictThreads + tid, x[j]);
-                s_key[j * kEvictThreads + tid] = k;
-                count_first(k);
-            }
-    }
-    const int r0 = wave * per, r1 = min(r0 + per, n);
-    // f(keys of rows i0 + 64 u + lane, i0) for all of the wave's, from memory: 16 loads at once,
-    // the next 16 while these are used
-    auto each_read = [&](auto f) __attribute__((always_inline)) {
-        float now[16], next[16] = {};
-        auto fetch = [&](int i0, float (&x)[16]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < 16; ++u) x[u] = w[min(i0 + 64 * u + lane, n - 1)];
-        };
-        if (r0 < r1) fetch(r0, now);
-        for (int b0 = r0; b0 < r1; b0 += 1024) {
-            if (b0 + 1024 < r1) fetch(b0 + 1024, next);
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int i0 = b0 + 256 * v;
-                if (i0 >= r1) break;  // the next wave's
-                uint32_t k[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) k[u] = evict_key(now[4 * v + u]);
-                if (i0 < lo || i0 + 256 > hi) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) k[u] = key_of(i0 + 64 * u + lane, now[4 * v + u]);
-                }
-                f(k, i0);
-            }
-#pragma unroll
-            for (int u = 0; u < 16; ++u) now[u] = next[u];
+        for (int u = 0; u < 4; ++u) {
+            if (cached) s_key[i0 + 64 * u + lane] = k[u];
+            count_first(k[u]);
         }
-    };
+    });
     // f(four keys) for all of the wave's, in any order
     auto each = [&](auto f) __attribute__((always_inline)) {
         if (!cached) {
+            fetch(r0, even);
             each_read(f);
             return;
         }
@@ -313,11 +332,6 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
             f(k4, i0);
         }
     };
-    if (!cached)
-        each_read([&](const uint32_t(&k)[4], int) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) count_first(k[u]);
-        });
     uint32_t prefix = 0, need = keep;  // digits found so far, keys still to take at or below them
     auto round = [&](auto number) __attribute__((always_inline)) {
         constexpr int R = decltype(number)::value, shift = R == 0 ? 21 : R == 1 ? 10 : 0, bits = R == 2 ? 10 : 11;
@@ -356,6 +370,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
             const bool first = above + b.y >= need;
             s_pick[0] = kEvictBins - 1 - 2 * tid - (first ? 0 : 1);
             s_pick[1] = above + (first ? 0 : b.y);
+            s_pick[2] = first ? b.y : b.x;
         }
         __syncthreads();
         prefix = (prefix << bits) | s_pick[0];
@@ -363,8 +378,15 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
     };
     round(std::integral_constant<int, 0>{});
     round(std::integral_constant<int, 1>{});
-    round(std::integral_constant<int, 2>{});
-    const uint32_t cut = prefix;  // keys above it stay, and the first `need` equal to it
+    uint32_t cut;  // keys above it stay, and the first `need` equal to it
+    if (prefix != 0 && s_pick[2] == need) {  // all that begin like this, often one: the last digit does not matter
+        cut = (prefix << 10) - 1;
+        need = 0;
+    } else {
+        __syncthreads();  // s_pick is read
+        round(std::integral_constant<int, 2>{});
+        cut = prefix;
+    }
     int sure_n = 0, tie_n = 0;
     each([&](const uint32_t(&k)[4], int) {
 #pragma unroll
@@ -402,16 +424,18 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_select_kernel(const f
             at += __popcll(take);
         }
     };
-    if (!cached) {
-        each_read(write);
-        return;
-    }
-    for (int i0 = r0; i0 < r1; i0 += 256) {
-        uint32_t k[4];
+    if (cached) {
+        for (int i0 = r0; i0 < r1; i0 += 256) {
+            uint32_t k[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = s_key[i0 + 64 * u + lane];
-        write(k, i0);
+            for (int u = 0; u < 4; ++u) k[u] = s_key[i0 + 64 * u + lane];
+            write(k, i0);
+        }
+    } else {
+        fetch(r0, even);
+        each_read(write);
     }
+    finish();
 }
 
 struct EvictMove {
@@ -492,8 +516,9 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(EvictMove
         else move_rows<u32x4, 2, 5, 12>(rows + 3, list, p.keep);
         return;
     }
+    const EvictHead head = evict_head(p.evicted, p.ctl, h, p.keep, p.max_seq);
     move_rows<float, 1, 1, 8>(p.out_weights + base, list, p.keep);
-    evict_finish(p.out_weights, p.evicted, p.out_evicted, p.ctl, h, p.keep, p.max_seq);
+    evict_finish(p.out_weights, p.out_evicted, head, h, p.max_seq);
 }
 
 // two buffers are one and the same, or share no byte

@@ -100,3 +100,47 @@ def test_context_limit(qe):
     with pytest.raises(RuntimeError, match="context window"):
         e.decode(1)
     e.close()
+
+
+def test_file_round_trip(qe, tmp_path):
+    """An engine read from a file holds 4-bit rows too, and says the same."""
+    a = _engine(qe, 1)
+    first = a.prefill(PROMPT)
+    tokens = a.decode(10)
+    path = str(tmp_path / "kv4.qwenbin")
+    a.save_qwenbin(path)
+    qe.set_tuning("engine_kv4", 1)
+    try:
+        b = qe.Engine.from_qwenbin(path, max_seq_len=256, prefill_chunk=64)
+    finally:
+        qe.set_tuning("engine_kv4", 0)
+    assert b.prefill(PROMPT) == first and b.decode(10) == tokens
+    assert np.array_equal(a.logits().view(np.uint16), b.logits().view(np.uint16))
+    rows = [e.read("kcache", np.uint8, 2 * 256 * ref.ROW) for e in (a, b)]
+    assert np.array_equal(*rows) and rows[0].any()
+    a.close(), b.close()
+
+
+def test_what_an_engine_says_and_how_likely_it_was(qe):
+    """Tokens of an engine on a 4-bit cache are the most likely ones of its logits, with the probability of the definition."""
+    import torch
+
+    e = _engine(qe, 1)
+    token = e.prefill(PROMPT)
+    for _ in range(5):
+        logits = e.logits()
+        x = torch.from_numpy(logits.copy()).cuda()
+        ids = torch.tensor([token], dtype=torch.int32, device="cuda")
+        lp, entropy = (torch.empty(1, device="cuda") for _ in range(2))
+        top, top_ids = torch.empty((1, 8), device="cuda"), torch.empty((1, 8), dtype=torch.int32, device="cuda")
+        ws = torch.empty(qe.token_logprobs_workspace_bytes(1, x.numel(), 8), dtype=torch.uint8, device="cuda")
+        qe.launch_token_logprobs(x, ids, lp, entropy, top, top_ids, ws, 1, vocab_size=x.numel(), top_k=8)
+        want, want_entropy, want_top, want_ids, spread = ref.logprobs(logits[None], [token], 8)
+        assert int(top_ids[0, 0]) == token and np.array_equal(top_ids.cpu().numpy(), want_ids)
+        # fp32: the logit, the maximum and the logarithm are added with three roundings; sums of 4096 terms
+        size = np.abs(logits.astype(np.float64)).max() + 20
+        assert abs(float(lp) - want[0]) <= 2.0 ** -20 * size
+        assert abs(float(entropy) - want_entropy[0]) <= 2.0 ** -20 * (size + spread[0])
+        assert float(top[0, 0]) == float(lp)
+        token = e.decode(1)[0]
+    e.close()

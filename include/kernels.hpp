@@ -385,12 +385,14 @@ inline void launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_
                   "launch_kv4_evict");
 }
 
+// row_stride 0: rows of vocab_size logits behind each other.
 inline void launch_token_logprobs(const half* logits, const int32_t* token_ids, float* out_logprob,
                                   float* out_entropy, float* out_top_logprob, int32_t* out_top_ids, void* workspace,
                                   int num_rows, hipStream_t stream, int vocab_size = VOCAB_SIZE,
-                                  long long row_stride = VOCAB_SIZE, int top_k = 0) {
+                                  long long row_stride = 0, int top_k = 0) {
     detail::check(qe_launch_token_logprobs(detail::h(logits), token_ids, out_logprob, out_entropy, out_top_logprob,
-                                           out_top_ids, workspace, num_rows, vocab_size, row_stride, top_k, stream),
+                                           out_top_ids, workspace, num_rows, vocab_size,
+                                           row_stride == 0 ? vocab_size : row_stride, top_k, stream),
                   "launch_token_logprobs");
 }
 

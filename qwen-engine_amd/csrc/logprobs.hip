@@ -25,6 +25,8 @@ constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
 // segment of any length, is seldom; with few 4 (8192), so that a row is spread over the chip.
 constexpr int kLpFew = 4, kLpMany = 16;
 constexpr int lp_segment(int chunks) { return 8 * kLpThreads * chunks; }
+// Vocabularies, at most: a row's last segment, which begins before index vocab + 7, ends within 31 bits.
+constexpr int kLpMaxVocab = INT32_MAX - 7 - lp_segment(kLpMany);
 
 // Candidates of a wave in LDS.
 constexpr int kLpCandidates = 1024;
@@ -416,7 +418,7 @@ using namespace qe;
 extern "C" int qe_token_logprobs_workspace_bytes(int num_rows, int vocab_size, int top_k, size_t* bytes) {
     const char* what = "token_logprobs_workspace_bytes";
     QE_REQUIRE(bytes != nullptr, "%s: NULL pointer", what);
-    QE_REQUIRE(num_rows >= 0 && vocab_size > 0 && vocab_size <= INT32_MAX - lp_segment(kLpMany) && top_k >= 0 && top_k <= kLpMaxTop,
+    QE_REQUIRE(num_rows >= 0 && vocab_size > 0 && vocab_size <= kLpMaxVocab && top_k >= 0 && top_k <= kLpMaxTop,
                "%s: num_rows=%d vocab_size=%d top_k=%d", what, num_rows, vocab_size, top_k);
     *bytes = static_cast<size_t>(num_rows) * lp_segments(vocab_size, kLpFew) * lp_words(top_k) * sizeof(uint32_t);
     return QE_OK;
@@ -430,7 +432,7 @@ extern "C" int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* t
     QE_REQUIRE(logits && workspace, "%s: NULL pointer", what);
     QE_REQUIRE((token_ids == nullptr) == (out_logprob == nullptr), "%s: token_ids and out_logprob are given together",
                what);
-    QE_REQUIRE(vocab_size > 0 && vocab_size <= INT32_MAX - lp_segment(kLpMany), "%s: vocab_size=%d", what, vocab_size);
+    QE_REQUIRE(vocab_size > 0 && vocab_size <= kLpMaxVocab, "%s: vocab_size=%d", what, vocab_size);
     QE_REQUIRE(row_stride >= vocab_size || num_rows <= 1, "%s: row_stride=%lld < vocab_size=%d", what, row_stride,
                vocab_size);
     QE_REQUIRE(top_k >= 0 && top_k <= kLpMaxTop && top_k <= vocab_size, "%s: top_k=%d (0..%d, at most vocab_size)", what,

@@ -1,0 +1,32 @@
+"""The largest sizes that the 4-bit cache and log probability entry points take: what their kernels' 32-bit indices
+can count.  Decided on the host before any HIP call (no GPU needed)."""
+import ctypes
+
+import pytest
+
+P = 0x100000  # an aligned address; nothing is launched
+INT_MAX = 2**31 - 1
+
+
+@pytest.fixture(scope="module")
+def L():
+    import qe_amd
+    return qe_amd.lib()
+
+
+def _says(L, rc, text):
+    assert rc == 1 and text in L.qe_last_error().decode(), (rc, L.qe_last_error())
+
+
+def test_vocabularies_whose_last_segment_ends_past_32_bits(L):
+    """Segments of up to 32768 logits begin up to 7 logits before the row, and a thread counts its chunk's end: the
+    last segment's end has to be an int.  vocab + 7 + 32767 is the sum that says how many segments there are."""
+    n = ctypes.c_size_t()
+    for vocab in (INT_MAX - 32768, INT_MAX - 32773):
+        last = (vocab + 6) // 32768 * 32768
+        assert vocab + 7 + 32767 > INT_MAX and last + 32768 > INT_MAX
+        _says(L, L.qe_token_logprobs_workspace_bytes(1, vocab, 0, ctypes.byref(n)), "vocab_size")
+        _says(L, L.qe_launch_token_logprobs(P, P, P, None, None, None, P, 1, vocab, ctypes.c_longlong(vocab), 0, None),
+              "vocab_size")
+    assert L.qe_token_logprobs_workspace_bytes(1, INT_MAX - 32775, 0, ctypes.byref(n)) == 0
+    assert n.value == -(-(INT_MAX - 32775 + 7) // 8192) * 3 * 4

@@ -57,6 +57,8 @@ constexpr int kKd4MaxSplits = 128;   // runs of a kv head, at most
 constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each of four waves
 constexpr int kKd4MaxGroup = 64;     // q heads of a kv head
 constexpr int kKd4ManyWaves = 16;    // of a block where runs may be longer (waves without rows do nothing)
+// rows of a cache, at most: the last run ends up to 32 kKd4MaxSplits rows behind it, a wave's next tile 32 kKd4ManyWaves
+constexpr int kKd4MaxRows = INT32_MAX - 8191;
 
 // rows of a run for `ctx` rows over at most `splits` runs
 __host__ __device__ __forceinline__ int kd4_run(int ctx, int splits) {
@@ -1034,7 +1036,7 @@ using namespace qe;
 
 extern "C" int qe_kv4_decode_workspace_bytes(int num_q_heads, int max_seq_len, int with_key_weights, size_t* bytes) {
     QE_REQUIRE(bytes != nullptr, "kv4_decode_workspace_bytes: NULL pointer");
-    QE_REQUIRE(num_q_heads > 0 && max_seq_len > 0 && max_seq_len <= INT32_MAX - 31,
+    QE_REQUIRE(num_q_heads > 0 && max_seq_len > 0 && max_seq_len <= kKd4MaxRows,
                "kv4_decode_workspace_bytes: num_q_heads=%d max_seq_len=%d", num_q_heads, max_seq_len);
     size_t floats = static_cast<size_t>(num_q_heads) * kKd4MaxSplits * (kKv4Dim + 2);
     if (with_key_weights) floats += static_cast<size_t>(num_q_heads) * score_stride(max_seq_len);
@@ -1054,7 +1056,7 @@ extern "C" int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const
     QE_REQUIRE(q && workspace && attn_out, "%s: NULL pointer", what);
     QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
     QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
-    QE_REQUIRE(max_seq_len <= INT32_MAX - 31, "%s: max_seq_len=%d", what, max_seq_len);
+    QE_REQUIRE(max_seq_len <= kKd4MaxRows, "%s: max_seq_len=%d", what, max_seq_len);
     QE_REQUIRE(aligned(q, 16) && aligned(workspace, 16), "%s: q and the workspace must be 16-byte aligned", what);
     QE_REQUIRE(key_weights_in == nullptr || key_weights_out != nullptr, "%s: key_weights_in without key_weights_out",
                what);

@@ -30,3 +30,19 @@ def test_vocabularies_whose_last_segment_ends_past_32_bits(L):
               "vocab_size")
     assert L.qe_token_logprobs_workspace_bytes(1, INT_MAX - 32775, 0, ctypes.byref(n)) == 0
     assert n.value == -(-(INT_MAX - 32775 + 7) // 8192) * 3 * 4
+
+
+def test_caches_whose_runs_end_past_32_bits(L):
+    """Decode cuts a cache into up to 128 runs, each rounded up to 32 rows: the end of the last one, up to 128 * 32 rows
+    behind the cache, and a wave's next 32 * 16 rows have to be ints."""
+    n = ctypes.c_size_t()
+    for rows in (INT_MAX - 31, INT_MAX - 4094):
+        run = -(-(-(-rows // 128)) // 32) * 32
+        assert rows + 127 > INT_MAX or 128 * run > INT_MAX
+        for weights in (0, 1):
+            _says(L, L.qe_kv4_decode_workspace_bytes(1, rows, weights, ctypes.byref(n)), "max_seq_len")
+        _says(L, L.qe_launch_attention_gqa_flash_decode_kv4(P, P, P, P, P, None, None, None, 1, 1, 128, rows, None, None,
+                                                            None, None, None), "max_seq_len")
+    rows = INT_MAX - 8191
+    assert L.qe_kv4_decode_workspace_bytes(1, rows, 1, ctypes.byref(n)) == 0
+    assert n.value == (128 * 130 + rows + (-rows) % 32) * 4

@@ -1145,6 +1145,10 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     const long long rows = static_cast<long long>(num_tokens) * p.group;
     QE_REQUIRE(rows <= (1 << 29) && max_seq_len <= (1 << 29), "%s: num_tokens=%d max_seq_len=%d", what, num_tokens,
                max_seq_len);
+    // the weights' kernel counts a tile of q rows in 32 bits of bytes
+    QE_REQUIRE(key_weights_out == nullptr ||
+                   static_cast<long long>(kW4Rows / p.group) * num_q_heads * kKv4Dim * 2 <= (1LL << 32),
+               "%s: num_q_heads=%d with key weights", what, num_q_heads);
     // Eight waves and one block per CU expand a tile for 256 rows; four waves for
     // 128, two blocks per CU, where there are few row blocks: their splits are shorter and
     // fewer rows idle.  (12 q heads, 2 kv heads, all in us: 40 tokens at 1200 13.1 against

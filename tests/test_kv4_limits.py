@@ -46,3 +46,16 @@ def test_caches_whose_runs_end_past_32_bits(L):
     rows = INT_MAX - 8191
     assert L.qe_kv4_decode_workspace_bytes(1, rows, 1, ctypes.byref(n)) == 0
     assert n.value == (128 * 130 + rows + (-rows) % 32) * 4
+
+
+def test_key_weights_of_more_heads_than_a_tile_of_q_rows_can_address(L):
+    """A tile of q rows holds the 128 // group tokens that 128 rows of one kv head hold; their places in q are byte
+    offsets of 32 bits from the tile's first."""
+    def prefill(nq, nkv, T=128):
+        far = P + T * nq * 256
+        return L.qe_launch_attention_gqa_prefill_kv4(P, P, P, far, None, None, T, None, nq, nkv, 128, 64, nq * 128, None,
+                                                     P, P)
+    for nq, nkv in ((131073, 131073), (2 * 131073, 131073), (64 * 131073, 131073)):
+        group = nq // nkv
+        assert (128 // group) * nq * 256 > 2**32
+        _says(L, prefill(nq, nkv), "num_q_heads")

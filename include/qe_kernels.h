@@ -513,7 +513,8 @@ int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint8_t* layer_
  * d_control->seq_pos - keep.  Heads with n <= keep keep everything.  kept_rows
  * (int32 [num_kv_heads][keep]) receives the old rows of the new ones, -1 behind the last.
  * K, V and weights are all moved in place (the outputs are the inputs) or all into memory
- * apart from them, which is faster; out_evicted may be d_evicted either way. */
+ * apart from them, which is faster; out_evicted may be d_evicted either way.  No other two of
+ * the buffers written, and of those and the buffers read, may share memory (refused). */
 int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, const float* key_weights,
                         const int32_t* d_evicted, uint8_t* out_k_cache, uint8_t* out_v_cache, float* out_key_weights,
                         int32_t* out_evicted, int32_t* kept_rows, const qe_device_control_block* d_control, int keep,

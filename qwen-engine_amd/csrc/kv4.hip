@@ -599,10 +599,23 @@ extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* 
     const bool in_place = layer_k_cache == out_k_cache;
     QE_REQUIRE(in_place == (layer_v_cache == out_v_cache) && in_place == (key_weights == out_key_weights),
                "%s: K, V and weights are all in place or all apart", what);
-    QE_REQUIRE(same_or_apart(layer_k_cache, out_k_cache, rows * kKv4Row) &&
-                   same_or_apart(layer_v_cache, out_v_cache, rows * kKv4Row) &&
-                   same_or_apart(key_weights, out_key_weights, rows * sizeof(float)),
-               "%s: an output overlaps its input without being it", what);
+    // Blocks do not wait for each other: an output may be its own input, and otherwise meets nothing.
+    struct Span {
+        const void* at;
+        size_t bytes;
+    };
+    const size_t counts = num_kv_heads * sizeof(int32_t);
+    const Span in[] = {{layer_k_cache, rows * kKv4Row}, {layer_v_cache, rows * kKv4Row}, {key_weights, rows * sizeof(float)},
+                       {d_evicted, d_evicted ? counts : 0}};
+    const Span out[] = {{out_k_cache, rows * kKv4Row}, {out_v_cache, rows * kKv4Row}, {out_key_weights, rows * sizeof(float)},
+                        {out_evicted, counts}, {kept_rows, static_cast<size_t>(num_kv_heads) * keep * sizeof(int32_t)}};
+    bool clear = true;
+    for (int o = 0; o < 5; ++o) {
+        for (int i = 0; i < 4; ++i)
+            clear &= (i == o && in[i].at == out[o].at) || apart(in[i].at, in[i].bytes, out[o].at, out[o].bytes);
+        for (int u = 0; u < o; ++u) clear &= apart(out[u].at, out[u].bytes, out[o].at, out[o].bytes);
+    }
+    QE_REQUIRE(clear, "%s: an output overlaps another, or an input without being it", what);
     const size_t lds = std::min(kEvictWaves * evict_run(max_seq_len), kEvictCached) * sizeof(uint32_t);
     kv4_evict_select_kernel<<<num_kv_heads, kEvictThreads, lds, stream>>>(key_weights, d_evicted, d_control, kept_rows,
                                                                           keep, sinks, recent, max_seq_len,

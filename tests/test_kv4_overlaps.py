@@ -1,0 +1,51 @@
+"""Buffers of the 4-bit cache calls that share memory where kernels would read what others have written: refused on
+the host before any HIP call (no GPU needed)."""
+import ctypes
+
+import pytest
+
+MB = 1 << 20
+
+
+@pytest.fixture(scope="module")
+def L():
+    import qe_amd
+    return qe_amd.lib()
+
+
+def _says(L, rc, text):
+    assert rc == 1 and text in L.qe_last_error().decode(), (rc, L.qe_last_error())
+
+
+def test_evict(L):
+    """2 heads, 64 rows: caches of 10240 bytes, weights of 512, counts of 8, kept rows of 256.  Rows, weights and counts
+    are moved by blocks that do not wait for each other: no two outputs meet, and an output meets no input but its own."""
+    cache, weights = 2 * 64 * 80, 2 * 64 * 4
+    inputs = dict(kc=MB, vc=2 * MB, w=3 * MB, gone=4 * MB)
+    apart = dict(ok=5 * MB, ov=6 * MB, ow=7 * MB, og=8 * MB, kept=9 * MB)
+
+    def evict(**kw):
+        a = {**inputs, **apart, **kw}
+        return L.qe_launch_kv4_evict(a["kc"], a["vc"], a["w"], a["gone"], a["ok"], a["ov"], a["ow"], a["og"], a["kept"],
+                                     10 * MB, 32, 4, 8, None, 2, 128, 64)
+
+    in_place = dict(ok=MB, ov=2 * MB, ow=3 * MB, og=4 * MB)
+    last = dict(kc=cache - 16, vc=cache - 16, w=weights - 16, gone=4, ok=cache - 16, ov=cache - 16, ow=weights - 16, og=4,
+                kept=252)
+    # apart: each output on another's last bytes, and on the last bytes of an input that is not its own
+    for out in apart:
+        for other in (*inputs, *apart):
+            if other == out or (out, other) in (("ok", "kc"), ("ov", "vc"), ("ow", "w")):
+                continue
+            if (out, other) == ("og", "gone"):  # may be it, but not part of it
+                _says(L, evict(og=inputs["gone"] + 4), "overlap")
+                continue
+            at = {**inputs, **apart}[other] + last[other]
+            _says(L, evict(**{out: at // 16 * 16 if out in ("ok", "ov") else at}), "overlap")
+    # swapped: K moves to where V comes from
+    _says(L, evict(ok=2 * MB, ov=MB, ow=7 * MB), "overlap")
+    # in place: one cache for both, lists and counts inside what moves
+    _says(L, evict(**{**in_place, "kc": MB, "vc": MB, "ok": MB, "ov": MB}), "overlap")
+    for kw in (dict(kept=MB), dict(kept=2 * MB + cache - 4), dict(kept=3 * MB), dict(kept=4 * MB + 4), dict(og=2 * MB),
+               dict(og=3 * MB + weights - 4), dict(og=4 * MB + 4)):
+        _says(L, evict(**{**in_place, **kw}), "overlap")

@@ -458,11 +458,12 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
 
 /* Bias, NeoX RoPE and append of num_tokens tokens from d_control->seq_pos on, as
  * qe_launch_qkv_bias_rope_kv_append does for an fp16 cache: q [T][num_q_heads][128]
- * biased, rotated and written to q_out (which may be q; no other overlap), k and v
+ * biased, rotated and written to q_out (which may be q), k and v
  * [T][num_kv_heads][128] biased, k rotated, both stored in 4 bits (k and v themselves
  * are not written).  Biases may be NULL.  Sums and rotation in fp32, angles in 64 bits,
  * one rounding at the end.  head_dim 128; rotary_dim 0 (= 128) or a multiple of 16 up
- * to 128; q, k, v and the biases 16-byte aligned. */
+ * to 128; q, k, v and the biases 16-byte aligned.  Apart from q_out over q, what is written
+ * shares memory with nothing (refused). */
 int qe_launch_qkv_bias_rope_kv4_append(const uint16_t* q, uint16_t* q_out, const uint16_t* k, const uint16_t* v,
                                        const uint16_t* q_bias, const uint16_t* k_bias, const uint16_t* v_bias,
                                        uint8_t* layer_k_cache, uint8_t* layer_v_cache,

@@ -521,8 +521,11 @@ __global__ __launch_bounds__(kEvictThreads) void kv4_evict_move_kernel(EvictMove
     evict_finish(p.out_weights, p.out_evicted, head, h, p.max_seq);
 }
 
-// two buffers are one and the same, or share no byte
-inline bool same_or_apart(const void* a, const void* b, size_t bytes) { return a == b || apart(a, bytes, b, bytes); }
+struct Span {
+    const void* at;
+    size_t bytes;
+};
+inline bool apart(const Span& a, const Span& b) { return qe::apart(a.at, a.bytes, b.at, b.bytes); }
 
 }  // namespace
 }  // namespace qe
@@ -548,8 +551,17 @@ extern "C" int qe_launch_qkv_bias_rope_kv4_append(const uint16_t* q, uint16_t* q
                    aligned(k_bias, 16) && aligned(v_bias, 16),
                "%s: q, k, v and the biases must be 16-byte aligned", what);
     if (num_tokens <= 0) return QE_OK;
-    QE_REQUIRE(same_or_apart(q, q_out, static_cast<size_t>(num_tokens) * num_q_heads * kKv4Dim * 2),
-               "%s: q_out overlaps q", what);
+    // Blocks do not wait for each other: q_out may be q, and otherwise what is written meets nothing.
+    const size_t head = kKv4Dim * 2, q_row = num_q_heads * head, kv_row = num_kv_heads * head;
+    const size_t cache = static_cast<size_t>(num_kv_heads) * max_seq_len * kKv4Row;
+    const Span in[] = {{q, num_tokens * q_row},       {k, num_tokens * kv_row},       {v, num_tokens * kv_row},
+                       {q_bias, q_bias ? q_row : 0},  {k_bias, k_bias ? kv_row : 0},  {v_bias, v_bias ? kv_row : 0},
+                       {d_evicted, d_evicted ? num_kv_heads * sizeof(int32_t) : 0}};
+    const Span out[] = {{q_out, num_tokens * q_row}, {layer_k_cache, cache}, {layer_v_cache, cache}};
+    bool clear = apart(out[0], out[1]) && apart(out[0], out[2]) && apart(out[1], out[2]);
+    for (const Span& o : out)
+        for (const Span& i : in) clear &= apart(i, o) || (&o == out && &i == in && q == q_out);
+    QE_REQUIRE(clear, "%s: q_out or a cache overlaps another buffer", what);
     const long long heads = static_cast<long long>(num_q_heads) + num_kv_heads;
     QE_REQUIRE(heads <= 65535 * 16, "%s: %lld heads", what, heads);
     const dim3 grid(num_tokens, static_cast<unsigned>((heads + 15) / 16));
@@ -600,10 +612,6 @@ extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* 
     QE_REQUIRE(in_place == (layer_v_cache == out_v_cache) && in_place == (key_weights == out_key_weights),
                "%s: K, V and weights are all in place or all apart", what);
     // Blocks do not wait for each other: an output may be its own input, and otherwise meets nothing.
-    struct Span {
-        const void* at;
-        size_t bytes;
-    };
     const size_t counts = num_kv_heads * sizeof(int32_t);
     const Span in[] = {{layer_k_cache, rows * kKv4Row}, {layer_v_cache, rows * kKv4Row}, {key_weights, rows * sizeof(float)},
                        {d_evicted, d_evicted ? counts : 0}};
@@ -611,9 +619,8 @@ extern "C" int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* 
                         {out_evicted, counts}, {kept_rows, static_cast<size_t>(num_kv_heads) * keep * sizeof(int32_t)}};
     bool clear = true;
     for (int o = 0; o < 5; ++o) {
-        for (int i = 0; i < 4; ++i)
-            clear &= (i == o && in[i].at == out[o].at) || apart(in[i].at, in[i].bytes, out[o].at, out[o].bytes);
-        for (int u = 0; u < o; ++u) clear &= apart(out[u].at, out[u].bytes, out[o].at, out[o].bytes);
+        for (int i = 0; i < 4; ++i) clear &= apart(in[i], out[o]) || (i == o && in[i].at == out[o].at);
+        for (int u = 0; u < o; ++u) clear &= apart(out[u], out[o]);
     }
     QE_REQUIRE(clear, "%s: an output overlaps another, or an input without being it", what);
     const size_t lds = std::min(kEvictWaves * evict_run(max_seq_len), kEvictCached) * sizeof(uint32_t);

@@ -49,3 +49,27 @@ def test_evict(L):
     for kw in (dict(kept=MB), dict(kept=2 * MB + cache - 4), dict(kept=3 * MB), dict(kept=4 * MB + 4), dict(og=2 * MB),
                dict(og=3 * MB + weights - 4), dict(og=4 * MB + 4)):
         _says(L, evict(**{**in_place, **kw}), "overlap")
+
+
+def test_append(L):
+    """3 tokens, 4 q heads, 2 kv heads, 64 rows.  Heads are rotated and stored by blocks that do not wait for each other:
+    q_out may be q and meets nothing else that is read, the caches meet nothing."""
+    q, kv, cache, counts = 3 * 4 * 256, 3 * 2 * 256, 2 * 64 * 80, 8
+    at = dict(q=MB, k=2 * MB, v=3 * MB, qb=4 * MB, kb=5 * MB, vb=6 * MB, q_out=MB, kc=7 * MB, vc=8 * MB, gone=9 * MB)
+    size = dict(q=q, k=kv, v=kv, qb=4 * 256, kb=2 * 256, vb=2 * 256, q_out=q, kc=cache, vc=cache, gone=counts)
+
+    def append(T=3, **kw):
+        a = {**at, **kw}
+        return L.qe_launch_qkv_bias_rope_kv4_append(a["q"], a["q_out"], a["k"], a["v"], a["qb"], a["kb"], a["vb"], a["kc"],
+                                                    a["vc"], None, a["gone"], T, None, 4, 2, 128, 64, 0,
+                                                    ctypes.c_float(1e6))
+    for out in ("q_out", "kc", "vc"):
+        for other in at:
+            if other in (out, "q_out") or (out, other) == ("q_out", "q"):
+                continue
+            _says(L, append(**{out: at[other] + (size[other] - 1) // 16 * 16}), "overlap")
+            if out != "q_out" and other != "q":
+                _says(L, append(**{out: at[other] + 16 - size[out]}), "overlap")
+    _says(L, append(q_out=MB + 16), "overlap")
+    _says(L, append(kc=MB, vc=7 * MB), "overlap")
+    assert append(T=0, kc=MB) == 0

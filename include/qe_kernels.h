@@ -449,8 +449,8 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
  * Key weights: float [num_kv_heads][max_seq_len], what the queries have given to a
  * cache row so far: the sum of its softmax weights over queries and over the q heads of
  * the kv head.  Attention reads key_weights_in (NULL = zeros) and writes key_weights_out
- * for the rows in use, in place when both are the same pointer; rows behind them keep
- * what they hold, and the rows of the launch's own tokens start from zero.
+ * for the rows in use, in place when both are the same pointer (they may not share memory
+ * otherwise); rows behind them keep what they hold, and the rows of the launch's own tokens start from zero.
  *
  * Streams and graphs: launches keep no state and allocate nothing.  Recorded into a
  * graph they read d_control and d_evicted at replay. */
@@ -498,7 +498,8 @@ int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const uint8_t* l
  * (appended before) over the 4-bit cache: the counterpart of
  * qe_launch_attention_gqa_prefill, which also says when the split workspace is used.
  * row_lse (float [T][num_q_heads], NULL = not wanted) receives the natural logarithm
- * of each row's softmax sum; key weights need it, and an attn_out apart from q. */
+ * of each row's softmax sum; key weights need it.  attn_out shares no memory with q, or, without
+ * key weights and with rows behind each other (hidden_size = 128 num_q_heads), is q. */
 int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
                                         uint16_t* attn_out, const qe_device_control_block* d_control,
                                         const int32_t* d_evicted, int num_tokens, hipStream_t stream,

@@ -1027,6 +1027,15 @@ inline int check_heads(const char* what, int nq, int nkv) {
     return QE_OK;
 }
 
+// key weights in place or apart
+inline int check_weights(const char* what, const float* in, const float* out, int nkv, int max_seq) {
+    QE_REQUIRE(in == nullptr || out != nullptr, "%s: key_weights_in without key_weights_out", what);
+    const size_t bytes = static_cast<size_t>(nkv) * max_seq * sizeof(float);
+    QE_REQUIRE(in == nullptr || in == out || apart(in, bytes, out, bytes),
+               "%s: key_weights_out overlaps key_weights_in without being it", what);
+    return QE_OK;
+}
+
 inline int score_stride(int max_seq) { return (max_seq + 31) / 32 * 32; }
 
 }  // namespace
@@ -1058,8 +1067,7 @@ extern "C" int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const
     QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
     QE_REQUIRE(max_seq_len <= kKd4MaxRows, "%s: max_seq_len=%d", what, max_seq_len);
     QE_REQUIRE(aligned(q, 16) && aligned(workspace, 16), "%s: q and the workspace must be 16-byte aligned", what);
-    QE_REQUIRE(key_weights_in == nullptr || key_weights_out != nullptr, "%s: key_weights_in without key_weights_out",
-               what);
+    QE_TRY(check_weights(what, key_weights_in, key_weights_out, num_kv_heads, max_seq_len));
     Decode4Params p{};
     p.q = q;
     p.kc = layer_k_cache;
@@ -1116,14 +1124,13 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
     QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
     QE_REQUIRE(hidden_size >= num_q_heads * head_dim && hidden_size % 4 == 0, "%s: hidden_size=%d", what, hidden_size);
-    QE_REQUIRE(key_weights_in == nullptr || key_weights_out != nullptr, "%s: key_weights_in without key_weights_out",
-               what);
+    QE_TRY(check_weights(what, key_weights_in, key_weights_out, num_kv_heads, max_seq_len));
     QE_REQUIRE(key_weights_out == nullptr || row_lse != nullptr, "%s: key weights need row_lse", what);
     QE_REQUIRE(aligned(q, 16) && aligned(attn_out, 8), "%s: q must be 16-byte and attn_out 8-byte aligned", what);
     if (num_tokens <= 0) return QE_OK;
-    // the weights' kernel reads q after the outputs are written
+    // a block writes its rows while others read theirs, and the weights' kernel reads q after that
     const size_t q_row = static_cast<size_t>(num_q_heads) * kKv4Dim * 2;
-    QE_REQUIRE(key_weights_out == nullptr ||
+    QE_REQUIRE((key_weights_out == nullptr && q == attn_out && (hidden_size == num_q_heads * kKv4Dim || num_tokens == 1)) ||
                    apart(q, num_tokens * q_row, attn_out, (num_tokens - 1) * static_cast<size_t>(hidden_size) * 2 + q_row),
                "%s: attn_out overlaps q", what);
     Prefill4Params p{};

@@ -73,3 +73,26 @@ def test_append(L):
     _says(L, append(q_out=MB + 16), "overlap")
     _says(L, append(kc=MB, vc=7 * MB), "overlap")
     assert append(T=0, kc=MB) == 0
+
+
+def test_attention(L):
+    """Key weights are added in place or apart, never shifted; a chunk's outputs are its q rows or apart from them (a
+    block writes its rows while others still read theirs)."""
+    T, nq, nkv, rows = 3, 4, 2, 64
+    weights, q = nkv * rows * 4, T * nq * 256
+
+    def decode(w_in, w_out):
+        return L.qe_launch_attention_gqa_flash_decode_kv4(MB, 2 * MB, 3 * MB, 4 * MB, 6 * MB, None, None, None, nq, nkv, 128,
+                                                          rows, None, None, None, w_in, w_out)
+
+    def prefill(out=6 * MB, w_in=None, w_out=None, hidden=nq * 128, lse=5 * MB, T=T):
+        return L.qe_launch_attention_gqa_prefill_kv4(MB, 2 * MB, 3 * MB, out, None, None, T, None, nq, nkv, 128, rows,
+                                                     hidden, w_in, w_out, lse)
+    for shift in (4, weights - 4, -4, 4 - weights):
+        _says(L, decode(7 * MB, 7 * MB + shift), "overlap")
+        _says(L, prefill(w_in=7 * MB, w_out=7 * MB + shift), "overlap")
+    for shift in (8, 256, q - 8, -8, 8 - q):
+        _says(L, prefill(out=MB + shift), "attn_out overlaps q")
+    _says(L, prefill(out=MB, hidden=nq * 128 + 4), "attn_out overlaps q")
+    _says(L, prefill(out=MB - 8 - (T - 1) * 2 * 1024, hidden=1024), "attn_out overlaps q")
+    assert prefill(out=MB + 8, T=0) == 0

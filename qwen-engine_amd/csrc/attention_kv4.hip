@@ -1123,7 +1123,8 @@ extern "C" int qe_launch_attention_gqa_prefill_kv4(const uint16_t* q, const uint
     QE_REQUIRE(q && attn_out, "%s: NULL pointer", what);
     QE_TRY(kv4_check(what, layer_k_cache, layer_v_cache, num_kv_heads, head_dim, max_seq_len));
     QE_TRY(check_heads(what, num_q_heads, num_kv_heads));
-    QE_REQUIRE(hidden_size >= num_q_heads * head_dim && hidden_size % 4 == 0, "%s: hidden_size=%d", what, hidden_size);
+    QE_REQUIRE(hidden_size >= static_cast<long long>(num_q_heads) * head_dim && hidden_size % 4 == 0, "%s: hidden_size=%d", what,
+               hidden_size);
     QE_TRY(check_weights(what, key_weights_in, key_weights_out, num_kv_heads, max_seq_len));
     QE_REQUIRE(key_weights_out == nullptr || row_lse != nullptr, "%s: key weights need row_lse", what);
     QE_REQUIRE(aligned(q, 16) && aligned(attn_out, 8), "%s: q must be 16-byte and attn_out 8-byte aligned", what);

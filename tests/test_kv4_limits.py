@@ -59,3 +59,10 @@ def test_key_weights_of_more_heads_than_a_tile_of_q_rows_can_address(L):
         group = nq // nkv
         assert (128 // group) * nq * 256 > 2**32
         _says(L, prefill(nq, nkv), "num_q_heads")
+
+
+def test_rows_of_outputs_shorter_than_the_q_heads_past_32_bits(L):
+    """128 values of 2^25 heads are 2^32, which an int would take for 0."""
+    rc = L.qe_launch_attention_gqa_prefill_kv4(P, P, P, 1 << 45, None, None, 1, None, 1 << 25, 1 << 25, 128, 64, 128, None,
+                                               None, None)
+    _says(L, rc, "hidden_size")

@@ -154,11 +154,21 @@ def _ptr(t):
 _raw_stream = None
 
 
-def _stream(stream, on=None):
-    """The stream's handle (None: torch's current one).  `on`: a tensor of the call; it must be on the current GPU."""
-    at = None if on is None or isinstance(on, int) else on.get_device()
-    if at == -1:
-        raise RuntimeError(f"the tensors must be on a GPU, not on {on.device}")
+def _stream(stream, *tensors):
+    """The stream's handle (None: torch's current one) for a call on `tensors`, of which all that are tensors (not
+    None, not addresses) must be on one GPU: the stream's, where it says which."""
+    at = None
+    for t in tensors:
+        if t is None or isinstance(t, int):
+            continue
+        gpu = t.get_device()
+        if gpu == at:
+            continue
+        if gpu < 0:
+            raise RuntimeError(f"the tensors must be on a GPU, not on {t.device}")
+        if at is not None:
+            raise RuntimeError(f"the tensors must be on one GPU, not on cuda:{at} and {t.device}")
+        at = gpu
     if stream is None:
         # the handle alone: a Stream object for each call costs 2.9 us, this 0.2
         global _raw_stream
@@ -169,10 +179,12 @@ def _stream(stream, on=None):
         get, device = _raw_stream
         current = device()
         if at is not None and at != current:
-            raise RuntimeError(f"the tensors are on {on.device}, the current GPU is cuda:{current}")
+            raise RuntimeError(f"the tensors are on cuda:{at}, the current GPU is cuda:{current}")
         return get(current)
     if isinstance(stream, int):
         return stream
+    if at is not None and at != getattr(stream, "device_index", at):
+        raise RuntimeError(f"the tensors are on cuda:{at}, the stream is of cuda:{stream.device_index}")
     return stream.cuda_stream
 
 
@@ -426,14 +438,14 @@ def launch_qkv_bias_rope_kv4_append(q, q_out, k, v, q_bias, k_bias, v_bias, laye
                                     max_seq_len=4096, rotary_dim=0, rope_theta=1000000.0):
     _call("qe_launch_qkv_bias_rope_kv4_append", _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_bias), _ptr(k_bias),
           _ptr(v_bias), _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(d_control), _ptr(d_evicted), num_tokens,
-          _stream(stream, q), num_q_heads, num_kv_heads, head_dim, max_seq_len, rotary_dim, rope_theta)
+          _stream(stream, q, q_out, k, v, q_bias, k_bias, v_bias, layer_k_cache, layer_v_cache, d_control, d_evicted),
+          num_q_heads, num_kv_heads, head_dim, max_seq_len, rotary_dim, rope_theta)
 
 
 def launch_kv4_unpack(layer_k_cache, layer_v_cache, out_k, out_v, first_row, num_rows, stream=None, num_kv_heads=2,
                       head_dim=128, max_seq_len=4096):
-    given = layer_v_cache if layer_k_cache is None else layer_k_cache
     _call("qe_launch_kv4_unpack", _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(out_k), _ptr(out_v), first_row,
-          num_rows, _stream(stream, given), num_kv_heads, head_dim, max_seq_len)
+          num_rows, _stream(stream, layer_k_cache, layer_v_cache, out_k, out_v), num_kv_heads, head_dim, max_seq_len)
 
 
 def kv4_decode_workspace_bytes(num_q_heads=12, max_seq_len=4096, key_weights=False) -> int:
@@ -449,17 +461,21 @@ def launch_attention_gqa_flash_decode_kv4(q, layer_k_cache, layer_v_cache, works
                                           out_q8=None, out_scale=None, out_sum8=None, key_weights_in=None,
                                           key_weights_out=None):
     _call("qe_launch_attention_gqa_flash_decode_kv4", _ptr(q), _ptr(layer_k_cache), _ptr(layer_v_cache),
-          _ptr(workspace), _ptr(attn_out), _ptr(d_control), _ptr(d_evicted), _stream(stream, q), num_q_heads,
-          num_kv_heads, head_dim, max_seq_len, _ptr(out_q8), _ptr(out_scale), _ptr(out_sum8), _ptr(key_weights_in),
-          _ptr(key_weights_out))
+          _ptr(workspace), _ptr(attn_out), _ptr(d_control), _ptr(d_evicted),
+          _stream(stream, q, layer_k_cache, layer_v_cache, workspace, attn_out, d_control, d_evicted, out_q8, out_scale,
+                  out_sum8, key_weights_in, key_weights_out),
+          num_q_heads, num_kv_heads, head_dim, max_seq_len, _ptr(out_q8), _ptr(out_scale), _ptr(out_sum8),
+          _ptr(key_weights_in), _ptr(key_weights_out))
 
 
 def launch_attention_gqa_prefill_kv4(q, layer_k_cache, layer_v_cache, attn_out, d_control, d_evicted, num_tokens,
                                      stream=None, num_q_heads=12, num_kv_heads=2, head_dim=128, max_seq_len=4096,
                                      hidden_size=1536, key_weights_in=None, key_weights_out=None, row_lse=None):
     _call("qe_launch_attention_gqa_prefill_kv4", _ptr(q), _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(attn_out),
-          _ptr(d_control), _ptr(d_evicted), num_tokens, _stream(stream, q), num_q_heads, num_kv_heads, head_dim,
-          max_seq_len, hidden_size, _ptr(key_weights_in), _ptr(key_weights_out), _ptr(row_lse))
+          _ptr(d_control), _ptr(d_evicted), num_tokens,
+          _stream(stream, q, layer_k_cache, layer_v_cache, attn_out, d_control, d_evicted, key_weights_in,
+                  key_weights_out, row_lse),
+          num_q_heads, num_kv_heads, head_dim, max_seq_len, hidden_size, _ptr(key_weights_in), _ptr(key_weights_out), _ptr(row_lse))
 
 
 def launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
@@ -467,7 +483,10 @@ def launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k
                      head_dim=128, max_seq_len=4096):
     _call("qe_launch_kv4_evict", _ptr(layer_k_cache), _ptr(layer_v_cache), _ptr(key_weights), _ptr(d_evicted),
           _ptr(out_k_cache), _ptr(out_v_cache), _ptr(out_key_weights), _ptr(out_evicted), _ptr(kept_rows),
-          _ptr(d_control), keep, sinks, recent, _stream(stream, layer_k_cache), num_kv_heads, head_dim, max_seq_len)
+          _ptr(d_control), keep, sinks, recent,
+          _stream(stream, layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
+                  out_evicted, kept_rows, d_control),
+          num_kv_heads, head_dim, max_seq_len)
 
 
 # ---- log probabilities ---------------------------------------------------------------
@@ -483,7 +502,8 @@ def launch_token_logprobs(logits, token_ids, out_logprob, out_entropy, out_top_l
                           num_rows, vocab_size=151936, row_stride=None, top_k=0, stream=None):
     _call("qe_launch_token_logprobs", _ptr(logits), _ptr(token_ids), _ptr(out_logprob), _ptr(out_entropy),
           _ptr(out_top_logprob), _ptr(out_top_ids), _ptr(workspace), num_rows, vocab_size,
-          vocab_size if row_stride is None else row_stride, top_k, _stream(stream, logits))
+          vocab_size if row_stride is None else row_stride, top_k,
+          _stream(stream, logits, token_ids, out_logprob, out_entropy, out_top_logprob, out_top_ids, workspace))
 
 
 # ---- engine ------------------------------------------------------------------------

@@ -507,7 +507,7 @@ __device__ __forceinline__ float xor32_max(float x) {
 template <int KG, bool DMA>
 __global__ __launch_bounds__(256 * KG, 2) void prefill_attention_kernel(PrefillAttnParams p) {
     // per key group: K buffers 0 and 1, V buffers 0 and 1
-    __shared__ __align__(16) char smem[KG * 4 * kPaTileBytes];
+    __shared__ __align__(256) char smem[KG * 4 * kPaTileBytes];  // for reads that turn address bits 5 to 7
     const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wave = wave_all & 3, kg = wave_all >> 2;
     const int fr = lane & 31, h = lane >> 5;

@@ -535,8 +535,9 @@ int qe_token_logprobs_workspace_bytes(int num_rows, int vocab_size, int top_k, s
  * qe_launch_sample_and_advance settles them.  NULL outputs are skipped.  -inf logits have
  * probability 0; a row of nothing else has log probabilities -inf and entropy 0; a
  * row with a NaN or +inf has NaN log probabilities, and NaN logits are never among the
- * alternatives (id -1 where there are too few).  `workspace` (4-byte aligned, the size
- * above) is scratch that two launches in flight must not share. */
+ * alternatives (id -1 where there are too few).  With no rows the buffers may be NULL.
+ * `workspace` (4-byte aligned, the size above) is scratch that two launches in flight must
+ * not share. */
 int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* token_ids, float* out_logprob, float* out_entropy,
                              float* out_top_logprob, int32_t* out_top_ids, void* workspace, int num_rows,
                              int vocab_size, long long row_stride, int top_k, hipStream_t stream);

@@ -429,18 +429,18 @@ extern "C" int qe_launch_token_logprobs(const uint16_t* logits, const int32_t* t
                                         void* workspace, int num_rows, int vocab_size, long long row_stride, int top_k,
                                         hipStream_t stream) {
     const char* what = "token_logprobs";
-    QE_REQUIRE(logits && workspace, "%s: NULL pointer", what);
-    QE_REQUIRE((token_ids == nullptr) == (out_logprob == nullptr), "%s: token_ids and out_logprob are given together",
-               what);
     QE_REQUIRE(vocab_size > 0 && vocab_size <= kLpMaxVocab, "%s: vocab_size=%d", what, vocab_size);
     QE_REQUIRE(row_stride >= vocab_size || num_rows <= 1, "%s: row_stride=%lld < vocab_size=%d", what, row_stride,
                vocab_size);
     QE_REQUIRE(top_k >= 0 && top_k <= kLpMaxTop && top_k <= vocab_size, "%s: top_k=%d (0..%d, at most vocab_size)", what,
                top_k, kLpMaxTop);
+    if (num_rows <= 0) return QE_OK;  // buffers of no rows may be NULL
+    QE_REQUIRE(logits && workspace, "%s: NULL pointer", what);
+    QE_REQUIRE((token_ids == nullptr) == (out_logprob == nullptr), "%s: token_ids and out_logprob are given together",
+               what);
     QE_REQUIRE((out_top_logprob == nullptr && out_top_ids == nullptr) || top_k > 0, "%s: top outputs with top_k=0", what);
     QE_REQUIRE(top_k == 0 || out_top_logprob || out_top_ids, "%s: top_k=%d without an output", what, top_k);
     QE_REQUIRE(aligned(logits, 2) && aligned(workspace, 4), "%s: alignment", what);
-    if (num_rows <= 0) return QE_OK;
     // many: enough rows for two blocks of long segments on every CU
     const bool many = static_cast<long long>(num_rows) * lp_segments(vocab_size, kLpMany) >= 2LL * cu_count();
     const int chunks = many ? kLpMany : kLpFew, segments = lp_segments(vocab_size, chunks);

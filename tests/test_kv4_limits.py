@@ -1,5 +1,5 @@
-"""The largest sizes that the 4-bit cache and log probability entry points take: what their kernels' 32-bit indices
-can count.  Decided on the host before any HIP call (no GPU needed)."""
+"""The largest and smallest sizes that the 4-bit cache and log probability entry points take: what their kernels'
+32-bit indices can count, and no rows.  Decided on the host before any HIP call (no GPU needed)."""
 import ctypes
 
 import pytest
@@ -66,3 +66,16 @@ def test_rows_of_outputs_shorter_than_the_q_heads_past_32_bits(L):
     rc = L.qe_launch_attention_gqa_prefill_kv4(P, P, P, 1 << 45, None, None, 1, None, 1 << 25, 1 << 25, 128, 64, 128, None,
                                                None, None)
     _says(L, rc, "hidden_size")
+
+
+def test_no_rows(L):
+    """The size query says 0 bytes for no rows, and an allocation of none may be NULL, as that of no logits."""
+    n = ctypes.c_size_t(1)
+    assert L.qe_token_logprobs_workspace_bytes(0, 100, 5, ctypes.byref(n)) == 0 and n.value == 0
+
+    def lp(x, ws, rows):
+        return L.qe_launch_token_logprobs(x, P, P, None, None, None, ws, rows, 100, ctypes.c_longlong(100), 0, None)
+    assert lp(None, None, 0) == 0 and lp(P, None, 0) == 0 and lp(None, P, 0) == 0
+    assert L.qe_launch_token_logprobs(*[None] * 7, 0, 100, ctypes.c_longlong(100), 5, None) == 0
+    for x, ws in ((None, P), (P, None)):
+        _says(L, lp(x, ws, 1), "NULL")

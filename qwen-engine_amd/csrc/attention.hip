@@ -969,14 +969,6 @@ extern "C" int qe_launch_attention_gqa_flash_decode_combine(const float* splitk_
 
 namespace qe {
 
-// Whether launches on the stream are being recorded into a graph (or the runtime will not say).
-static bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &st) == hipSuccess) return st != hipStreamCaptureStatusNone;
-    (void)hipGetLastError();
-    return true;
-}
-
 // Prefill attention; max_context bounds the positions the rows see (the
 // engine knows it on the host, the public entry point only max_seq_len).
 int launch_prefill_attention(const uint16_t* q, const uint16_t* layer_k_cache, const uint16_t* layer_v_cache,

@@ -1017,13 +1017,6 @@ __global__ __launch_bounds__(256) void kv4_prefill_weights_merge_kernel(Prefill4
     p.w_out[at] = (key < base ? was : 0.0f) + x;
 }
 
-inline bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &st) == hipSuccess) return st != hipStreamCaptureStatusNone;
-    (void)hipGetLastError();
-    return true;
-}
-
 inline int check_heads(const char* what, int nq, int nkv) {
     QE_REQUIRE(nq > 0 && nq % nkv == 0, "%s: %d q heads over %d kv heads", what, nq, nkv);
     QE_REQUIRE(nq / nkv <= kKd4MaxGroup, "%s: %d q heads for each kv head (at most %d)", what, nq / nkv, kKd4MaxGroup);

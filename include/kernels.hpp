@@ -359,16 +359,18 @@ inline void launch_attention_gqa_flash_decode_kv4(const half* q, const uint8_t* 
                   "launch_attention_gqa_flash_decode_kv4");
 }
 
+// hidden_size 0: rows of num_q_heads * head_dim outputs behind each other.
 inline void launch_attention_gqa_prefill_kv4(const half* q, const uint8_t* layer_k_cache, const uint8_t* layer_v_cache,
                                              half* attn_out, const DeviceControlBlock* d_control,
                                              const int32_t* d_evicted, int num_tokens, hipStream_t stream,
                                              int num_q_heads = NUM_Q_HEADS, int num_kv_heads = NUM_KV_HEADS,
                                              int head_dim = HEAD_DIM, int max_seq_len = MAX_SEQ_LEN,
-                                             int hidden_size = HIDDEN_SIZE, const float* key_weights_in = nullptr,
+                                             int hidden_size = 0, const float* key_weights_in = nullptr,
                                              float* key_weights_out = nullptr, float* row_lse = nullptr) {
     detail::check(qe_launch_attention_gqa_prefill_kv4(detail::h(q), layer_k_cache, layer_v_cache, detail::h(attn_out),
                                                       d_control, d_evicted, num_tokens, stream, num_q_heads,
-                                                      num_kv_heads, head_dim, max_seq_len, hidden_size,
+                                                      num_kv_heads, head_dim, max_seq_len,
+                                                      hidden_size == 0 ? num_q_heads * head_dim : hidden_size,
                                                       key_weights_in, key_weights_out, row_lse),
                   "launch_attention_gqa_prefill_kv4");
 }

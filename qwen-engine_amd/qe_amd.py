@@ -472,11 +472,11 @@ def launch_attention_gqa_flash_decode_kv4(q, layer_k_cache, layer_v_cache, works
 
 def launch_attention_gqa_prefill_kv4(q, layer_k_cache, layer_v_cache, attn_out, d_control, d_evicted, num_tokens,
                                      stream=None, num_q_heads=12, num_kv_heads=2, head_dim=128, max_seq_len=4096,
-                                     hidden_size=1536, key_weights_in=None, key_weights_out=None, row_lse=None):
+                                     hidden_size=None, key_weights_in=None, key_weights_out=None, row_lse=None):
     s, p = _on_gpu(stream, q, layer_k_cache, layer_v_cache, attn_out, d_control, d_evicted, key_weights_in,
                    key_weights_out, row_lse)
     _call("qe_launch_attention_gqa_prefill_kv4", *p[:6], num_tokens, s, num_q_heads, num_kv_heads, head_dim, max_seq_len,
-          hidden_size, *p[6:])
+          num_q_heads * head_dim if hidden_size is None else hidden_size, *p[6:])
 
 
 def launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,

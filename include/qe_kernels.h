@@ -483,7 +483,8 @@ int qe_kv4_decode_workspace_bytes(int num_q_heads, int max_seq_len, int with_key
 
 /* Attention of one token (position d_control->seq_pos, its row appended before) over
  * the 4-bit cache: the counterpart of qe_launch_attention_gqa_flash_decode, Q8_1
- * outputs included (out_q8 NULL = none).  `workspace` (16-byte aligned, the size
+ * outputs included (out_q8 NULL = none; a head whose attn_out is NaN has q8 of 0 and a scale
+ * of 1e-8, as there).  `workspace` (16-byte aligned, the size
  * above) is scratch that two launches in flight must not share.  At most 64 q heads
  * for each kv head.  The cache is split over blocks by max_seq_len, the number of heads
  * and the rows in use; a launch's bits depend on those alone. */

@@ -749,7 +749,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv4_prefill_kernel(Prefill4Para
     lsum += __shfl_xor(lsum, 32);
     if (r >= rows) return;
     if (live == 1) {
-        const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+        const float inv = 1.0f / lsum;  // (0 only where every score is -inf: NaN)
         uint16_t* o = p.out + static_cast<size_t>(qi) * p.out_stride + qh * kKv4Dim;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -826,7 +826,7 @@ __global__ __launch_bounds__(256 * GROUPS) void kv4_prefill_merge_kernel(Prefill
         }
         const float l = qwen::seg_sum<32>(w[0] * ml[0].y + w[1] * ml[1].y);
         if (lane == 0) {
-            s_inv[row] = l > 0.0f ? 1.0f / l : 0.0f;
+            s_inv[row] = 1.0f / l;
             if (p.lse != nullptr && r0 + row < rows)
                 p.lse[static_cast<size_t>(rr / p.group) * p.nq + kvh * p.group + rr % p.group] =
                     (m == -INFINITY ? 0.0f : m) * kLn2 + logf(l);

@@ -98,3 +98,40 @@ def test_eight_waves_and_the_poison_of_a_later_token(qe, workspace):
             _check(qe, kv, q[:at], at, nq, base, [0, 0], ms, got[:at], lse[:at])
         w = host(w)
         assert np.all(np.isnan(w[:, :base + at + 1])) and np.all(w[:, base + T:] == 0)
+
+
+def test_rows_whose_every_score_is_minus_infinity(qe, workspace):
+    """A query with an infinity where every key is of the other sign: no softmax, so NaN, from every form alike."""
+    rng = np.random.default_rng(61)
+    nq, nkv, ms, ctx = 12, 2, 2048, 1500
+    kv = _cache(rng, nkv, ms, ctx)
+    k = rng.standard_normal((nkv, ctx, 128)) + 3.0
+    group = np.clip(k, 0.5, None).reshape(nkv, ctx, 4, 32)  # every key value positive
+    low = group.min(-1).astype(np.float16)
+    scale = ((group.max(-1) - low) / 15).astype(np.float16)
+    kv[0, :, :ctx] = ref.pack(np.clip(np.rint((group - low[..., None]) / scale[..., None]), 0, 15).reshape(nkv, ctx, 128),
+                              scale, low)
+    assert (ref.values(kv[0, :, :ctx]) > 0).all()
+    for T, base in ((40, 1400), (40, 3), (600, 800)):  # splits, none, eight waves
+        q = rng.standard_normal((T, nq * 128)).astype(np.float16)
+        q[5, 4 * 128 + 9] = -np.inf
+        out, lse = _prefill(qe, kv, q, T, nq, base, None, ms, lse=True)
+        assert np.all(np.isnan(out[5, 4 * 128:5 * 128])) and lse[5, 4] == -np.inf
+        out[5, 4 * 128:5 * 128] = 0
+        assert np.all(np.isfinite(out))
+    assert np.all(np.isnan(_decode(qe, kv, q[5], nq, 1000, None, ms)[4 * 128:5 * 128]))
+
+
+def test_q8_of_a_head_that_is_nan(qe):
+    """attn_out is NaN; Q8_1 cannot say so: zeros with the smallest scale, as the fp16 flash decode's epilogue."""
+    rng = np.random.default_rng(62)
+    nq, nkv, ms = 12, 2, 500
+    kv = _cache(rng, nkv, ms, 400)
+    clean = _decode(qe, kv, np.ones(nq * 128, np.float16), nq, 399, None, ms, q8=True)
+    kv[0, 1, 250, 64:] = np.frombuffer(np.full(8, 0x7E00, np.uint16).tobytes(), np.uint8)
+    out, q8, scale, sum8 = _decode(qe, kv, np.ones(nq * 128, np.float16), nq, 399, None, ms, q8=True)
+    half = nq // 2 * 128
+    assert np.all(np.isnan(out[half:])) and np.all(q8[half:] == 0) and np.all(sum8[half // 8:] == 0)
+    assert np.all(scale[nq // 2:] == np.float32(1e-8))
+    for got, want in zip((out, q8, scale, sum8), clean):
+        assert np.array_equal(got[:got.size // 2], want[:want.size // 2])

@@ -434,9 +434,14 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
  * word w, then four pairs (scale, low) of fp16, one for every 32 elements.  A nibble
  * n stands for fp16(n * scale + low), rounded once.  Storing x: low = fp16(min),
  * scale = fp16((max - low) / 15), or the fp16 below where 15 * scale + low would be
- * infinite, n = clamp(rint((x - low) / scale), 0, 15), n = 0 for a scale of 0.  A token whose K or V holds a value that fp16 cannot (infinite,
- * NaN, 65520 and more) is stored with NaN pairs in its K row: every row that
- * attends to it gives NaN, rows that do not are untouched.
+ * infinite, n = clamp(rint((x - low) / scale), 0, 15), n = 0 for a scale of 0.  A token
+ * whose K or V holds a value that fp16 cannot (infinite, NaN, 65520 and more) is stored
+ * with NaN pairs in its K row: every row that attends to it gives NaN, rows that do not
+ * are untouched.
+ *
+ * Attention on this cache: scores, softmax sums and outputs in fp32; the softmax weights
+ * are rounded to fp16 (2^-11) for the product with V, in decode too, where
+ * qe_launch_attention_gqa_flash_decode keeps them in fp32; outputs rounded once to fp16.
  *
  * The row of position p is p - d_evicted[kv_head]: d_evicted (device int32
  * [num_kv_heads], NULL = zeros) counts the positions that eviction has taken out of
@@ -450,7 +455,8 @@ int qe_launch_attention_gqa_prefill(const uint16_t* q, const uint16_t* layer_k_c
  * cache row so far: the sum of its softmax weights over queries and over the q heads of
  * the kv head.  Attention reads key_weights_in (NULL = zeros) and writes key_weights_out
  * for the rows in use, in place when both are the same pointer (they may not share memory
- * otherwise); rows behind them keep what they hold, and the rows of the launch's own tokens start from zero.
+ * otherwise); rows behind them keep what they hold, and the rows of the launch's own
+ * tokens start from zero.
  *
  * Streams and graphs: launches keep no state and allocate nothing.  Recorded into a
  * graph they read d_control and d_evicted at replay. */
@@ -484,10 +490,10 @@ int qe_kv4_decode_workspace_bytes(int num_q_heads, int max_seq_len, int with_key
 /* Attention of one token (position d_control->seq_pos, its row appended before) over
  * the 4-bit cache: the counterpart of qe_launch_attention_gqa_flash_decode, Q8_1
  * outputs included (out_q8 NULL = none; a head whose attn_out is NaN has q8 of 0 and a scale
- * of 1e-8, as there).  `workspace` (16-byte aligned, the size
- * above) is scratch that two launches in flight must not share.  At most 64 q heads
- * for each kv head.  The cache is split over blocks by max_seq_len, the number of heads
- * and the rows in use; a launch's bits depend on those alone. */
+ * of 1e-8, as there).  `workspace` (16-byte aligned, the size above) is scratch that two
+ * launches in flight must not share.  At most 64 q heads for each kv head.  The cache is
+ * split over blocks by max_seq_len, the number of heads and the rows in use; a launch's
+ * bits depend on those alone. */
 int qe_launch_attention_gqa_flash_decode_kv4(const uint16_t* q, const uint8_t* layer_k_cache,
                                              const uint8_t* layer_v_cache, void* workspace, uint16_t* attn_out,
                                              const qe_device_control_block* d_control, const int32_t* d_evicted,

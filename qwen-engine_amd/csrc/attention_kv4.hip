@@ -49,10 +49,14 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 // A run is short where the cache is short (a block's start and end cost 2 us, a tile
 // of 32 rows 0.15), and there are at most 128: the merge reads them all.  12 q heads
 // on 2 kv heads, with the merge's 3 to 4 us behind it: 300 rows 4.3 us, 16001 with the
-// scores kept 5.1, 131000 12.3 (42 MB, 3.4 TB/s; a plain read of as much takes 7.6).
-// Short caches wait for the launch and one round of loads; long ones issue vector
-// instructions (24 for a word of eight nibbles, the matrix cores busy 9 %): neither more
-// rows in flight nor 8 waves for 16 changes them.
+// scores kept 5.1, 131000 12.1 (42 MB, 3.5 TB/s; a plain read of as much takes 7.6).
+// Short caches wait for the launch and one round of loads.  At 131000 rows a wave has two
+// tiles: its vector instructions (24 for each MFMA) fill 57 % of the cycles, the matrix
+// cores 9 %, and the rest is the start, the two waits for loads, the meeting in LDS and
+// the end.  Neither more rows in flight nor 8 waves for 16 changed it.
+// Probabilities are rounded to fp16 for the product with V, their sum l is not (the
+// fp16 flash decode keeps both in fp32): 2^-11 of each, as prefill does, and below what a
+// nibble leaves of V.
 constexpr int kKd4MaxSplits = 128;   // runs of a kv head, at most
 constexpr int kKd4MinRun = 128;      // rows of a run, at least: 32 for each of four waves
 constexpr int kKd4MaxGroup = 64;     // q heads of a kv head
@@ -294,7 +298,7 @@ __device__ __forceinline__ void kd4_run_weights(Kd4RunSums& r, int live, int lan
 
 // Blocks 0..nq-1: one q head each, its runs merged (32 lanes x 4 dims, 16 groups
 // of runs), rounded once to fp16, and the Q8_1 of it when asked for.  The blocks
-// behind them, with key weights: 256 rows of one kv head, the sum over its q
+// behind them, with key weights: 512 rows of one kv head, the sum over its q
 // heads of exp2(score - M) / L added to the weight so far; the newest row
 // starts at its own sum.  A launch and two rounds of loads: 3.0 us with 3 runs,
 // 3.8 with 128, 4.2 with the weights of 16001 rows.
@@ -403,14 +407,18 @@ __global__ __launch_bounds__(kKd4MergeThreads) void kv4_decode_merge_kernel(Deco
 // before they are expanded; a split's first two tiles are requested at once, and four
 // waves with no more than two take them from there (17 tokens at 1200: 12.9 -> 10.4 us in
 // all, a third of it the coalesced partials below).
-// Bound by the vector instructions between the products (6.5 for each MFMA, one of them
-// an exponential at a quarter of the rate), which overlap the MFMAs in part: 2048 tokens
-// at 14000 (12 q heads, 2 kv heads) take 222 us with the merge, 0.85 PFLOP/s of the 1.25
-// that a large fp16 product reaches, MFMAs busy 54 %; without the exponentials or without
-// the expansion they would take a tenth less, without the barrier 3 %.  Slower: 64 rows a
-// wave (by 15 %: the scores move through the accumulation registers), the block's halves
-// half a step apart (by 24 %: the probabilities that cross the barrier do not fit the
-// registers).
+// 2048 tokens at 14000 (12 q heads, 2 kv heads) take 224 us with the merge, 0.84 PFLOP/s of
+// the 1.5 to 1.6 that a large product reaches.  Two things bound them.  Splits are whole
+// per row block: 96 row blocks make 192 blocks of one per CU, and a quarter of the CUs has
+// none.  On the others MFMAs are busy 54 %, beside the vector instructions between them
+// (6.5 for each MFMA, one of them an exponential at a quarter of the rate), which overlap in
+// part; without the exponentials or without the expansion they would take a tenth less,
+// without the barrier 3 %.  Slower: 64 rows a wave (by 15 %: the scores move through the
+// accumulation registers), the block's halves half a step apart (by 24 %: the
+// probabilities that cross the barrier do not fit the registers).
+// Registers: all 256, and scratch where a wave ends with two tiles: with four waves 70
+// values (216 bytes a lane), with eight 2, stored and read back once; the steps have none.
+// Probabilities are rounded to fp16 for the product with V, their sum is not.
 constexpr int kP4Keys = 64;
 constexpr int kP4TileBytes = kP4Keys * kKv4Dim * 2;
 // Tiles of a split, at least, and of the splits beyond the eighth, whose merge costs
@@ -876,8 +884,8 @@ __global__ __launch_bounds__(256 * GROUPS) void kv4_prefill_merge_kernel(Prefill
 // places in a tile are always the same), comes to LDS by DMA, whole rows of 256 bytes,
 // while the one before is used, and wave w takes its rows 32 (w % 4).. for its K
 // rows.  A lane keeps 16 sums; lanes, then waves, then the splits of the q rows add
-// up in one order.  Bound by the exponentials and what little is around them (MFMAs
-// busy 29 %).  1000 rows on 2900..3900 positions (12 q heads, 2 kv heads): 50 us with
+// up in one order.  The log sum's rounding, 2^-24 of it, is in every weight of its row.
+// Bound by the exponentials and what little is around them (MFMAs busy 29 %).  1000 rows on 2900..3900 positions (12 q heads, 2 kv heads): 50 us with
 // operands read from memory, 32 bytes of 32 rows at a time (their addresses alone), 29
 // with 32 K rows a block and a q tile for each wave, 22 and 5 for the splits' merge now.
 constexpr int kW4Keys = 64, kW4Rows = 128;

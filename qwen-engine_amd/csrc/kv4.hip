@@ -212,16 +212,17 @@ __device__ __forceinline__ void evict_finish(float* out_weights, int32_t* out_ev
 // largest keys, equal ones by the lowest index: radix selection of the keep-th
 // largest, then one ordered pass that writes the kept indices.
 // Up to 32768 rows the keys are read from memory once and stay in LDS; more rows are
-// read again in every pass, eight loads a lane ahead (60000 rows, copy included, 48 us; with
+// read again in every pass, eight loads a lane ahead (60000 rows, copy included, 40 to 48 us; with
 // four loads and their wait at a time 81).  A wave owns a run of rows, a multiple of 256
 // so that a lane can take four keys with one LDS read wherever their order does not
 // matter.  Digits of 11, 11 and 10 bits: the first holds the sign, the exponent and two
 // bits of the mantissa, so that weights of like size still spread over the bins and
 // lanes seldom meet in one; the third is looked at only where some, not all, of
-// the keys with the same first 22 bits stay.  One CU a head, so instructions count: 4096
-// rows take 6.0 us (2 heads), 32000 17.7 (8 heads); with the loads waited for before
-// the first count and always three digits 7.3 and 21, with digits of 8 bits, four rounds over
-// memory and a branch for every key 10.3 and 53.
+// the keys with the same first 22 bits stay.  One CU a head, its vector units busy a
+// little over half the time, then waits, barriers and LDS: 4096 rows take 6.0 us (2
+// heads), 32000 17.7 (8 heads); with the loads waited for before the first count and always
+// three digits 7.3 and 21, with digits of 8 bits, four rounds over memory and a branch for
+// every key 10.3 and 53.
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictCached = 32768;  // keys in LDS

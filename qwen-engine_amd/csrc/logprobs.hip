@@ -104,8 +104,10 @@ __device__ __forceinline__ T lp_merge(T a, T b, int lane) {
 // with c = m L rounded; what the rounding leaves, r = m L - c, is the same for every
 // logit of the wave and comes off at the end: S = 2^-r S', T = ln 2 (T' - r S') 2^-r.
 // Per logit that is a conversion, the multiply-add, the exponential, two sums, a clamp
-// (-inf times 0) and a comparison: bound by these beside the memory.  1024 rows of 151936
-// with five alternatives 61 us (311 MB, 5.1 TB/s; a plain read takes 47), one row 6.1.
+// (-inf times 0) and a comparison, 6.5 vector instructions, and with long segments as many
+// again that a wave has whatever its logits are (filling with -inf, the row's edges, the
+// alternatives' cut and sorts): 12.7 counted, beside the memory.  1024 rows of 151936 with
+// five alternatives 61 us (311 MB, 5.1 TB/s; a plain read takes 47), one row 6.2.
 template <int CHUNKS>
 __global__ __launch_bounds__(kLpThreads, 4) void token_logprobs_segment_kernel(const uint16_t* __restrict__ logits,
                                                                                float* __restrict__ stats,

@@ -177,7 +177,7 @@ def _stream(stream, gpu=None):
 
 def _on_gpu(stream, *tensors):
     """The stream's handle and the addresses of a call's tensors, None and addresses as they are; the tensors must all
-    be on one GPU, the stream's where it says which.  (One loop for both: 0.1 us more than the addresses alone.)"""
+    be on one GPU, the stream's where it says which.  (One loop for both: 0.05 us a tensor more than the addresses alone.)"""
     gpu, addresses = None, []
     for t in tensors:
         if t is None or isinstance(t, int):

@@ -478,8 +478,8 @@ int qe_launch_qkv_bias_rope_kv4_append(const uint16_t* q, uint16_t* q_out, const
                                        int head_dim, int max_seq_len, int rotary_dim, float rope_theta);
 
 /* Rows first_row .. first_row + num_rows - 1 of every head as fp16
- * [num_kv_heads][num_rows][128] (16-byte aligned).  Either cache may be left out,
- * together with its output. */
+ * [num_kv_heads][num_rows][128] (16-byte aligned, apart from the caches and each other).
+ * Either cache may be left out, together with its output. */
 int qe_launch_kv4_unpack(const uint8_t* layer_k_cache, const uint8_t* layer_v_cache, uint16_t* out_k, uint16_t* out_v,
                          int first_row, int num_rows, hipStream_t stream, int num_kv_heads, int head_dim,
                          int max_seq_len);

@@ -587,6 +587,14 @@ extern "C" int qe_launch_kv4_unpack(const uint8_t* layer_k_cache, const uint8_t*
     if (num_rows <= 0) return QE_OK;
     QE_REQUIRE(first_row >= 0 && first_row <= max_seq_len - num_rows, "%s: rows %d..%lld of %d", what, first_row,
                static_cast<long long>(first_row) + num_rows - 1, max_seq_len);
+    const size_t cache = static_cast<size_t>(num_kv_heads) * max_seq_len * kKv4Row;
+    const size_t rows = static_cast<size_t>(num_kv_heads) * num_rows * kKv4Dim * 2;
+    const Span in[] = {{layer_k_cache, layer_k_cache ? cache : 0}, {layer_v_cache, layer_v_cache ? cache : 0}};
+    const Span out[] = {{out_k, out_k ? rows : 0}, {out_v, out_v ? rows : 0}};
+    bool clear = apart(out[0], out[1]);
+    for (const Span& x : out)
+        for (const Span& i : in) clear &= apart(i, x);
+    QE_REQUIRE(clear, "%s: an output overlaps another buffer", what);
     const dim3 grid((static_cast<unsigned>(num_rows) + 15) / 16, num_kv_heads, 2);
     kv4_unpack_kernel<<<grid, 256, 0, stream>>>(layer_k_cache, layer_v_cache, out_k, out_v, first_row, num_rows,
                                                 max_seq_len);

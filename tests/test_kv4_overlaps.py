@@ -96,3 +96,16 @@ def test_attention(L):
     _says(L, prefill(out=MB, hidden=nq * 128 + 4), "attn_out overlaps q")
     _says(L, prefill(out=MB - 8 - (T - 1) * 2 * 1024, hidden=1024), "attn_out overlaps q")
     assert prefill(out=MB + 8, T=0) == 0
+
+
+def test_unpack(L):
+    """Rows come out 3.2 times as wide, by blocks that do not wait for each other: outputs meet neither cache nor each
+    other."""
+    cache, out = 2 * 64 * 80, 2 * 10 * 256
+
+    def unpack(kc=MB, vc=2 * MB, ok=3 * MB, ov=4 * MB, n=10):
+        return L.qe_launch_kv4_unpack(kc, vc, ok, ov, 5, n, None, 2, 128, 64)
+    for kw in (dict(ok=MB), dict(ok=2 * MB + cache - 16), dict(ov=MB + 16 - out), dict(ov=2 * MB), dict(ov=3 * MB + out - 16),
+               dict(kc=None, ok=None, ov=2 * MB + 16), dict(vc=None, ov=None, ok=MB + cache - 16)):
+        _says(L, unpack(**kw), "overlap")
+    assert unpack(ok=MB, n=0) == 0

@@ -529,6 +529,141 @@ int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cac
                         int32_t* out_evicted, int32_t* kept_rows, const qe_device_control_block* d_control, int keep,
                         int sinks, int recent, hipStream_t stream, int num_kv_heads, int head_dim, int max_seq_len);
 
+/* ---- paged key/value cache: many sequences ------------------------------------------ */
+/* No counterpart in the reference (one sequence, one contiguous cache).  A layer's K and
+ * V lie in pages of page_size tokens (16, 32, 64, 128 or 256), fp16
+ * [page][num_kv_heads][page_size][128], page_stride elements from page to page (0 =
+ * behind each other; K and V may take turns in one allocation), 16-byte aligned.
+ * Position p of sequence s is row p % page_size of page block_table[s][p / page_size].
+ * Table entries outside [0, num_pages), and positions of max_pages * page_size and more,
+ * have no row: nothing is stored there, and nobody attends to them. */
+typedef struct qe_paged_cache {
+    uint16_t* k;
+    uint16_t* v;
+    long long page_stride;
+    int num_pages, page_size, num_kv_heads, head_dim;
+} qe_paged_cache;
+
+/* The rows of a launch (device arrays, read when the kernels run; a recorded launch reads
+ * them at replay).  Rows query_start[s] .. query_start[s + 1] - 1 are the new tokens of
+ * sequence s, at positions context_len[s], context_len[s] + 1, ...; query_start NULL: row s
+ * is the one new token of sequence s (num_tokens = num_seqs).  query_start does not
+ * decrease.  num_tokens is the number of rows the buffers hold: rows of no sequence, and
+ * those of sequences with a negative context_len, are neither read nor written (a batch
+ * padded to a recorded size).  Each entry point says which rows of a cache it writes; two
+ * sequences may share pages that neither writes. */
+typedef struct qe_paged_batch {
+    const int32_t* block_table; /* [num_seqs][max_pages] */
+    const int32_t* query_start; /* [num_seqs + 1] or NULL */
+    const int32_t* context_len; /* [num_seqs] */
+    int num_seqs, num_tokens, max_pages;
+} qe_paged_batch;
+
+/* Rotary positions: pair i of the first rotary_dim (a multiple of 16 up to 128) elements
+ * of a head turns by position * turns[i] full turns (device doubles, [rotary_dim / 2]),
+ * and is multiplied by `scale`.  The pair is elements i and i + rotary_dim / 2, or, when
+ * interleaved, 2 i and 2 i + 1. */
+typedef struct qe_rope {
+    const double* turns;
+    int rotary_dim, interleaved;
+    float scale;
+} qe_rope;
+
+/* Fills `turns` (host memory, [rotary_dim / 2]) and the factor for qe_rope.  With f_i =
+ * theta^(-2i / rotary_dim) / (2 pi), the plain frequencies, and L = original_positions, the
+ * length trained on:
+ *   QE_ROPE_PLAIN   f_i, factor 1;
+ *   QE_ROPE_LINEAR  f_i / factor, factor 1;
+ *   QE_ROPE_RAMP    (1 - r_i) f_i + r_i f_i / factor, where r_i goes evenly from 0 to 1 between
+ *                   the pair (rounded down) that turns high_turns times within L and the one
+ *                   (rounded up) that turns low_turns times; 0.1 ln(factor) + 1;
+ *   QE_ROPE_BANDS   the same with r_i = (high_turns - L f_i) / (high_turns - low_turns) within
+ *                   [0, 1]: evenly in the number of turns; factor 1.
+ * factor >= 1, 0 < low_turns < high_turns (usual: 1 and 32, or 1 and 4).  Host only. */
+#define QE_ROPE_PLAIN 0
+#define QE_ROPE_LINEAR 1
+#define QE_ROPE_RAMP 2
+#define QE_ROPE_BANDS 3
+int qe_rope_turns(double* turns, float* scale, int rotary_dim, double theta, int kind, double factor,
+                  double original_positions, double low_turns, double high_turns);
+
+/* Bias, norm of each q and k head, rotation and append of the batch's tokens: the
+ * counterpart of qe_launch_qkv_bias_rope_kv_append.  q [num_tokens][num_q_heads][128],
+ * rows q_stride elements apart, goes to q_out (rows behind each other; may be q itself where
+ * q's are too); k and v, rows kv_stride apart, go to the cache and are not written.  A stride of
+ * 0 means rows behind each other.  x = x + bias; then, where the norm's weights [128] are given, x =
+ * x * weight / sqrt(mean(x^2) + norm_eps) for each head; then the rotation (rope NULL: none).
+ * Biases and norms may be NULL.  Sums, norm and rotation in fp32, angles in 64 bits, one
+ * rounding at the end.  A token whose V holds a value that fp16 cannot (infinite, NaN,
+ * 65520 and more) is stored with NaN in its K row and zeros in its V row, head by head: who
+ * attends to it gets NaN, and who does not is untouched.  All buffers 16-byte aligned, strides
+ * multiples of 8.  Apart from q_out over q, what is written shares memory with nothing (refused). */
+int qe_launch_qkv_norm_rope_paged_append(const uint16_t* q, uint16_t* q_out, const uint16_t* k, const uint16_t* v,
+                                         const uint16_t* q_bias, const uint16_t* k_bias, const uint16_t* v_bias,
+                                         const uint16_t* q_norm, const uint16_t* k_norm, const qe_rope* rope,
+                                         const qe_paged_cache* cache, const qe_paged_batch* batch, hipStream_t stream,
+                                         int num_q_heads, long long q_stride, long long kv_stride, float norm_eps);
+
+/* Attention on this cache: the row at position p attends to the positions up to p, with
+ * window > 0 the last `window` of them, that have a row in the cache; scale 1 / sqrt(128).
+ * Scores, softmax sums and outputs in fp32; the softmax weights are rounded to fp16 (2^-11) for
+ * the product with V; outputs rounded once to fp16.  row_lse (float [num_tokens][num_q_heads],
+ * NULL = not wanted) receives the natural logarithm of each row's softmax sum.  A row with
+ * nothing to attend to gives zeros and -inf; one whose every score is -inf gives NaN and -inf.
+ * Rows of a page that nobody attends to may hold anything.  q and attn_out are
+ * [num_tokens][num_q_heads][128], at most 64 q heads for each kv head; q and `workspace`
+ * 16-byte, attn_out 8-byte aligned.  `workspace` is scratch of the size that the _bytes call
+ * gives (for any batch on any cache), which two launches in flight must not share.  What is
+ * written shares memory with nothing (refused).  The work is divided evenly over the chip by
+ * what block_table, query_start and context_len say: a row's bits depend on them, for the
+ * whole batch, and on nothing else. */
+
+/* One token of each sequence (query_start NULL): the counterpart of
+ * qe_launch_attention_gqa_flash_decode. */
+int qe_paged_decode_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, size_t* bytes);
+int qe_launch_attention_gqa_paged_decode(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                                         void* workspace, uint16_t* attn_out, float* row_lse, hipStream_t stream,
+                                         int num_q_heads, int window);
+
+/* Chunks of new tokens, single ones among them: the counterpart of
+ * qe_launch_attention_gqa_prefill.  The chunk's own K and V are in the cache.  An infinity or
+ * NaN in V (which append stores as a NaN in K) of a position may reach rows up to 128 before it. */
+int qe_paged_prefill_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, size_t* bytes);
+int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                                          void* workspace, uint16_t* attn_out, float* row_lse, hipStream_t stream,
+                                          int num_q_heads, int window);
+
+/* Bounds of the keys of each page: bounds int8 [num_pages][num_kv_heads][256] (16-byte
+ * aligned), bound_steps float [num_pages][num_kv_heads].  With m = max |k| over the rows of a
+ * page in use, bytes 0..127 are ceil(127 max / m) of each of the 128 dims, bytes 128..255
+ * floor(127 min / m), and the step is m; a page with an infinity or NaN has zeros and an infinite
+ * step.  Renewed for the pages that the batch's tokens lie in, whose keys are in the cache
+ * (appended before); others keep what they hold. */
+int qe_launch_paged_key_bounds(const qe_paged_cache* cache, const qe_paged_batch* batch, int8_t* bounds,
+                               float* bound_steps, hipStream_t stream);
+
+/* For each row and kv head the blocks (of page_size positions) worth attending to, of those
+ * up to the row's own that have a page: the first `sinks`, the last `recent` and, of the rest,
+ * those with the highest scores (equal scores: the lower block), num_selected in all; selected
+ * (int32 [num_tokens][num_kv_heads][num_selected]) receives them in ascending order, -1 behind the
+ * last.  A block's score is the largest that its bounds allow a key in it to get from any of the
+ * kv head's q heads, in whole steps: with m_h = max |q| and n = rint(127 q / m_h) of q head h (an
+ * infinity or NaN: zeros), fp32(step * max_h fp32(m_h * sum_d max(n_d high_d, n_d low_d))); an
+ * infinite step comes before every score.  `workspace` (4-byte aligned, the size that the _bytes
+ * call gives) is scratch that two launches in flight must not share. */
+int qe_paged_select_workspace_bytes(int num_tokens, int num_kv_heads, int max_pages, size_t* bytes);
+int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                           const int8_t* bounds, const float* bound_steps, int32_t* selected, void* workspace,
+                           hipStream_t stream, int num_q_heads, int num_selected, int sinks, int recent);
+
+/* Attention of each row to the positions up to its own in the blocks listed for it
+ * (selected int32 [num_tokens][num_kv_heads][num_selected], in any order; negative and other
+ * entries that are no block of the sequence are skipped, a block listed twice counts twice).  The
+ * workspace is qe_paged_decode_workspace_bytes'. */
+int qe_launch_attention_gqa_paged_sparse(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                                         const int32_t* selected, void* workspace, uint16_t* attn_out, float* row_lse,
+                                         hipStream_t stream, int num_q_heads, int num_selected);
+
 /* ---- log probabilities ------------------------------------------------------------- */
 
 /* Bytes of the workspace of qe_launch_token_logprobs (host only). */

@@ -1,0 +1,1129 @@
+// Attention over the paged key/value cache: single tokens, selected blocks, and
+// chunks of many sequences.
+#include <algorithm>
+#include <type_traits>
+
+#include "lds_dma.hpp"
+#include "paged_common.hpp"
+
+namespace qe {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kPgScale = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
+constexpr float kPgLowest = -3.4e38f;  // the maximum of keys whose every score is -inf: a sum of 0, so NaN
+// A row's reference value (what its scores are lowered by before the exponential) is its
+// running maximum, renewed only when that has grown by more than this: weights then reach
+// at most 2^8, and their relative precision in fp16 does not change.
+constexpr float kPgLag = 8.0f;
+
+// ---- shares of the work ------------------------------------------------------
+// The lengths are on the device, so the division of the work is made there.  A
+// segment is one row tile of one kv head of one sequence (or row): a list of key
+// tiles, none of whose parts depend on another's.  All segments behind each other,
+// each as long as its weight (about its number of key tiles), form a line, which is
+// cut into equal shares, one for each block of the launch: every block has the same
+// work whatever the lengths, and a segment that is cut leaves partial results (row
+// maximum, sum and unnormalized outputs), which a second kernel merges.  A block has
+// at most two cut segments: the one that its share begins in (slot 0) and the one
+// that it ends in (slot 1).  Tile t of a segment of n tiles and weight w belongs to the
+// place t * w / n of its stretch; the bits of a row depend on the lengths of the whole
+// batch, through where the cuts fall, and on nothing else.
+struct SegmentCut {    // of the block that has a segment's beginning but not its end
+    long long at, share, weight;  // where the segment begins; the length of a share
+    int tiles, item, head, row_tile;  // tiles 0: there is no such segment
+};
+
+__device__ __forceinline__ long long uniform(long long x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(x) >> 32));
+    return static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Tiles of a segment that lie before place x of the line.
+__device__ __forceinline__ int tiles_before(long long x, long long at, long long weight, int tiles) {
+    if (x <= at) return 0;
+    if (x >= at + weight) return tiles;
+    return min(tiles, static_cast<int>(static_cast<double>(x - at) * tiles / static_cast<double>(weight)));
+}
+
+// One sequence on the line: `heads` times row tiles whose weights are first + step *
+// (i + 1), but at most `most`.
+struct SeqWork {
+    long long first, step, most;
+    int row_tiles, heads;
+
+    __device__ __forceinline__ long long before(long long i) const {  // weight of the first i row tiles
+        long long m = i;
+        if (step > 0) m = min(i, max(0LL, (most - first) / step));
+        return m * first + step * (m * (m + 1) / 2) + (i - m) * most;
+    }
+    __device__ __forceinline__ long long weight(int i) const { return min(most, first + step * (i + 1)); }
+    __device__ __forceinline__ long long all() const { return row_tiles > 0 ? heads * before(row_tiles) : 0; }
+};
+
+// Sum over a wave up to and with each lane.
+__device__ __forceinline__ long long wave_scan(long long x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const long long y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Runs body(sequence, head, row tile, tiles, first tile, end tile, slot) for each piece of a
+// segment in this block's share, by all waves of the block alike, and leaves the cut
+// that its last segment makes.  slot: -1 for a whole segment, else where its partials go.
+// work(s): the SeqWork of sequence s of `seqs`, tiles(s, row tile): its key tiles.
+template <class Work, class Tiles, class Body, class Cut>
+__device__ __forceinline__ void for_share(int block, int blocks, int seqs, long long least_share, Work work, Tiles tiles,
+                                          Body body, Cut cut) {
+    const int lane = threadIdx.x & 63;
+    // the whole line, then the sequence in which the share begins
+    long long total = 0;
+    for (int s0 = 0; s0 < seqs; s0 += 64) {
+        long long w = s0 + lane < seqs ? work(s0 + lane).all() : 0;
+        w = wave_scan(w);
+        total += uniform(__shfl(w, 63));
+    }
+    const long long share = max(least_share, (total + blocks - 1) / blocks);
+    const long long x0 = share * block, x1 = min(total, x0 + share);
+    SegmentCut last{};
+    if (x0 >= x1) {
+        cut(last);
+        return;
+    }
+    int s = 0;
+    long long at = 0;
+    for (int s0 = 0; s0 < seqs; s0 += 64) {
+        long long w = s0 + lane < seqs ? work(s0 + lane).all() : 0;
+        w = wave_scan(w);
+        const long long chunk = uniform(__shfl(w, 63));
+        if (x0 < at + chunk) {
+            const int k = __popcll(__builtin_amdgcn_ballot_w64(at + w <= x0));  // sequences before
+            s = s0 + k;
+            if (k > 0) at += uniform(__shfl(w, k - 1));
+            break;
+        }
+        at += chunk;
+    }
+    s = uniform(s);
+    SeqWork q = work(s);
+    int head, rt;
+    {
+        const long long one = q.before(q.row_tiles);
+        head = static_cast<int>((x0 - at) / one);
+        at += one * head;
+        int lo = 0, hi = q.row_tiles;  // before(lo) <= x0 - at < before(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (q.before(mid) <= x0 - at) lo = mid; else hi = mid;
+        }
+        rt = lo;
+        at += q.before(rt);
+    }
+    head = uniform(head);
+    rt = uniform(rt);
+    at = uniform(at);
+    while (true) {
+        const long long w = q.weight(rt);
+        const int n = tiles(s, rt);
+        const int t0 = tiles_before(x0, at, w, n), t1 = tiles_before(x1, at, w, n);
+        const bool whole = t0 == 0 && t1 == n;
+        if (whole ? n > 0 || x0 <= at : t0 < t1) body(s, head, rt, n, t0, t1, whole ? -1 : t0 == 0 ? 1 : 0);
+        if (t0 == 0 && t1 > 0 && t1 < n) {
+            last = SegmentCut{at, share, w, n, s, head, rt};
+        }
+        at += w;
+        if (at >= x1) break;
+        if (++rt == q.row_tiles) {
+            rt = 0;
+            if (++head == q.heads) {
+                head = 0;
+                do q = work(++s); while (q.row_tiles == 0);
+            }
+        }
+    }
+    cut(last);
+}
+
+// ---- partial results and their merge ------------------------------------------
+// Workspace of a launch of `blocks` blocks and segments of ROWS rows: the cuts, then a
+// (reference value, sum) for each block, slot and row, then 128 unnormalized outputs.
+struct Partials {
+    SegmentCut* cuts;
+    float2* ml;
+    float* o;
+};
+template <int ROWS>
+__host__ __device__ __forceinline__ Partials partials(void* ws, int blocks) {
+    char* at = static_cast<char*>(ws);
+    Partials p;
+    p.cuts = reinterpret_cast<SegmentCut*>(at);
+    at += (sizeof(SegmentCut) * blocks + 255) / 256 * 256;
+    p.ml = reinterpret_cast<float2*>(at);
+    p.o = reinterpret_cast<float*>(at + sizeof(float2) * 2 * blocks * ROWS);
+    return p;
+}
+template <int ROWS>
+constexpr size_t partials_bytes(int blocks) {
+    return (sizeof(SegmentCut) * blocks + 255) / 256 * 256 +
+           static_cast<size_t>(2) * blocks * ROWS * (sizeof(float2) + kPgDim * sizeof(float));
+}
+
+// Where the rows of a segment are: row r of it is q row first + (r0 + r) / per_row (in the
+// order of q rows and, within one, of the group's heads) and head head0 + (r0 + r) % per_row.
+struct RowMap {
+    int first, r0, per_row, head0;
+    __device__ __forceinline__ int row(int r) const { return first + (r0 + r) / per_row; }
+    __device__ __forceinline__ int head(int r) const { return head0 + (r0 + r) % per_row; }
+};
+
+// A merged row: o / sum, and the logarithm of the sum.  No key at all: zeros and -inf.
+__device__ __forceinline__ float row_inverse(float m, float l) { return m == -INFINITY ? 0.0f : 1.0f / l; }
+__device__ __forceinline__ float row_log_sum(float m, float l) {
+    return m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+// What a part with reference value m counts against the common one.
+__device__ __forceinline__ float part_weight(float m, float common) {
+    return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - common);
+}
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    return make_uint2(static_cast<uint32_t>(f2h(a)) | static_cast<uint32_t>(f2h(b)) << 16,
+                      static_cast<uint32_t>(f2h(c)) | static_cast<uint32_t>(f2h(d)) << 16);
+}
+
+// Merges the parts of the segments that were cut: block b looks after the segment that
+// main block b began and did not end.  8 / GROUPS rows a block, GROUPS times 32
+// lanes a row (4 dims each): the groups take every GROUPS-th part.
+template <int ROWS, int GROUPS, class Map>
+__device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out, float* lse, int nq, Map map) {
+    constexpr int kRows = 8 / GROUPS;  // rows of a block
+    constexpr int kParts = 512;        // weights kept at once
+    __shared__ float s_w[kRows][kParts], s_l[kRows][kParts];
+    __shared__ float s_red[kRows][8];
+    __shared__ float4 s_o[GROUPS > 1 ? 8 : 1][32];
+    const Partials p = partials<ROWS>(ws, blocks);
+    const int b = blockIdx.x;
+    const SegmentCut c = p.cuts[b];
+    if (c.tiles == 0) return;
+    RowMap rows;
+    const int live = map(c, rows);
+    const int r_first = blockIdx.y * kRows;
+    if (r_first >= live) return;
+    const long long end = c.at + c.weight;
+    const int parts = static_cast<int>((end - 1) / c.share) - b + 1;  // blocks that share the segment
+    const int tid = threadIdx.x, grp = tid >> 5, lane = tid & 31;
+    const int row_in = GROUPS == 1 ? grp : 0, part_in = GROUPS == 1 ? 0 : grp;
+    const int r = r_first + row_in;
+    auto slot = [&](int i) { return static_cast<size_t>(2 * (b + i) + (i == 0 ? 1 : 0)) * ROWS; };
+    auto holds = [&](int i) {  // block b + i has tiles of the segment
+        const long long x = (b + i) * c.share;
+        return tiles_before(x, c.at, c.weight, c.tiles) < tiles_before(x + c.share, c.at, c.weight, c.tiles);
+    };
+    // the common reference value of each row
+    constexpr int kPer = 256 / kRows;  // threads that read a row's values
+    const int vr = tid / kPer, vi = tid % kPer;
+    float m = -INFINITY;
+    for (int i = vi; i < parts; i += kPer) {
+        float2 v = make_float2(-INFINITY, 0.0f);
+        if (r_first + vr < live && holds(i)) v = p.ml[slot(i) + r_first + vr];
+        if (i < kParts) s_w[vr][i] = v.x, s_l[vr][i] = v.y;
+        m = fmaxf(m, v.x);
+    }
+#pragma unroll
+    for (int d = 1; d < (kPer < 64 ? kPer : 64); d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if constexpr (kPer > 64) {
+        if ((tid & 63) == 0) s_red[0][tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+    } else {
+        if (vi == 0) s_red[vr][0] = m;
+        __syncthreads();
+        m = s_red[row_in][0];
+    }
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < live) {
+        for (int i = part_in; i < parts; i += GROUPS) {
+            float mi, li;
+            if (i < kParts) {
+                mi = s_w[row_in][i], li = s_l[row_in][i];
+            } else {
+                const float2 v = holds(i) ? p.ml[slot(i) + r] : make_float2(-INFINITY, 0.0f);
+                mi = v.x, li = v.y;
+            }
+            if (mi == -INFINITY) continue;
+            const float w = part_weight(mi, m);
+            const float4 v = *reinterpret_cast<const float4*>(p.o + (slot(i) + r) * kPgDim + 4 * lane);
+            l += w * li;
+            o.x += w * v.x;
+            o.y += w * v.y;
+            o.z += w * v.z;
+            o.w += w * v.w;
+        }
+    }
+    if constexpr (GROUPS > 1) {
+        __syncthreads();
+        s_o[grp][lane] = o;
+        if (lane == 0) s_red[0][grp] = l;
+        __syncthreads();
+        if (grp != 0) return;
+        l = s_red[0][0];
+        for (int g = 1; g < GROUPS; ++g) {
+            const float4 v = s_o[g][lane];
+            l += s_red[0][g];
+            o.x += v.x;
+            o.y += v.y;
+            o.z += v.z;
+            o.w += v.w;
+        }
+    }
+    if (r >= live) return;
+    const float inv = row_inverse(m, l);
+    const size_t at = static_cast<size_t>(rows.row(r)) * nq + rows.head(r);
+    *reinterpret_cast<uint2*>(out + at * kPgDim + 4 * lane) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (lse != nullptr && lane == 0) lse[at] = row_log_sum(m, l);
+}
+
+// ---- single tokens and selected blocks -----------------------------------------
+// o = softmax(q K^T / sqrt(128)) V for one token: its q heads of one kv head, 16 at a
+// time, are the columns of v_mfma_f32_16x16x32_f16; a tile is 32 keys, a wave's own.
+//   S^T (16 keys x 16 heads) = K . Q^T: lane l (c = l % 16, g = l / 16) gives K row m = c and Q^T
+//   column c, dims 32 kk + 8 g .. + 7, and receives S of head c and m = 4 g + r;
+//   O^T (16 dims x 16 heads) += V^T . P^T: lane l gives eight keys of dim c and of head c.  The
+//   order of the keys within the product is free: P^T uses what the lane holds of S, m = 4 g + r of
+//   both halves of the tile, so row m of half u stands for key 16 u + 4 r + g, and then V^T's
+//   eight keys of a lane are those of its own eight 16-byte loads (load i: key 4 i + g, dims 8 c .. 8 c + 7):
+//   product j takes element j of each, put together by v_perm, and belongs to dims 8 c + j.
+// So K and V go from memory to registers to the matrix cores with no trip through LDS, and a
+// lane ends with dims 32 g .. 32 g + 31 of head c.  The softmax weights are rounded to fp16 for
+// the product with V (2^-11, as everywhere in this library's matrix-core attention); scores, sums
+// and outputs are fp32.
+constexpr int kDecWaves = 4;    // waves of a block
+constexpr int kDecBlocks = 768; // of a launch
+constexpr int kDecKeys = 32;    // keys of a tile
+constexpr int kDecRows = 16;    // rows of a segment
+
+struct DecodeParams {
+    PagedView c;
+    const uint16_t* q;
+    const int32_t* selected;  // [row][kv head][num_selected]
+    uint16_t* out;
+    float* lse;
+    void* ws;
+    int nq, group, window, num_selected, blocks;
+};
+
+__device__ __forceinline__ float xor32_max(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float xor16_max(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// The keys of a token, in tiles of 32: of the whole context or window (tile t: positions 32 t ..),
+// or of the list of selected blocks (tile t: entries from 32 t / page size on).
+struct DecodeRange {
+    int pos, lo, lim, first_tile, tiles;
+};
+template <bool SPARSE>
+__device__ __forceinline__ DecodeRange decode_range(const DecodeParams& p, const PagedSeq& s, int row) {
+    DecodeRange r;
+    r.pos = s.ctx + row - s.first;
+    r.lim = min(r.pos, p.c.capacity() - 1);
+    r.lo = !SPARSE && p.window > 0 ? max(0, r.pos - p.window + 1) : 0;
+    if (SPARSE) {
+        r.first_tile = 0;
+        r.tiles = static_cast<int>(((static_cast<long long>(p.num_selected) << p.c.shift) + kDecKeys - 1) / kDecKeys);
+    } else {
+        r.first_tile = r.lo / kDecKeys;
+        r.tiles = r.lim < r.lo ? 0 : r.lim / kDecKeys - r.first_tile + 1;
+    }
+    return r;
+}
+
+template <bool SPARSE>
+__global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeParams p) {
+    constexpr int NW = kDecWaves, kPad = kPgDim + 4;
+    __shared__ float s_m[NW][kDecRows], s_l[NW][kDecRows];
+    __shared__ __align__(16) float s_o[NW][kDecRows][kPad];
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int c = lane & 15, g = lane >> 4;
+    const Partials part = partials<kDecRows>(p.ws, p.blocks);
+    const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
+    const ptrdiff_t v_minus_k = reinterpret_cast<const char*>(p.c.v) - reinterpret_cast<const char*>(p.c.k);
+
+    // On the line: each sequence has its token's heads; or one sequence has those of all rows, the heads of
+    // a row behind each other (all alike: which rows have a token is seen when their turn comes).
+    constexpr int kOver = 4;  // what starting a segment costs, in tiles
+    auto token = [&](int item, int head, int& row, int& h, int& seq, PagedSeq& s) __attribute__((always_inline)) {
+        row = SPARSE ? head / p.c.nkv : item;
+        h = SPARSE ? head - row * p.c.nkv : head;
+        seq = SPARSE ? uniform(paged_seq_of_row(p.c, row)) : item;
+        if (seq < 0) return false;
+        s = paged_seq(p.c, seq);
+        return row >= s.first && row < s.first + s.n;
+    };
+    auto work = [&](int item) __attribute__((always_inline)) {
+        SeqWork w{0, 0, 0, row_tiles, p.c.nkv};
+        if constexpr (SPARSE) {
+            w.heads = p.c.rows * p.c.nkv;
+            w.first = w.most = decode_range<SPARSE>(p, PagedSeq{0, 1, 0}, 0).tiles + kOver;
+        } else {
+            const PagedSeq s = paged_seq(p.c, item);
+            if (s.n > 0) w.first = w.most = decode_range<SPARSE>(p, s, item).tiles + kOver;
+            else w.row_tiles = 0;
+        }
+        return w;
+    };
+    auto tiles = [&](int item, int) __attribute__((always_inline)) {
+        return uniform(decode_range<SPARSE>(p, SPARSE ? PagedSeq{0, 1, 0} : paged_seq(p.c, item), item).tiles);
+    };
+
+    auto body = [&](int item, int head, int rt, int, int t0, int t1, int slot) __attribute__((always_inline)) {
+        int row, h, seq;
+        PagedSeq s;
+        if (!token(item, head, row, h, seq, s)) return;  // a row of no sequence: not written
+        const DecodeRange range = decode_range<SPARSE>(p, s, row);
+        const int lim = uniform(range.lim), lo = uniform(range.lo);
+        const int live = min(kDecRows, p.group - rt * kDecRows);
+        const int head0 = h * p.group + rt * kDecRows;
+        f16x8 qf[4];
+        {
+            const uint16_t* q = p.q + (static_cast<size_t>(row) * p.nq + head0 + min(c, live - 1)) * kPgDim + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
+        }
+        // this wave's run of tiles
+        const int a = range.first_tile + t0 + static_cast<int>(static_cast<long long>(t1 - t0) * wave / NW);
+        const int e = range.first_tile + t0 + static_cast<int>(static_cast<long long>(t1 - t0) * (wave + 1) / NW);
+        const int* list = SPARSE ? p.selected + (static_cast<size_t>(row) * p.c.nkv + h) * p.num_selected : nullptr;
+        // 64 entries of the list or of the table from `base` on, one a lane: page and block number
+        int base = 0, page_l = -1, block_l = 0;
+        auto refill = [&](int entry) __attribute__((always_inline)) {
+            base = entry;
+            block_l = entry + lane;
+            if constexpr (SPARSE) block_l = block_l < p.num_selected ? list[block_l] : -1;
+            page_l = block_l >= 0 && block_l < p.c.max_pages && (block_l << p.c.shift) <= lim
+                         ? paged_page(p.c, seq, block_l) : -1;
+        };
+        struct Tile {
+            const char* k[2];  // of the first key of each half
+            int pos[2];        // its position
+            bool there[2];     // it has a page
+        };
+        auto tile_at = [&](int t) __attribute__((always_inline)) {
+            Tile x;
+            const int per_page = p.c.shift - 5;  // log2 of the tiles of a page, -1 for two pages a tile
+            const int entry = per_page >= 0 ? t >> per_page : 2 * t;
+            const int span = per_page >= 0 ? 1 : 2;
+            if (entry + span > base + 64) refill(entry);
+            const int in_page = per_page >= 0 ? (t & ((1 << per_page) - 1)) * kDecKeys : 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int at = entry - base + (span == 2 ? u : 0);
+                const int page = __builtin_amdgcn_readlane(page_l, at);
+                const int row0 = in_page + (span == 2 ? 0 : 16 * u);
+                x.there[u] = page >= 0;
+                x.pos[u] = (__builtin_amdgcn_readlane(block_l, at) << p.c.shift) + row0;
+                x.k[u] = reinterpret_cast<const char*>(p.c.k + static_cast<long long>(max(page, 0)) * p.c.page_stride +
+                                                       ((static_cast<long long>(h) << p.c.shift) + row0) * kPgDim);
+            }
+            return x;
+        };
+        const uint32_t k_off = static_cast<uint32_t>((4 * (c & 3) + (c >> 2)) * kPgDim * 2 + 16 * g);
+        const uint32_t v_off = static_cast<uint32_t>(g * kPgDim * 2 + 16 * c);
+        u32x4 kf[8], vf[8];
+        auto request_k = [&](const Tile& x) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) kf[i] = *reinterpret_cast<const u32x4*>(x.k[i >> 2] + (k_off + 64 * (i & 3)));
+        };
+        auto request_v = [&](const Tile& x) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                vf[i] = *reinterpret_cast<const u32x4*>(x.k[i >> 2] + v_minus_k + (v_off + 4 * (i & 3) * kPgDim * 2));
+        };
+        f32x4 acc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = f32x4{};
+        float mref = -INFINITY, lsum = 0.0f;
+        bool any = false;
+        Tile cur{};
+        if (a < e) {
+            const int entry = p.c.shift >= 5 ? a >> (p.c.shift - 5) : 2 * a;
+            refill(entry);
+            cur = tile_at(a);
+            request_k(cur);
+            request_v(cur);
+        }
+        for (int t = a; t < e; ++t) {
+            f32x4 sc[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sc[u] = f32x4{};
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[4 * u + kk]), qf[kk], sc[u],
+                                                                   0, 0, 0);
+            }
+            Tile nxt = cur;
+            if (t + 1 < e) {
+                nxt = tile_at(t + 1);
+                request_k(nxt);
+            }
+            // keys out of sight (and rows that are none): the weights are 0, but what lies in the rows may be anything
+            const bool plain = cur.there[0] && cur.there[1] && cur.pos[0] >= lo && cur.pos[0] + 15 <= lim &&
+                               cur.pos[1] >= lo && cur.pos[1] + 15 <= lim;
+            if (plain) {
+                any = true;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int key = cur.pos[u] + 4 * r + g;
+                        const bool seen = cur.there[u] && key >= lo && key <= lim;
+                        any = any || seen;
+                        sc[u][r] = seen ? sc[u][r] : -INFINITY;
+                    }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = cur.pos[i >> 2] + 4 * (i & 3) + g;
+                    const bool seen = cur.there[i >> 2] && key >= lo && key <= lim;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) vf[i][d] = seen ? vf[i][d] : 0u;
+                }
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+            mx = xor32_max(xor16_max(mx)) * kPgScale;
+            const bool grow = mx > mref + kPgLag;
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+                const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
+                mref = grow ? mx : mref;
+                lsum *= alpha;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
+            }
+            const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
+            f16x8 pf;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 2][i & 3], kPgScale, neg));
+                lsum += w;
+                pf[i] = static_cast<_Float16>(w);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t take = j & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(vf[2 * i + 1][j >> 1], vf[2 * i][j >> 1], take);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf, acc[j], 0, 0, 0);
+            }
+            if (t + 1 < e) request_v(nxt);
+            cur = nxt;
+        }
+        // the waves meet: each row's common reference value, then the sum of the rescaled outputs
+        lsum += __shfl_xor(lsum, 16);
+        lsum += __shfl_xor(lsum, 32);
+        if (__builtin_amdgcn_ballot_w64(any) != 0) mref = fmaxf(mref, kPgLowest);
+        if (g == 0) s_m[wave][c] = mref, s_l[wave][c] = lsum;
+        __syncthreads();
+        {
+            float m = s_m[0][c];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][c]);
+            const float f = part_weight(mref, m);
+            float* o = &s_o[wave][c][32 * g];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)  // dims 32 g + 4 i .. + 3: r = i / 2, j = 4 (i % 2) ..
+                *reinterpret_cast<float4*>(o + 4 * i) =
+                    make_float4(acc[4 * (i & 1)][i >> 1] * f, acc[4 * (i & 1) + 1][i >> 1] * f,
+                                acc[4 * (i & 1) + 2][i >> 1] * f, acc[4 * (i & 1) + 3][i >> 1] * f);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < kDecRows * kPgDim / 4; i += 64 * NW) {
+            const int r = i / (kPgDim / 4), d = 4 * (i % (kPgDim / 4));
+            if (r >= live) continue;
+            float m = s_m[0][r], l = 0.0f;
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][r]);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int w = 0; w < NW; ++w) {
+                l += s_m[w][r] == -INFINITY ? 0.0f : s_l[w][r] * part_weight(s_m[w][r], m);
+                const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
+                o.x += x.x;
+                o.y += x.y;
+                o.z += x.z;
+                o.w += x.w;
+            }
+            if (slot < 0) {
+                const float inv = row_inverse(m, l);
+                const size_t at = static_cast<size_t>(row) * p.nq + head0 + r;
+                *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
+            } else {
+                const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * kDecRows + r;
+                *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
+                if (d == 0) part.ml[at] = make_float2(m, l);
+            }
+        }
+        __syncthreads();  // the next segment writes s_m
+    };
+    for_share(blockIdx.x, p.blocks, SPARSE ? 1 : p.c.seqs, NW + kOver, work, tiles, body, [&](SegmentCut cut) {
+        if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
+    });
+}
+
+template <bool SPARSE>
+__global__ __launch_bounds__(256) void paged_decode_merge_kernel(DecodeParams p) {
+    merge_parts<kDecRows, 8>(p.ws, p.blocks, p.out, p.lse, p.nq, [&](const SegmentCut& c, RowMap& rows) {
+        const int row = SPARSE ? c.head / p.c.nkv : c.item, h = SPARSE ? c.head - row * p.c.nkv : c.head;
+        const int live = min(kDecRows, p.group - c.row_tile * kDecRows);
+        rows = RowMap{row, 0, live, h * p.group + c.row_tile * kDecRows};
+        if constexpr (SPARSE) {  // a row of no sequence has no parts
+            const int seq = paged_seq_of_row(p.c, row);
+            if (seq < 0) return 0;
+            const PagedSeq s = paged_seq(p.c, seq);
+            if (row < s.first || row >= s.first + s.n) return 0;
+        }
+        return live;
+    });
+}
+
+// ---- chunks -----------------------------------------------------------------------
+// Causal attention of the rows of many sequences.  The q heads of a kv head and a
+// sequence's new tokens form one list of rows, row r = token r / group, head kvh *
+// group + r % group; a segment is 128 of them (32 a wave), whatever the group.  The
+// waves share tiles of 64 keys in LDS, filled from the pages by DMA a step ahead of
+// their use.  v_mfma_f32_32x32x16_f16 with the rows as columns:
+//   S^T (32 keys x 32 rows) = K . Q^T: lane l holds key l % 32 and row l % 32, dims 8 (l / 32) +
+//   16 kk; Q stays in registers; the result has lane l = row l % 32 with the keys
+//   8 (v / 4) + 4 (l / 32) + v % 4, so a row's maximum and sum are in-lane and one swap;
+//   O^T (128 dims x 32 rows) += V^T . P^T: P^T is the lane's own weights as fp16, V^T comes
+//   out of the row-major tile by ds_read_b64_tr_b16.
+// A tile row is 256 bytes, its 16-byte chunk c stored at c ^ swz(key), so that the reads
+// of K (16 keys, one chunk) and of V (4 keys x 4 chunks a half wave) meet no bank twice.
+// Rows that no one may see (behind the sequence's end, before every window, of missing
+// pages) are filled from a row of zeros: their weights are 0, and what lies there may be
+// anything.
+constexpr int kPfRows = 128;     // rows of a segment
+constexpr int kPfKeys = 64;      // keys of a tile
+constexpr int kPfTileBytes = kPfKeys * kPgDim * 2;
+constexpr int kPfBlocks = 512;   // of a launch: two a CU
+
+__device__ __align__(256) const uint16_t g_zero_row[kPgDim] = {};
+
+struct PrefillParams {
+    PagedView c;
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    void* ws;
+    int nq, group, window;
+};
+
+struct PrefillRange {
+    int r0, rows;           // first row of the segment, rows of the sequence
+    int first_tile, tiles;  // key tiles that its rows see
+    int low;                // the first key that one of them sees
+};
+__device__ __forceinline__ PrefillRange prefill_range(const PrefillParams& p, const PagedSeq& s, int rt) {
+    PrefillRange r;
+    r.r0 = rt * kPfRows;
+    r.rows = s.n * p.group;
+    const int first = s.ctx + r.r0 / p.group;
+    const int last = min(s.ctx + (min(r.r0 + kPfRows, r.rows) - 1) / p.group, p.c.capacity() - 1);
+    r.low = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    r.first_tile = r.low / kPfKeys;
+    r.tiles = last < r.low ? 0 : last / kPfKeys - r.first_tile + 1;
+    return r;
+}
+
+// ONE: pages of 64 tokens and more (a tile lies in one page).
+template <bool ONE>
+__global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) {
+    __shared__ __align__(256) char smem[4 * kPfTileBytes];  // K buffers 0 and 1, V buffers 0 and 1
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int fr = lane & 31, h = lane >> 5;
+    // blocks of one XCD take neighbouring shares: they read the same pages
+    const int block = static_cast<int>(blockIdx.x & 7) * (kPfBlocks / 8) + static_cast<int>(blockIdx.x >> 3);
+    const Partials part = partials<kPfRows>(p.ws, kPfBlocks);
+    const ptrdiff_t v_minus_k = p.c.v - p.c.k;  // elements
+    constexpr int NP = ONE ? 1 : 4;             // pages of a tile, at most
+
+    const uint32_t lds0 =
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)smem));
+    // tile load i of a wave: tile rows 16 i + 4 wave + lane / 16, stored chunk lane % 16, i.e. chunk
+    // (lane % 16) ^ swz(row) of memory
+    const int lrow = 4 * wave + (lane >> 4);
+    const int lcol = 8 * ((lane & 15) ^ (((lane >> 4) << 2) | wave));
+    const uint32_t loff = static_cast<uint32_t>(2 * (lrow * kPgDim + lcol));  // bytes
+    // LDS addresses: K chunk 2 kk + h of key fr; V^T reads (dt: 32 dims, u: keys + 8)
+    uint32_t ka[8], va[4][2];
+    {
+        const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
+        const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
+        const int s16 = lane & 15, b16 = (lane >> 4) & 1;
+        const uint32_t v0 = lds0 + 2 * kPfTileBytes + (4 * h + (s16 >> 2)) * 256 +
+                            16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+            va[dt][0] = v0 ^ (64 * dt);
+            va[dt][1] = (v0 ^ (64 * dt) ^ 32) + 8 * 256;
+        }
+    }
+    // K operand of MFMA i of a tile: 32-key half i % 2, dims 16 (i / 2); V^T operand: 16-key quarter i / 4,
+    // dims 32 (i % 4)
+    auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
+        typedef const __attribute__((address_space(3))) f16x8* lptr;
+        return *reinterpret_cast<lptr>(ka[i >> 1] + buf * kPfTileBytes + (i & 1) * 32 * 256);
+    };
+    auto read_v = [&](int buf, int i) __attribute__((always_inline)) {
+        typedef __attribute__((address_space(3))) s16x4* lptr;
+        const uint32_t off = (buf - 2) * kPfTileBytes + (i >> 2) * 16 * 256;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][0] + off));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][1] + off));
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // every tile requested so far is in LDS, for every wave, and what was read before is read
+    auto tile_barrier = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    constexpr int kOver = 2 * kPfKeys;  // what a segment costs beside its keys, in keys
+    auto work = [&](int seq) __attribute__((always_inline)) {
+        const PagedSeq s = paged_seq(p.c, seq);
+        // weights: keys times group, as if the rows were cut between tokens
+        const long long g = p.group, cap = p.c.capacity();
+        SeqWork w{g * (s.ctx + kOver), kPfRows, g * (cap + kOver), 0, p.c.nkv};
+        if (p.window > 0) w.most = min(w.most, g * (p.window + kPfRows / g + kPfKeys + kOver));
+        w.row_tiles = static_cast<int>((s.n * g + kPfRows - 1) / kPfRows);
+        return w;
+    };
+    auto tiles = [&](int seq, int rt) __attribute__((always_inline)) {
+        return uniform(prefill_range(p, paged_seq(p.c, seq), rt).tiles);
+    };
+
+    auto body = [&](int seq, int kvh, int rt, int, int t0, int t1, int slot) __attribute__((always_inline)) {
+        const PagedSeq s = paged_seq(p.c, seq);
+        const PrefillRange range = prefill_range(p, s, rt);
+        const int rows = uniform(range.rows), first_tile = uniform(range.first_tile), low = uniform(range.low);
+        const int it0 = first_tile + t0, it1 = first_tile + t1;
+        const int r = rt * kPfRows + wave * 32 + fr;
+        const int rc = min(r, rows - 1);
+        const int qi = rc / p.group, qh = kvh * p.group + rc - qi * p.group;
+        const int pos = s.ctx + qi;
+        const bool dead = rt * kPfRows + wave * 32 >= rows;  // the wave has no row
+        // the keys that this row takes here: lo .. lim
+        const int lim = min(min(pos, p.c.capacity() - 1), it1 * kPfKeys - 1);
+        const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        // tiles within these take no mask; the last key that any row of the wave takes
+        const int wave_lim = __builtin_amdgcn_readlane(lim, 0), wave_lo = __builtin_amdgcn_readlane(lo, 31);
+        const int wave_last = dead ? -1 : __builtin_amdgcn_readlane(lim, 31);
+        const int keys = uniform(min(s.ctx + s.n, p.c.capacity()));  // of the sequence
+
+        u32x4 qf[8];
+        {
+            const uint16_t* qr = p.q + (static_cast<size_t>(s.first + qi) * p.nq + qh) * kPgDim + 8 * h;
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
+        }
+        // 64 entries of the table from `base` on, one a lane
+        int base = 0, page_l = -1;
+        auto refill = [&](int entry) __attribute__((always_inline)) {
+            base = entry;
+            page_l = paged_page(p.c, seq, entry + lane);
+        };
+        struct Pages {
+            int at[NP];
+        };
+        auto pages_of = [&](int t) __attribute__((always_inline)) {
+            t = min(t, it1 - 1);  // the steps ask for up to two tiles behind the last
+            Pages x;
+            if constexpr (ONE) {
+                const int entry = t >> (p.c.shift - 6);
+                if (entry >= base + 64) refill(entry);
+                x.at[0] = __builtin_amdgcn_readlane(page_l, entry - base);
+            } else {
+                const int per = p.c.shift == 4 ? 0 : 1;  // log2 of the 16-key quarters of a page
+                const int entry = t << (2 - per);
+                if (entry + (4 >> per) > base + 64) refill(entry);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.at[i] = __builtin_amdgcn_readlane(page_l, entry - base + (i >> per));
+            }
+            return x;
+        };
+        auto there = [&](const Pages& x, int i) __attribute__((always_inline)) { return x.at[ONE ? 0 : i] >= 0; };
+        auto whole = [&](const Pages& x) __attribute__((always_inline)) {
+            bool all = true;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) all = all && x.at[i] >= 0;
+            return all;
+        };
+        // Tile t, whose pages are x, into buffer `buf` (0, 1: K; 2, 3: V); tile_barrier holds the waits.
+        auto load_tile = [&](int t, const Pages& x, int buf) __attribute__((always_inline)) {
+            t = min(t, it1 - 1);
+            const uint32_t dst = lds0 + buf * kPfTileBytes + wave * 1024;
+            const uint16_t* from[4];  // of quarter i
+            const int mask = p.c.page_size() - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (ONE && i > 0) {
+                    from[i] = from[0] + 16 * i * kPgDim;
+                } else {
+                    const int row0 = (t * kPfKeys + 16 * i) & mask;
+                    from[i] = p.c.k + (buf >= 2 ? v_minus_k : 0) +
+                              static_cast<long long>(max(x.at[ONE ? 0 : i], 0)) * p.c.page_stride +
+                              ((static_cast<long long>(kvh) << p.c.shift) + row0) * kPgDim;
+                }
+            }
+            if (t * kPfKeys >= low && (t + 1) * kPfKeys <= keys && whole(x)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lds_load_x4(dst + 4096 * i, from[i], loff);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = t * kPfKeys + 16 * i + lrow;
+                    const bool seen = key >= low && key < keys && there(x, i);
+                    lds_load_x4(dst + 4096 * i, seen ? from[i] + lrow * kPgDim + lcol : g_zero_row + lcol);
+                }
+            }
+        };
+
+        f32x16 acc[4];
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
+        float mref = -INFINITY, lsum = 0.0f;
+        bool any = false;  // the row has had a key
+        auto mask = [&](int t, const Pages& x, f32x16 (&sc)[2]) __attribute__((always_inline)) {
+            if ((t + 1) * kPfKeys - 1 <= wave_lim && t * kPfKeys >= wave_lo && whole(x)) {  // wave-uniform
+                any = true;
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int key = t * kPfKeys + 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
+                    const bool seen = key <= lim && key >= lo && there(x, 2 * j + (v >> 3));
+                    any = any || seen;
+                    sc[j][v] = seen ? sc[j][v] : -INFINITY;
+                }
+        };
+        auto renew_ref = [&](float mx) __attribute__((always_inline)) {
+            const bool grow = mx > mref + kPgLag;
+            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+                const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
+                mref = grow ? mx : mref;
+                lsum *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+            }
+        };
+        auto row_max = [&](const f32x16 (&sc)[2]) __attribute__((always_inline)) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[j][v]);
+            return xor32_max(mx) * kPgScale;  // scaling is monotonic
+        };
+        // weights 2 i and 2 i + 1 of a tile's scores (32-key half i / 8), packed
+        auto probs = [&](const f32x16 (&sc)[2], int i, float neg, float (&ps)[2]) __attribute__((always_inline)) {
+            const int j = i >> 3, v = 2 * (i & 7);
+            const f32x2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v], kPgScale, neg)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v + 1], kPgScale, neg))};
+            ps[0] += e.x;
+            ps[1] += e.y;
+            uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, f16x2));
+            asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]));  // here, not past the mask's branch
+            return w;
+        };
+        constexpr int AHEAD = 4;  // operand reads in flight before their MFMA
+        // Scores of the K tile in `buf`; beside them, when EXP, the weights of the scores `cur`.  Each MFMA is
+        // fenced together with its share of the vector work: left alone, the scheduler puts all of the one
+        // before all of the other.
+        auto scores = [&](auto exp_too, int buf, f32x16 (&sc)[2], const f32x16 (&cur)[2],
+                          uint32_t (&pw)[2][8]) __attribute__((always_inline)) {
+            const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
+            float ps[2] = {0.0f, 0.0f};
+            f16x8 kf[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) kf[i] = read_k(buf, i);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % AHEAD], __builtin_bit_cast(f16x8, qf[i >> 1]),
+                                                                   i < 2 ? f32x16{} : sc[i & 1], 0, 0, 0);
+                if (i + AHEAD < 16) kf[i % AHEAD] = read_k(buf, i + AHEAD);
+                if constexpr (decltype(exp_too)::value) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (decltype(exp_too)::value) lsum += ps[0] + ps[1];
+        };
+        // O^T += V^T . P^T; beside it, when MAX, the (scaled) row maximum of nxt
+        auto add_pv = [&](auto max_too, const uint32_t (&pw)[2][8], int buf, const f32x16 (&nxt)[2]) __attribute__((always_inline)) {
+            f16x8 vf[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) vf[i] = read_v(buf, i);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = i >> 3, ks = (i >> 2) & 1, dt = i & 3;
+                const u32x4 pf = {pw[j][4 * ks], pw[j][4 * ks + 1], pw[j][4 * ks + 2], pw[j][4 * ks + 3]};
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % AHEAD], __builtin_bit_cast(f16x8, pf), acc[dt], 0, 0, 0);
+                if (i + AHEAD < 16) vf[i % AHEAD] = read_v(buf, i + AHEAD);
+                if constexpr (decltype(max_too)::value)
+                    mx = fmaxf(fmaxf(mx, nxt[j][2 * (i & 7)]), nxt[j][2 * (i & 7) + 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return decltype(max_too)::value ? xor32_max(mx) * kPgScale : 0.0f;
+        };
+        typedef std::true_type yes;
+        typedef std::false_type no;
+        // The scores of tile t are in cur: the scores of the next tile beside the weights of t, then V of t
+        // beside the next tile's maximum.  b: parity of the tile; x: pages of tile t + 1, of t + 2 after it.
+        auto step = [&](int t, int b, Pages& x, f32x16 (&cur)[2], f32x16 (&nxt)[2]) __attribute__((always_inline)) {
+            uint32_t pw[2][8];
+            load_tile(t + 1, x, 2 + (b ^ 1));
+            const Pages y = pages_of(t + 2);
+            load_tile(t + 2, y, b);
+            scores(yes{}, b ^ 1, nxt, cur, pw);
+            mask(t + 1, x, nxt);
+            const float mx = add_pv(yes{}, pw, 2 + b, nxt);
+            renew_ref(mx);
+            x = y;
+            tile_barrier();
+        };
+        auto finish = [&](int b, f32x16 (&cur)[2]) __attribute__((always_inline)) {
+            uint32_t pw[2][8];
+            const float neg = mref == -INFINITY ? 0.0f : -mref;
+            float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
+            lsum += ps[0] + ps[1];
+            add_pv(no{}, pw, 2 + b, cur);
+        };
+        if (it0 < it1) {
+            const int n = it1 - it0;
+            int t = it0;
+            refill(ONE ? t >> (p.c.shift - 6) : t << (p.c.shift == 4 ? 2 : 1));
+            Pages x = pages_of(t);
+            load_tile(t, x, 0);
+            load_tile(t, x, 2);
+            Pages y = pages_of(t + 1);
+            load_tile(t + 1, y, 1);
+            tile_barrier();
+            f32x16 s0[2] = {}, s1[2];
+            if (wave_last >= t * kPfKeys) {
+                uint32_t pw[2][8];
+                scores(no{}, 0, s0, s1, pw);
+                mask(t, x, s0);
+                renew_ref(row_max(s0));
+            }
+            tile_barrier();  // K buffer 0 is read
+            // Tiles past the wave's last key are not multiplied.
+            const int mine = wave_last < t * kPfKeys ? 0 : min(n, wave_last / kPfKeys - t + 1);
+            int left = mine;
+            for (; left > 2; left -= 2) {
+                step(t, 0, y, s0, s1);
+                step(t + 1, 1, y, s1, s0);
+                t += 2;
+            }
+            if (left == 2) {
+                step(t, 0, y, s0, s1);
+                finish(1, s1);
+            } else if (left == 1) {
+                finish(0, s0);
+            }
+            for (int i = max(mine - 1, 0); i < n - 1; ++i) {  // the tiles of the other waves
+                load_tile(it0 + i + 1, y, 2 + ((i & 1) ^ 1));
+                y = pages_of(it0 + i + 2);
+                load_tile(it0 + i + 2, y, i & 1);
+                tile_barrier();
+            }
+        }
+        lsum += __shfl_xor(lsum, 32);
+        if (any || __shfl_xor(static_cast<int>(any), 32) != 0) mref = fmaxf(mref, kPgLowest);
+        if (r < rows) {
+            if (slot < 0) {
+                const float inv = row_inverse(mref, lsum);
+                const size_t at = static_cast<size_t>(s.first + qi) * p.nq + qh;
+                uint16_t* o = p.out + at * kPgDim;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)  // dims 32dt + 8g + 4h .. +3
+                        *reinterpret_cast<uint2*>(o + 32 * dt + 8 * g + 4 * h) =
+                            pack4(acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv);
+                if (p.lse != nullptr && h == 0) p.lse[at] = row_log_sum(mref, lsum);
+            } else {
+                const size_t at = static_cast<size_t>(2 * block + slot) * kPfRows + wave * 32 + fr;
+                if (h == 0) part.ml[at] = make_float2(mref, lsum);
+                float* po = part.o + at * kPgDim;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4*>(po + 32 * dt + 8 * g + 4 * h) =
+                            make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+            }
+        }
+        tile_barrier();  // the tiles are read: the next segment fills them
+    };
+    constexpr int kLeastTiles = 4;
+    for_share(block, kPfBlocks, p.c.seqs, static_cast<long long>(p.group) * kLeastTiles * kPfKeys, work, tiles, body,
+              [&](SegmentCut cut) {
+                  if (threadIdx.x == 0) part.cuts[block] = cut;
+              });
+}
+
+__global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillParams p) {
+    merge_parts<kPfRows, 1>(p.ws, kPfBlocks, p.out, p.lse, p.nq, [&](const SegmentCut& c, RowMap& rows) {
+        const PagedSeq s = paged_seq(p.c, c.item);
+        rows = RowMap{s.first, c.row_tile * kPfRows, p.group, c.head * p.group};
+        return min(kPfRows, s.n * p.group - c.row_tile * kPfRows);
+    });
+}
+
+// The checks that the attention entry points share.
+int check_attention(const char* what, const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                    uint16_t* attn_out, float* row_lse, void* workspace, size_t workspace_bytes, const int32_t* selected,
+                    int num_q_heads, int num_selected) {
+    QE_REQUIRE(q && attn_out && workspace, "%s: NULL pointer", what);
+    QE_REQUIRE(aligned(q, 16) && aligned(attn_out, 8) && aligned(workspace, 16) && aligned(row_lse, 4) &&
+                   aligned(selected, 4),
+               "%s: q and the workspace must be 16-byte and attn_out 8-byte aligned", what);
+    const size_t n = batch->num_tokens, q_bytes = 2 * n * num_q_heads * kPgDim;
+    const PagedSpan spans[] = {{attn_out, q_bytes, "attn_out"},
+                               {row_lse, 4 * n * num_q_heads, "row_lse"},
+                               {workspace, workspace_bytes, "the workspace"},
+                               {q, q_bytes, "q"},
+                               {selected, 4 * n * cache->num_kv_heads * num_selected, "selected"},
+                               paged_k_span(cache),
+                               paged_v_span(cache),
+                               paged_table_span(batch),
+                               paged_starts_span(batch),
+                               paged_context_span(batch)};
+    return paged_check_apart(what, spans, 3);
+}
+
+template <bool SPARSE>
+int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
+                  const int32_t* selected, uint16_t* attn_out, float* row_lse, void* workspace, hipStream_t stream,
+                  int num_q_heads, int window, int num_selected) {
+    DecodeParams p{};
+    QE_TRY(paged_check(what, cache, batch, &p.c));
+    QE_TRY(paged_check_heads(what, cache, num_q_heads));
+    if (batch->num_tokens == 0 || batch->num_seqs == 0) return QE_OK;
+    QE_TRY(check_attention(what, q, cache, batch, attn_out, row_lse, workspace, partials_bytes<kDecRows>(kDecBlocks),
+                           selected, num_q_heads, num_selected));
+    p.q = q;
+    p.selected = selected;
+    p.out = attn_out;
+    p.lse = row_lse;
+    p.ws = workspace;
+    p.nq = num_q_heads;
+    p.group = num_q_heads / cache->num_kv_heads;
+    p.window = window;
+    p.num_selected = num_selected;
+    p.blocks = kDecBlocks;
+    paged_decode_kernel<SPARSE><<<p.blocks, 64 * kDecWaves, 0, stream>>>(p);
+    paged_decode_merge_kernel<SPARSE><<<dim3(p.blocks, std::min(p.group, kDecRows)), 256, 0, stream>>>(p);
+    return check_launch(what);
+}
+
+}  // namespace
+}  // namespace qe
+
+using namespace qe;
+
+extern "C" int qe_paged_decode_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, size_t* bytes) {
+    QE_REQUIRE(bytes, "paged_decode_workspace_bytes: NULL pointer");
+    QE_REQUIRE(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+               "paged_decode_workspace_bytes: num_tokens=%d, %d q heads over %d kv heads", num_tokens, num_q_heads,
+               num_kv_heads);
+    *bytes = partials_bytes<kDecRows>(kDecBlocks);
+    clear_error();
+    return QE_OK;
+}
+
+extern "C" int qe_launch_attention_gqa_paged_decode(const uint16_t* q, const qe_paged_cache* cache,
+                                                    const qe_paged_batch* batch, void* workspace, uint16_t* attn_out,
+                                                    float* row_lse, hipStream_t stream, int num_q_heads, int window) {
+    const char* what = "attention_gqa_paged_decode";
+    QE_REQUIRE(batch == nullptr || batch->query_start == nullptr, "%s: query_start is for chunks", what);
+    QE_REQUIRE(window >= 0, "%s: window=%d", what, window);
+    return launch_decode<false>(what, q, cache, batch, nullptr, attn_out, row_lse, workspace, stream, num_q_heads, window, 0);
+}
+
+extern "C" int qe_launch_attention_gqa_paged_sparse(const uint16_t* q, const qe_paged_cache* cache,
+                                                    const qe_paged_batch* batch, const int32_t* selected, void* workspace,
+                                                    uint16_t* attn_out, float* row_lse, hipStream_t stream,
+                                                    int num_q_heads, int num_selected) {
+    const char* what = "attention_gqa_paged_sparse";
+    QE_REQUIRE(selected, "%s: NULL pointer", what);
+    QE_REQUIRE(num_selected > 0 && num_selected <= (1 << 20), "%s: num_selected=%d", what, num_selected);
+    QE_REQUIRE(!cache || !batch || static_cast<long long>(batch->num_tokens) * cache->num_kv_heads <= (1 << 30),
+               "%s: num_tokens=%d", what, batch->num_tokens);
+    return launch_decode<true>(what, q, cache, batch, selected, attn_out, row_lse, workspace, stream, num_q_heads, 0,
+                               num_selected);
+}
+
+extern "C" int qe_paged_prefill_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, size_t* bytes) {
+    QE_REQUIRE(bytes, "paged_prefill_workspace_bytes: NULL pointer");
+    QE_REQUIRE(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+               "paged_prefill_workspace_bytes: num_tokens=%d, %d q heads over %d kv heads", num_tokens, num_q_heads,
+               num_kv_heads);
+    *bytes = partials_bytes<kPfRows>(kPfBlocks);
+    clear_error();
+    return QE_OK;
+}
+
+extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe_paged_cache* cache,
+                                                     const qe_paged_batch* batch, void* workspace, uint16_t* attn_out,
+                                                     float* row_lse, hipStream_t stream, int num_q_heads, int window) {
+    const char* what = "attention_gqa_paged_prefill";
+    PrefillParams p{};
+    QE_TRY(paged_check(what, cache, batch, &p.c));
+    QE_TRY(paged_check_heads(what, cache, num_q_heads));
+    QE_REQUIRE(window >= 0, "%s: window=%d", what, window);
+    if (batch->num_tokens == 0 || batch->num_seqs == 0) return QE_OK;
+    QE_TRY(check_attention(what, q, cache, batch, attn_out, row_lse, workspace, partials_bytes<kPfRows>(kPfBlocks), nullptr,
+                           num_q_heads, 0));
+    p.q = q;
+    p.out = attn_out;
+    p.lse = row_lse;
+    p.ws = workspace;
+    p.nq = num_q_heads;
+    p.group = num_q_heads / cache->num_kv_heads;
+    p.window = window;
+    if (p.c.shift >= 6)
+        paged_prefill_kernel<true><<<kPfBlocks, 256, 0, stream>>>(p);
+    else
+        paged_prefill_kernel<false><<<kPfBlocks, 256, 0, stream>>>(p);
+    paged_prefill_merge_kernel<<<dim3(kPfBlocks, kPfRows / 8), 256, 0, stream>>>(p);
+    return check_launch(what);
+}

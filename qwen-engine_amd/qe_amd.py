@@ -62,6 +62,13 @@ SIGNATURES = {
     "qe_launch_attention_gqa_flash_decode_kv4": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "qe_launch_attention_gqa_prefill_kv4": [_P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P],
     "qe_launch_kv4_evict": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _I],
+    "qe_launch_qkv_norm_rope_paged_append": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, ctypes.c_longlong,
+                                             ctypes.c_longlong, ctypes.c_float],
+    "qe_launch_attention_gqa_paged_decode": [_P, _P, _P, _P, _P, _P, _P, _I, _I],
+    "qe_launch_attention_gqa_paged_prefill": [_P, _P, _P, _P, _P, _P, _P, _I, _I],
+    "qe_launch_paged_key_bounds": [_P, _P, _P, _P, _P],
+    "qe_launch_paged_select": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I],
+    "qe_launch_attention_gqa_paged_sparse": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I],
     "qe_launch_token_logprobs": [_P, _P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_longlong, _I, _P],
 }
 
@@ -76,6 +83,11 @@ OTHER_SIGNATURES = {
     "qe_gemm_prefill_plan": [_I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)],
     "qe_gemm_prefill_launch_plan": [_I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)],
     "qe_kv4_decode_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "qe_rope_turns": [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_float), _I, ctypes.c_double, _I,
+                      ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double],
+    "qe_paged_decode_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "qe_paged_prefill_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "qe_paged_select_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
     "qe_token_logprobs_workspace_bytes": [_I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
 }
 
@@ -485,6 +497,171 @@ def launch_kv4_evict(layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k
     s, p = _on_gpu(stream, layer_k_cache, layer_v_cache, key_weights, d_evicted, out_k_cache, out_v_cache, out_key_weights,
                    out_evicted, kept_rows, d_control)
     _call("qe_launch_kv4_evict", *p, keep, sinks, recent, s, num_kv_heads, head_dim, max_seq_len)
+
+
+# ---- paged key/value cache: many sequences --------------------------------------------
+class _PagedCache(ctypes.Structure):
+    """qe_paged_cache (include/qe_kernels.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("page_stride", ctypes.c_longlong), ("num_pages", _I), ("page_size", _I),
+                ("num_kv_heads", _I), ("head_dim", _I)]
+
+
+class _PagedBatch(ctypes.Structure):
+    """qe_paged_batch."""
+    _fields_ = [("block_table", _P), ("query_start", _P), ("context_len", _P), ("num_seqs", _I), ("num_tokens", _I),
+                ("max_pages", _I)]
+
+
+class _Rope(ctypes.Structure):
+    """qe_rope."""
+    _fields_ = [("turns", _P), ("rotary_dim", _I), ("interleaved", _I), ("scale", ctypes.c_float)]
+
+
+class _Described:
+    """A description of device tensors for the library: the structure, its address, and the tensors, kept alive."""
+
+    def __init__(self, struct, *tensors):
+        self.struct, self.address, self.tensors = struct, ctypes.addressof(struct), tensors
+        self.gpu = None
+        for t in tensors:
+            if t is None:
+                continue
+            at = t.get_device()
+            if at < 0:
+                raise RuntimeError(f"the tensors must be on a GPU, not on {t.device}")
+            if self.gpu not in (None, at):
+                raise RuntimeError(f"the tensors must be on one GPU, not on cuda:{self.gpu} and {t.device}")
+            self.gpu = at
+
+
+def _typed(t, dtype, what):
+    if t.dtype != dtype:
+        raise RuntimeError(f"{what} must be {dtype}, not {t.dtype}")
+    return t
+
+
+def paged_cache(k, v):
+    """The pages of one layer for the paged launchers (qe_paged_cache): fp16 tensors [pages][kv heads][page size][128],
+    whose pages may lie apart (views of one allocation), and what lies in a page must not."""
+    import torch
+    for t in (k, v):
+        _typed(t, torch.float16, "pages")
+        if t.dim() != 4 or t.shape != k.shape:
+            raise RuntimeError(f"pages of shapes {tuple(k.shape)} and {tuple(v.shape)}")
+        if t.stride()[1:] != (t.shape[2] * t.shape[3], t.shape[3], 1) or (t.shape[0] > 1 and t.stride(0) != k.stride(0)):
+            raise RuntimeError(f"pages of strides {k.stride()} and {v.stride()}")
+    n, heads, size, dim = k.shape
+    stride = k.stride(0) if n > 1 else heads * size * dim
+    return _Described(_PagedCache(k.data_ptr(), v.data_ptr(), stride, n, size, heads, dim), k, v)
+
+
+def paged_batch(block_table, context_len, query_start=None, num_tokens=None):
+    """The rows of a launch (qe_paged_batch): int32 block_table [sequences][max pages], context_len [sequences],
+    query_start [sequences + 1] or None (a row for each sequence); num_tokens: the rows of the buffers."""
+    import torch
+    for name, t in (("block_table", block_table), ("context_len", context_len), ("query_start", query_start)):
+        if t is not None and not _typed(t, torch.int32, name).is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+    if block_table.dim() != 2 or context_len.dim() != 1 or context_len.shape[0] != block_table.shape[0]:
+        raise RuntimeError(f"block_table {tuple(block_table.shape)} and context_len {tuple(context_len.shape)}")
+    seqs, pages = block_table.shape
+    if query_start is None:
+        num_tokens = seqs if num_tokens is None else num_tokens
+    elif query_start.shape != (seqs + 1,) or num_tokens is None:
+        raise RuntimeError(f"query_start {tuple(query_start.shape)} for {seqs} sequences, num_tokens {num_tokens}")
+    return _Described(_PagedBatch(block_table.data_ptr(), _ptr(query_start), context_len.data_ptr(), seqs, num_tokens,
+                                  pages), block_table, context_len, query_start)
+
+
+def rope(turns, scale=1.0, interleaved=False):
+    """Rotary positions (qe_rope) from device turns a position, float64 [rotary_dim / 2] (see rope_turns)."""
+    import torch
+    if not _typed(turns, torch.float64, "turns").is_contiguous():
+        raise RuntimeError("turns must be contiguous")
+    return _Described(_Rope(turns.data_ptr(), 2 * turns.numel(), int(interleaved), scale), turns)
+
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "ramp": 2, "bands": 3}  # QE_ROPE_*
+
+
+def rope_turns(rotary_dim=128, theta=1000000.0, kind="plain", factor=1.0, original_positions=32768, low_turns=1.0,
+               high_turns=32.0):
+    """(turns a position as a float64 host tensor [rotary_dim / 2], factor) for rope (qe_rope_turns)."""
+    import torch
+    turns, scale = (ctypes.c_double * (max(rotary_dim, 2) // 2))(), ctypes.c_float()
+    if kind not in ROPE_KINDS:
+        raise RuntimeError(f"rope_turns: kind {kind!r}")
+    _check(lib().qe_rope_turns(turns, ctypes.byref(scale), rotary_dim, theta, ROPE_KINDS[kind], factor, original_positions,
+                               low_turns, high_turns), "qe_rope_turns")
+    return torch.tensor(list(turns), dtype=torch.float64), scale.value
+
+
+def _on_gpu_with(stream, described, *tensors):
+    """_on_gpu for a call that also takes descriptions, which must be of the tensors' GPU."""
+    gpu = described[0].gpu
+    for d in described:
+        if d.gpu != gpu:
+            raise RuntimeError(f"the tensors must be on one GPU, not on cuda:{gpu} and cuda:{d.gpu}")
+    s, p = _on_gpu(stream, described[0].tensors[0], *tensors)
+    return s, p[1:]
+
+
+def launch_qkv_norm_rope_paged_append(q, q_out, k, v, q_bias, k_bias, v_bias, q_norm, k_norm, rope, cache, batch,
+                                      stream=None, num_q_heads=12, q_stride=0, kv_stride=0, norm_eps=1e-6):
+    described = (cache, batch) if rope is None else (cache, batch, rope)
+    s, p = _on_gpu_with(stream, described, q, q_out, k, v, q_bias, k_bias, v_bias, q_norm, k_norm)
+    _call("qe_launch_qkv_norm_rope_paged_append", *p, None if rope is None else rope.address, cache.address, batch.address,
+          s, num_q_heads, q_stride, kv_stride, norm_eps)
+
+
+def _paged_bytes(name, *args) -> int:
+    n = ctypes.c_size_t()
+    _check(getattr(lib(), name)(*args, ctypes.byref(n)), name)
+    return n.value
+
+
+def paged_decode_workspace_bytes(num_tokens, num_q_heads=12, num_kv_heads=2) -> int:
+    """Bytes of the workspace of launch_attention_gqa_paged_decode and _sparse (qe_paged_decode_workspace_bytes)."""
+    return _paged_bytes("qe_paged_decode_workspace_bytes", num_tokens, num_q_heads, num_kv_heads)
+
+
+def paged_prefill_workspace_bytes(num_tokens, num_q_heads=12, num_kv_heads=2) -> int:
+    """Bytes of launch_attention_gqa_paged_prefill's workspace (qe_paged_prefill_workspace_bytes)."""
+    return _paged_bytes("qe_paged_prefill_workspace_bytes", num_tokens, num_q_heads, num_kv_heads)
+
+
+def paged_select_workspace_bytes(num_tokens, num_kv_heads=2, max_pages=64) -> int:
+    """Bytes of launch_paged_select's workspace (qe_paged_select_workspace_bytes)."""
+    return _paged_bytes("qe_paged_select_workspace_bytes", num_tokens, num_kv_heads, max_pages)
+
+
+def launch_attention_gqa_paged_decode(q, cache, batch, workspace, attn_out, stream=None, num_q_heads=12, window=0,
+                                      row_lse=None):
+    s, p = _on_gpu_with(stream, (cache, batch), q, workspace, attn_out, row_lse)
+    _call("qe_launch_attention_gqa_paged_decode", p[0], cache.address, batch.address, *p[1:], s, num_q_heads, window)
+
+
+def launch_attention_gqa_paged_prefill(q, cache, batch, workspace, attn_out, stream=None, num_q_heads=12, window=0,
+                                       row_lse=None):
+    s, p = _on_gpu_with(stream, (cache, batch), q, workspace, attn_out, row_lse)
+    _call("qe_launch_attention_gqa_paged_prefill", p[0], cache.address, batch.address, *p[1:], s, num_q_heads, window)
+
+
+def launch_paged_key_bounds(cache, batch, bounds, bound_steps, stream=None):
+    s, p = _on_gpu_with(stream, (cache, batch), bounds, bound_steps)
+    _call("qe_launch_paged_key_bounds", cache.address, batch.address, *p, s)
+
+
+def launch_paged_select(q, cache, batch, bounds, bound_steps, selected, workspace, stream=None, num_q_heads=12,
+                        num_selected=32, sinks=1, recent=2):
+    s, p = _on_gpu_with(stream, (cache, batch), q, bounds, bound_steps, selected, workspace)
+    _call("qe_launch_paged_select", p[0], cache.address, batch.address, *p[1:], s, num_q_heads, num_selected, sinks, recent)
+
+
+def launch_attention_gqa_paged_sparse(q, cache, batch, selected, workspace, attn_out, stream=None, num_q_heads=12,
+                                      num_selected=32, row_lse=None):
+    s, p = _on_gpu_with(stream, (cache, batch), q, selected, workspace, attn_out, row_lse)
+    _call("qe_launch_attention_gqa_paged_sparse", p[0], cache.address, batch.address, *p[1:], s, num_q_heads, num_selected)
 
 
 # ---- log probabilities ---------------------------------------------------------------

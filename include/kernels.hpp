@@ -387,6 +387,62 @@ inline void launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_
                   "launch_kv4_evict");
 }
 
+// ---- paged key/value cache: many sequences (no counterpart in kernels.cuh) ----
+using PagedCache = qe_paged_cache;
+using PagedBatch = qe_paged_batch;
+using Rope = qe_rope;
+
+inline void launch_qkv_norm_rope_paged_append(const half* q, half* q_out, const half* k, const half* v,
+                                              const half* q_bias, const half* k_bias, const half* v_bias,
+                                              const half* q_norm, const half* k_norm, const Rope* rope,
+                                              const PagedCache& cache, const PagedBatch& batch, hipStream_t stream,
+                                              int num_q_heads = NUM_Q_HEADS, long long q_stride = 0,
+                                              long long kv_stride = 0, float norm_eps = RMS_NORM_EPS) {
+    detail::check(qe_launch_qkv_norm_rope_paged_append(detail::h(q), detail::h(q_out), detail::h(k), detail::h(v),
+                                                       detail::h(q_bias), detail::h(k_bias), detail::h(v_bias),
+                                                       detail::h(q_norm), detail::h(k_norm), rope, &cache, &batch,
+                                                       stream, num_q_heads, q_stride, kv_stride, norm_eps),
+                  "launch_qkv_norm_rope_paged_append");
+}
+
+inline void launch_attention_gqa_paged_decode(const half* q, const PagedCache& cache, const PagedBatch& batch,
+                                              void* workspace, half* attn_out, hipStream_t stream,
+                                              int num_q_heads = NUM_Q_HEADS, int window = 0, float* row_lse = nullptr) {
+    detail::check(qe_launch_attention_gqa_paged_decode(detail::h(q), &cache, &batch, workspace, detail::h(attn_out),
+                                                       row_lse, stream, num_q_heads, window),
+                  "launch_attention_gqa_paged_decode");
+}
+
+inline void launch_attention_gqa_paged_prefill(const half* q, const PagedCache& cache, const PagedBatch& batch,
+                                               void* workspace, half* attn_out, hipStream_t stream,
+                                               int num_q_heads = NUM_Q_HEADS, int window = 0, float* row_lse = nullptr) {
+    detail::check(qe_launch_attention_gqa_paged_prefill(detail::h(q), &cache, &batch, workspace, detail::h(attn_out),
+                                                        row_lse, stream, num_q_heads, window),
+                  "launch_attention_gqa_paged_prefill");
+}
+
+inline void launch_paged_key_bounds(const PagedCache& cache, const PagedBatch& batch, int8_t* bounds,
+                                    float* bound_steps, hipStream_t stream) {
+    detail::check(qe_launch_paged_key_bounds(&cache, &batch, bounds, bound_steps, stream), "launch_paged_key_bounds");
+}
+
+inline void launch_paged_select(const half* q, const PagedCache& cache, const PagedBatch& batch, const int8_t* bounds,
+                                const float* bound_steps, int32_t* selected, void* workspace, hipStream_t stream,
+                                int num_q_heads = NUM_Q_HEADS, int num_selected = 32, int sinks = 1, int recent = 2) {
+    detail::check(qe_launch_paged_select(detail::h(q), &cache, &batch, bounds, bound_steps, selected, workspace, stream,
+                                         num_q_heads, num_selected, sinks, recent),
+                  "launch_paged_select");
+}
+
+inline void launch_attention_gqa_paged_sparse(const half* q, const PagedCache& cache, const PagedBatch& batch,
+                                              const int32_t* selected, void* workspace, half* attn_out,
+                                              hipStream_t stream, int num_q_heads = NUM_Q_HEADS, int num_selected = 32,
+                                              float* row_lse = nullptr) {
+    detail::check(qe_launch_attention_gqa_paged_sparse(detail::h(q), &cache, &batch, selected, workspace,
+                                                       detail::h(attn_out), row_lse, stream, num_q_heads, num_selected),
+                  "launch_attention_gqa_paged_sparse");
+}
+
 // row_stride 0: rows of vocab_size logits behind each other.
 inline void launch_token_logprobs(const half* logits, const int32_t* token_ids, float* out_logprob,
                                   float* out_entropy, float* out_top_logprob, int32_t* out_top_ids, void* workspace,

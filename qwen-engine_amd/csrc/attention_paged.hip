@@ -716,7 +716,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         const PagedSeq s = paged_seq(p.c, seq);
         // weights: keys times group, as if the rows were cut between tokens
         const long long g = p.group, cap = p.c.capacity();
-        SeqWork w{g * (s.ctx + kOver), kPfRows, g * (cap + kOver), 0, p.c.nkv};
+        SeqWork w{g * (static_cast<long long>(s.ctx) + kOver), kPfRows, g * (cap + kOver), 0, p.c.nkv};
         if (p.window > 0) w.most = min(w.most, g * (p.window + kPfRows / g + kPfKeys + kOver));
         w.row_tiles = static_cast<int>((s.n * g + kPfRows - 1) / kPfRows);
         return w;

@@ -31,93 +31,126 @@ constexpr float kPgLag = 8.0f;
 // that it ends in (slot 1).  Tile t of a segment of n tiles and weight w belongs to the
 // place t * w / n of its stretch; the bits of a row depend on the lengths of the whole
 // batch, through where the cuts fall, and on nothing else.
-struct SegmentCut {    // of the block that has a segment's beginning but not its end
-    long long at, share, weight;  // where the segment begins; the length of a share
+//
+// Weights are whole numbers whose sum is below 2^30: the launcher says by how many
+// bits they have to be shortened (kernels: `coarse`).
+struct SegmentCut {  // of the block that has a segment's beginning but not its end
+    int at, share, weight;            // where the segment begins; the length of a share
     int tiles, item, head, row_tile;  // tiles 0: there is no such segment
+    int pad;
 };
 
-__device__ __forceinline__ long long uniform(long long x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(x) >> 32));
-    return static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo);
-}
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Tiles of a segment that lie before place x of the line.
-__device__ __forceinline__ int tiles_before(long long x, long long at, long long weight, int tiles) {
+// Tiles of a segment that lie before place x of the line.  (In fp32: it rises with x, and everyone
+// who asks gets the same.)
+__device__ __forceinline__ int tiles_before(int x, int at, int weight, int tiles) {
     if (x <= at) return 0;
     if (x >= at + weight) return tiles;
-    return min(tiles, static_cast<int>(static_cast<double>(x - at) * tiles / static_cast<double>(weight)));
+    return min(tiles, static_cast<int>(static_cast<float>(x - at) * (static_cast<float>(tiles) / static_cast<float>(weight))));
 }
 
 // One sequence on the line: `heads` times row tiles whose weights are first + step *
 // (i + 1), but at most `most`.
 struct SeqWork {
-    long long first, step, most;
+    int first, step, most;
     int row_tiles, heads;
 
-    __device__ __forceinline__ long long before(long long i) const {  // weight of the first i row tiles
-        long long m = i;
-        if (step > 0) m = min(i, max(0LL, (most - first) / step));
+    __device__ __forceinline__ int before(int i) const {  // weight of the first i row tiles
+        if (step == 0) return i * min(first, most);
+        const int m = min(i, max(0, most - first) / step);
         return m * first + step * (m * (m + 1) / 2) + (i - m) * most;
     }
-    __device__ __forceinline__ long long weight(int i) const { return min(most, first + step * (i + 1)); }
-    __device__ __forceinline__ long long all() const { return row_tiles > 0 ? heads * before(row_tiles) : 0; }
+    __device__ __forceinline__ int weight(int i) const { return min(most, first + step * (i + 1)); }
+    __device__ __forceinline__ int all() const { return row_tiles > 0 ? heads * before(row_tiles) : 0; }
 };
 
-// Sum over a wave up to and with each lane.
-__device__ __forceinline__ long long wave_scan(long long x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const long long y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+// Sum over a wave up to and with each lane, in the vector unit: 1, 2, 4 and 8 lanes on within rows
+// of 16, then the rows' sums.
+__device__ __forceinline__ int wave_scan(int x) {
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    typedef std::integral_constant<int, 0xF> all;
+    add(std::integral_constant<int, 0x111>{}, all{});
+    add(std::integral_constant<int, 0x112>{}, all{});
+    add(std::integral_constant<int, 0x114>{}, all{});
+    add(std::integral_constant<int, 0x118>{}, all{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row 15's and 47's sum
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row 31's
     return x;
 }
 
-// Runs body(sequence, head, row tile, tiles, first tile, end tile, slot) for each piece of a
-// segment in this block's share, by all waves of the block alike, and leaves the cut
-// that its last segment makes.  slot: -1 for a whole segment, else where its partials go.
-// work(s): the SeqWork of sequence s of `seqs`, tiles(s, row tile): its key tiles.
-template <class Work, class Tiles, class Body, class Cut>
-__device__ __forceinline__ void for_share(int block, int blocks, int seqs, long long least_share, Work work, Tiles tiles,
-                                          Body body, Cut cut) {
-    const int lane = threadIdx.x & 63;
-    // the whole line, then the sequence in which the share begins
-    long long total = 0;
-    for (int s0 = 0; s0 < seqs; s0 += 64) {
-        long long w = s0 + lane < seqs ? work(s0 + lane).all() : 0;
-        w = wave_scan(w);
-        total += uniform(__shfl(w, 63));
+// 64 sequences of the batch, one a lane.
+struct SeqChunk {
+    int base, first, n, ctx;
+    __device__ __forceinline__ void read(const PagedView& c, int at) {
+        base = at;
+        const int s = at + (threadIdx.x & 63);
+        PagedSeq q{0, 0, 0};
+        if (s < c.seqs) q = paged_seq(c, s);
+        first = q.first;
+        n = q.n;
+        ctx = q.ctx;
     }
-    const long long share = max(least_share, (total + blocks - 1) / blocks);
-    const long long x0 = share * block, x1 = min(total, x0 + share);
+    __device__ __forceinline__ PagedSeq lane() const { return PagedSeq{first, n, ctx}; }
+    __device__ __forceinline__ PagedSeq seq(const PagedView& c, int s) {  // s: the same in all lanes
+        if (s < base || s >= base + 64) read(c, s);
+        const int k = s - base;
+        return PagedSeq{__builtin_amdgcn_readlane(first, k), __builtin_amdgcn_readlane(n, k), __builtin_amdgcn_readlane(ctx, k)};
+    }
+};
+
+// Runs body(item, its sequence, head, row tile, first tile, end tile, slot) for each piece of a segment
+// in this block's share, by all waves of the block alike; then cut(the cut that its last
+// segment makes).  slot: -1 for a whole segment, else where its partials go.  work(sequence):
+// the SeqWork of one of the batch's sequences; tiles(sequence, row tile): its key tiles.
+// LISTED: there is only one item, whose work is work({}).
+template <bool LISTED, class Work, class Tiles, class Body, class Cut>
+__device__ __forceinline__ void for_share(const PagedView& c, int block, int blocks, int least_share, Work work,
+                                          Tiles tiles, Body body, Cut cut) {
+    // the whole line, then the sequence in which the share begins
+    SeqChunk chunk{};
+    const int seqs = LISTED ? 1 : c.seqs;
+    int total = 0, s = 0, at = 0, w = 0;
+    if constexpr (LISTED) {
+        total = work(PagedSeq{0, 1, 0}).all();
+    } else {
+        for (int s0 = 0; s0 < seqs; s0 += 64) {
+            chunk.read(c, s0);
+            w = wave_scan(work(chunk.lane()).all());
+            total += __builtin_amdgcn_readlane(w, 63);
+        }
+    }
+    const int share = max(least_share, (total + blocks - 1) / blocks);
+    const int x0 = min(total, share * block), x1 = min(total, x0 + share);
     SegmentCut last{};
     if (x0 >= x1) {
         cut(last);
         return;
     }
-    int s = 0;
-    long long at = 0;
-    for (int s0 = 0; s0 < seqs; s0 += 64) {
-        long long w = s0 + lane < seqs ? work(s0 + lane).all() : 0;
-        w = wave_scan(w);
-        const long long chunk = uniform(__shfl(w, 63));
-        if (x0 < at + chunk) {
-            const int k = __popcll(__builtin_amdgcn_ballot_w64(at + w <= x0));  // sequences before
-            s = s0 + k;
-            if (k > 0) at += uniform(__shfl(w, k - 1));
-            break;
+    if constexpr (!LISTED) {
+        for (int s0 = 0; s0 < seqs; s0 += 64) {
+            if (seqs > 64) {
+                chunk.read(c, s0);
+                w = wave_scan(work(chunk.lane()).all());
+            }
+            const int all = __builtin_amdgcn_readlane(w, 63);
+            if (x0 < at + all) {
+                const int k = __popcll(__builtin_amdgcn_ballot_w64(at + w <= x0));  // sequences before
+                s = s0 + k;
+                if (k > 0) at += __builtin_amdgcn_readlane(w, k - 1);
+                break;
+            }
+            at += all;
         }
-        at += chunk;
     }
-    s = uniform(s);
-    SeqWork q = work(s);
+    PagedSeq seq = LISTED ? PagedSeq{0, 1, 0} : chunk.seq(c, s);
+    SeqWork q = work(seq);
     int head, rt;
     {
-        const long long one = q.before(q.row_tiles);
-        head = static_cast<int>((x0 - at) / one);
+        const int one = q.before(q.row_tiles);
+        head = static_cast<int>(static_cast<uint32_t>(x0 - at) / static_cast<uint32_t>(one));
         at += one * head;
         int lo = 0, hi = q.row_tiles;  // before(lo) <= x0 - at < before(hi)
         while (hi - lo > 1) {
@@ -131,21 +164,23 @@ __device__ __forceinline__ void for_share(int block, int blocks, int seqs, long 
     rt = uniform(rt);
     at = uniform(at);
     while (true) {
-        const long long w = q.weight(rt);
-        const int n = tiles(s, rt);
-        const int t0 = tiles_before(x0, at, w, n), t1 = tiles_before(x1, at, w, n);
+        const int weight = q.weight(rt);
+        const int n = uniform(tiles(seq, rt));
+        const int t0 = uniform(tiles_before(x0, at, weight, n)), t1 = uniform(tiles_before(x1, at, weight, n));
         const bool whole = t0 == 0 && t1 == n;
-        if (whole ? n > 0 || x0 <= at : t0 < t1) body(s, head, rt, n, t0, t1, whole ? -1 : t0 == 0 ? 1 : 0);
-        if (t0 == 0 && t1 > 0 && t1 < n) {
-            last = SegmentCut{at, share, w, n, s, head, rt};
-        }
-        at += w;
+        if (whole ? n > 0 || x0 <= at : t0 < t1) body(s, seq, head, rt, t0, t1, whole ? -1 : t0 == 0 ? 1 : 0);
+        if (t0 == 0 && t1 > 0 && t1 < n) last = SegmentCut{at, share, weight, n, s, head, rt, 0};
+        at += weight;
         if (at >= x1) break;
         if (++rt == q.row_tiles) {
             rt = 0;
             if (++head == q.heads) {
                 head = 0;
-                do q = work(++s); while (q.row_tiles == 0);
+                do {
+                    if (++s >= seqs) return cut(last);  // (only where query_start decreases)
+                    seq = chunk.seq(c, s);
+                    q = work(seq);
+                } while (q.row_tiles == 0);
             }
         }
     }
@@ -216,14 +251,13 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
     const int live = map(c, rows);
     const int r_first = blockIdx.y * kRows;
     if (r_first >= live) return;
-    const long long end = c.at + c.weight;
-    const int parts = static_cast<int>((end - 1) / c.share) - b + 1;  // blocks that share the segment
+    const int parts = (c.at + c.weight - 1) / c.share - b + 1;  // blocks that share the segment
     const int tid = threadIdx.x, grp = tid >> 5, lane = tid & 31;
     const int row_in = GROUPS == 1 ? grp : 0, part_in = GROUPS == 1 ? 0 : grp;
     const int r = r_first + row_in;
     auto slot = [&](int i) { return static_cast<size_t>(2 * (b + i) + (i == 0 ? 1 : 0)) * ROWS; };
     auto holds = [&](int i) {  // block b + i has tiles of the segment
-        const long long x = (b + i) * c.share;
+        const int x = (b + i) * c.share;
         return tiles_before(x, c.at, c.weight, c.tiles) < tiles_before(x + c.share, c.at, c.weight, c.tiles);
     };
     // the common reference value of each row
@@ -250,22 +284,32 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
     float l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (r < live) {
-        for (int i = part_in; i < parts; i += GROUPS) {
-            float mi, li;
-            if (i < kParts) {
-                mi = s_w[row_in][i], li = s_l[row_in][i];
-            } else {
-                const float2 v = holds(i) ? p.ml[slot(i) + r] : make_float2(-INFINITY, 0.0f);
-                mi = v.x, li = v.y;
+        constexpr int B = 8;  // partial outputs requested at once
+        for (int i0 = part_in; i0 < parts; i0 += GROUPS * B) {
+            float mi[B], li[B];
+            float4 v[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const int i = i0 + k * GROUPS;
+                mi[k] = -INFINITY;
+                if (i < kParts) {
+                    if (i < parts) mi[k] = s_w[row_in][i], li[k] = s_l[row_in][i];
+                } else if (i < parts && holds(i)) {
+                    const float2 ml = p.ml[slot(i) + r];
+                    mi[k] = ml.x, li[k] = ml.y;
+                }
+                if (mi[k] != -INFINITY) v[k] = *reinterpret_cast<const float4*>(p.o + (slot(i) + r) * kPgDim + 4 * lane);
             }
-            if (mi == -INFINITY) continue;
-            const float w = part_weight(mi, m);
-            const float4 v = *reinterpret_cast<const float4*>(p.o + (slot(i) + r) * kPgDim + 4 * lane);
-            l += w * li;
-            o.x += w * v.x;
-            o.y += w * v.y;
-            o.z += w * v.z;
-            o.w += w * v.w;
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                if (mi[k] == -INFINITY) continue;
+                const float w = part_weight(mi[k], m);
+                l += w * li[k];
+                o.x += w * v[k].x;
+                o.y += w * v[k].y;
+                o.z += w * v[k].z;
+                o.w += w * v[k].w;
+            }
         }
     }
     if constexpr (GROUPS > 1) {
@@ -309,6 +353,7 @@ constexpr int kDecWaves = 4;    // waves of a block
 constexpr int kDecBlocks = 768; // of a launch
 constexpr int kDecKeys = 32;    // keys of a tile
 constexpr int kDecRows = 16;    // rows of a segment
+constexpr int kDecOver = 4;     // what starting a segment costs, in tiles
 
 struct DecodeParams {
     PagedView c;
@@ -317,7 +362,7 @@ struct DecodeParams {
     uint16_t* out;
     float* lse;
     void* ws;
-    int nq, group, window, num_selected, blocks;
+    int nq, group, window, num_selected, blocks, coarse;
 };
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -367,35 +412,22 @@ __global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeP
 
     // On the line: each sequence has its token's heads; or one sequence has those of all rows, the heads of
     // a row behind each other (all alike: which rows have a token is seen when their turn comes).
-    constexpr int kOver = 4;  // what starting a segment costs, in tiles
-    auto token = [&](int item, int head, int& row, int& h, int& seq, PagedSeq& s) __attribute__((always_inline)) {
-        row = SPARSE ? head / p.c.nkv : item;
-        h = SPARSE ? head - row * p.c.nkv : head;
-        seq = SPARSE ? uniform(paged_seq_of_row(p.c, row)) : item;
-        if (seq < 0) return false;
-        s = paged_seq(p.c, seq);
-        return row >= s.first && row < s.first + s.n;
-    };
-    auto work = [&](int item) __attribute__((always_inline)) {
-        SeqWork w{0, 0, 0, row_tiles, p.c.nkv};
-        if constexpr (SPARSE) {
-            w.heads = p.c.rows * p.c.nkv;
-            w.first = w.most = decode_range<SPARSE>(p, PagedSeq{0, 1, 0}, 0).tiles + kOver;
-        } else {
-            const PagedSeq s = paged_seq(p.c, item);
-            if (s.n > 0) w.first = w.most = decode_range<SPARSE>(p, s, item).tiles + kOver;
-            else w.row_tiles = 0;
-        }
+    auto work = [&](const PagedSeq& s) __attribute__((always_inline)) {
+        SeqWork w{0, 0, 0, s.n > 0 ? row_tiles : 0, SPARSE ? p.c.rows * p.c.nkv : p.c.nkv};
+        w.first = w.most = (decode_range<SPARSE>(p, s, s.first).tiles >> p.coarse) + kDecOver;
         return w;
     };
-    auto tiles = [&](int item, int) __attribute__((always_inline)) {
-        return uniform(decode_range<SPARSE>(p, SPARSE ? PagedSeq{0, 1, 0} : paged_seq(p.c, item), item).tiles);
-    };
+    auto tiles = [&](const PagedSeq& s, int) __attribute__((always_inline)) { return decode_range<SPARSE>(p, s, s.first).tiles; };
 
-    auto body = [&](int item, int head, int rt, int, int t0, int t1, int slot) __attribute__((always_inline)) {
-        int row, h, seq;
-        PagedSeq s;
-        if (!token(item, head, row, h, seq, s)) return;  // a row of no sequence: not written
+    auto body = [&](int item, PagedSeq s, int head, int rt, int t0, int t1, int slot) __attribute__((always_inline)) {
+        const int row = SPARSE ? head / p.c.nkv : s.first, h = SPARSE ? head - row * p.c.nkv : head;
+        int seq = item;
+        if constexpr (SPARSE) {
+            seq = uniform(paged_seq_of_row(p.c, row));
+            if (seq < 0) return;
+            s = paged_seq(p.c, seq);
+            if (row < s.first || row >= s.first + s.n) return;  // a row of no sequence: not written
+        }
         const DecodeRange range = decode_range<SPARSE>(p, s, row);
         const int lim = uniform(range.lim), lo = uniform(range.lo);
         const int live = min(kDecRows, p.group - rt * kDecRows);
@@ -585,7 +617,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeP
         }
         __syncthreads();  // the next segment writes s_m
     };
-    for_share(blockIdx.x, p.blocks, SPARSE ? 1 : p.c.seqs, NW + kOver, work, tiles, body, [&](SegmentCut cut) {
+    for_share<SPARSE>(p.c, blockIdx.x, p.blocks, (NW >> p.coarse) + kDecOver, work, tiles, body, [&](SegmentCut cut) {
         if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
     });
 }
@@ -626,6 +658,7 @@ constexpr int kPfRows = 128;     // rows of a segment
 constexpr int kPfKeys = 64;      // keys of a tile
 constexpr int kPfTileBytes = kPfKeys * kPgDim * 2;
 constexpr int kPfBlocks = 512;   // of a launch: two a CU
+constexpr int kPfOver = 2 * kPfKeys;  // what a segment costs beside its keys, in keys
 
 __device__ __align__(256) const uint16_t g_zero_row[kPgDim] = {};
 
@@ -635,7 +668,7 @@ struct PrefillParams {
     uint16_t* out;
     float* lse;
     void* ws;
-    int nq, group, window;
+    int nq, group, window, coarse;
 };
 
 struct PrefillRange {
@@ -653,6 +686,12 @@ __device__ __forceinline__ PrefillRange prefill_range(const PrefillParams& p, co
     r.first_tile = r.low / kPfKeys;
     r.tiles = last < r.low ? 0 : last / kPfKeys - r.first_tile + 1;
     return r;
+}
+
+// Weight of so many keys for a token's group: shortened as the launch says, 1 to 2^29.
+__device__ __forceinline__ int weight_of(const PrefillParams& p, int keys) {
+    const long long w = static_cast<long long>(p.group) * (static_cast<long long>(keys) + kPfOver) >> p.coarse;
+    return static_cast<int>(max(1LL, min(w, 1LL << 29)));
 }
 
 // ONE: pages of 64 tokens and more (a tile lies in one page).
@@ -711,22 +750,16 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    constexpr int kOver = 2 * kPfKeys;  // what a segment costs beside its keys, in keys
-    auto work = [&](int seq) __attribute__((always_inline)) {
-        const PagedSeq s = paged_seq(p.c, seq);
+    auto work = [&](const PagedSeq& s) __attribute__((always_inline)) {
         // weights: keys times group, as if the rows were cut between tokens
-        const long long g = p.group, cap = p.c.capacity();
-        SeqWork w{g * (static_cast<long long>(s.ctx) + kOver), kPfRows, g * (cap + kOver), 0, p.c.nkv};
-        if (p.window > 0) w.most = min(w.most, g * (p.window + kPfRows / g + kPfKeys + kOver));
-        w.row_tiles = static_cast<int>((s.n * g + kPfRows - 1) / kPfRows);
+        const int g = p.group;
+        SeqWork w{weight_of(p, s.ctx), kPfRows >> p.coarse, weight_of(p, p.c.capacity()), (s.n * g + kPfRows - 1) / kPfRows, p.c.nkv};
+        if (p.window > 0) w.most = min(w.most, weight_of(p, min(p.window, p.c.capacity()) + kPfRows / g + kPfKeys));
         return w;
     };
-    auto tiles = [&](int seq, int rt) __attribute__((always_inline)) {
-        return uniform(prefill_range(p, paged_seq(p.c, seq), rt).tiles);
-    };
+    auto tiles = [&](const PagedSeq& s, int rt) __attribute__((always_inline)) { return prefill_range(p, s, rt).tiles; };
 
-    auto body = [&](int seq, int kvh, int rt, int, int t0, int t1, int slot) __attribute__((always_inline)) {
-        const PagedSeq s = paged_seq(p.c, seq);
+    auto body = [&](int seq, const PagedSeq& s, int kvh, int rt, int t0, int t1, int slot) __attribute__((always_inline)) {
         const PrefillRange range = prefill_range(p, s, rt);
         const int rows = uniform(range.rows), first_tile = uniform(range.first_tile), low = uniform(range.low);
         const int it0 = first_tile + t0, it1 = first_tile + t1;
@@ -994,10 +1027,10 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         tile_barrier();  // the tiles are read: the next segment fills them
     };
     constexpr int kLeastTiles = 4;
-    for_share(block, kPfBlocks, p.c.seqs, static_cast<long long>(p.group) * kLeastTiles * kPfKeys, work, tiles, body,
-              [&](SegmentCut cut) {
-                  if (threadIdx.x == 0) part.cuts[block] = cut;
-              });
+    for_share<false>(p.c, block, kPfBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, body,
+                     [&](SegmentCut cut) {
+                         if (threadIdx.x == 0) part.cuts[block] = cut;
+                     });
 }
 
 __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillParams p) {
@@ -1050,6 +1083,15 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
     p.window = window;
     p.num_selected = num_selected;
     p.blocks = kDecBlocks;
+    const long long row_tiles = (p.group + kDecRows - 1) / kDecRows;
+    const long long most = SPARSE ? static_cast<long long>(num_selected) * cache->page_size
+                                  : static_cast<long long>(batch->max_pages) * cache->page_size;
+    const long long segments = row_tiles * cache->num_kv_heads * batch->num_tokens;
+    while (segments * (((most / kDecKeys + 1) >> p.coarse) + kDecOver) >= (1 << 30)) {
+        QE_REQUIRE(most / kDecKeys >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens,
+                   cache->num_kv_heads);
+        ++p.coarse;
+    }
     paged_decode_kernel<SPARSE><<<p.blocks, 64 * kDecWaves, 0, stream>>>(p);
     paged_decode_merge_kernel<SPARSE><<<dim3(p.blocks, std::min(p.group, kDecRows)), 256, 0, stream>>>(p);
     return check_launch(what);
@@ -1120,6 +1162,12 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     p.nq = num_q_heads;
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
+    const long long row_tiles = static_cast<long long>(batch->num_tokens) * p.group / kPfRows + batch->num_seqs;
+    const long long most = static_cast<long long>(p.group) * (static_cast<long long>(batch->max_pages) * cache->page_size + kPfOver);
+    while (row_tiles * cache->num_kv_heads > ((1LL << 30) - 1) / ((most >> p.coarse) + 1)) {
+        QE_REQUIRE(most >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens, cache->num_kv_heads);
+        ++p.coarse;
+    }
     if (p.c.shift >= 6)
         paged_prefill_kernel<true><<<kPfBlocks, 256, 0, stream>>>(p);
     else

@@ -36,8 +36,8 @@ constexpr float kPgLag = 8.0f;
 // bits they have to be shortened (kernels: `coarse`).
 struct SegmentCut {  // of the block that has a segment's beginning but not its end
     int at, share, weight;            // where the segment begins; the length of a share
-    int tiles, item, head, row_tile;  // tiles 0: there is no such segment
-    int pad;
+    int tiles, item, head, row_tile;
+    int rows;  // of the segment; 0: there is no such segment
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -104,11 +104,12 @@ struct SeqChunk {
 // Runs body(item, its sequence, head, row tile, first tile, end tile, slot) for each piece of a segment
 // in this block's share, by all waves of the block alike; then cut(the cut that its last
 // segment makes).  slot: -1 for a whole segment, else where its partials go.  work(sequence):
-// the SeqWork of one of the batch's sequences; tiles(sequence, row tile): its key tiles.
+// the SeqWork of one of the batch's sequences; tiles(sequence, row tile): its key tiles; rows(sequence,
+// head, row tile): its rows.
 // LISTED: there is only one item, whose work is work({}).
-template <bool LISTED, class Work, class Tiles, class Body, class Cut>
+template <bool LISTED, class Work, class Tiles, class Rows, class Body, class Cut>
 __device__ __forceinline__ void for_share(const PagedView& c, int block, int blocks, int least_share, Work work,
-                                          Tiles tiles, Body body, Cut cut) {
+                                          Tiles tiles, Rows rows, Body body, Cut cut) {
     // the whole line, then the sequence in which the share begins
     SeqChunk chunk{};
     const int seqs = LISTED ? 1 : c.seqs;
@@ -169,7 +170,7 @@ __device__ __forceinline__ void for_share(const PagedView& c, int block, int blo
         const int t0 = uniform(tiles_before(x0, at, weight, n)), t1 = uniform(tiles_before(x1, at, weight, n));
         const bool whole = t0 == 0 && t1 == n;
         if (whole ? n > 0 || x0 <= at : t0 < t1) body(s, seq, head, rt, t0, t1, whole ? -1 : t0 == 0 ? 1 : 0);
-        if (t0 == 0 && t1 > 0 && t1 < n) last = SegmentCut{at, share, weight, n, s, head, rt, 0};
+        if (t0 == 0 && t1 > 0 && t1 < n) last = SegmentCut{at, share, weight, n, s, head, rt, rows(seq, head, rt)};
         at += weight;
         if (at >= x1) break;
         if (++rt == q.row_tiles) {
@@ -233,106 +234,132 @@ __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
                       static_cast<uint32_t>(f2h(c)) | static_cast<uint32_t>(f2h(d)) << 16);
 }
 
-// Merges the parts of the segments that were cut: block b looks after the segment that
-// main block b began and did not end.  8 / GROUPS rows a block, GROUPS times 32
-// lanes a row (4 dims each): the groups take every GROUPS-th part.
-template <int ROWS, int GROUPS, class Map>
+// Merges the parts of the segments that were cut.  An item is THREADS / 32 / GROUPS rows of one cut
+// segment, GROUPS times 32 lanes a row (4 dims each): the groups take every GROUPS-th part, eight
+// partial outputs requested at once.  Every block counts the cuts and takes its share of the items.
+constexpr int kMergeCuts = 512;  // cuts of a launch, at most
+template <int ROWS, int GROUPS, int THREADS, class Map>
 __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out, float* lse, int nq, Map map) {
-    constexpr int kRows = 8 / GROUPS;  // rows of a block
-    constexpr int kParts = 512;        // weights kept at once
+    constexpr int kRows = THREADS / 32 / GROUPS;  // rows of an item
+    constexpr int kParts = GROUPS > 1 ? 512 : 32;  // weights kept at once
+    constexpr int kWaves = THREADS / 64;
     __shared__ float s_w[kRows][kParts], s_l[kRows][kParts];
-    __shared__ float s_red[kRows][8];
-    __shared__ float4 s_o[GROUPS > 1 ? 8 : 1][32];
+    __shared__ float s_red[THREADS / 32];
+    __shared__ float4 s_o[GROUPS > 1 ? THREADS / 32 : 1][32];
+    __shared__ int s_first[kMergeCuts + 1];  // the items before those of each cut
+    __shared__ short s_cut[kMergeCuts];      // its block
+    __shared__ int2 s_count[kWaves];
+    __shared__ int s_found;
     const Partials p = partials<ROWS>(ws, blocks);
-    const int b = blockIdx.x;
-    const SegmentCut c = p.cuts[b];
-    if (c.tiles == 0) return;
-    RowMap rows;
-    const int live = map(c, rows);
-    const int r_first = blockIdx.y * kRows;
-    if (r_first >= live) return;
-    const int parts = (c.at + c.weight - 1) / c.share - b + 1;  // blocks that share the segment
     const int tid = threadIdx.x, grp = tid >> 5, lane = tid & 31;
-    const int row_in = GROUPS == 1 ? grp : 0, part_in = GROUPS == 1 ? 0 : grp;
-    const int r = r_first + row_in;
-    auto slot = [&](int i) { return static_cast<size_t>(2 * (b + i) + (i == 0 ? 1 : 0)) * ROWS; };
-    auto holds = [&](int i) {  // block b + i has tiles of the segment
-        const int x = (b + i) * c.share;
-        return tiles_before(x, c.at, c.weight, c.tiles) < tiles_before(x + c.share, c.at, c.weight, c.tiles);
-    };
-    // the common reference value of each row
-    constexpr int kPer = 256 / kRows;  // threads that read a row's values
-    const int vr = tid / kPer, vi = tid % kPer;
-    float m = -INFINITY;
-    for (int i = vi; i < parts; i += kPer) {
-        float2 v = make_float2(-INFINITY, 0.0f);
-        if (r_first + vr < live && holds(i)) v = p.ml[slot(i) + r_first + vr];
-        if (i < kParts) s_w[vr][i] = v.x, s_l[vr][i] = v.y;
-        m = fmaxf(m, v.x);
-    }
-#pragma unroll
-    for (int d = 1; d < (kPer < 64 ? kPer : 64); d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    if constexpr (kPer > 64) {
-        if ((tid & 63) == 0) s_red[0][tid >> 6] = m;
+    // the blocks with a cut, in their order
+    int cuts = 0, items = 0;
+    for (int b0 = 0; b0 < blocks; b0 += THREADS) {
+        const int b = b0 + tid;
+        const int mine = b < blocks ? (p.cuts[b].rows + kRows - 1) / kRows : 0;
+        const uint64_t live = __builtin_amdgcn_ballot_w64(mine != 0);
+        const int upto = wave_scan(mine);
+        if ((tid & 63) == 63) s_count[tid >> 6] = make_int2(__popcll(live), upto);
         __syncthreads();
-        m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-    } else {
-        if (vi == 0) s_red[vr][0] = m;
+        int at = cuts + __popcll(live & ((1ull << (tid & 63)) - 1)), first = items + upto - mine;
+        for (int w = 0; w < kWaves; ++w) {
+            at += w < (tid >> 6) ? s_count[w].x : 0;
+            first += w < (tid >> 6) ? s_count[w].y : 0;
+            cuts += s_count[w].x;
+            items += s_count[w].y;
+        }
+        if (mine != 0) s_cut[at] = static_cast<short>(b), s_first[at] = first;
         __syncthreads();
-        m = s_red[row_in][0];
     }
-    float l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (r < live) {
-        constexpr int B = 8;  // partial outputs requested at once
-        for (int i0 = part_in; i0 < parts; i0 += GROUPS * B) {
-            float mi[B], li[B];
-            float4 v[B];
+    if (tid == 0) s_first[cuts] = items;
+    __syncthreads();
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        for (int k = tid; k < cuts; k += THREADS)
+            if (s_first[k] <= item && item < s_first[k + 1]) s_found = k;
+        __syncthreads();
+        const int b = s_cut[s_found], r_first = (item - s_first[s_found]) * kRows;
+        const SegmentCut c = p.cuts[b];
+        const RowMap rows = map(c);
+        const int live = c.rows;
+        const int parts = (c.at + c.weight - 1) / c.share - b + 1;  // blocks that share the segment
+        const int row_in = grp / GROUPS, part_in = grp % GROUPS, r = r_first + row_in;
+        auto slot = [&](int i) { return static_cast<size_t>(2 * (b + i) + (i == 0 ? 1 : 0)) * ROWS; };
+        auto holds = [&](int i) {  // block b + i has tiles of the segment
+            const int x = (b + i) * c.share;
+            return tiles_before(x, c.at, c.weight, c.tiles) < tiles_before(x + c.share, c.at, c.weight, c.tiles);
+        };
+        // the common reference value of each row
+        constexpr int kPer = THREADS / kRows;  // threads of a row
+        const int vi = tid % kPer;
+        float m = -INFINITY;
+        for (int i = vi; i < parts; i += kPer) {
+            float2 v = make_float2(-INFINITY, 0.0f);
+            if (r < live && holds(i)) v = p.ml[slot(i) + r];
+            if (i < kParts) s_w[row_in][i] = v.x, s_l[row_in][i] = v.y;
+            m = fmaxf(m, v.x);
+        }
 #pragma unroll
-            for (int k = 0; k < B; ++k) {
-                const int i = i0 + k * GROUPS;
-                mi[k] = -INFINITY;
-                if (i < kParts) {
-                    if (i < parts) mi[k] = s_w[row_in][i], li[k] = s_l[row_in][i];
-                } else if (i < parts && holds(i)) {
-                    const float2 ml = p.ml[slot(i) + r];
-                    mi[k] = ml.x, li[k] = ml.y;
+        for (int d = 1; d < 32; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        if (lane == 0) s_red[grp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, s_red[row_in * GROUPS + g]);
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < live) {
+            constexpr int B = 8;
+            for (int i0 = part_in; i0 < parts; i0 += GROUPS * B) {
+                float mi[B], li[B];
+                float4 v[B];
+#pragma unroll
+                for (int k = 0; k < B; ++k) {
+                    const int i = i0 + k * GROUPS;
+                    mi[k] = -INFINITY;
+                    if (i < kParts) {
+                        if (i < parts) mi[k] = s_w[row_in][i], li[k] = s_l[row_in][i];
+                    } else if (i < parts && holds(i)) {
+                        const float2 ml = p.ml[slot(i) + r];
+                        mi[k] = ml.x, li[k] = ml.y;
+                    }
+                    if (mi[k] != -INFINITY) v[k] = *reinterpret_cast<const float4*>(p.o + (slot(i) + r) * kPgDim + 4 * lane);
                 }
-                if (mi[k] != -INFINITY) v[k] = *reinterpret_cast<const float4*>(p.o + (slot(i) + r) * kPgDim + 4 * lane);
-            }
 #pragma unroll
-            for (int k = 0; k < B; ++k) {
-                if (mi[k] == -INFINITY) continue;
-                const float w = part_weight(mi[k], m);
-                l += w * li[k];
-                o.x += w * v[k].x;
-                o.y += w * v[k].y;
-                o.z += w * v[k].z;
-                o.w += w * v[k].w;
+                for (int k = 0; k < B; ++k) {
+                    if (mi[k] == -INFINITY) continue;
+                    const float w = part_weight(mi[k], m);
+                    l += w * li[k];
+                    o.x += w * v[k].x;
+                    o.y += w * v[k].y;
+                    o.z += w * v[k].z;
+                    o.w += w * v[k].w;
+                }
             }
         }
-    }
-    if constexpr (GROUPS > 1) {
-        __syncthreads();
-        s_o[grp][lane] = o;
-        if (lane == 0) s_red[0][grp] = l;
-        __syncthreads();
-        if (grp != 0) return;
-        l = s_red[0][0];
-        for (int g = 1; g < GROUPS; ++g) {
-            const float4 v = s_o[g][lane];
-            l += s_red[0][g];
-            o.x += v.x;
-            o.y += v.y;
-            o.z += v.z;
-            o.w += v.w;
+        if constexpr (GROUPS > 1) {
+            __syncthreads();  // s_red is read
+            s_o[grp][lane] = o;
+            if (lane == 0) s_red[grp] = l;
+            __syncthreads();
+            l = 0.0f;
+            o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (part_in == 0)
+                for (int g = 0; g < GROUPS; ++g) {
+                    const float4 v = s_o[grp + g][lane];
+                    l += s_red[grp + g];
+                    o.x += v.x;
+                    o.y += v.y;
+                    o.z += v.z;
+                    o.w += v.w;
+                }
         }
+        if (r < live && part_in == 0) {
+            const float inv = row_inverse(m, l);
+            const size_t at = static_cast<size_t>(rows.row(r)) * nq + rows.head(r);
+            *reinterpret_cast<uint2*>(out + at * kPgDim + 4 * lane) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            if (lse != nullptr && lane == 0) lse[at] = row_log_sum(m, l);
+        }
+        __syncthreads();  // the next item writes s_w, s_red and s_o
     }
-    if (r >= live) return;
-    const float inv = row_inverse(m, l);
-    const size_t at = static_cast<size_t>(rows.row(r)) * nq + rows.head(r);
-    *reinterpret_cast<uint2*>(out + at * kPgDim + 4 * lane) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (lse != nullptr && lane == 0) lse[at] = row_log_sum(m, l);
 }
 
 // ---- single tokens and selected blocks -----------------------------------------
@@ -349,11 +376,11 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
 // lane ends with dims 32 g .. 32 g + 31 of head c.  The softmax weights are rounded to fp16 for
 // the product with V (2^-11, as everywhere in this library's matrix-core attention); scores, sums
 // and outputs are fp32.
-constexpr int kDecWaves = 4;    // waves of a block
-constexpr int kDecBlocks = 768; // of a launch
-constexpr int kDecKeys = 32;    // keys of a tile
-constexpr int kDecRows = 16;    // rows of a segment
-constexpr int kDecOver = 4;     // what starting a segment costs, in tiles
+constexpr int kDecWaves = 8;     // waves of a block
+constexpr int kDecBlocks = 256;  // of a launch: one a CU
+constexpr int kDecKeys = 32;     // keys of a tile
+constexpr int kDecRows = 16;     // rows of a segment
+constexpr int kDecOver = 4;      // what starting a segment costs, in tiles
 
 struct DecodeParams {
     PagedView c;
@@ -362,7 +389,7 @@ struct DecodeParams {
     uint16_t* out;
     float* lse;
     void* ws;
-    int nq, group, window, num_selected, blocks, coarse;
+    int nq, group, window, num_selected, coarse;
 };
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -400,13 +427,13 @@ __device__ __forceinline__ DecodeRange decode_range(const DecodeParams& p, const
 }
 
 template <bool SPARSE>
-__global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeParams p) {
+__global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeParams p) {
     constexpr int NW = kDecWaves, kPad = kPgDim + 4;
     __shared__ float s_m[NW][kDecRows], s_l[NW][kDecRows];
     __shared__ __align__(16) float s_o[NW][kDecRows][kPad];
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int c = lane & 15, g = lane >> 4;
-    const Partials part = partials<kDecRows>(p.ws, p.blocks);
+    const Partials part = partials<kDecRows>(p.ws, kDecBlocks);
     const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
     const ptrdiff_t v_minus_k = reinterpret_cast<const char*>(p.c.v) - reinterpret_cast<const char*>(p.c.k);
 
@@ -484,8 +511,11 @@ __global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeP
         };
         auto request_v = [&](const Tile& x) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                vf[i] = *reinterpret_cast<const u32x4*>(x.k[i >> 2] + v_minus_k + (v_off + 4 * (i & 3) * kPgDim * 2));
+            for (int i = 0; i < 8; ++i) {
+                // a row of V is read once by each wave: not kept, unless the rows of other tokens read it too
+                const u32x4* v = reinterpret_cast<const u32x4*>(x.k[i >> 2] + v_minus_k + (v_off + 4 * (i & 3) * kPgDim * 2));
+                vf[i] = SPARSE ? *v : __builtin_nontemporal_load(v);
+            }
         };
         f32x4 acc[8];
 #pragma unroll
@@ -617,24 +647,26 @@ __global__ __launch_bounds__(64 * kDecWaves, 3) void paged_decode_kernel(DecodeP
         }
         __syncthreads();  // the next segment writes s_m
     };
-    for_share<SPARSE>(p.c, blockIdx.x, p.blocks, (NW >> p.coarse) + kDecOver, work, tiles, body, [&](SegmentCut cut) {
-        if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
-    });
-}
-
-template <bool SPARSE>
-__global__ __launch_bounds__(256) void paged_decode_merge_kernel(DecodeParams p) {
-    merge_parts<kDecRows, 8>(p.ws, p.blocks, p.out, p.lse, p.nq, [&](const SegmentCut& c, RowMap& rows) {
-        const int row = SPARSE ? c.head / p.c.nkv : c.item, h = SPARSE ? c.head - row * p.c.nkv : c.head;
-        const int live = min(kDecRows, p.group - c.row_tile * kDecRows);
-        rows = RowMap{row, 0, live, h * p.group + c.row_tile * kDecRows};
-        if constexpr (SPARSE) {  // a row of no sequence has no parts
-            const int seq = paged_seq_of_row(p.c, row);
+    auto rows = [&](const PagedSeq&, int head, int rt) __attribute__((always_inline)) {
+        if constexpr (SPARSE) {
+            const int row = head / p.c.nkv, seq = paged_seq_of_row(p.c, row);
             if (seq < 0) return 0;
             const PagedSeq s = paged_seq(p.c, seq);
             if (row < s.first || row >= s.first + s.n) return 0;
         }
-        return live;
+        return min(kDecRows, p.group - rt * kDecRows);
+    };
+    for_share<SPARSE>(p.c, blockIdx.x, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
+        if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
+    });
+}
+
+template <bool SPARSE, int GROUPS, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParams p) {
+    static_assert(kDecBlocks <= kMergeCuts, "a cut for each block");
+    merge_parts<kDecRows, GROUPS, THREADS>(p.ws, kDecBlocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
+        const int row = SPARSE ? c.head / p.c.nkv : paged_seq(p.c, c.item).first, h = SPARSE ? c.head - row * p.c.nkv : c.head;
+        return RowMap{row, 0, kDecRows, h * p.group + c.row_tile * kDecRows};
     });
 }
 
@@ -1027,17 +1059,17 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         tile_barrier();  // the tiles are read: the next segment fills them
     };
     constexpr int kLeastTiles = 4;
-    for_share<false>(p.c, block, kPfBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, body,
+    auto rows = [&](const PagedSeq& s, int, int rt) __attribute__((always_inline)) { return min(kPfRows, s.n * p.group - rt * kPfRows); };
+    for_share<false>(p.c, block, kPfBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, rows, body,
                      [&](SegmentCut cut) {
                          if (threadIdx.x == 0) part.cuts[block] = cut;
                      });
 }
 
 __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillParams p) {
-    merge_parts<kPfRows, 1>(p.ws, kPfBlocks, p.out, p.lse, p.nq, [&](const SegmentCut& c, RowMap& rows) {
-        const PagedSeq s = paged_seq(p.c, c.item);
-        rows = RowMap{s.first, c.row_tile * kPfRows, p.group, c.head * p.group};
-        return min(kPfRows, s.n * p.group - c.row_tile * kPfRows);
+    static_assert(kPfBlocks <= kMergeCuts, "a cut for each block");
+    merge_parts<kPfRows, 1, 256>(p.ws, kPfBlocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
+        return RowMap{paged_seq(p.c, c.item).first, c.row_tile * kPfRows, p.group, c.head * p.group};
     });
 }
 
@@ -1082,7 +1114,6 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
     p.num_selected = num_selected;
-    p.blocks = kDecBlocks;
     const long long row_tiles = (p.group + kDecRows - 1) / kDecRows;
     const long long most = SPARSE ? static_cast<long long>(num_selected) * cache->page_size
                                   : static_cast<long long>(batch->max_pages) * cache->page_size;
@@ -1092,8 +1123,14 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
                    cache->num_kv_heads);
         ++p.coarse;
     }
-    paged_decode_kernel<SPARSE><<<p.blocks, 64 * kDecWaves, 0, stream>>>(p);
-    paged_decode_merge_kernel<SPARSE><<<dim3(p.blocks, std::min(p.group, kDecRows)), 256, 0, stream>>>(p);
+    paged_decode_kernel<SPARSE><<<kDecBlocks, 64 * kDecWaves, 0, stream>>>(p);
+    // Few segments have many parts each: a block a row, 32 parts at once.  (131000 keys, 12 heads: 5.8 us, with two
+    // rows a block 8.2; 48 sequences 13.1 and 5.)
+    const long long cuts = std::min<long long>(segments, kDecBlocks);
+    if (segments < 16)
+        paged_decode_merge_kernel<SPARSE, 32, 1024><<<static_cast<unsigned>(cuts * std::min(p.group, kDecRows)), 1024, 0, stream>>>(p);
+    else
+        paged_decode_merge_kernel<SPARSE, 4, 256><<<static_cast<unsigned>(cuts * ((std::min(p.group, kDecRows) + 1) / 2)), 256, 0, stream>>>(p);
     return check_launch(what);
 }
 
@@ -1172,6 +1209,7 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
         paged_prefill_kernel<true><<<kPfBlocks, 256, 0, stream>>>(p);
     else
         paged_prefill_kernel<false><<<kPfBlocks, 256, 0, stream>>>(p);
-    paged_prefill_merge_kernel<<<dim3(kPfBlocks, kPfRows / 8), 256, 0, stream>>>(p);
+    const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, kPfBlocks) * (kPfRows / 8);
+    paged_prefill_merge_kernel<<<static_cast<unsigned>(std::min(items, 2048LL)), 256, 0, stream>>>(p);
     return check_launch(what);
 }

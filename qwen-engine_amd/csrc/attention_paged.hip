@@ -15,8 +15,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float kPgScale = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 constexpr float kPgLowest = -3.4e38f;  // the maximum of keys whose every score is -inf: a sum of 0, so NaN
 // A row's reference value (what its scores are lowered by before the exponential) is its
-// running maximum, renewed only when that has grown by more than this: weights then reach
-// at most 2^8, and their relative precision in fp16 does not change.
+// running maximum (in chunks rounded down to a whole number), renewed only when that has grown
+// by more than this: weights then stay below 2^9, and their relative precision in fp16 does
+// not change.
 constexpr float kPgLag = 8.0f;
 
 // ---- shares of the work ------------------------------------------------------
@@ -686,11 +687,18 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // Rows that no one may see (behind the sequence's end, before every window, of missing
 // pages) are filled from a row of zeros: their weights are 0, and what lies there may be
 // anything.
-constexpr int kPfRows = 128;     // rows of a segment
-constexpr int kPfKeys = 64;      // keys of a tile
-constexpr int kPfTileBytes = kPfKeys * kPgDim * 2;
-constexpr int kPfBlocks = 512;   // of a launch: two a CU
+constexpr int kPfKeys = 64;           // keys of a tile: what shares are cut between
+constexpr int kPfHalf = 32;           // keys of a stage
+constexpr int kPfHalfBytes = kPfHalf * kPgDim * 2;
 constexpr int kPfOver = 2 * kPfKeys;  // what a segment costs beside its keys, in keys
+// Blocks of WAVES waves, 32 rows each; a CU holds eight waves.
+template <int WAVES>
+struct PrefillShape {
+    static constexpr int rows = 32 * WAVES;          // rows of a segment
+    static constexpr int blocks = 256 * 8 / WAVES;   // of a launch
+    static constexpr int period = WAVES / 2;         // stages between barriers
+    static constexpr int ring = 2 * period;          // halves of K, and of V, in LDS
+};
 
 __device__ __align__(256) const uint16_t g_zero_row[kPgDim] = {};
 
@@ -708,12 +716,14 @@ struct PrefillRange {
     int first_tile, tiles;  // key tiles that its rows see
     int low;                // the first key that one of them sees
 };
+template <int WAVES>
 __device__ __forceinline__ PrefillRange prefill_range(const PrefillParams& p, const PagedSeq& s, int rt) {
+    constexpr int kRows = PrefillShape<WAVES>::rows;
     PrefillRange r;
-    r.r0 = rt * kPfRows;
+    r.r0 = rt * kRows;
     r.rows = s.n * p.group;
     const int first = s.ctx + r.r0 / p.group;
-    const int last = min(s.ctx + (min(r.r0 + kPfRows, r.rows) - 1) / p.group, p.c.capacity() - 1);
+    const int last = min(s.ctx + (min(r.r0 + kRows, r.rows) - 1) / p.group, p.c.capacity() - 1);
     r.low = p.window > 0 ? max(0, first - p.window + 1) : 0;
     r.first_tile = r.low / kPfKeys;
     r.tiles = last < r.low ? 0 : last / kPfKeys - r.first_tile + 1;
@@ -726,32 +736,34 @@ __device__ __forceinline__ int weight_of(const PrefillParams& p, int keys) {
     return static_cast<int>(max(1LL, min(w, 1LL << 29)));
 }
 
-// ONE: pages of 64 tokens and more (a tile lies in one page).
-template <bool ONE>
-__global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) {
-    __shared__ __align__(256) char smem[4 * kPfTileBytes];  // K buffers 0 and 1, V buffers 0 and 1
+// ONE: pages of 32 tokens and more (a half tile lies in one page).
+template <bool ONE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillParams p) {
+    typedef PrefillShape<WAVES> Shape;
+    constexpr int kRows = Shape::rows, kBlocks = Shape::blocks, P = Shape::period, R = Shape::ring;
+    __shared__ __align__(256) char smem[2 * R * kPfHalfBytes];  // the last R halves of K, of V
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int fr = lane & 31, h = lane >> 5;
     // blocks of one XCD take neighbouring shares: they read the same pages
-    const int block = static_cast<int>(blockIdx.x & 7) * (kPfBlocks / 8) + static_cast<int>(blockIdx.x >> 3);
-    const Partials part = partials<kPfRows>(p.ws, kPfBlocks);
-    const ptrdiff_t v_minus_k = p.c.v - p.c.k;  // elements
-    constexpr int NP = ONE ? 1 : 4;             // pages of a tile, at most
+    const int block = static_cast<int>(blockIdx.x & 7) * (kBlocks / 8) + static_cast<int>(blockIdx.x >> 3);
+    const Partials part = partials<kRows>(p.ws, kBlocks);
+    constexpr int NP = ONE ? 1 : 2;             // pages of a half tile, at most
 
     const uint32_t lds0 =
         static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)smem));
-    // tile load i of a wave: tile rows 16 i + 4 wave + lane / 16, stored chunk lane % 16, i.e. chunk
-    // (lane % 16) ^ swz(row) of memory
-    const int lrow = 4 * wave + (lane >> 4);
-    const int lcol = 8 * ((lane & 15) ^ (((lane >> 4) << 2) | wave));
-    const uint32_t loff = static_cast<uint32_t>(2 * (lrow * kPgDim + lcol));  // bytes
+    // A wave loads whole halves, by eight loads of four rows: load i its rows 4 i + lane / 16, stored chunk lane % 16,
+    // i.e. chunk (lane % 16) ^ swz(row) of memory.  The first four lanes' offsets (the others are 16 rows on):
+    uint32_t loff[4];  // bytes
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        loff[i] = static_cast<uint32_t>((4 * i + (lane >> 4)) * (2 * kPgDim) + 16 * ((lane & 15) ^ (((lane >> 4) << 2) | i)));
     // LDS addresses: K chunk 2 kk + h of key fr; V^T reads (dt: 32 dims, u: keys + 8)
     uint32_t ka[8], va[4][2];
     {
         const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
         const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
         const int s16 = lane & 15, b16 = (lane >> 4) & 1;
-        const uint32_t v0 = lds0 + 2 * kPfTileBytes + (4 * h + (s16 >> 2)) * 256 +
+        const uint32_t v0 = lds0 + (R + P) * kPfHalfBytes + (4 * h + (s16 >> 2)) * 256 +
                             16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
@@ -761,15 +773,26 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
             va[dt][1] = (v0 ^ (64 * dt) ^ 32) + 8 * 256;
         }
     }
-    // K operand of MFMA i of a tile: 32-key half i % 2, dims 16 (i / 2); V^T operand: 16-key quarter i / 4,
-    // dims 32 (i % 4)
-    auto read_k = [&](int buf, int i) __attribute__((always_inline)) {
-        typedef const __attribute__((address_space(3))) f16x8* lptr;
-        return *reinterpret_cast<lptr>(ka[i >> 1] + buf * kPfTileBytes + (i & 1) * 32 * 256);
+    // The ring is two frames of P slots, and these addresses are of one of them: of K's first at first, of V's second.
+    int k_turn = P * kPfHalfBytes, v_turn = -P * kPfHalfBytes;
+    auto turn_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) ka[kk] += k_turn;
+        k_turn = -k_turn;
     };
-    auto read_v = [&](int buf, int i) __attribute__((always_inline)) {
+    auto turn_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) va[dt][0] += v_turn, va[dt][1] += v_turn;
+        v_turn = -v_turn;
+    };
+    // K operand of MFMA i of the half in the frame's `slot`: dims 16 i; V^T operand: 16-key quarter i / 4, dims 32 (i % 4)
+    auto read_k = [&](int slot, int i) __attribute__((always_inline)) {
+        typedef const __attribute__((address_space(3))) f16x8* lptr;
+        return *reinterpret_cast<lptr>(ka[i] + slot * kPfHalfBytes);
+    };
+    auto read_v = [&](int slot, int i) __attribute__((always_inline)) {
         typedef __attribute__((address_space(3))) s16x4* lptr;
-        const uint32_t off = (buf - 2) * kPfTileBytes + (i >> 2) * 16 * 256;
+        const uint32_t off = slot * kPfHalfBytes + (i >> 2) * 16 * 256;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][0] + off));
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][1] + off));
         return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -785,21 +808,21 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
     auto work = [&](const PagedSeq& s) __attribute__((always_inline)) {
         // weights: keys times group, as if the rows were cut between tokens
         const int g = p.group;
-        SeqWork w{weight_of(p, s.ctx), kPfRows >> p.coarse, weight_of(p, p.c.capacity()), (s.n * g + kPfRows - 1) / kPfRows, p.c.nkv};
-        if (p.window > 0) w.most = min(w.most, weight_of(p, min(p.window, p.c.capacity()) + kPfRows / g + kPfKeys));
+        SeqWork w{weight_of(p, s.ctx), kRows >> p.coarse, weight_of(p, p.c.capacity()), (s.n * g + kRows - 1) / kRows, p.c.nkv};
+        if (p.window > 0) w.most = min(w.most, weight_of(p, min(p.window, p.c.capacity()) + kRows / g + kPfKeys));
         return w;
     };
-    auto tiles = [&](const PagedSeq& s, int rt) __attribute__((always_inline)) { return prefill_range(p, s, rt).tiles; };
+    auto tiles = [&](const PagedSeq& s, int rt) __attribute__((always_inline)) { return prefill_range<WAVES>(p, s, rt).tiles; };
 
     auto body = [&](int seq, const PagedSeq& s, int kvh, int rt, int t0, int t1, int slot) __attribute__((always_inline)) {
-        const PrefillRange range = prefill_range(p, s, rt);
+        const PrefillRange range = prefill_range<WAVES>(p, s, rt);
         const int rows = uniform(range.rows), first_tile = uniform(range.first_tile), low = uniform(range.low);
         const int it0 = first_tile + t0, it1 = first_tile + t1;
-        const int r = rt * kPfRows + wave * 32 + fr;
+        const int r = rt * kRows + wave * 32 + fr;
         const int rc = min(r, rows - 1);
         const int qi = rc / p.group, qh = kvh * p.group + rc - qi * p.group;
         const int pos = s.ctx + qi;
-        const bool dead = rt * kPfRows + wave * 32 >= rows;  // the wave has no row
+        const bool dead = rt * kRows + wave * 32 >= rows;  // the wave has no row
         // the keys that this row takes here: lo .. lim
         const int lim = min(min(pos, p.c.capacity() - 1), it1 * kPfKeys - 1);
         const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
@@ -814,66 +837,79 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) qf[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
         }
-        // 64 entries of the table from `base` on, one a lane
-        int base = 0, page_l = -1;
-        auto refill = [&](int entry) __attribute__((always_inline)) {
-            base = entry;
-            page_l = paged_page(p.c, seq, entry + lane);
+        const int key0 = it0 * kPfKeys, halves = 2 * (it1 - it0);  // the run: halves 0 .. halves - 1
+        // 64 entries of the table from `base` on, one a lane, as the distance of their page from the first
+        // (-1: no page); and the next ones, on their way
+        int base = 0, next_base = -1, next_l = 0, page_lo = 0, page_hi = -1;
+        auto entry_of = [&](int half) __attribute__((always_inline)) {
+            return (key0 + kPfHalf * min(half, halves - 1)) >> p.c.shift;
         };
-        struct Pages {
-            int at[NP];
+        bool holes = false;  // some of the run's pages among them are missing
+        auto request_entries = [&](int entry) __attribute__((always_inline)) {
+            next_base = entry;
+            next_l = p.c.table[static_cast<size_t>(seq) * p.c.max_pages + min(entry + lane, p.c.max_pages - 1)];
         };
-        auto pages_of = [&](int t) __attribute__((always_inline)) {
-            t = min(t, it1 - 1);  // the steps ask for up to two tiles behind the last
-            Pages x;
-            if constexpr (ONE) {
-                const int entry = t >> (p.c.shift - 6);
-                if (entry >= base + 64) refill(entry);
-                x.at[0] = __builtin_amdgcn_readlane(page_l, entry - base);
-            } else {
-                const int per = p.c.shift == 4 ? 0 : 1;  // log2 of the 16-key quarters of a page
-                const int entry = t << (2 - per);
-                if (entry + (4 >> per) > base + 64) refill(entry);
+        auto take_entries = [&]() __attribute__((always_inline)) {
+            base = next_base;
+            next_base = -1;
+            const bool page = base + lane < p.c.max_pages && next_l >= 0 && next_l < p.c.num_pages;
+            const long long far = page ? 2 * static_cast<long long>(next_l) * p.c.page_stride : -1;
+            page_lo = static_cast<int>(far);
+            page_hi = static_cast<int>(far >> 32);
+            holes = __builtin_amdgcn_ballot_w64(!page && base + lane <= entry_of(halves - 1) + NP - 1) != 0;
+        };
+        auto page_at = [&](int entry) __attribute__((always_inline)) {
+            const uint32_t lo = __builtin_amdgcn_readlane(page_lo, entry - base), hi = __builtin_amdgcn_readlane(page_hi, entry - base);
+            return static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo);
+        };
+        // Halves that are filled without a look at their keys, and those that no row of the wave masks (both as
+        // the first one and how many).
+        const int fill0 = (max(low - key0, 0) + kPfHalf - 1) / kPfHalf;
+        const int fill_n = min(halves, (keys - key0) / kPfHalf) - fill0;
+        const int bare0 = (max(wave_lo - key0, 0) + kPfHalf - 1) / kPfHalf;
+        const int bare_n = min(halves, (wave_lim + 1 - key0) / kPfHalf) - bare0;
+        auto within = [](int x, int first, int n) __attribute__((always_inline)) { return n > 0 && static_cast<uint32_t>(x - first) < static_cast<uint32_t>(n); };
+        // bytes from the first page's to this head's first row
+        const long long head_at = 2 * ((static_cast<long long>(kvh) << p.c.shift) * kPgDim);
+        const int in_page = p.c.page_size() - 1;
+        // K or V of a half on its way into its slot; tile_barrier holds the waits.  The half before the first is
+        // zeros, halves behind the last are left out.
+        struct Job {
+            const char* from[2];  // of its rows 0 and 16
+            uint32_t dst;
+            bool plain;           // every row is there
+        };
+        auto job_of = [&](int half, bool v) __attribute__((always_inline)) {
+            Job j;
+            j.dst = lds0 + ((v ? R : 0) + (half & (R - 1))) * kPfHalfBytes;
+            j.plain = !holes && within(half, fill0, fill_n);
+            j.from[0] = j.from[1] = nullptr;
+            const int key1 = key0 + kPfHalf * half;
+            const char* const pool = reinterpret_cast<const char*>(v ? p.c.v : p.c.k) + head_at;
+            if (__builtin_expect(j.plain, 1)) {
+                const int entry = key1 >> p.c.shift;
+                j.from[0] = pool + page_at(entry) + (ONE ? (key1 & in_page) * (2 * kPgDim) : 0);
+                j.from[1] = ONE ? j.from[0] + 16 * 2 * kPgDim : pool + page_at(entry + 1);
+            } else if (half < halves) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x.at[i] = __builtin_amdgcn_readlane(page_l, entry - base + (i >> per));
-            }
-            return x;
-        };
-        auto there = [&](const Pages& x, int i) __attribute__((always_inline)) { return x.at[ONE ? 0 : i] >= 0; };
-        auto whole = [&](const Pages& x) __attribute__((always_inline)) {
-            bool all = true;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) all = all && x.at[i] >= 0;
-            return all;
-        };
-        // Tile t, whose pages are x, into buffer `buf` (0, 1: K; 2, 3: V); tile_barrier holds the waits.
-        auto load_tile = [&](int t, const Pages& x, int buf) __attribute__((always_inline)) {
-            t = min(t, it1 - 1);
-            const uint32_t dst = lds0 + buf * kPfTileBytes + wave * 1024;
-            const uint16_t* from[4];  // of quarter i
-            const int mask = p.c.page_size() - 1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (ONE && i > 0) {
-                    from[i] = from[0] + 16 * i * kPgDim;
-                } else {
-                    const int row0 = (t * kPfKeys + 16 * i) & mask;
-                    from[i] = p.c.k + (buf >= 2 ? v_minus_k : 0) +
-                              static_cast<long long>(max(x.at[ONE ? 0 : i], 0)) * p.c.page_stride +
-                              ((static_cast<long long>(kvh) << p.c.shift) + row0) * kPgDim;
+                for (int i = 0; i < 8; ++i) {
+                    const int row = 4 * i + (lane >> 4), key = key1 + row;
+                    const long long page = half < 0 ? -1 : page_at((key1 + (ONE ? 0 : 16 * (i / 4))) >> p.c.shift);
+                    const uint32_t chunk = 16 * ((lane & 15) ^ (((lane >> 4) << 2) | (i & 3)));
+                    const bool seen = page >= 0 && key >= low && key < keys;
+                    lds_load_x4(j.dst + 1024 * i, seen ? pool + page + (key & in_page) * (2 * kPgDim) + chunk
+                                                       : reinterpret_cast<const char*>(g_zero_row) + chunk);
                 }
             }
-            if (t * kPfKeys >= low && (t + 1) * kPfKeys <= keys && whole(x)) {
+            return j;
+        };
+        auto load_part = [&](const Job& j, int i) __attribute__((always_inline)) {
+            if (__builtin_expect(j.plain, 1)) lds_load_x4(j.dst + 1024 * i, j.from[i >> 2], loff[i & 3]);
+        };
+        auto load_half = [&](int half, bool v) __attribute__((always_inline)) {
+            const Job j = job_of(half, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds_load_x4(dst + 4096 * i, from[i], loff);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = t * kPfKeys + 16 * i + lrow;
-                    const bool seen = key >= low && key < keys && there(x, i);
-                    lds_load_x4(dst + 4096 * i, seen ? from[i] + lrow * kPgDim + lcol : g_zero_row + lcol);
-                }
-            }
+            for (int i = 0; i < 8; ++i) load_part(j, i);
         };
 
         f32x16 acc[4];
@@ -881,154 +917,201 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
         float mref = -INFINITY, lsum = 0.0f;
         bool any = false;  // the row has had a key
-        auto mask = [&](int t, const Pages& x, f32x16 (&sc)[2]) __attribute__((always_inline)) {
-            if ((t + 1) * kPfKeys - 1 <= wave_lim && t * kPfKeys >= wave_lo && whole(x)) {  // wave-uniform
+        auto mask = [&](int half, f32x16& sc) __attribute__((always_inline)) {
+            if (__builtin_expect(!holes && within(half, bare0, bare_n), 1)) {
                 any = true;
                 return;
             }
+            const int key1 = key0 + kPfHalf * half;
+            const bool there0 = page_at(entry_of(half)) >= 0, there1 = ONE ? there0 : page_at(entry_of(half) + 1) >= 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int key = t * kPfKeys + 32 * j + 8 * (v >> 2) + 4 * h + (v & 3);
-                    const bool seen = key <= lim && key >= lo && there(x, 2 * j + (v >> 3));
-                    any = any || seen;
-                    sc[j][v] = seen ? sc[j][v] : -INFINITY;
-                }
+            for (int v = 0; v < 16; ++v) {
+                const int key = key1 + 8 * (v >> 2) + 4 * h + (v & 3);
+                const bool seen = key <= lim && key >= lo && (v < 8 ? there0 : there1);
+                any = any || seen;
+                sc[v] = seen ? sc[v] : -INFINITY;
+            }
         };
-        auto renew_ref = [&](float mx) __attribute__((always_inline)) {
+        // Reference values are whole numbers (exponents of two), so what was weighed by an old one, the
+        // weights pw in wait among it, is scaled without rounding.
+        auto renew_ref = [&](float mx, uint32_t (&pw)[8]) __attribute__((always_inline)) {
             const bool grow = mx > mref + kPgLag;
-            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-                const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
-                mref = grow ? mx : mref;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(grow) != 0, 0)) {
+                const float to = grow ? floorf(mx) : mref;
+                const float alpha = !grow ? 1.0f : __builtin_amdgcn_exp2f(mref - to);
+                mref = to;
                 lsum *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+                const f16x2 a = {static_cast<_Float16>(alpha), static_cast<_Float16>(alpha)};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pw[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pw[i]) * a);
             }
         };
-        auto row_max = [&](const f32x16 (&sc)[2]) __attribute__((always_inline)) {
-            float mx = -INFINITY;
+        auto max_of = [&](const f32x16& sc, int v0, int n, float mx) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[j][v]);
-            return xor32_max(mx) * kPgScale;  // scaling is monotonic
+            for (int v = v0; v < v0 + n; ++v) mx = fmaxf(mx, sc[v]);
+            return mx;
         };
-        // weights 2 i and 2 i + 1 of a tile's scores (32-key half i / 8), packed
-        auto probs = [&](const f32x16 (&sc)[2], int i, float neg, float (&ps)[2]) __attribute__((always_inline)) {
-            const int j = i >> 3, v = 2 * (i & 7);
-            const f32x2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v], kPgScale, neg)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][v + 1], kPgScale, neg))};
+        // weights 2 i and 2 i + 1 of a half's scores, packed
+        auto weights = [&](const f32x16& sc, int i, float neg, float (&ps)[2]) __attribute__((always_inline)) {
+            const f32x2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], kPgScale, neg)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], kPgScale, neg))};
             ps[0] += e.x;
             ps[1] += e.y;
             uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, f16x2));
             asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]));  // here, not past the mask's branch
             return w;
         };
+        auto times_q = [&](const f16x8& k, int i, f32x16& sc) __attribute__((always_inline)) {
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(f16x8, qf[i]), i == 0 ? f32x16{} : sc, 0, 0, 0);
+        };
+        auto add_pv = [&](const f16x8& v, int i, const uint32_t (&pw)[8]) __attribute__((always_inline)) {
+            const u32x4 pf = {pw[4 * (i >> 2)], pw[4 * (i >> 2) + 1], pw[4 * (i >> 2) + 2], pw[4 * (i >> 2) + 3]};
+            acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(f16x8, pf), acc[i & 3], 0, 0, 0);
+        };
+        // Stage t: the scores of half t + 1 (nxt) and the outputs of half t - 1 (weights pp) beside the weights of
+        // half t (scores cur, weights pc).  ks, vs: slots of K t + 1 and V t - 1; f: the first operands of K t + 1,
+        // then those of K t + 2 in slot `then` (-1: not there yet); mx: the lane's part of the maximum of cur, then of
+        // nxt; parts: the first of the four parts of `job` that the stage asks for.  Each MFMA is fenced together with its share of the vector work: left alone, the scheduler puts
+        // all of the one before all of the other.
         constexpr int AHEAD = 4;  // operand reads in flight before their MFMA
-        // Scores of the K tile in `buf`; beside them, when EXP, the weights of the scores `cur`.  Each MFMA is
-        // fenced together with its share of the vector work: left alone, the scheduler puts all of the one
-        // before all of the other.
-        auto scores = [&](auto exp_too, int buf, f32x16 (&sc)[2], const f32x16 (&cur)[2],
-                          uint32_t (&pw)[2][8]) __attribute__((always_inline)) {
-            const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
-            float ps[2] = {0.0f, 0.0f};
-            f16x8 kf[AHEAD];
+        f16x8 f[AHEAD];
+        // In the P stages from t on K of the halves t + P + 1 .. t + 2 P and V of t + P - 1 .. t + 2 P - 2 come in, a
+        // half by each wave.
+        static_assert(WAVES == 2 * P, "a half of K or V for each wave");
+        const bool loads_v = wave < P;
+        auto job_at = [&](int t) __attribute__((always_inline)) { return job_of(t + P + (loads_v ? wave - 1 : wave - P + 1), loads_v); };
+        auto first_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) kf[i] = read_k(buf, i);
+            for (int i = 0; i < AHEAD; ++i) f[i] = read_k(slot, i);
+        };
+        auto stage = [&](int t, int ks, int vs, int then, const Job& job, auto parts, const f32x16& cur, f32x16& nxt, uint32_t (&pc)[8], uint32_t (&pp)[8],
+                         float& mx) __attribute__((always_inline)) {
+            constexpr int first_part = decltype(parts)::value;
+            float ps[2] = {0.0f, 0.0f}, neg = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % AHEAD], __builtin_bit_cast(f16x8, qf[i >> 1]),
-                                                                   i < 2 ? f32x16{} : sc[i & 1], 0, 0, 0);
-                if (i + AHEAD < 16) kf[i % AHEAD] = read_k(buf, i + AHEAD);
-                if constexpr (decltype(exp_too)::value) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
+            for (int i = 0; i < 8; ++i) {
+                times_q(f[i % AHEAD], i, nxt);
+                f[i % AHEAD] = i + AHEAD < 8 ? read_k(ks, i + AHEAD) : read_v(vs, i + AHEAD - 8);
+                if (i == 1) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    renew_ref(xor32_max(mx) * kPgScale, pp);  // (scaling is monotonic)
+                    neg = mref == -INFINITY ? 0.0f : -mref;   // masked scores give exp2(-inf) = 0
+                }
+                if (i & 1) pc[i >> 1] = weights(cur, i >> 1, neg, ps);
+                if (i == 4 && first_part + 0 < 8) load_part(job, first_part + 0);
+                if (i == 7 && first_part + 1 < 8) load_part(job, first_part + 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr (decltype(exp_too)::value) lsum += ps[0] + ps[1];
-        };
-        // O^T += V^T . P^T; beside it, when MAX, the (scaled) row maximum of nxt
-        auto add_pv = [&](auto max_too, const uint32_t (&pw)[2][8], int buf, const f32x16 (&nxt)[2]) __attribute__((always_inline)) {
-            f16x8 vf[AHEAD];
+            mask(t + 1, nxt);
+            mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) vf[i] = read_v(buf, i);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = i >> 3, ks = (i >> 2) & 1, dt = i & 3;
-                const u32x4 pf = {pw[j][4 * ks], pw[j][4 * ks + 1], pw[j][4 * ks + 2], pw[j][4 * ks + 3]};
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % AHEAD], __builtin_bit_cast(f16x8, pf), acc[dt], 0, 0, 0);
-                if (i + AHEAD < 16) vf[i % AHEAD] = read_v(buf, i + AHEAD);
-                if constexpr (decltype(max_too)::value)
-                    mx = fmaxf(fmaxf(mx, nxt[j][2 * (i & 7)]), nxt[j][2 * (i & 7) + 1]);
+            for (int i = 0; i < 8; ++i) {
+                add_pv(f[i % AHEAD], i, pp);
+                if (i + AHEAD < 8) f[i % AHEAD] = read_v(vs, i + AHEAD);
+                else if (then >= 0) f[i % AHEAD] = read_k(then, i + AHEAD - 8);
+                if (i & 1) pc[4 + (i >> 1)] = weights(cur, 4 + (i >> 1), neg, ps);
+                if (i >= 2) mx = i < 6 ? max_of(nxt, 3 * (i - 2), 3, mx) : max_of(nxt, 12 + 2 * (i - 6), 2, mx);
+                if (i == 2 && first_part + 2 < 8) load_part(job, first_part + 2);
+                if (i == 5 && first_part + 3 < 8) load_part(job, first_part + 3);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            return decltype(max_too)::value ? xor32_max(mx) * kPgScale : 0.0f;
-        };
-        typedef std::true_type yes;
-        typedef std::false_type no;
-        // The scores of tile t are in cur: the scores of the next tile beside the weights of t, then V of t
-        // beside the next tile's maximum.  b: parity of the tile; x: pages of tile t + 1, of t + 2 after it.
-        auto step = [&](int t, int b, Pages& x, f32x16 (&cur)[2], f32x16 (&nxt)[2]) __attribute__((always_inline)) {
-            uint32_t pw[2][8];
-            load_tile(t + 1, x, 2 + (b ^ 1));
-            const Pages y = pages_of(t + 2);
-            load_tile(t + 2, y, b);
-            scores(yes{}, b ^ 1, nxt, cur, pw);
-            mask(t + 1, x, nxt);
-            const float mx = add_pv(yes{}, pw, 2 + b, nxt);
-            renew_ref(mx);
-            x = y;
-            tile_barrier();
-        };
-        auto finish = [&](int b, f32x16 (&cur)[2]) __attribute__((always_inline)) {
-            uint32_t pw[2][8];
-            const float neg = mref == -INFINITY ? 0.0f : -mref;
-            float ps[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = probs(cur, i, neg, ps);
             lsum += ps[0] + ps[1];
-            add_pv(no{}, pw, 2 + b, cur);
+        };
+        // The same where the wave has no half t + 1, or none of the others.
+        const int mine = wave_last < key0 ? 0 : min(halves, (wave_last - key0) / kPfHalf + 1);  // its halves
+        auto last_stage = [&](int t, int ks, int vs, const f32x16& cur, f32x16& nxt, uint32_t (&pc)[8], uint32_t (&pp)[8],
+                              float& mx) __attribute__((always_inline)) {
+            if (t < mine) renew_ref(xor32_max(mx) * kPgScale, pp);
+            if (t + 1 < mine) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) times_q(read_k(ks, i), i, nxt);
+                mask(t + 1, nxt);
+                mx = max_of(nxt, 0, 16, -INFINITY);
+            }
+            if (t > 0 && t - 1 < mine) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) add_pv(read_v(vs, i), i, pp);
+            }
+            if (t < mine) {
+                const float neg = mref == -INFINITY ? 0.0f : -mref;
+                float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pc[i] = weights(cur, i, neg, ps);
+                lsum += ps[0] + ps[1];
+            }
         };
         if (it0 < it1) {
-            const int n = it1 - it0;
-            int t = it0;
-            refill(ONE ? t >> (p.c.shift - 6) : t << (p.c.shift == 4 ? 2 : 1));
-            Pages x = pages_of(t);
-            load_tile(t, x, 0);
-            load_tile(t, x, 2);
-            Pages y = pages_of(t + 1);
-            load_tile(t + 1, y, 1);
+            f32x16 s0, s1;
+            uint32_t p0[8] = {}, p1[8] = {};
+            float mx = -INFINITY;
+            request_entries(entry_of(0));
+            take_entries();
+            if (wave == 0) load_half(0, false);
+            load_half(loads_v ? wave - 1 : wave - P + 1, loads_v);
             tile_barrier();
-            f32x16 s0[2] = {}, s1[2];
-            if (wave_last >= t * kPfKeys) {
-                uint32_t pw[2][8];
-                scores(no{}, 0, s0, s1, pw);
-                mask(t, x, s0);
-                renew_ref(row_max(s0));
+            if (mine > 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) times_q(read_k(0, i), i, s0);
+                mask(0, s0);
+                mx = max_of(s0, 0, 16, -INFINITY);
             }
-            tile_barrier();  // K buffer 0 is read
-            // Tiles past the wave's last key are not multiplied.
-            const int mine = wave_last < t * kPfKeys ? 0 : min(n, wave_last / kPfKeys - t + 1);
-            int left = mine;
-            for (; left > 2; left -= 2) {
-                step(t, 0, y, s0, s1);
-                step(t + 1, 1, y, s1, s0);
-                t += 2;
-            }
-            if (left == 2) {
-                step(t, 0, y, s0, s1);
-                finish(1, s1);
-            } else if (left == 1) {
-                finish(0, s0);
-            }
-            for (int i = max(mine - 1, 0); i < n - 1; ++i) {  // the tiles of the other waves
-                load_tile(it0 + i + 1, y, 2 + ((i & 1) ^ 1));
-                y = pages_of(it0 + i + 2);
-                load_tile(it0 + i + 2, y, i & 1);
+            tile_barrier();  // K's slot 0 is read
+            // P stages from t on between two barriers.  A wave asks for the parts of its half one by one within the
+            // first stages (in one go, and with an address for each part of every half, the loads held the waves up
+            // for a third of the time), which leaves them time to come in.  Halves past the wave's last key are not
+            // multiplied.
+            auto entries = [&](int t) __attribute__((always_inline)) {
+                if (__builtin_expect(next_base >= 0, 0)) take_entries();
+                if (__builtin_expect(entry_of(t + 3 * P) + NP > base + 64, 0)) request_entries(entry_of(t + P + 1));  // for the next time
+            };
+            typedef std::integral_constant<int, 0> first;
+            typedef std::integral_constant<int, 4> second;
+            typedef std::integral_constant<int, 8> none;
+            int t = 0;
+            for (; t + P < mine; t += P) {
+                entries(t);
+                first_k(1);
+                const Job job = job_at(t);
+                if constexpr (P == 4) {
+                    stage(t, 1, 3, 2, job, first{}, s0, s1, p0, p1, mx);
+                    turn_v();
+                    stage(t + 1, 2, 0, 3, job, second{}, s1, s0, p1, p0, mx);
+                    stage(t + 2, 3, 1, -1, job, none{}, s0, s1, p0, p1, mx);
+                    turn_k();  // K t + P lies in the other frame
+                    first_k(0);
+                    stage(t + 3, 0, 2, -1, job, none{}, s1, s0, p1, p0, mx);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_part(job, i);
+                    stage(t, 1, 1, -1, job, second{}, s0, s1, p0, p1, mx);
+                    turn_v();
+                    turn_k();
+                    first_k(0);
+                    stage(t + 1, 0, 0, -1, job, none{}, s1, s0, p1, p0, mx);
+                }
                 tile_barrier();
             }
+            for (; t <= halves; t += P) {
+                entries(t);
+                const Job job = job_at(t);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) load_part(job, i);
+#pragma unroll
+                for (int j = 0; j < P; j += 2) {
+                    last_stage(t + j, j + 1, j == 0 ? P - 1 : j - 1, s0, s1, p0, p1, mx);
+                    if (j == 0) turn_v();
+                    if (j + 1 == P - 1) turn_k();
+                    last_stage(t + j + 1, j + 1 == P - 1 ? 0 : j + 2, j, s1, s0, p1, p0, mx);
+                }
+                tile_barrier();
+            }
+            // the addresses as they were at first
+            if (k_turn < 0) turn_k();
+            if (v_turn > 0) turn_v();
         }
         lsum += __shfl_xor(lsum, 32);
         if (any || __shfl_xor(static_cast<int>(any), 32) != 0) mref = fmaxf(mref, kPgLowest);
@@ -1045,7 +1128,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
                             pack4(acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv);
                 if (p.lse != nullptr && h == 0) p.lse[at] = row_log_sum(mref, lsum);
             } else {
-                const size_t at = static_cast<size_t>(2 * block + slot) * kPfRows + wave * 32 + fr;
+                const size_t at = static_cast<size_t>(2 * block + slot) * kRows + wave * 32 + fr;
                 if (h == 0) part.ml[at] = make_float2(mref, lsum);
                 float* po = part.o + at * kPgDim;
 #pragma unroll
@@ -1059,17 +1142,19 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_kernel(PrefillParams p) 
         tile_barrier();  // the tiles are read: the next segment fills them
     };
     constexpr int kLeastTiles = 4;
-    auto rows = [&](const PagedSeq& s, int, int rt) __attribute__((always_inline)) { return min(kPfRows, s.n * p.group - rt * kPfRows); };
-    for_share<false>(p.c, block, kPfBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, rows, body,
+    auto rows = [&](const PagedSeq& s, int, int rt) __attribute__((always_inline)) { return min(kRows, s.n * p.group - rt * kRows); };
+    for_share<false>(p.c, block, kBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, rows, body,
                      [&](SegmentCut cut) {
                          if (threadIdx.x == 0) part.cuts[block] = cut;
                      });
 }
 
+template <int WAVES>
 __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillParams p) {
-    static_assert(kPfBlocks <= kMergeCuts, "a cut for each block");
-    merge_parts<kPfRows, 1, 256>(p.ws, kPfBlocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
-        return RowMap{paged_seq(p.c, c.item).first, c.row_tile * kPfRows, p.group, c.head * p.group};
+    typedef PrefillShape<WAVES> Shape;
+    static_assert(Shape::blocks <= kMergeCuts, "a cut for each block");
+    merge_parts<Shape::rows, 1, 256>(p.ws, Shape::blocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
+        return RowMap{paged_seq(p.c, c.item).first, c.row_tile * Shape::rows, p.group, c.head * p.group};
     });
 }
 
@@ -1134,6 +1219,30 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
     return check_launch(what);
 }
 
+constexpr size_t prefill_bytes() {
+    return std::max(partials_bytes<PrefillShape<4>::rows>(PrefillShape<4>::blocks),
+                    partials_bytes<PrefillShape<8>::rows>(PrefillShape<8>::blocks));
+}
+
+template <int WAVES>
+int launch_prefill(PrefillParams p, const qe_paged_batch* batch, const qe_paged_cache* cache, hipStream_t stream,
+                   const char* what) {
+    typedef PrefillShape<WAVES> Shape;
+    const long long row_tiles = static_cast<long long>(batch->num_tokens) * p.group / Shape::rows + batch->num_seqs;
+    const long long most = static_cast<long long>(p.group) * (static_cast<long long>(batch->max_pages) * cache->page_size + kPfOver);
+    while (row_tiles * cache->num_kv_heads > ((1LL << 30) - 1) / ((most >> p.coarse) + 1)) {
+        QE_REQUIRE(most >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens, cache->num_kv_heads);
+        ++p.coarse;
+    }
+    if (p.c.shift >= 5)
+        paged_prefill_kernel<true, WAVES><<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
+    else
+        paged_prefill_kernel<false, WAVES><<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
+    const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, Shape::blocks) * (Shape::rows / 8);
+    paged_prefill_merge_kernel<WAVES><<<static_cast<unsigned>(std::min(items, 2048LL)), 256, 0, stream>>>(p);
+    return QE_OK;
+}
+
 }  // namespace
 }  // namespace qe
 
@@ -1176,7 +1285,7 @@ extern "C" int qe_paged_prefill_workspace_bytes(int num_tokens, int num_q_heads,
     QE_REQUIRE(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
                "paged_prefill_workspace_bytes: num_tokens=%d, %d q heads over %d kv heads", num_tokens, num_q_heads,
                num_kv_heads);
-    *bytes = partials_bytes<kPfRows>(kPfBlocks);
+    *bytes = prefill_bytes();
     clear_error();
     return QE_OK;
 }
@@ -1190,7 +1299,7 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     QE_TRY(paged_check_heads(what, cache, num_q_heads));
     QE_REQUIRE(window >= 0, "%s: window=%d", what, window);
     if (batch->num_tokens == 0 || batch->num_seqs == 0) return QE_OK;
-    QE_TRY(check_attention(what, q, cache, batch, attn_out, row_lse, workspace, partials_bytes<kPfRows>(kPfBlocks), nullptr,
+    QE_TRY(check_attention(what, q, cache, batch, attn_out, row_lse, workspace, prefill_bytes(), nullptr,
                            num_q_heads, 0));
     p.q = q;
     p.out = attn_out;
@@ -1199,17 +1308,6 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     p.nq = num_q_heads;
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
-    const long long row_tiles = static_cast<long long>(batch->num_tokens) * p.group / kPfRows + batch->num_seqs;
-    const long long most = static_cast<long long>(p.group) * (static_cast<long long>(batch->max_pages) * cache->page_size + kPfOver);
-    while (row_tiles * cache->num_kv_heads > ((1LL << 30) - 1) / ((most >> p.coarse) + 1)) {
-        QE_REQUIRE(most >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens, cache->num_kv_heads);
-        ++p.coarse;
-    }
-    if (p.c.shift >= 6)
-        paged_prefill_kernel<true><<<kPfBlocks, 256, 0, stream>>>(p);
-    else
-        paged_prefill_kernel<false><<<kPfBlocks, 256, 0, stream>>>(p);
-    const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, kPfBlocks) * (kPfRows / 8);
-    paged_prefill_merge_kernel<<<static_cast<unsigned>(std::min(items, 2048LL)), 256, 0, stream>>>(p);
+    QE_TRY(launch_prefill<8>(p, batch, cache, stream, what));
     return check_launch(what);
 }

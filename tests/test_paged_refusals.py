@@ -281,7 +281,7 @@ for size in (16, 32, 64, 256):
     c, t = describe(100, True, size)
     ok(L.qe_launch_attention_gqa_paged_prefill(q, c, t, ws, out, V(0), s, I(12), I(0)))
     e = events()
-    near(names(), "paged_prefill_kernelILb%d" % (size >= 64), "paged_prefill_merge")
+    near(names(), "paged_prefill_kernelILb%d" % (size >= 32), "paged_prefill_merge")
     assert all(x.stream == 0x5000 for x in e), e
 ok(L.qe_launch_paged_key_bounds(c, t, a, b, s))
 ok(L.qe_launch_paged_select(q, c, t, a, b, out, ws, s, I(12), I(8), I(1), I(1)))

@@ -33,6 +33,10 @@ constexpr float kPgLag = 8.0f;
 // place t * w / n of its stretch; the bits of a row depend on the lengths of the whole
 // batch, through where the cuts fall, and on nothing else.
 //
+// Where there are few segments for the blocks (at most one for four), every segment is
+// given whole shares, so that no block has two: a second one costs as much again as a
+// short share (17 rows on 1200 positions: 20 us of a launch instead of 13).
+//
 // Weights are whole numbers whose sum is below 2^30: the launcher says by how many
 // bits they have to be shortened (kernels: `coarse`).
 struct SegmentCut {  // of the block that has a segment's beginning but not its end
@@ -51,19 +55,24 @@ __device__ __forceinline__ int tiles_before(int x, int at, int weight, int tiles
     return min(tiles, static_cast<int>(static_cast<float>(x - at) * (static_cast<float>(tiles) / static_cast<float>(weight))));
 }
 
-// One sequence on the line: `heads` times row tiles whose weights are first + step *
-// (i + 1), but at most `most`.
+// One sequence on the line: `heads` times row tiles whose weights are first + (i + 1 << step)
+// (step < 0: first), but at most `most`.
 struct SeqWork {
     int first, step, most;
     int row_tiles, heads;
 
     __device__ __forceinline__ int before(int i) const {  // weight of the first i row tiles
-        if (step == 0) return i * min(first, most);
-        const int m = min(i, max(0, most - first) / step);
-        return m * first + step * (m * (m + 1) / 2) + (i - m) * most;
+        if (step < 0) return i * min(first, most);
+        const int m = min(i, max(0, most - first) >> step);
+        return m * first + ((m * (m + 1) / 2) << step) + (i - m) * most;
     }
-    __device__ __forceinline__ int weight(int i) const { return min(most, first + step * (i + 1)); }
-    __device__ __forceinline__ int all() const { return row_tiles > 0 ? heads * before(row_tiles) : 0; }
+    __device__ __forceinline__ int weight(int i) const { return min(most, step < 0 ? first : first + ((i + 1) << step)); }
+    __device__ __forceinline__ int segments() const { return heads * row_tiles; }
+    // every row tile with the weight of the last, rounded up to whole shares
+    __device__ __forceinline__ void fill_shares(int share) {
+        first = most = (weight(row_tiles - 1) + share - 1) / share * share;
+        step = -1;
+    }
 };
 
 // Sum over a wave up to and with each lane, in the vector unit: 1, 2, 4 and 8 lanes on within rows
@@ -114,17 +123,46 @@ __device__ __forceinline__ void for_share(const PagedView& c, int block, int blo
     // the whole line, then the sequence in which the share begins
     SeqChunk chunk{};
     const int seqs = LISTED ? 1 : c.seqs;
-    int total = 0, s = 0, at = 0, w = 0;
+    int total = 0, segments = 0, level = 0, s = 0, at = 0, w = 0;  // level: were every row tile as heavy as its sequence's last
+    auto sum = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(x), 63); };
     if constexpr (LISTED) {
-        total = work(PagedSeq{0, 1, 0}).all();
+        const SeqWork q = work(PagedSeq{0, 1, 0});
+        segments = q.segments();
+        total = level = segments * q.first;
     } else {
         for (int s0 = 0; s0 < seqs; s0 += 64) {
             chunk.read(c, s0);
-            w = wave_scan(work(chunk.lane()).all());
+            const SeqWork q = work(chunk.lane());
+            w = wave_scan(q.heads * q.before(q.row_tiles));
             total += __builtin_amdgcn_readlane(w, 63);
+            segments += sum(q.segments());
+            level += sum(q.row_tiles > 0 ? q.segments() * q.weight(q.row_tiles - 1) : 0);
         }
     }
-    const int share = max(least_share, (total + blocks - 1) / blocks);
+    const bool few = segments <= blocks / 4;
+    const int share = few ? max(least_share, (level + blocks - segments - 1) / (blocks - segments))
+                          : max(least_share, (total + blocks - 1) / blocks);
+    auto work_of = [&](const PagedSeq& q) __attribute__((always_inline)) {
+        SeqWork x = work(q);
+        if (few && x.row_tiles > 0) x.fill_shares(share);
+        return x;
+    };
+    auto all_of = [&](const PagedSeq& q) __attribute__((always_inline)) {
+        const SeqWork x = work_of(q);
+        return x.row_tiles > 0 ? x.heads * x.before(x.row_tiles) : 0;
+    };
+    if (few) {
+        total = 0;
+        if constexpr (LISTED) {
+            total = all_of(PagedSeq{0, 1, 0});
+        } else {
+            for (int s0 = 0; s0 < seqs; s0 += 64) {
+                if (seqs > 64) chunk.read(c, s0);
+                w = wave_scan(all_of(chunk.lane()));
+                total += __builtin_amdgcn_readlane(w, 63);
+            }
+        }
+    }
     const int x0 = min(total, share * block), x1 = min(total, x0 + share);
     SegmentCut last{};
     if (x0 >= x1) {
@@ -135,7 +173,7 @@ __device__ __forceinline__ void for_share(const PagedView& c, int block, int blo
         for (int s0 = 0; s0 < seqs; s0 += 64) {
             if (seqs > 64) {
                 chunk.read(c, s0);
-                w = wave_scan(work(chunk.lane()).all());
+                w = wave_scan(all_of(chunk.lane()));
             }
             const int all = __builtin_amdgcn_readlane(w, 63);
             if (x0 < at + all) {
@@ -148,7 +186,7 @@ __device__ __forceinline__ void for_share(const PagedView& c, int block, int blo
         }
     }
     PagedSeq seq = LISTED ? PagedSeq{0, 1, 0} : chunk.seq(c, s);
-    SeqWork q = work(seq);
+    SeqWork q = work_of(seq);
     int head, rt;
     {
         const int one = q.before(q.row_tiles);
@@ -181,7 +219,7 @@ __device__ __forceinline__ void for_share(const PagedView& c, int block, int blo
                 do {
                     if (++s >= seqs) return cut(last);  // (only where query_start decreases)
                     seq = chunk.seq(c, s);
-                    q = work(seq);
+                    q = work_of(seq);
                 } while (q.row_tiles == 0);
             }
         }
@@ -441,7 +479,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
     // On the line: each sequence has its token's heads; or one sequence has those of all rows, the heads of
     // a row behind each other (all alike: which rows have a token is seen when their turn comes).
     auto work = [&](const PagedSeq& s) __attribute__((always_inline)) {
-        SeqWork w{0, 0, 0, s.n > 0 ? row_tiles : 0, SPARSE ? p.c.rows * p.c.nkv : p.c.nkv};
+        SeqWork w{0, -1, 0, s.n > 0 ? row_tiles : 0, SPARSE ? p.c.rows * p.c.nkv : p.c.nkv};
         w.first = w.most = (decode_range<SPARSE>(p, s, s.first).tiles >> p.coarse) + kDecOver;
         return w;
     };
@@ -690,7 +728,7 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 constexpr int kPfKeys = 64;           // keys of a tile: what shares are cut between
 constexpr int kPfHalf = 32;           // keys of a stage
 constexpr int kPfHalfBytes = kPfHalf * kPgDim * 2;
-constexpr int kPfOver = 2 * kPfKeys;  // what a segment costs beside its keys, in keys
+constexpr int kPfOver = 4 * kPfKeys;  // what a segment costs beside its keys, in keys
 // Blocks of WAVES waves, 32 rows each; a CU holds eight waves.
 template <int WAVES>
 struct PrefillShape {
@@ -808,7 +846,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
     auto work = [&](const PagedSeq& s) __attribute__((always_inline)) {
         // weights: keys times group, as if the rows were cut between tokens
         const int g = p.group;
-        SeqWork w{weight_of(p, s.ctx), kRows >> p.coarse, weight_of(p, p.c.capacity()), (s.n * g + kRows - 1) / kRows, p.c.nkv};
+        constexpr int kStep = WAVES == 8 ? 8 : 7;
+        static_assert(1 << kStep == kRows, "the weight of a row tile's own tokens");
+        SeqWork w{weight_of(p, s.ctx), max(kStep - p.coarse, -1), weight_of(p, p.c.capacity()), (s.n * g + kRows - 1) / kRows, p.c.nkv};
         if (p.window > 0) w.most = min(w.most, weight_of(p, min(p.window, p.c.capacity()) + kRows / g + kPfKeys));
         return w;
     };
@@ -1141,7 +1181,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         }
         tile_barrier();  // the tiles are read: the next segment fills them
     };
-    constexpr int kLeastTiles = 4;
+    constexpr int kLeastTiles = 2;
     auto rows = [&](const PagedSeq& s, int, int rt) __attribute__((always_inline)) { return min(kRows, s.n * p.group - rt * kRows); };
     for_share<false>(p.c, block, kBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, rows, body,
                      [&](SegmentCut cut) {
@@ -1308,6 +1348,11 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     p.nq = num_q_heads;
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
-    QE_TRY(launch_prefill<8>(p, batch, cache, stream, what));
+    // Blocks of eight waves read K and V once for 256 rows, those of four waves waste less on sequences of few rows
+    // (2048 rows at 14000: 205 and 232 us; 40 single tokens and three prompts: 68 and 58).
+    if (static_cast<long long>(batch->num_tokens) * p.group >= 512LL * batch->num_seqs)
+        QE_TRY(launch_prefill<8>(p, batch, cache, stream, what));
+    else
+        QE_TRY(launch_prefill<4>(p, batch, cache, stream, what));
     return check_launch(what);
 }

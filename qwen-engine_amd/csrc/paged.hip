@@ -162,10 +162,12 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_paged_append_kernel(AppendP
 // from one than its rounding: the bytes are those of exact arithmetic.  A page with an infinity or
 // NaN has m = inf and bytes of 0.
 //
-// grid (rows), 256 threads: a block works where its row is the first of its page or of its
-// sequence; a wave a head, 16 lanes a row of keys.
+// grid (rows, kv heads), 256 threads: a block works where its row is the first of its page or of its
+// sequence; 16 lanes a row of keys, 16 rows at once, up to four rounds of them requested together.
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(PagedView c, int8_t* bounds, float* step) {
-    const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __shared__ __align__(16) uint16_t s_high[4][kPgDim], s_low[4][kPgDim];
+    __shared__ uint32_t s_odd[4];
+    const int t = blockIdx.x, h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int seq = paged_seq_of_row(c, t);
     if (seq < 0) return;
     const PagedSeq s = paged_seq(c, seq);
@@ -176,51 +178,72 @@ __global__ __launch_bounds__(256) void paged_key_bounds_kernel(PagedView c, int8
     if (page < 0) return;
     // rows of the page in use once all new tokens are there (ctx + n is below 2^31)
     const int live = min(c.page_size(), s.ctx + s.n - (block << c.shift));
-    const int j = lane & 15, g = lane >> 4;
-    for (int h = wave; h < c.nkv; h += 4) {
-        const uint16_t* k = c.k + static_cast<long long>(page) * c.page_stride + (static_cast<long long>(h) << c.shift) * kPgDim + 8 * j;
-        f16x8 high, low;
-        uint32_t odd = 0;  // exponent of all ones somewhere
+    const int j = lane & 15, row0 = threadIdx.x >> 4;
+    const uint16_t* k = c.k + static_cast<long long>(page) * c.page_stride + (static_cast<long long>(h) << c.shift) * kPgDim + 8 * j;
+    f16x8 high, low;
+    uint32_t odd = 0;  // exponent of all ones somewhere
 #pragma unroll
-        for (int e = 0; e < 8; ++e) high[e] = static_cast<_Float16>(-65504.0f), low[e] = static_cast<_Float16>(65504.0f);
-#pragma unroll 8
-        for (int r = g; r < live; r += 4) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(k + static_cast<size_t>(r) * kPgDim);
-            const f16x8 x = __builtin_bit_cast(f16x8, w);
+    for (int e = 0; e < 8; ++e) high[e] = static_cast<_Float16>(-65504.0f), low[e] = static_cast<_Float16>(65504.0f);
+    for (int r0 = 0; r0 < live; r0 += 64) {
+        u32x4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (a row behind the last: the last again)
+            w[i] = *reinterpret_cast<const u32x4*>(k + static_cast<size_t>(min(r0 + 16 * i + row0, live - 1)) * kPgDim);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x8 x = __builtin_bit_cast(f16x8, w[i]);
             high = __builtin_elementwise_max(high, x);
             low = __builtin_elementwise_min(low, x);
 #pragma unroll
             for (int d = 0; d < 4; ++d)
-                odd |= static_cast<uint32_t>((w[d] & 0x7C00u) == 0x7C00u || (w[d] & 0x7C000000u) == 0x7C000000u);
+                odd |= static_cast<uint32_t>((w[i][d] & 0x7C00u) == 0x7C00u || (w[i][d] & 0x7C000000u) == 0x7C000000u);
         }
-        float hi[8], lo[8], m = 0.0f;
+    }
+    // over the four rows of the wave, then over the waves
+#pragma unroll
+    for (int d = 16; d < 64; d *= 2) {
+        u32x4 a = __builtin_bit_cast(u32x4, high), b = __builtin_bit_cast(u32x4, low);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = __shfl_xor(a[i], d);
+            b[i] = __shfl_xor(b[i], d);
+        }
+        high = __builtin_elementwise_max(high, __builtin_bit_cast(f16x8, a));
+        low = __builtin_elementwise_min(low, __builtin_bit_cast(f16x8, b));
+    }
+    const bool spoilt_here = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
+    if (lane < 16) {
+        *reinterpret_cast<f16x8*>(&s_high[wave][8 * j]) = high;
+        *reinterpret_cast<f16x8*>(&s_low[wave][8 * j]) = low;
+        if (lane == 0) s_odd[wave] = spoilt_here;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        high = __builtin_elementwise_max(high, *reinterpret_cast<const f16x8*>(&s_high[w][8 * j]));
+        low = __builtin_elementwise_min(low, *reinterpret_cast<const f16x8*>(&s_low[w][8 * j]));
+    }
+    const bool spoilt = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) != 0;
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(static_cast<float>(high[e])), fabsf(static_cast<float>(low[e]))));
+    m = qwen::seg_max_nonneg<16>(m);
+    const float div = m > 0.0f ? m : 1.0f;
+    uint32_t bytes[4] = {0, 0, 0, 0};
+    if (!spoilt) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            hi[e] = static_cast<float>(high[e]);
-            lo[e] = static_cast<float>(low[e]);
-            for (int d = 16; d < 64; d *= 2) {
-                hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], d));
-                lo[e] = fminf(lo[e], __shfl_xor(lo[e], d));
-            }
-            m = fmaxf(m, fmaxf(fabsf(hi[e]), fabsf(lo[e])));
+            const int a = static_cast<int>(ceilf(127.0f * static_cast<float>(high[e]) / div));
+            const int b = static_cast<int>(floorf(127.0f * static_cast<float>(low[e]) / div));
+            bytes[e >> 2] |= static_cast<uint32_t>(a & 0xFF) << (8 * (e & 3));
+            bytes[2 + (e >> 2)] |= static_cast<uint32_t>(b & 0xFF) << (8 * (e & 3));
         }
-        for (int d = 1; d < 16; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-        const bool spoilt = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
-        const float div = m > 0.0f ? m : 1.0f;
-        uint32_t bytes[4] = {0, 0, 0, 0};
-        if (!spoilt) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int a = static_cast<int>(ceilf(127.0f * hi[e] / div)), b = static_cast<int>(floorf(127.0f * lo[e] / div));
-                bytes[e >> 2] |= static_cast<uint32_t>(a & 0xFF) << (8 * (e & 3));
-                bytes[2 + (e >> 2)] |= static_cast<uint32_t>(b & 0xFF) << (8 * (e & 3));
-            }
-        }
-        const size_t at = static_cast<size_t>(page) * c.nkv + h;
-        if (g == 0) *reinterpret_cast<uint2*>(bounds + at * 2 * kPgDim + 8 * j) = make_uint2(bytes[0], bytes[1]);
-        if (g == 1) *reinterpret_cast<uint2*>(bounds + at * 2 * kPgDim + kPgDim + 8 * j) = make_uint2(bytes[2], bytes[3]);
-        if (lane == 0) step[at] = spoilt ? INFINITY : m;
     }
+    const size_t at = static_cast<size_t>(page) * c.nkv + h;
+    *reinterpret_cast<uint2*>(bounds + at * 2 * kPgDim + 8 * j) = make_uint2(bytes[0], bytes[1]);
+    *reinterpret_cast<uint2*>(bounds + at * 2 * kPgDim + kPgDim + 8 * j) = make_uint2(bytes[2], bytes[3]);
+    if (j == 0) step[at] = spoilt ? INFINITY : m;
 }
 
 // ---- selection of blocks ---------------------------------------------------------
@@ -243,14 +266,16 @@ struct SelectParams {
 constexpr uint32_t kForced = 0xFFFFFFFFu, kSpoilt = 0xFFFFFFFEu;  // above every score
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-// grid (row tiles * chunks of 64 blocks, kv heads), 256 threads: a wave 16 blocks.  A row tile is as many
-// rows as 16 columns hold, of one or more sequences; more than 16 q heads take several columns runs.
+// grid (row tiles * chunks of 64 GROUPS blocks, kv heads), 256 threads: a wave 16 GROUPS blocks.  A row
+// tile is as many rows as 16 columns hold, of one or more sequences; more than 16 q heads take several
+// runs of columns.  q is quantized by every wave for itself, which costs more than the products.
+template <int GROUPS>
 __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     __shared__ float s_t[4][16][17];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int tile = blockIdx.x / p.chunks, chunk = blockIdx.x - tile * p.chunks, h = blockIdx.y;
     const int r_end = min((tile + 1) * p.rows_per_tile, p.c.rows);
-    const int b0 = chunk * 64 + wave * 16, cols = min(p.group, 16);
+    const int b0 = (chunk * 4 + wave) * 16 * GROUPS, cols = min(p.group, 16);
     for (int r = tile * p.rows_per_tile; r < r_end;) {
         const int seq = paged_seq_of_row(p.c, r);
         if (seq < 0) {
@@ -263,16 +288,27 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
             continue;
         }
         const int end = min(r_end, s.first + s.n), n = end - r, pos = s.ctx + r - s.first;
-        if (b0 <= (pos + n - 1) >> p.c.shift && b0 < p.c.max_pages) {
-            const int page = paged_page(p.c, seq, b0 + c);
-            const size_t at = static_cast<size_t>(max(page, 0)) * p.c.nkv + h;
-            i32x4 a[4];
+        const int b_end = min(((pos + n - 1) >> p.c.shift) + 1, p.c.max_pages);
+        if (b0 < b_end) {
+            int page[GROUPS];
+            i32x4 a[GROUPS][4];
+            float m_b[GROUPS];
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                a[kk] = *reinterpret_cast<const i32x4*>(p.bounds + at * 2 * kPgDim + 64 * kk + 16 * g);
-            const float m_b = p.step[at];
-            // lane (c, g) of the result: block c, rows g, g + 4, ... of the tile
-            float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int i = 0; i < GROUPS; ++i) page[i] = paged_page(p.c, seq, b0 + 16 * i + c);
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const size_t at = static_cast<size_t>(max(page[i], 0)) * p.c.nkv + h;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    a[i][kk] = *reinterpret_cast<const i32x4*>(p.bounds + at * 2 * kPgDim + 64 * kk + 16 * g);
+                m_b[i] = p.step[at];
+            }
+            // lane (c, g) of the result: block c of each group, rows g, g + 4, ... of the tile
+            float best[GROUPS][4];
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) best[i][k] = -INFINITY;
             for (int hb = 0; hb < p.group; hb += 16) {
                 const int col_row = min(c / cols, n - 1), col_head = min(hb + c % cols, p.group - 1);
                 const uint16_t* q = p.q + (static_cast<size_t>(r + col_row) * p.nq + h * p.group + col_head) * kPgDim + 16 * g;
@@ -309,41 +345,47 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
                         up[i][w] = static_cast<int>(u);
                         down[i][w] = static_cast<int>(d);
                     }
-                i32x4 dot = {0, 0, 0, 0};
-                dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[0], up[0], dot, 0, 0, 0);
-                dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[1], up[1], dot, 0, 0, 0);
-                dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[2], down[0], dot, 0, 0, 0);
-                dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[3], down[1], dot, 0, 0, 0);
                 const float m_h = none ? 0.0f : m;
-                __builtin_amdgcn_wave_barrier();  // the last run's values are read
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s_t[wave][4 * g + i][c] = static_cast<float>(dot[i]) * m_h;
-                __builtin_amdgcn_wave_barrier();
                 const int heads = min(cols, p.group - hb);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = g + 4 * i;
-                    if (row >= n) break;
-                    for (int k = 0; k < heads; ++k) best[i] = fmaxf(best[i], s_t[wave][c][row * cols + k]);
+                for (int i = 0; i < GROUPS; ++i) {
+                    i32x4 dot = {0, 0, 0, 0};
+                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][0], up[0], dot, 0, 0, 0);
+                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][1], up[1], dot, 0, 0, 0);
+                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][2], down[0], dot, 0, 0, 0);
+                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][3], down[1], dot, 0, 0, 0);
+                    __builtin_amdgcn_wave_barrier();  // the last group's values are read
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s_t[wave][4 * g + k][c] = static_cast<float>(dot[k]) * m_h;
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = g + 4 * k;
+                        if (row >= n) break;
+                        for (int e = 0; e < heads; ++e) best[i][k] = fmaxf(best[i][k], s_t[wave][c][row * cols + e]);
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = g + 4 * i, own = (pos + row) >> p.c.shift, b = b0 + c;
-                if (row >= n || b > own || b >= p.c.max_pages) continue;
-                const uint32_t u = __builtin_bit_cast(uint32_t, best[i] * m_b + 0.0f);  // (no -0)
-                uint32_t key = u >> 31 ? ~u : u | 0x80000000u;
-                if (m_b == INFINITY) key = kSpoilt;
-                if (b < p.sinks || b > own - p.recent) key = kForced;
-                if (page < 0) key = 0;
-                p.keys[(static_cast<size_t>(r + row) * p.c.nkv + h) * p.c.max_pages + b] = key;
-            }
+            for (int i = 0; i < GROUPS; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = g + 4 * k, own = (pos + row) >> p.c.shift, b = b0 + 16 * i + c;
+                    if (row >= n || b > own || b >= p.c.max_pages) continue;
+                    const uint32_t u = __builtin_bit_cast(uint32_t, best[i][k] * m_b[i] + 0.0f);  // (no -0)
+                    uint32_t key = u >> 31 ? ~u : u | 0x80000000u;
+                    if (m_b[i] == INFINITY) key = kSpoilt;
+                    if (b < p.sinks || b > own - p.recent) key = kForced;
+                    if (page[i] < 0) key = 0;
+                    p.keys[(static_cast<size_t>(r + row) * p.c.nkv + h) * p.c.max_pages + b] = key;
+                }
         }
         r = end;
     }
 }
 
-// Sum over the 256 threads of a block up to and without each; `all` gets the sum.  Two barriers.
+// Sum over the threads of a block up to and without each; `all` gets the sum.  Two barriers.
+template <int THREADS>
 __device__ __forceinline__ int block_scan(int x, int& all, int* s_part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int y = x;
@@ -358,38 +400,126 @@ __device__ __forceinline__ int block_scan(int x, int& all, int* s_part) {
     int before = 0;
     all = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         before += w < wave ? s_part[w] : 0;
         all += s_part[w];
     }
     return before + y - x;
 }
 
-// The num_selected largest keys of a (row, kv head), equal ones the lower block first, as ascending
-// blocks and -1 behind.  A block each: the last key that is in is found digit by digit (8 bits,
-// counts in LDS), keys in LDS up to kSelectCached.
-constexpr int kSelectCached = 8192;
-__global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
-    __shared__ uint32_t s_key[kSelectCached];
-    __shared__ int s_count[256], s_part[4], s_found[2];
-    const int row = blockIdx.x / p.c.nkv, tid = threadIdx.x;
+// Which row and kv head a block of the selection has, and how many blocks it chooses from; false: none.
+__device__ __forceinline__ bool select_range(const SelectParams& p, int& n) {
+    const int row = blockIdx.x / p.c.nkv;
     const int seq = paged_seq_of_row(p.c, row);
-    if (seq < 0) return;
+    if (seq < 0) return false;
     const PagedSeq s = paged_seq(p.c, seq);
-    if (row < s.first || row >= s.first + s.n) return;
-    const int n = min(((s.ctx + row - s.first) >> p.c.shift) + 1, p.c.max_pages);
+    if (row < s.first || row >= s.first + s.n) return false;
+    n = min(((s.ctx + row - s.first) >> p.c.shift) + 1, p.c.max_pages);
+    return true;
+}
+
+// The num_selected largest keys of a (row, kv head), equal ones the lower block first, as ascending
+// blocks and -1 behind.  A block each, KEYS keys a thread in registers: the last key that is in is
+// found bit by bit, from the highest in which the scores differ (two ballots' worth of work a key and
+// bit), until as many keys as wanted are left above.  2048 keys of 131000 positions 3.6 us of 13.1 with a
+// count of digits in LDS: scores have few different first digits, so its counters were met by all lanes.
+template <int THREADS, int KEYS>
+__global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
+    constexpr int kWaves = THREADS / 64;
+    __shared__ int s_part[kWaves], s_count[2][kWaves];
+    __shared__ uint2 s_bits[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int n;
+    if (!select_range(p, n)) return;
     const uint32_t* keys = p.keys + static_cast<size_t>(blockIdx.x) * p.c.max_pages;
     int32_t* out = p.selected + static_cast<size_t>(blockIdx.x) * p.num_selected;
-    const bool cached = n <= kSelectCached;
-    int mine = 0;
-    for (int i = tid; i < n; i += 256) {
-        const uint32_t k = keys[i];
-        if (cached) s_key[i] = k;
-        mine += k != 0;
+    // each thread a stretch of blocks, so that they come out in order
+    const int per = (n + THREADS - 1) / THREADS, i0 = tid * per;
+    uint32_t k[KEYS];
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) k[j] = j < per && i0 + j < n ? keys[i0 + j] : 0u;
+    auto count = [&](uint32_t from, int turn) __attribute__((always_inline)) {  // keys of at least `from`; one barrier
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j)
+            if (j < per) mine += __popcll(__builtin_amdgcn_ballot_w64(k[j] >= from));
+        if (lane == 0) s_count[turn & 1][wave] = mine;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) all += s_count[turn & 1][w];
+        return all;
+    };
+    // bits that are set in some score and in every one
+    uint32_t some = 0, every = ~0u;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)
+        if (k[j] != 0 && k[j] < kSpoilt) some |= k[j], every &= k[j];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) some |= __shfl_xor(some, d), every &= __shfl_xor(every, d);
+    if (lane == 0) s_bits[wave] = make_uint2(some, every);
+    const int there = count(1u, 0);  // (its barrier is that of s_bits too)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) some |= s_bits[w].x, every &= s_bits[w].y;
+    const int need = min(p.num_selected, there);
+    uint32_t limit = 1;       // keys of at least this are in, but of those equal to it
+    int equal = INT32_MAX;    // only so many
+    int turn = 1;
+    if (need < there) {
+        const int above = count(kSpoilt, turn++), forced = count(kForced, turn++);
+        if (need <= forced) {
+            limit = kForced;
+            equal = need;
+        } else if (need <= above) {
+            limit = kSpoilt;
+            equal = need - forced;
+        } else {
+            const uint32_t differ = some & ~every;
+            int bit = differ == 0 ? -1 : 31 - __clz(differ);
+            limit = bit < 0 ? every : every & ~((2u << bit) - 1u);  // what all scores begin with
+            bool exact = false;
+            for (; bit >= 0 && !exact; --bit) {
+                const uint32_t x = limit | 1u << bit;
+                const int c = count(x, turn++);
+                if (c >= need) {
+                    limit = x;
+                    exact = c == need;
+                }
+            }
+            if (!exact) equal = need - count(limit + 1, turn++);
+        }
     }
-    auto key = [&](int i) { return cached ? s_key[i] : keys[i]; };
+    int above = 0, same = 0;
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+        above += k[j] > limit;
+        same += k[j] == limit;
+    }
+    int all;
+    const int both = block_scan<THREADS>(above << 16 | same, all, s_part);  // (neither passes 2^15)
+    int same_before = both & 0xFFFF;
+    int at = (both >> 16) + min(same_before, equal);
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+        if (k[j] > limit || (k[j] == limit && same_before < equal)) out[at++] = i0 + j;
+        same_before += k[j] == limit;
+    }
+    for (int i = need + tid; i < p.num_selected; i += THREADS) out[i] = -1;
+}
+
+// The same for longer lists: digit by digit (8 bits, counts in LDS), the keys read again for each.
+__global__ __launch_bounds__(1024) void paged_select_long_kernel(SelectParams p) {
+    constexpr int kThreads = 1024;
+    __shared__ int s_count[256], s_part[kThreads / 64], s_found[2];
+    const int tid = threadIdx.x;
+    int n;
+    if (!select_range(p, n)) return;
+    const uint32_t* keys = p.keys + static_cast<size_t>(blockIdx.x) * p.c.max_pages;
+    int32_t* out = p.selected + static_cast<size_t>(blockIdx.x) * p.num_selected;
+    int mine = 0;
+    for (int i = tid; i < n; i += kThreads) mine += keys[i] != 0;
     int there;
-    block_scan(mine, there, s_part);
+    block_scan<kThreads>(mine, there, s_part);
     const int need = min(p.num_selected, there);
     uint32_t limit = 1;  // keys above it are in, and the first `equal` of those equal to it
     int equal = INT32_MAX;
@@ -397,41 +527,39 @@ __global__ __launch_bounds__(256) void paged_select_kernel(SelectParams p) {
         equal = need;
         limit = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            s_count[tid] = 0;
+            if (tid < 256) s_count[tid] = 0;
             __syncthreads();
             const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            for (int i = tid; i < n; i += 256) {
-                const uint32_t k = key(i);
+            for (int i = tid; i < n; i += kThreads) {
+                const uint32_t k = keys[i];
                 if ((k & mask) == limit) atomicAdd(&s_count[(k >> shift) & 255], 1);
             }
             __syncthreads();
-            const int digit = 255 - tid, here = s_count[digit];  // from the largest down
+            const int digit = 255 - tid, here = tid < 256 ? s_count[digit & 255] : 0;  // from the largest down
             int all;
-            const int above = block_scan(here, all, s_part);
-            if (above < equal && equal <= above + here) s_found[0] = digit, s_found[1] = above;
+            const int above = block_scan<kThreads>(here, all, s_part);
+            if (tid < 256 && above < equal && equal <= above + here) s_found[0] = digit, s_found[1] = above;
             __syncthreads();
             limit |= static_cast<uint32_t>(s_found[0]) << shift;
             equal -= s_found[1];
         }
     }
-    // each thread a stretch of blocks, so that they come out in order
-    const int per = (n + 255) / 256, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    const int per = (n + kThreads - 1) / kThreads, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     int above = 0, same = 0;
     for (int i = i0; i < i1; ++i) {
-        const uint32_t k = key(i);
-        above += k > limit;
-        same += k == limit;
+        above += keys[i] > limit;
+        same += keys[i] == limit;
     }
     int all;
-    const int above_before = block_scan(above, all, s_part);
-    int same_before = block_scan(same, all, s_part);
+    const int above_before = block_scan<kThreads>(above, all, s_part);
+    int same_before = block_scan<kThreads>(same, all, s_part);
     int at = above_before + min(same_before, equal);
     for (int i = i0; i < i1; ++i) {
-        const uint32_t k = key(i);
+        const uint32_t k = keys[i];
         if (k > limit || (k == limit && same_before < equal)) out[at++] = i;
         same_before += k == limit;
     }
-    for (int i = need + tid; i < p.num_selected; i += 256) out[i] = -1;
+    for (int i = need + tid; i < p.num_selected; i += kThreads) out[i] = -1;
 }
 
 }  // namespace
@@ -563,7 +691,7 @@ extern "C" int qe_launch_paged_key_bounds(const qe_paged_cache* cache, const qe_
                                paged_v_span(cache), paged_table_span(batch), paged_starts_span(batch),
                                paged_context_span(batch)};
     QE_TRY(paged_check_apart(what, spans, 2));
-    paged_key_bounds_kernel<<<batch->num_tokens, 256, 0, stream>>>(c, bounds, bound_steps);
+    paged_key_bounds_kernel<<<dim3(batch->num_tokens, cache->num_kv_heads), 256, 0, stream>>>(c, bounds, bound_steps);
     return check_launch(what);
 }
 
@@ -605,8 +733,12 @@ extern "C" int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* c
     const long long n = batch->num_tokens;
     p.group = num_q_heads / nkv;
     p.rows_per_tile = batch->query_start == nullptr ? 1 : std::max(1, 16 / p.group);
-    p.chunks = (batch->max_pages + 63) / 64;
     const long long tiles = (n + p.rows_per_tile - 1) / p.rows_per_tile;
+    // Four groups of 16 blocks a wave where there is work for the whole chip all the same (200 rows on 1563 blocks:
+    // 39 us with one group), else one: a single row waits for its loads.
+    const bool wide = tiles * nkv * ((batch->max_pages + 63) / 64) >= 4096;
+    const int per_block = wide ? 256 : 64;
+    p.chunks = (batch->max_pages + per_block - 1) / per_block;
     size_t bytes = 0;
     QE_REQUIRE(select_workspace(n, nkv, batch->max_pages, &bytes) && tiles * p.chunks <= INT32_MAX && n * nkv <= INT32_MAX,
                "%s: num_tokens=%d max_pages=%d", what, batch->num_tokens, batch->max_pages);
@@ -631,7 +763,17 @@ extern "C" int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* c
     p.num_selected = num_selected;
     p.sinks = sinks;
     p.recent = recent;
-    paged_score_kernel<<<dim3(static_cast<unsigned>(tiles * p.chunks), nkv), 256, 0, stream>>>(p);
-    paged_select_kernel<<<static_cast<unsigned>(n * nkv), 256, 0, stream>>>(p);
+    const dim3 grid(static_cast<unsigned>(tiles * p.chunks), nkv);
+    if (wide)
+        paged_score_kernel<4><<<grid, 256, 0, stream>>>(p);
+    else
+        paged_score_kernel<1><<<grid, 256, 0, stream>>>(p);
+    const unsigned lists = static_cast<unsigned>(n * nkv);
+    if (batch->max_pages <= 256 * 8)
+        paged_select_kernel<256, 8><<<lists, 256, 0, stream>>>(p);
+    else if (batch->max_pages <= 1024 * 16)
+        paged_select_kernel<1024, 16><<<lists, 1024, 0, stream>>>(p);
+    else
+        paged_select_long_kernel<<<lists, 1024, 0, stream>>>(p);
     return check_launch(what);
 }

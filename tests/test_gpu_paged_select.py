@@ -151,9 +151,10 @@ def test_selection_with_the_bounds_of_the_keys(qe):
 
 
 def test_ties_and_a_table_of_thousands_of_blocks(qe):
-    """9000 blocks on 40 pages: hundreds of equal scores, the lower blocks first; the longest list kept in LDS is 8192."""
+    """Thousands of blocks on a few pages: hundreds of equal scores, the lower blocks first.  Lists of up to 2048, 16384 and
+    more blocks are selected by different kernels."""
     rng = np.random.default_rng(6)
-    for blocks in (8192, 9000):
+    for blocks in (2048, 2049, 9000, 16384, 17000):
         w = World(rng, [(20, 1)], 16, 12, 2)
         w.lens = [(16 * blocks - 5, 1)]
         w.context = np.array([16 * blocks - 5], np.int32)

@@ -75,22 +75,6 @@ struct SeqWork {
     }
 };
 
-// Sum over a wave up to and with each lane, in the vector unit: 1, 2, 4 and 8 lanes on within rows
-// of 16, then the rows' sums.
-__device__ __forceinline__ int wave_scan(int x) {
-    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
-        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-    };
-    typedef std::integral_constant<int, 0xF> all;
-    add(std::integral_constant<int, 0x111>{}, all{});
-    add(std::integral_constant<int, 0x112>{}, all{});
-    add(std::integral_constant<int, 0x114>{}, all{});
-    add(std::integral_constant<int, 0x118>{}, all{});
-    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row 15's and 47's sum
-    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row 31's
-    return x;
-}
-
 // 64 sequences of the batch, one a lane.
 struct SeqChunk {
     int base, first, n, ctx;
@@ -473,6 +457,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int c = lane & 15, g = lane >> 4;
     const Partials part = partials<kDecRows>(p.ws, kDecBlocks);
+    const int block = blockIdx.x;
     const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
     const ptrdiff_t v_minus_k = reinterpret_cast<const char*>(p.c.v) - reinterpret_cast<const char*>(p.c.k);
 
@@ -679,7 +664,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
                 *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
                 if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
             } else {
-                const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * kDecRows + r;
+                const size_t at = static_cast<size_t>(2 * block + slot) * kDecRows + r;
                 *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
                 if (d == 0) part.ml[at] = make_float2(m, l);
             }
@@ -695,8 +680,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
         }
         return min(kDecRows, p.group - rt * kDecRows);
     };
-    for_share<SPARSE>(p.c, blockIdx.x, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
-        if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
+    for_share<SPARSE>(p.c, block, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
+        if (threadIdx.x == 0) part.cuts[block] = cut;
     });
 }
 

@@ -261,22 +261,28 @@ struct SelectParams {
     const float* step;
     uint32_t* keys;  // [row][kv head][max_pages]: scores as whole numbers of the same order
     int32_t* selected;
-    int nq, group, rows_per_tile, chunks, num_selected, sinks, recent;
+    int nq, group, rows_per_tile, rows_per_run, chunks, num_selected, sinks, recent;
 };
 constexpr uint32_t kForced = 0xFFFFFFFFu, kSpoilt = 0xFFFFFFFEu;  // above every score
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-// grid (row tiles * chunks of 64 GROUPS blocks, kv heads), 256 threads: a wave 16 GROUPS blocks.  A row
-// tile is as many rows as 16 columns hold, of one or more sequences; more than 16 q heads take several
-// runs of columns.  q is quantized by every wave for itself, which costs more than the products.
-template <int GROUPS>
+// grid (runs of rows * chunks of 64 blocks, kv heads), 256 threads: a wave 16 blocks, whose bounds stay in
+// registers for the rows of the run that are of one sequence.  Rows are taken as many at a time as 16
+// columns hold; more than 16 q heads take several runs of columns.  The block quantizes q once, 16
+// threads a column (every wave for itself, and the bounds read again for every 16 columns, 200 rows on
+// 1563 blocks took 39 us).
 __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     __shared__ float s_t[4][16][17];
+    __shared__ __align__(16) int8_t s_q[16][2 * kPgDim + 16];  // positive and negative parts of each column (and 16 bytes, for the banks)
+    __shared__ float s_m[16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x / p.chunks, chunk = blockIdx.x - tile * p.chunks, h = blockIdx.y;
-    const int r_end = min((tile + 1) * p.rows_per_tile, p.c.rows);
-    const int b0 = (chunk * 4 + wave) * 16 * GROUPS, cols = min(p.group, 16);
-    for (int r = tile * p.rows_per_tile; r < r_end;) {
+    const int run = blockIdx.x / p.chunks, chunk = blockIdx.x - run * p.chunks, h = blockIdx.y;
+    const int r_end = min((run + 1) * p.rows_per_run, p.c.rows);
+    const int b = (chunk * 4 + wave) * 16 + c, cols = min(p.group, 16);  // the lane's block
+    int loaded = -1, page = -1;  // the sequence whose bounds are in a
+    i32x4 a[4];
+    float m_b = 0.0f;
+    for (int r = run * p.rows_per_run; r < r_end;) {
         const int seq = paged_seq_of_row(p.c, r);
         if (seq < 0) {
             ++r;
@@ -287,115 +293,93 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
             ++r;
             continue;
         }
-        const int end = min(r_end, s.first + s.n), n = end - r, pos = s.ctx + r - s.first;
-        const int b_end = min(((pos + n - 1) >> p.c.shift) + 1, p.c.max_pages);
-        if (b0 < b_end) {
-            int page[GROUPS];
-            i32x4 a[GROUPS][4];
-            float m_b[GROUPS];
+        for (const int seq_end = min(r_end, s.first + s.n); r < seq_end;) {
+            const int n = min(p.rows_per_tile, seq_end - r), pos = s.ctx + r - s.first;
+            const int b_end = min(((pos + n - 1) >> p.c.shift) + 1, p.c.max_pages);
+            if (chunk * 64 < b_end) {  // (the same for the whole block)
+                if (seq != loaded) page = paged_page(p.c, seq, b);
+                // lane (c, g) of the result: block c, rows g, g + 4, ... of the tile
+                float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int hb = 0; hb < p.group; hb += 16) {
+                    {
+                        const int col = threadIdx.x >> 4, j = threadIdx.x & 15;
+                        const int col_row = min(col / cols, n - 1), col_head = min(hb + col % cols, p.group - 1);
+                        const f16x8 x = *reinterpret_cast<const f16x8*>(
+                            p.q + (static_cast<size_t>(r + col_row) * p.nq + h * p.group + col_head) * kPgDim + 8 * j);
+                        if (seq != loaded) {  // asked for behind q
+                            loaded = seq;
+                            const size_t at = static_cast<size_t>(max(page, 0)) * p.c.nkv + h;
 #pragma unroll
-            for (int i = 0; i < GROUPS; ++i) page[i] = paged_page(p.c, seq, b0 + 16 * i + c);
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const size_t at = static_cast<size_t>(max(page[i], 0)) * p.c.nkv + h;
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    a[i][kk] = *reinterpret_cast<const i32x4*>(p.bounds + at * 2 * kPgDim + 64 * kk + 16 * g);
-                m_b[i] = p.step[at];
-            }
-            // lane (c, g) of the result: block c of each group, rows g, g + 4, ... of the tile
-            float best[GROUPS][4];
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) best[i][k] = -INFINITY;
-            for (int hb = 0; hb < p.group; hb += 16) {
-                const int col_row = min(c / cols, n - 1), col_head = min(hb + c % cols, p.group - 1);
-                const uint16_t* q = p.q + (static_cast<size_t>(r + col_row) * p.nq + h * p.group + col_head) * kPgDim + 16 * g;
-                f16x8 x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const f16x8*>(q + 64 * (i >> 1) + 8 * (i & 1));
-                float m = 0.0f;
-                bool odd = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = fabsf(static_cast<float>(x[i][e]));
-                        odd = odd || !(v < INFINITY);
-                        m = fmaxf(m, v);
-                    }
-                m = odd ? INFINITY : m;
-                m = fmaxf(m, __shfl_xor(m, 16));
-                m = fmaxf(m, __shfl_xor(m, 32));
-                const bool none = !(m > 0.0f && m < INFINITY);
-                i32x4 up[2], down[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t u = 0, d = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = static_cast<float>(x[2 * i + (w >> 1)][4 * (w & 1) + e]);
-                            const int y = none ? 0 : static_cast<int>(rintf(127.0f * v / m));
-                            u |= static_cast<uint32_t>(max(y, 0)) << (8 * e);
-                            d |= static_cast<uint32_t>(min(y, 0) & 0xFF) << (8 * e);
+                            for (int kk = 0; kk < 4; ++kk)
+                                a[kk] = *reinterpret_cast<const i32x4*>(p.bounds + at * 2 * kPgDim + 64 * kk + 16 * g);
+                            m_b = p.step[at];
                         }
-                        up[i][w] = static_cast<int>(u);
-                        down[i][w] = static_cast<int>(d);
-                    }
-                const float m_h = none ? 0.0f : m;
-                const int heads = min(cols, p.group - hb);
+                        float m = 0.0f;
+                        bool odd = false;
 #pragma unroll
-                for (int i = 0; i < GROUPS; ++i) {
+                        for (int e = 0; e < 8; ++e) {
+                            const float v = fabsf(static_cast<float>(x[e]));
+                            odd = odd || !(v < INFINITY);
+                            m = fmaxf(m, v);
+                        }
+                        m = qwen::seg_max_nonneg<16>(odd ? INFINITY : m);
+                        const bool none = !(m > 0.0f && m < INFINITY);
+                        uint32_t up[2] = {0, 0}, down[2] = {0, 0};
+                        if (!none) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int y = static_cast<int>(rintf(127.0f * static_cast<float>(x[e]) / m));
+                                up[e >> 2] |= static_cast<uint32_t>(max(y, 0)) << (8 * (e & 3));
+                                down[e >> 2] |= static_cast<uint32_t>(min(y, 0) & 0xFF) << (8 * (e & 3));
+                            }
+                        }
+                        __syncthreads();  // the last columns are read
+                        *reinterpret_cast<uint2*>(&s_q[col][8 * j]) = make_uint2(up[0], up[1]);
+                        *reinterpret_cast<uint2*>(&s_q[col][kPgDim + 8 * j]) = make_uint2(down[0], down[1]);
+                        if (j == 0) s_m[col] = none ? 0.0f : m;
+                        __syncthreads();
+                    }
+                    const float m_h = s_m[c];
                     i32x4 dot = {0, 0, 0, 0};
-                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][0], up[0], dot, 0, 0, 0);
-                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][1], up[1], dot, 0, 0, 0);
-                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][2], down[0], dot, 0, 0, 0);
-                    dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][3], down[1], dot, 0, 0, 0);
-                    __builtin_amdgcn_wave_barrier();  // the last group's values are read
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[kk], *reinterpret_cast<const i32x4*>(&s_q[c][64 * kk + 16 * g]),
+                                                                    dot, 0, 0, 0);
+                    __builtin_amdgcn_wave_barrier();  // the last columns' values are read
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s_t[wave][4 * g + k][c] = static_cast<float>(dot[k]) * m_h;
                     __builtin_amdgcn_wave_barrier();
+                    const int heads = min(cols, p.group - hb);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int row = g + 4 * k;
                         if (row >= n) break;
-                        for (int e = 0; e < heads; ++e) best[i][k] = fmaxf(best[i][k], s_t[wave][c][row * cols + e]);
+                        for (int e = 0; e < heads; ++e) best[k] = fmaxf(best[k], s_t[wave][c][row * cols + e]);
                     }
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int row = g + 4 * k, own = (pos + row) >> p.c.shift, b = b0 + 16 * i + c;
+                    const int row = g + 4 * k, own = (pos + row) >> p.c.shift;
                     if (row >= n || b > own || b >= p.c.max_pages) continue;
-                    const uint32_t u = __builtin_bit_cast(uint32_t, best[i][k] * m_b[i] + 0.0f);  // (no -0)
+                    const uint32_t u = __builtin_bit_cast(uint32_t, best[k] * m_b + 0.0f);  // (no -0)
                     uint32_t key = u >> 31 ? ~u : u | 0x80000000u;
-                    if (m_b[i] == INFINITY) key = kSpoilt;
+                    if (m_b == INFINITY) key = kSpoilt;
                     if (b < p.sinks || b > own - p.recent) key = kForced;
-                    if (page[i] < 0) key = 0;
+                    if (page < 0) key = 0;
                     p.keys[(static_cast<size_t>(r + row) * p.c.nkv + h) * p.c.max_pages + b] = key;
                 }
+            }
+            r += n;
         }
-        r = end;
     }
 }
 
 // Sum over the threads of a block up to and without each; `all` gets the sum.  Two barriers.
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int x, int& all, int* s_part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int y = x;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int z = __shfl_up(y, d);
-        if (lane >= d) y += z;
-    }
+    const int wave = threadIdx.x >> 6, y = wave_scan(x);
     __syncthreads();
-    if (lane == 63) s_part[wave] = y;
+    if ((threadIdx.x & 63) == 63) s_part[wave] = y;
     __syncthreads();
     int before = 0;
     all = 0;
@@ -420,13 +404,15 @@ __device__ __forceinline__ bool select_range(const SelectParams& p, int& n) {
 
 // The num_selected largest keys of a (row, kv head), equal ones the lower block first, as ascending
 // blocks and -1 behind.  A block each, KEYS keys a thread in registers: the last key that is in is
-// found bit by bit, from the highest in which the scores differ (two ballots' worth of work a key and
-// bit), until as many keys as wanted are left above.  2048 keys of 131000 positions 3.6 us of 13.1 with a
-// count of digits in LDS: scores have few different first digits, so its counters were met by all lanes.
+// found by two bits at once, from the highest in which the scores differ, until as many keys as wanted
+// are left above: three counts by ballots, and one barrier, each time.  (A count of digits in LDS, as
+// below, took 12.8 us for the 2048 keys of 131000 positions: scores have few different first digits,
+// so the lanes met at the same counters.)
 template <int THREADS, int KEYS>
 __global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
     constexpr int kWaves = THREADS / 64;
-    __shared__ int s_part[kWaves], s_count[2][kWaves];
+    __shared__ int s_part[kWaves];
+    __shared__ int4 s_count[2][kWaves];
     __shared__ uint2 s_bits[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int n;
@@ -438,16 +424,28 @@ __global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
     uint32_t k[KEYS];
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) k[j] = j < per && i0 + j < n ? keys[i0 + j] : 0u;
-    auto count = [&](uint32_t from, int turn) __attribute__((always_inline)) {  // keys of at least `from`; one barrier
-        int mine = 0;
+    int turn = 0;
+    // keys of at least a, b and c each; one barrier
+    auto count = [&](uint32_t a, uint32_t b, uint32_t c) __attribute__((always_inline)) {
+        int3 mine = make_int3(0, 0, 0);
 #pragma unroll
         for (int j = 0; j < KEYS; ++j)
-            if (j < per) mine += __popcll(__builtin_amdgcn_ballot_w64(k[j] >= from));
-        if (lane == 0) s_count[turn & 1][wave] = mine;
+            if (j < per) {
+                mine.x += __popcll(__builtin_amdgcn_ballot_w64(k[j] >= a));
+                mine.y += __popcll(__builtin_amdgcn_ballot_w64(k[j] >= b));
+                mine.z += __popcll(__builtin_amdgcn_ballot_w64(k[j] >= c));
+            }
+        if (lane == 0) s_count[turn][wave] = make_int4(mine.x, mine.y, mine.z, 0);
         __syncthreads();
-        int all = 0;
+        int3 all = make_int3(0, 0, 0);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) all += s_count[turn & 1][w];
+        for (int w = 0; w < kWaves; ++w) {
+            const int4 x = s_count[turn][w];
+            all.x += x.x;
+            all.y += x.y;
+            all.z += x.z;
+        }
+        turn ^= 1;
         return all;
     };
     // bits that are set in some score and in every one
@@ -458,35 +456,32 @@ __global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) some |= __shfl_xor(some, d), every &= __shfl_xor(every, d);
     if (lane == 0) s_bits[wave] = make_uint2(some, every);
-    const int there = count(1u, 0);  // (its barrier is that of s_bits too)
+    const int3 kinds = count(1u, kSpoilt, kForced);  // (its barrier is that of s_bits too)
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) some |= s_bits[w].x, every &= s_bits[w].y;
-    const int need = min(p.num_selected, there);
-    uint32_t limit = 1;       // keys of at least this are in, but of those equal to it
-    int equal = INT32_MAX;    // only so many
-    int turn = 1;
+    const int there = kinds.x, need = min(p.num_selected, there);
+    uint32_t limit = 1;     // keys of at least this are in, but of those equal to it
+    int equal = INT32_MAX;  // only so many
     if (need < there) {
-        const int above = count(kSpoilt, turn++), forced = count(kForced, turn++);
-        if (need <= forced) {
+        if (need <= kinds.z) {
             limit = kForced;
             equal = need;
-        } else if (need <= above) {
+        } else if (need <= kinds.y) {
             limit = kSpoilt;
-            equal = need - forced;
+            equal = need - kinds.z;
         } else {
             const uint32_t differ = some & ~every;
-            int bit = differ == 0 ? -1 : 31 - __clz(differ);
-            limit = bit < 0 ? every : every & ~((2u << bit) - 1u);  // what all scores begin with
+            int bit = differ == 0 ? -2 : (31 - __clz(differ)) & ~1;  // the lower of the two looked at
+            limit = bit < 0 ? every : every & ~((4u << bit) - 1u);   // what all scores begin with
             bool exact = false;
-            for (; bit >= 0 && !exact; --bit) {
-                const uint32_t x = limit | 1u << bit;
-                const int c = count(x, turn++);
-                if (c >= need) {
-                    limit = x;
-                    exact = c == need;
-                }
+            for (; bit >= 0 && !exact; bit -= 2) {
+                const uint32_t one = 1u << bit;
+                const int3 c = count(limit + one, limit + 2 * one, limit + 3 * one);
+                const int got = c.z >= need ? c.z : c.y >= need ? c.y : c.x >= need ? c.x : 0;
+                limit += c.z >= need ? 3 * one : c.y >= need ? 2 * one : c.x >= need ? one : 0;
+                exact = got == need;
             }
-            if (!exact) equal = need - count(limit + 1, turn++);
+            if (!exact) equal = need - count(limit + 1, ~0u, ~0u).x;
         }
     }
     int above = 0, same = 0;
@@ -734,13 +729,13 @@ extern "C" int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* c
     p.group = num_q_heads / nkv;
     p.rows_per_tile = batch->query_start == nullptr ? 1 : std::max(1, 16 / p.group);
     const long long tiles = (n + p.rows_per_tile - 1) / p.rows_per_tile;
-    // Four groups of 16 blocks a wave where there is work for the whole chip all the same (200 rows on 1563 blocks:
-    // 39 us with one group), else one: a single row waits for its loads.
-    const bool wide = tiles * nkv * ((batch->max_pages + 63) / 64) >= 4096;
-    const int per_block = wide ? 256 : 64;
-    p.chunks = (batch->max_pages + per_block - 1) / per_block;
+    p.chunks = (batch->max_pages + 63) / 64;
+    // several tiles a block where that leaves four blocks a CU
+    const long long tiles_per_run = std::max(1LL, std::min(8LL, tiles * p.chunks * nkv / 1024));
+    const long long runs = (tiles + tiles_per_run - 1) / tiles_per_run;
+    p.rows_per_run = static_cast<int>(p.rows_per_tile * tiles_per_run);
     size_t bytes = 0;
-    QE_REQUIRE(select_workspace(n, nkv, batch->max_pages, &bytes) && tiles * p.chunks <= INT32_MAX && n * nkv <= INT32_MAX,
+    QE_REQUIRE(select_workspace(n, nkv, batch->max_pages, &bytes) && runs * p.chunks <= INT32_MAX && n * nkv <= INT32_MAX,
                "%s: num_tokens=%d max_pages=%d", what, batch->num_tokens, batch->max_pages);
     const size_t pages = static_cast<size_t>(cache->num_pages) * nkv;
     const PagedSpan spans[] = {{selected, 4 * static_cast<size_t>(n) * nkv * num_selected, "selected"},
@@ -763,14 +758,12 @@ extern "C" int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* c
     p.num_selected = num_selected;
     p.sinks = sinks;
     p.recent = recent;
-    const dim3 grid(static_cast<unsigned>(tiles * p.chunks), nkv);
-    if (wide)
-        paged_score_kernel<4><<<grid, 256, 0, stream>>>(p);
-    else
-        paged_score_kernel<1><<<grid, 256, 0, stream>>>(p);
+    paged_score_kernel<<<dim3(static_cast<unsigned>(runs * p.chunks), nkv), 256, 0, stream>>>(p);
     const unsigned lists = static_cast<unsigned>(n * nkv);
     if (batch->max_pages <= 256 * 8)
         paged_select_kernel<256, 8><<<lists, 256, 0, stream>>>(p);
+    else if (batch->max_pages <= 512 * 8)
+        paged_select_kernel<512, 8><<<lists, 512, 0, stream>>>(p);
     else if (batch->max_pages <= 1024 * 16)
         paged_select_kernel<1024, 16><<<lists, 1024, 0, stream>>>(p);
     else

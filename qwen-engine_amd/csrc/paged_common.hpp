@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4_common.hpp"
 
@@ -64,6 +65,22 @@ __device__ __forceinline__ int paged_page(const PagedView& p, int seq, int block
     if (block >= p.max_pages) return -1;
     const int at = p.table[static_cast<size_t>(seq) * p.max_pages + block];
     return at >= 0 && at < p.num_pages ? at : -1;
+}
+
+// Sum over a wave up to and with each lane, in the vector unit: 1, 2, 4 and 8 lanes on within rows
+// of 16, then the rows' sums.
+__device__ __forceinline__ int wave_scan(int x) {
+    auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    typedef std::integral_constant<int, 0xF> all;
+    add(std::integral_constant<int, 0x111>{}, all{});
+    add(std::integral_constant<int, 0x112>{}, all{});
+    add(std::integral_constant<int, 0x114>{}, all{});
+    add(std::integral_constant<int, 0x118>{}, all{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row 15's and 47's sum
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row 31's
+    return x;
 }
 
 // ---- host: checks -------------------------------------------------------------

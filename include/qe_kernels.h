@@ -536,7 +536,8 @@ int qe_launch_kv4_evict(const uint8_t* layer_k_cache, const uint8_t* layer_v_cac
  * behind each other; K and V may take turns in one allocation), 16-byte aligned.
  * Position p of sequence s is row p % page_size of page block_table[s][p / page_size].
  * Table entries outside [0, num_pages), and positions of max_pages * page_size and more,
- * have no row: nothing is stored there, and nobody attends to them. */
+ * have no row: nothing is stored there, and nobody attends to them.  head_dim is 128,
+ * num_kv_heads at most 1024. */
 typedef struct qe_paged_cache {
     uint16_t* k;
     uint16_t* v;
@@ -550,7 +551,7 @@ typedef struct qe_paged_cache {
  * is the one new token of sequence s (num_tokens = num_seqs).  query_start does not
  * decrease.  num_tokens is the number of rows the buffers hold: rows of no sequence, and
  * those of sequences with a negative context_len, are neither read nor written (a batch
- * padded to a recorded size).  Each entry point says which rows of a cache it writes; two
+ * padded to a recorded size).  Positions stay below 2^31; at most 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
  * sequences may share pages that neither writes. */
 typedef struct qe_paged_batch {
     const int32_t* block_table; /* [num_seqs][max_pages] */
@@ -627,7 +628,8 @@ int qe_launch_attention_gqa_paged_decode(const uint16_t* q, const qe_paged_cache
 
 /* Chunks of new tokens, single ones among them: the counterpart of
  * qe_launch_attention_gqa_prefill.  The chunk's own K and V are in the cache.  An infinity or
- * NaN in V (which append stores as a NaN in K) of a position may reach rows up to 128 before it. */
+ * NaN in V (which append stores as a NaN in K) of a position may reach rows up to 62 before it
+ * and, with a window, rows of the chunk up to window + 255 behind it. */
 int qe_paged_prefill_workspace_bytes(int num_tokens, int num_q_heads, int num_kv_heads, size_t* bytes);
 int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
                                           void* workspace, uint16_t* attn_out, float* row_lse, hipStream_t stream,

@@ -252,6 +252,19 @@ __device__ __forceinline__ float row_log_sum(float m, float l) {
 __device__ __forceinline__ float part_weight(float m, float common) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - common);
 }
+__device__ __forceinline__ float xor32_max(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float xor16_max(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
 __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
     return make_uint2(static_cast<uint32_t>(f2h(a)) | static_cast<uint32_t>(f2h(b)) << 16,
                       static_cast<uint32_t>(f2h(c)) | static_cast<uint32_t>(f2h(d)) << 16);
@@ -399,6 +412,14 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
 // lane ends with dims 32 g .. 32 g + 31 of head c.  The softmax weights are rounded to fp16 for
 // the product with V (2^-11, as everywhere in this library's matrix-core attention); scores, sums
 // and outputs are fp32.
+//
+// Bound by memory: K and V are read once, 512 bytes a key and kv head.  The next tile's K is
+// requested as soon as this one's is in the matrix cores, and its V as soon as that is: 16 KB in
+// flight a wave, 128 KB a CU (8 waves with 2 a SIMD; with 4 waves a block and two blocks a CU the
+// merge has twice the parts and everything takes 5% longer).  V goes past the caches: 2% on the
+// long cases, and nothing where other tokens select the same blocks, which keep it.
+// 48 sequences of up to 4000 tokens (293 MB): 51 us, 5.7 TB/s, and 5.6 for the merge; one of
+// 131000 (134 MB): 24 and 5.3 us; one of 300: 7 and 5.3, of which 2 are the division of the work.
 constexpr int kDecWaves = 8;     // waves of a block
 constexpr int kDecBlocks = 256;  // of a launch: one a CU
 constexpr int kDecKeys = 32;     // keys of a tile
@@ -414,19 +435,6 @@ struct DecodeParams {
     void* ws;
     int nq, group, window, num_selected, coarse;
 };
-
-__device__ __forceinline__ float xor32_max(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    const uint32_t a = r[0], b = r[1];
-    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-}
-__device__ __forceinline__ float xor16_max(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t a = r[0], b = r[1];
-    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-}
 
 // The keys of a token, in tiles of 32: of the whole context or window (tile t: positions 32 t ..),
 // or of the list of selected blocks (tile t: entries from 32 t / page size on).
@@ -449,17 +457,207 @@ __device__ __forceinline__ DecodeRange decode_range(const DecodeParams& p, const
     return r;
 }
 
-template <bool SPARSE>
-__global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeParams p) {
-    constexpr int NW = kDecWaves, kPad = kPgDim + 4;
-    __shared__ float s_m[NW][kDecRows], s_l[NW][kDecRows];
-    __shared__ __align__(16) float s_o[NW][kDecRows][kPad];
+// Where the waves of a block meet: each row's reference value and sum, and its outputs.
+template <int WAVES>
+struct TokenShared {
+    float m[WAVES][kDecRows], l[WAVES][kDecRows];
+    __align__(16) float o[WAVES][kDecRows][kPgDim + 4];
+};
+
+// Up to 16 rows (lane (c, g): row c, with keys lo .. lim) of a kv head against tiles first .. end - 1 of a
+// sequence's keys, or of its list of blocks, the waves of the block a run each; store(row, dim, four
+// outputs, reference value, sum) for every row < live and every fourth dim.  KEEP: rows of V are read by others too.
+template <bool SPARSE, bool KEEP, int WAVES, class Store>
+__device__ __forceinline__ void token_rows(const PagedView& p, int seq, int h, const int32_t* list, int num_selected, int first,
+                                           int end, const f16x8 (&qf)[4], int lo, int lim, int live,
+                                           TokenShared<WAVES>& shared, Store store) {
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int c = lane & 15, g = lane >> 4;
+    const ptrdiff_t v_minus_k = reinterpret_cast<const char*>(p.v) - reinterpret_cast<const char*>(p.k);
+    // rows in the order of positions: the keys that all see, and those that any does
+    const int lo_all = __builtin_amdgcn_readlane(lo, live - 1), lo_any = __builtin_amdgcn_readlane(lo, 0);
+    const int lim_all = __builtin_amdgcn_readlane(lim, 0), lim_any = __builtin_amdgcn_readlane(lim, live - 1);
+    // this wave's run of tiles
+    const int a = first + static_cast<int>(static_cast<long long>(end - first) * wave / WAVES);
+    const int e = first + static_cast<int>(static_cast<long long>(end - first) * (wave + 1) / WAVES);
+    // 64 entries of the list or of the table from `base` on, one a lane: page and block number
+    int base = 0, page_l = -1, block_l = 0;
+    auto refill = [&](int entry) __attribute__((always_inline)) {
+        base = entry;
+        block_l = entry + lane;
+        if constexpr (SPARSE) block_l = block_l < num_selected ? list[block_l] : -1;
+        page_l = block_l >= 0 && block_l < p.max_pages && (block_l << p.shift) <= lim_any ? paged_page(p, seq, block_l) : -1;
+    };
+    struct Tile {
+        const char* k[2];  // of the first key of each half
+        int pos[2];        // its position
+        bool there[2];     // it has a page
+    };
+    auto tile_at = [&](int t) __attribute__((always_inline)) {
+        Tile x;
+        const int per_page = p.shift - 5;  // log2 of the tiles of a page, -1 for two pages a tile
+        const int entry = per_page >= 0 ? t >> per_page : 2 * t;
+        const int span = per_page >= 0 ? 1 : 2;
+        if (entry + span > base + 64) refill(entry);
+        const int in_page = per_page >= 0 ? (t & ((1 << per_page) - 1)) * kDecKeys : 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int at = entry - base + (span == 2 ? u : 0);
+            const int page = __builtin_amdgcn_readlane(page_l, at);
+            const int row0 = in_page + (span == 2 ? 0 : 16 * u);
+            x.there[u] = page >= 0;
+            x.pos[u] = (__builtin_amdgcn_readlane(block_l, at) << p.shift) + row0;
+            x.k[u] = reinterpret_cast<const char*>(p.k + static_cast<long long>(max(page, 0)) * p.page_stride +
+                                                   ((static_cast<long long>(h) << p.shift) + row0) * kPgDim);
+        }
+        return x;
+    };
+    const uint32_t k_off = static_cast<uint32_t>((4 * (c & 3) + (c >> 2)) * kPgDim * 2 + 16 * g);
+    const uint32_t v_off = static_cast<uint32_t>(g * kPgDim * 2 + 16 * c);
+    u32x4 kf[8], vf[8];
+    auto request_k = [&](const Tile& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kf[i] = *reinterpret_cast<const u32x4*>(x.k[i >> 2] + (k_off + 64 * (i & 3)));
+    };
+    auto request_v = [&](const Tile& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const u32x4* v = reinterpret_cast<const u32x4*>(x.k[i >> 2] + v_minus_k + (v_off + 4 * (i & 3) * kPgDim * 2));
+            vf[i] = KEEP ? *v : __builtin_nontemporal_load(v);
+        }
+    };
+    f32x4 acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = f32x4{};
+    float mref = -INFINITY, lsum = 0.0f;
+    bool any = false;
+    Tile cur{};
+    if (a < e) {
+        const int entry = p.shift >= 5 ? a >> (p.shift - 5) : 2 * a;
+        refill(entry);
+        cur = tile_at(a);
+        request_k(cur);
+        request_v(cur);
+    }
+    for (int t = a; t < e; ++t) {
+        f32x4 sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            sc[u] = f32x4{};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[4 * u + kk]), qf[kk], sc[u],
+                                                               0, 0, 0);
+        }
+        Tile nxt = cur;
+        if (t + 1 < e) {
+            nxt = tile_at(t + 1);
+            request_k(nxt);
+        }
+        // keys out of sight (and rows that are none): the weights are 0, but what lies in the rows may be anything
+        const bool plain = cur.there[0] && cur.there[1] && cur.pos[0] >= lo_all && cur.pos[0] + 15 <= lim_all &&
+                           cur.pos[1] >= lo_all && cur.pos[1] + 15 <= lim_all;
+        if (plain) {
+            any = true;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = cur.pos[u] + 4 * r + g;
+                    const bool seen = cur.there[u] && key >= lo && key <= lim;
+                    any = any || seen;
+                    sc[u][r] = seen ? sc[u][r] : -INFINITY;
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = cur.pos[i >> 2] + 4 * (i & 3) + g;
+                const bool seen = cur.there[i >> 2] && key >= lo_any && key <= lim_any;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) vf[i][d] = seen ? vf[i][d] : 0u;
+            }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
+        mx = xor32_max(xor16_max(mx)) * kPgScale;
+        const bool grow = mx > mref + kPgLag;
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+            const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
+            mref = grow ? mx : mref;
+            lsum *= alpha;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
+        }
+        const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
+        f16x8 pf;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 2][i & 3], kPgScale, neg));
+            lsum += w;
+            pf[i] = static_cast<_Float16>(w);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t take = j & 1 ? 0x07060302u : 0x05040100u;
+            u32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(vf[2 * i + 1][j >> 1], vf[2 * i][j >> 1], take);
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf, acc[j], 0, 0, 0);
+        }
+        if (t + 1 < e) request_v(nxt);
+        cur = nxt;
+    }
+    // the waves meet: each row's common reference value, then the sum of the rescaled outputs
+    lsum += __shfl_xor(lsum, 16);
+    lsum += __shfl_xor(lsum, 32);
+    // the row has had a key (all lanes ask: one that leaves early would answer the others with 0)
+    int some = any;
+    some |= __shfl_xor(some, 16);
+    some |= __shfl_xor(some, 32);
+    if (some != 0) mref = fmaxf(mref, kPgLowest);
+    if (g == 0) shared.m[wave][c] = mref, shared.l[wave][c] = lsum;
+    __syncthreads();
+    {
+        float m = shared.m[0][c];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, shared.m[w][c]);
+        const float f = part_weight(mref, m);
+        float* o = &shared.o[wave][c][32 * g];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // dims 32 g + 4 i .. + 3: r = i / 2, j = 4 (i % 2) ..
+            *reinterpret_cast<float4*>(o + 4 * i) =
+                make_float4(acc[4 * (i & 1)][i >> 1] * f, acc[4 * (i & 1) + 1][i >> 1] * f, acc[4 * (i & 1) + 2][i >> 1] * f,
+                            acc[4 * (i & 1) + 3][i >> 1] * f);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < live * (kPgDim / 4); i += 64 * WAVES) {
+        const int r = i / (kPgDim / 4), d = 4 * (i % (kPgDim / 4));
+        float m = shared.m[0][r], l = 0.0f;
+        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, shared.m[w][r]);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < WAVES; ++w) {
+            l += shared.m[w][r] == -INFINITY ? 0.0f : shared.l[w][r] * part_weight(shared.m[w][r], m);
+            const float4 x = *reinterpret_cast<const float4*>(&shared.o[w][r][d]);
+            o.x += x.x;
+            o.y += x.y;
+            o.z += x.z;
+            o.w += x.w;
+        }
+        store(r, d, o, m, l);
+    }
+    __syncthreads();  // the next segment writes shared.m
+}
+
+template <bool SPARSE>
+__global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeParams p) {
+    constexpr int NW = kDecWaves;
+    __shared__ TokenShared<NW> shared;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const Partials part = partials<kDecRows>(p.ws, kDecBlocks);
-    const int block = blockIdx.x;
     const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
-    const ptrdiff_t v_minus_k = reinterpret_cast<const char*>(p.c.v) - reinterpret_cast<const char*>(p.c.k);
 
     // On the line: each sequence has its token's heads; or one sequence has those of all rows, the heads of
     // a row behind each other (all alike: which rows have a token is seen when their turn comes).
@@ -484,192 +682,24 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
         const int live = min(kDecRows, p.group - rt * kDecRows);
         const int head0 = h * p.group + rt * kDecRows;
         f16x8 qf[4];
-        {
-            const uint16_t* q = p.q + (static_cast<size_t>(row) * p.nq + head0 + min(c, live - 1)) * kPgDim + 8 * g;
+        const uint16_t* q = p.q + (static_cast<size_t>(row) * p.nq + head0 + min(c, live - 1)) * kPgDim + 8 * g;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
-        }
-        // this wave's run of tiles
-        const int a = range.first_tile + t0 + static_cast<int>(static_cast<long long>(t1 - t0) * wave / NW);
-        const int e = range.first_tile + t0 + static_cast<int>(static_cast<long long>(t1 - t0) * (wave + 1) / NW);
+        for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
         const int* list = SPARSE ? p.selected + (static_cast<size_t>(row) * p.c.nkv + h) * p.num_selected : nullptr;
-        // 64 entries of the list or of the table from `base` on, one a lane: page and block number
-        int base = 0, page_l = -1, block_l = 0;
-        auto refill = [&](int entry) __attribute__((always_inline)) {
-            base = entry;
-            block_l = entry + lane;
-            if constexpr (SPARSE) block_l = block_l < p.num_selected ? list[block_l] : -1;
-            page_l = block_l >= 0 && block_l < p.c.max_pages && (block_l << p.c.shift) <= lim
-                         ? paged_page(p.c, seq, block_l) : -1;
-        };
-        struct Tile {
-            const char* k[2];  // of the first key of each half
-            int pos[2];        // its position
-            bool there[2];     // it has a page
-        };
-        auto tile_at = [&](int t) __attribute__((always_inline)) {
-            Tile x;
-            const int per_page = p.c.shift - 5;  // log2 of the tiles of a page, -1 for two pages a tile
-            const int entry = per_page >= 0 ? t >> per_page : 2 * t;
-            const int span = per_page >= 0 ? 1 : 2;
-            if (entry + span > base + 64) refill(entry);
-            const int in_page = per_page >= 0 ? (t & ((1 << per_page) - 1)) * kDecKeys : 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int at = entry - base + (span == 2 ? u : 0);
-                const int page = __builtin_amdgcn_readlane(page_l, at);
-                const int row0 = in_page + (span == 2 ? 0 : 16 * u);
-                x.there[u] = page >= 0;
-                x.pos[u] = (__builtin_amdgcn_readlane(block_l, at) << p.c.shift) + row0;
-                x.k[u] = reinterpret_cast<const char*>(p.c.k + static_cast<long long>(max(page, 0)) * p.c.page_stride +
-                                                       ((static_cast<long long>(h) << p.c.shift) + row0) * kPgDim);
-            }
-            return x;
-        };
-        const uint32_t k_off = static_cast<uint32_t>((4 * (c & 3) + (c >> 2)) * kPgDim * 2 + 16 * g);
-        const uint32_t v_off = static_cast<uint32_t>(g * kPgDim * 2 + 16 * c);
-        u32x4 kf[8], vf[8];
-        auto request_k = [&](const Tile& x) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) kf[i] = *reinterpret_cast<const u32x4*>(x.k[i >> 2] + (k_off + 64 * (i & 3)));
-        };
-        auto request_v = [&](const Tile& x) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // a row of V is read once by each wave: not kept, unless the rows of other tokens read it too
-                const u32x4* v = reinterpret_cast<const u32x4*>(x.k[i >> 2] + v_minus_k + (v_off + 4 * (i & 3) * kPgDim * 2));
-                vf[i] = SPARSE ? *v : __builtin_nontemporal_load(v);
-            }
-        };
-        f32x4 acc[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = f32x4{};
-        float mref = -INFINITY, lsum = 0.0f;
-        bool any = false;
-        Tile cur{};
-        if (a < e) {
-            const int entry = p.c.shift >= 5 ? a >> (p.c.shift - 5) : 2 * a;
-            refill(entry);
-            cur = tile_at(a);
-            request_k(cur);
-            request_v(cur);
-        }
-        for (int t = a; t < e; ++t) {
-            f32x4 sc[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                sc[u] = f32x4{};
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[4 * u + kk]), qf[kk], sc[u],
-                                                                   0, 0, 0);
-            }
-            Tile nxt = cur;
-            if (t + 1 < e) {
-                nxt = tile_at(t + 1);
-                request_k(nxt);
-            }
-            // keys out of sight (and rows that are none): the weights are 0, but what lies in the rows may be anything
-            const bool plain = cur.there[0] && cur.there[1] && cur.pos[0] >= lo && cur.pos[0] + 15 <= lim &&
-                               cur.pos[1] >= lo && cur.pos[1] + 15 <= lim;
-            if (plain) {
-                any = true;
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = cur.pos[u] + 4 * r + g;
-                        const bool seen = cur.there[u] && key >= lo && key <= lim;
-                        any = any || seen;
-                        sc[u][r] = seen ? sc[u][r] : -INFINITY;
-                    }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = cur.pos[i >> 2] + 4 * (i & 3) + g;
-                    const bool seen = cur.there[i >> 2] && key >= lo && key <= lim;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) vf[i][d] = seen ? vf[i][d] : 0u;
+        token_rows<SPARSE, SPARSE, NW>(
+            p.c, seq, h, list, p.num_selected, range.first_tile + t0, range.first_tile + t1, qf, lo, lim, live, shared,
+            [&](int r, int d, float4 o, float m, float l) __attribute__((always_inline)) {
+                if (slot < 0) {
+                    const float inv = row_inverse(m, l);
+                    const size_t at = static_cast<size_t>(row) * p.nq + head0 + r;
+                    *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                    if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
+                } else {
+                    const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * kDecRows + r;
+                    *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
+                    if (d == 0) part.ml[at] = make_float2(m, l);
                 }
-            }
-            float mx = sc[0][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
-            mx = xor32_max(xor16_max(mx)) * kPgScale;
-            const bool grow = mx > mref + kPgLag;
-            if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-                const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
-                mref = grow ? mx : mref;
-                lsum *= alpha;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
-            }
-            const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
-            f16x8 pf;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 2][i & 3], kPgScale, neg));
-                lsum += w;
-                pf[i] = static_cast<_Float16>(w);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t take = j & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(vf[2 * i + 1][j >> 1], vf[2 * i][j >> 1], take);
-                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf, acc[j], 0, 0, 0);
-            }
-            if (t + 1 < e) request_v(nxt);
-            cur = nxt;
-        }
-        // the waves meet: each row's common reference value, then the sum of the rescaled outputs
-        lsum += __shfl_xor(lsum, 16);
-        lsum += __shfl_xor(lsum, 32);
-        if (__builtin_amdgcn_ballot_w64(any) != 0) mref = fmaxf(mref, kPgLowest);
-        if (g == 0) s_m[wave][c] = mref, s_l[wave][c] = lsum;
-        __syncthreads();
-        {
-            float m = s_m[0][c];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][c]);
-            const float f = part_weight(mref, m);
-            float* o = &s_o[wave][c][32 * g];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)  // dims 32 g + 4 i .. + 3: r = i / 2, j = 4 (i % 2) ..
-                *reinterpret_cast<float4*>(o + 4 * i) =
-                    make_float4(acc[4 * (i & 1)][i >> 1] * f, acc[4 * (i & 1) + 1][i >> 1] * f,
-                                acc[4 * (i & 1) + 2][i >> 1] * f, acc[4 * (i & 1) + 3][i >> 1] * f);
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < kDecRows * kPgDim / 4; i += 64 * NW) {
-            const int r = i / (kPgDim / 4), d = 4 * (i % (kPgDim / 4));
-            if (r >= live) continue;
-            float m = s_m[0][r], l = 0.0f;
-            for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][r]);
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int w = 0; w < NW; ++w) {
-                l += s_m[w][r] == -INFINITY ? 0.0f : s_l[w][r] * part_weight(s_m[w][r], m);
-                const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
-                o.x += x.x;
-                o.y += x.y;
-                o.z += x.z;
-                o.w += x.w;
-            }
-            if (slot < 0) {
-                const float inv = row_inverse(m, l);
-                const size_t at = static_cast<size_t>(row) * p.nq + head0 + r;
-                *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
-            } else {
-                const size_t at = static_cast<size_t>(2 * block + slot) * kDecRows + r;
-                *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
-                if (d == 0) part.ml[at] = make_float2(m, l);
-            }
-        }
-        __syncthreads();  // the next segment writes s_m
+            });
     };
     auto rows = [&](const PagedSeq&, int head, int rt) __attribute__((always_inline)) {
         if constexpr (SPARSE) {
@@ -680,8 +710,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
         }
         return min(kDecRows, p.group - rt * kDecRows);
     };
-    for_share<SPARSE>(p.c, block, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
-        if (threadIdx.x == 0) part.cuts[block] = cut;
+    for_share<SPARSE>(p.c, blockIdx.x, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
+        if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
     });
 }
 
@@ -697,9 +727,9 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // ---- chunks -----------------------------------------------------------------------
 // Causal attention of the rows of many sequences.  The q heads of a kv head and a
 // sequence's new tokens form one list of rows, row r = token r / group, head kvh *
-// group + r % group; a segment is 128 of them (32 a wave), whatever the group.  The
-// waves share tiles of 64 keys in LDS, filled from the pages by DMA a step ahead of
-// their use.  v_mfma_f32_32x32x16_f16 with the rows as columns:
+// group + r % group; a segment is 32 of them for each wave of a block, whatever the group.  The
+// waves share the keys in LDS, in halves of 32, filled from the pages by DMA.
+// v_mfma_f32_32x32x16_f16 with the rows as columns:
 //   S^T (32 keys x 32 rows) = K . Q^T: lane l holds key l % 32 and row l % 32, dims 8 (l / 32) +
 //   16 kk; Q stays in registers; the result has lane l = row l % 32 with the keys
 //   8 (v / 4) + 4 (l / 32) + v % 4, so a row's maximum and sum are in-lane and one swap;
@@ -710,6 +740,21 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // Rows that no one may see (behind the sequence's end, before every window, of missing
 // pages) are filled from a row of zeros: their weights are 0, and what lies there may be
 // anything.
+//
+// Bound by the matrix cores where rows are many (4 * 128 operations a row and key): a wave's
+// stage is 16 MFMAs (32 cycles each) and the scores of half t + 1, the weights of half t and the outputs
+// of half t - 1, which do not depend on each other and share the issue slots MFMA by MFMA.
+// Between two barriers lie 4 such stages, and a CU holds one block of 8 waves with a ring of 8 halves of
+// K and V (128 KB): a segment of 256 rows reads each key once, and the waves drift apart and fill each
+// other's gaps.  Rows that are few for their sequences (num_tokens * group < 512 num_seqs) take two
+// blocks of 4 waves a CU, with 2 stages and rings of 4 halves: segments of 128 rows, half the waste on short
+// ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 205 us (920
+// TF) before the chip lowers its clock and 215 - 245 after, with 4 waves 275; a mixed batch of 43
+// sequences: 54 us, with 8 waves 76; 17 tokens at 1200: 14 us, with 8 waves 17.
+//
+// A sequence with up to 16 rows of a kv head (single tokens beside the chunks, drafts) is attended as in
+// the section above, each wave on keys of its own: a tile of 128 rows would be mostly empty.  It counts half
+// on the line (59 us for the mixed batch where such rows fill tiles, 54 so; 66 where they count whole, 67 where a quarter).
 constexpr int kPfKeys = 64;           // keys of a tile: what shares are cut between
 constexpr int kPfHalf = 32;           // keys of a stage
 constexpr int kPfHalfBytes = kPfHalf * kPgDim * 2;
@@ -759,12 +804,14 @@ __device__ __forceinline__ int weight_of(const PrefillParams& p, int keys) {
     return static_cast<int>(max(1LL, min(w, 1LL << 29)));
 }
 
-// ONE: pages of 32 tokens and more (a half tile lies in one page).
-template <bool ONE, int WAVES>
+// ONE: pages of 32 tokens and more (a half tile lies in one page).  FEW: sequences of few rows may be there (a
+// kernel that knows of none starts 3 us sooner: 17 tokens at 1200 14 us instead of 17).
+template <bool ONE, int WAVES, bool FEW>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillParams p) {
     typedef PrefillShape<WAVES> Shape;
     constexpr int kRows = Shape::rows, kBlocks = Shape::blocks, P = Shape::period, R = Shape::ring;
     __shared__ __align__(256) char smem[2 * R * kPfHalfBytes];  // the last R halves of K, of V
+    static_assert(sizeof(TokenShared<WAVES>) <= sizeof(smem), "segments of few rows meet there");
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int fr = lane & 31, h = lane >> 5;
     // blocks of one XCD take neighbouring shares: they read the same pages
@@ -772,54 +819,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
     const Partials part = partials<kRows>(p.ws, kBlocks);
     constexpr int NP = ONE ? 1 : 2;             // pages of a half tile, at most
 
-    const uint32_t lds0 =
-        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)smem));
-    // A wave loads whole halves, by eight loads of four rows: load i its rows 4 i + lane / 16, stored chunk lane % 16,
-    // i.e. chunk (lane % 16) ^ swz(row) of memory.  The first four lanes' offsets (the others are 16 rows on):
-    uint32_t loff[4];  // bytes
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        loff[i] = static_cast<uint32_t>((4 * i + (lane >> 4)) * (2 * kPgDim) + 16 * ((lane & 15) ^ (((lane >> 4) << 2) | i)));
-    // LDS addresses: K chunk 2 kk + h of key fr; V^T reads (dt: 32 dims, u: keys + 8)
-    uint32_t ka[8], va[4][2];
-    {
-        const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
-        const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
-        const int s16 = lane & 15, b16 = (lane >> 4) & 1;
-        const uint32_t v0 = lds0 + (R + P) * kPfHalfBytes + (4 * h + (s16 >> 2)) * 256 +
-                            16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-            va[dt][0] = v0 ^ (64 * dt);
-            va[dt][1] = (v0 ^ (64 * dt) ^ 32) + 8 * 256;
-        }
-    }
-    // The ring is two frames of P slots, and these addresses are of one of them: of K's first at first, of V's second.
-    int k_turn = P * kPfHalfBytes, v_turn = -P * kPfHalfBytes;
-    auto turn_k = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) ka[kk] += k_turn;
-        k_turn = -k_turn;
-    };
-    auto turn_v = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) va[dt][0] += v_turn, va[dt][1] += v_turn;
-        v_turn = -v_turn;
-    };
-    // K operand of MFMA i of the half in the frame's `slot`: dims 16 i; V^T operand: 16-key quarter i / 4, dims 32 (i % 4)
-    auto read_k = [&](int slot, int i) __attribute__((always_inline)) {
-        typedef const __attribute__((address_space(3))) f16x8* lptr;
-        return *reinterpret_cast<lptr>(ka[i] + slot * kPfHalfBytes);
-    };
-    auto read_v = [&](int slot, int i) __attribute__((always_inline)) {
-        typedef __attribute__((address_space(3))) s16x4* lptr;
-        const uint32_t off = slot * kPfHalfBytes + (i >> 2) * 16 * 256;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][0] + off));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][1] + off));
-        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
     // every tile requested so far is in LDS, for every wave, and what was read before is read
     auto tile_barrier = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -835,6 +834,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         static_assert(1 << kStep == kRows, "the weight of a row tile's own tokens");
         SeqWork w{weight_of(p, s.ctx), max(kStep - p.coarse, -1), weight_of(p, p.c.capacity()), (s.n * g + kRows - 1) / kRows, p.c.nkv};
         if (p.window > 0) w.most = min(w.most, weight_of(p, min(p.window, p.c.capacity()) + kRows / g + kPfKeys));
+        if (FEW && s.n * g <= kDecRows) {  // half: as measured
+            w.first = (w.first + 1) / 2;
+            w.most = (w.most + 1) / 2;
+        }
         return w;
     };
     auto tiles = [&](const PagedSeq& s, int rt) __attribute__((always_inline)) { return prefill_range<WAVES>(p, s, rt).tiles; };
@@ -843,6 +846,80 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         const PrefillRange range = prefill_range<WAVES>(p, s, rt);
         const int rows = uniform(range.rows), first_tile = uniform(range.first_tile), low = uniform(range.low);
         const int it0 = first_tile + t0, it1 = first_tile + t1;
+        if (FEW && rows <= kDecRows) {  // as single tokens are attended: each wave keys of its own, no rows to share them
+            const int c = lane & 15, rc = min(c, rows - 1), qi = rc / p.group, qh = kvh * p.group + rc - qi * p.group;
+            const int pos = s.ctx + qi, lim = min(pos, p.c.capacity() - 1), lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            const uint16_t* q = p.q + (static_cast<size_t>(s.first + qi) * p.nq + qh) * kPgDim + 8 * (lane >> 4);
+            f16x8 qf[4];
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
+            // (the last tile's second half may lie behind the last key)
+            const int end = min(2 * it1, __builtin_amdgcn_readlane(lim, rows - 1) / kPfHalf + 1);
+            token_rows<false, false, WAVES>(
+                p.c, seq, kvh, nullptr, 0, 2 * it0, max(end, 2 * it0), qf, lo, lim, rows, *reinterpret_cast<TokenShared<WAVES>*>(smem),
+                [&](int r, int d, float4 o, float m, float l) __attribute__((always_inline)) {
+                    const int token = r / p.group;
+                    if (slot < 0) {
+                        const float inv = row_inverse(m, l);
+                        const size_t at = static_cast<size_t>(s.first + token) * p.nq + kvh * p.group + r - token * p.group;
+                        *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                        if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
+                    } else {
+                        const size_t at = static_cast<size_t>(2 * block + slot) * kRows + r;
+                        *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
+                        if (d == 0) part.ml[at] = make_float2(m, l);
+                    }
+                });
+            return;
+        }
+        const uint32_t lds0 =
+            static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)smem));
+        // A wave loads whole halves, by eight loads of four rows: load i its rows 4 i + lane / 16, stored chunk lane % 16,
+        // i.e. chunk (lane % 16) ^ swz(row) of memory.  The first four lanes' offsets (the others are 16 rows on):
+        uint32_t loff[4];  // bytes
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            loff[i] = static_cast<uint32_t>((4 * i + (lane >> 4)) * (2 * kPgDim) + 16 * ((lane & 15) ^ (((lane >> 4) << 2) | i)));
+        // LDS addresses: K chunk 2 kk + h of key fr; V^T reads (dt: 32 dims, u: keys + 8)
+        uint32_t ka[8], va[4][2];
+        {
+            const int swz_k = ((fr & 3) << 2) | ((fr >> 2) & 3);
+            const uint32_t k0 = lds0 + fr * 256 + 16 * (h ^ swz_k);
+            const int s16 = lane & 15, b16 = (lane >> 4) & 1;
+            const uint32_t v0 = lds0 + (R + P) * kPfHalfBytes + (4 * h + (s16 >> 2)) * 256 +
+                                16 * ((2 * b16 + ((s16 & 3) >> 1)) ^ (((s16 >> 2) << 2) | h)) + 8 * (s16 & 1);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) ka[kk] = k0 ^ (32 * kk);
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                va[dt][0] = v0 ^ (64 * dt);
+                va[dt][1] = (v0 ^ (64 * dt) ^ 32) + 8 * 256;
+            }
+        }
+        // The ring is two frames of P slots, and these addresses are of one of them: of K's first at first, of V's second.
+        int k_turn = P * kPfHalfBytes, v_turn = -P * kPfHalfBytes;
+        auto turn_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) ka[kk] += k_turn;
+            k_turn = -k_turn;
+        };
+        auto turn_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) va[dt][0] += v_turn, va[dt][1] += v_turn;
+            v_turn = -v_turn;
+        };
+        // K operand of MFMA i of the half in the frame's `slot`: dims 16 i; V^T operand: 16-key quarter i / 4, dims 32 (i % 4)
+        auto read_k = [&](int slot, int i) __attribute__((always_inline)) {
+            typedef const __attribute__((address_space(3))) f16x8* lptr;
+            return *reinterpret_cast<lptr>(ka[i] + slot * kPfHalfBytes);
+        };
+        auto read_v = [&](int slot, int i) __attribute__((always_inline)) {
+            typedef __attribute__((address_space(3))) s16x4* lptr;
+            const uint32_t off = slot * kPfHalfBytes + (i >> 2) * 16 * 256;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][0] + off));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lptr>(va[i & 3][1] + off));
+            return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
         const int r = rt * kRows + wave * 32 + fr;
         const int rc = min(r, rows - 1);
         const int qi = rc / p.group, qh = kvh * p.group + rc - qi * p.group;
@@ -1000,8 +1077,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         // Stage t: the scores of half t + 1 (nxt) and the outputs of half t - 1 (weights pp) beside the weights of
         // half t (scores cur, weights pc).  ks, vs: slots of K t + 1 and V t - 1; f: the first operands of K t + 1,
         // then those of K t + 2 in slot `then` (-1: not there yet); mx: the lane's part of the maximum of cur, then of
-        // nxt; parts: the first of the four parts of `job` that the stage asks for.  Each MFMA is fenced together with its share of the vector work: left alone, the scheduler puts
-        // all of the one before all of the other.
+        // nxt; parts: the first of the four parts of `job` that the stage asks for.  Each MFMA is fenced
+        // together with its share of the vector work: left alone, the scheduler puts all of the one before all of
+        // the other.
         constexpr int AHEAD = 4;  // operand reads in flight before their MFMA
         f16x8 f[AHEAD];
         // In the P stages from t on K of the halves t + P + 1 .. t + 2 P and V of t + P - 1 .. t + 2 P - 2 come in, a
@@ -1134,12 +1212,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                 }
                 tile_barrier();
             }
-            // the addresses as they were at first
-            if (k_turn < 0) turn_k();
-            if (v_turn > 0) turn_v();
         }
         lsum += __shfl_xor(lsum, 32);
-        if (any || __shfl_xor(static_cast<int>(any), 32) != 0) mref = fmaxf(mref, kPgLowest);
+        const int other_any = __shfl_xor(static_cast<int>(any), 32);  // (asked by all lanes)
+        if (any || other_any != 0) mref = fmaxf(mref, kPgLowest);
         if (r < rows) {
             if (slot < 0) {
                 const float inv = row_inverse(mref, lsum);
@@ -1259,10 +1335,10 @@ int launch_prefill(PrefillParams p, const qe_paged_batch* batch, const qe_paged_
         QE_REQUIRE(most >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens, cache->num_kv_heads);
         ++p.coarse;
     }
-    if (p.c.shift >= 5)
-        paged_prefill_kernel<true, WAVES><<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
-    else
-        paged_prefill_kernel<false, WAVES><<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
+    const bool one = p.c.shift >= 5, few = batch->num_seqs > 1 || batch->num_tokens * p.group <= kDecRows;
+    auto* kernel = one ? few ? paged_prefill_kernel<true, WAVES, true> : paged_prefill_kernel<true, WAVES, false>
+                       : few ? paged_prefill_kernel<false, WAVES, true> : paged_prefill_kernel<false, WAVES, false>;
+    kernel<<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
     const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, Shape::blocks) * (Shape::rows / 8);
     paged_prefill_merge_kernel<WAVES><<<static_cast<unsigned>(std::min(items, 2048LL)), 256, 0, stream>>>(p);
     return QE_OK;

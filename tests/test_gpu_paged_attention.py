@@ -98,6 +98,23 @@ def test_chunks(qe, form, lens, page, nq, nkv, window):
     _try(qe, form, w, window)
 
 
+FEW_ROWS = [
+    ([(1500, 4), (2222, 5), (31, 3), (0, 4), (777, 1)], 16, 8, 2, 0),
+    ([(1500, 2), (2222, 5), (31, 3), (0, 1), (777, 16)], 64, 3, 3, 50),
+    ([(3000, 2), (1777, 600)], 32, 4, 2, 0),
+    ([(2500, 2), (900, 600)], 16, 4, 2, 700),
+    ([(5000, 2)], 32, 6, 1, 0),
+    ([(640, 16), (639, 15)], 128, 2, 2, 0),
+]
+
+
+@pytest.mark.parametrize("lens,page,nq,nkv,window", FEW_ROWS)
+def test_few_rows_beside_chunks(qe, lens, page, nq, nkv, window):
+    """Sequences of up to 16 rows of a kv head (15, 16, 17, ...), alone and beside longer ones."""
+    w = World(np.random.default_rng(page + nq + window), lens, page, nq, nkv, pad_rows=2, single=False)
+    _try(qe, "prefill", w, window)
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_many_short_sequences(qe, form):
     """Several segments a block, and more than one round of the search for a row's sequence."""
@@ -202,6 +219,20 @@ def test_every_score_minus_infinity(qe, form):
     want = w.attention(q)
     out[-1, 4], lse[-1, 4] = want[0][-1, 4], want[2][-1, 4]
     check(out, lse, want, -7)
+
+
+@pytest.mark.parametrize("form", ("decode", "prefill"))
+@pytest.mark.parametrize("nq", [2, 40])
+def test_the_only_key_scores_minus_infinity(qe, form, nq):
+    """A window of one key, wherever it lies among the lanes: NaN, as for any row whose every score is -inf."""
+    w = World(np.random.default_rng(24), [(i, 1) for i in range(40)], 16, nq, 1, pad_rows=0)
+    for s in range(40):
+        w.k[s] = np.abs(w.k[s]) + np.float16(0.1)
+        w.store(s)
+    q = w.queries()
+    q[:, :, 9] = -np.inf
+    out, lse = attend(qe, form, w, q, window=1)
+    assert np.isnan(out).all() and np.isneginf(lse).all()
 
 
 @pytest.mark.parametrize("form", FORMS)

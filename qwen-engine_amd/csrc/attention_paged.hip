@@ -651,11 +651,68 @@ __device__ __forceinline__ void token_rows(const PagedView& p, int seq, int h, c
     __syncthreads();  // the next segment writes shared.m
 }
 
+// The sequence of a row of a list; -1: the row is of none.
+__device__ __forceinline__ int seq_of_listed_row(const PagedView& p, int row, PagedSeq& s) {
+    const int seq = uniform(paged_seq_of_row(p, row));
+    if (seq < 0) return -1;
+    s = paged_seq(p, seq);
+    return row < s.first || row >= s.first + s.n ? -1 : seq;
+}
+
+// Tiles t0 .. t1 - 1 of a segment, into the output (at < 0) or into the partials from row `at` on.
+template <bool SPARSE, int WAVES>
+__device__ __forceinline__ void token_segment(const DecodeParams& p, const PagedSeq& s, int seq, int row, int h, int rt, int t0,
+                                              int t1, long long at, const Partials& part, TokenShared<WAVES>& shared) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const DecodeRange range = decode_range<SPARSE>(p, s, row);
+    const int live = min(kDecRows, p.group - rt * kDecRows);
+    const int head0 = h * p.group + rt * kDecRows;
+    f16x8 qf[4];
+    const uint16_t* q = p.q + (static_cast<size_t>(row) * p.nq + head0 + min(c, live - 1)) * kPgDim + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
+    const int* list = SPARSE ? p.selected + (static_cast<size_t>(row) * p.c.nkv + h) * p.num_selected : nullptr;
+    token_rows<SPARSE, SPARSE, WAVES>(
+        p.c, seq, h, list, p.num_selected, range.first_tile + t0, range.first_tile + t1, qf, uniform(range.lo), uniform(range.lim),
+        live, shared, [&](int r, int d, float4 o, float m, float l) __attribute__((always_inline)) {
+            if (at < 0) {
+                const float inv = row_inverse(m, l);
+                const size_t to = static_cast<size_t>(row) * p.nq + head0 + r;
+                *reinterpret_cast<uint2*>(p.out + to * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                if (p.lse != nullptr && d == 0) p.lse[to] = row_log_sum(m, l);
+            } else {
+                *reinterpret_cast<float4*>(part.o + (at + r) * kPgDim + d) = o;
+                if (d == 0) part.ml[at + r] = make_float2(m, l);
+            }
+        });
+}
+
+// A block for each segment, and nothing to merge: where no row has more than kShortKeys keys, or where there
+// are kManySegments and none is far longer than the others (lists are all alike; single tokens of up to twice
+// as many keys).  Blocks of 4 waves, three of them a CU.  (us, with the merge, shares against this: 1 token on
+// 300 keys 13.0 and 7.2, on 1000 14.8 and 12.8, on 2000 15.3 and 21.8; 200 on 1 to 2000 53.6 and 39.5; 400 lists of
+// 2048 keys 84 and 72, 200 of 4096 82 and 65, 128 of 4096 54 and 64.  With 8 waves a block: 7.8, 14.1, ... 75.)
+constexpr int kShortWaves = 4, kShortKeys = 1024, kManySegments = 192;
+template <bool SPARSE>
+__global__ __launch_bounds__(64 * kShortWaves, 3) void paged_short_kernel(DecodeParams p) {
+    __shared__ TokenShared<kShortWaves> shared;
+    const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
+    const int of_row = p.c.nkv * row_tiles, row = blockIdx.x / of_row, h = (blockIdx.x - row * of_row) / row_tiles;
+    PagedSeq s;
+    int seq = row;
+    if constexpr (SPARSE) {
+        seq = seq_of_listed_row(p.c, row, s);
+        if (seq < 0) return;
+    } else {
+        s = paged_seq(p.c, seq);
+        if (s.n == 0) return;
+    }
+    token_segment<SPARSE>(p, s, seq, row, h, blockIdx.x % row_tiles, 0, decode_range<SPARSE>(p, s, row).tiles, -1, Partials{}, shared);
+}
+
 template <bool SPARSE>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeParams p) {
-    constexpr int NW = kDecWaves;
-    __shared__ TokenShared<NW> shared;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    __shared__ TokenShared<kDecWaves> shared;
     const Partials part = partials<kDecRows>(p.ws, kDecBlocks);
     const int row_tiles = (p.group + kDecRows - 1) / kDecRows;
 
@@ -670,47 +727,19 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void paged_decode_kernel(DecodeP
 
     auto body = [&](int item, PagedSeq s, int head, int rt, int t0, int t1, int slot) __attribute__((always_inline)) {
         const int row = SPARSE ? head / p.c.nkv : s.first, h = SPARSE ? head - row * p.c.nkv : head;
-        int seq = item;
-        if constexpr (SPARSE) {
-            seq = uniform(paged_seq_of_row(p.c, row));
-            if (seq < 0) return;
-            s = paged_seq(p.c, seq);
-            if (row < s.first || row >= s.first + s.n) return;  // a row of no sequence: not written
-        }
-        const DecodeRange range = decode_range<SPARSE>(p, s, row);
-        const int lim = uniform(range.lim), lo = uniform(range.lo);
-        const int live = min(kDecRows, p.group - rt * kDecRows);
-        const int head0 = h * p.group + rt * kDecRows;
-        f16x8 qf[4];
-        const uint16_t* q = p.q + (static_cast<size_t>(row) * p.nq + head0 + min(c, live - 1)) * kPgDim + 8 * g;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const f16x8*>(q + 32 * kk);
-        const int* list = SPARSE ? p.selected + (static_cast<size_t>(row) * p.c.nkv + h) * p.num_selected : nullptr;
-        token_rows<SPARSE, SPARSE, NW>(
-            p.c, seq, h, list, p.num_selected, range.first_tile + t0, range.first_tile + t1, qf, lo, lim, live, shared,
-            [&](int r, int d, float4 o, float m, float l) __attribute__((always_inline)) {
-                if (slot < 0) {
-                    const float inv = row_inverse(m, l);
-                    const size_t at = static_cast<size_t>(row) * p.nq + head0 + r;
-                    *reinterpret_cast<uint2*>(p.out + at * kPgDim + d) = pack4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-                    if (p.lse != nullptr && d == 0) p.lse[at] = row_log_sum(m, l);
-                } else {
-                    const size_t at = static_cast<size_t>(2 * blockIdx.x + slot) * kDecRows + r;
-                    *reinterpret_cast<float4*>(part.o + at * kPgDim + d) = o;
-                    if (d == 0) part.ml[at] = make_float2(m, l);
-                }
-            });
+        const int seq = SPARSE ? seq_of_listed_row(p.c, row, s) : item;
+        if (SPARSE && seq < 0) return;  // not written
+        token_segment<SPARSE>(p, s, seq, row, h, rt, t0, t1, slot < 0 ? -1 : static_cast<long long>(2 * blockIdx.x + slot) * kDecRows,
+                              part, shared);
     };
     auto rows = [&](const PagedSeq&, int head, int rt) __attribute__((always_inline)) {
         if constexpr (SPARSE) {
-            const int row = head / p.c.nkv, seq = paged_seq_of_row(p.c, row);
-            if (seq < 0) return 0;
-            const PagedSeq s = paged_seq(p.c, seq);
-            if (row < s.first || row >= s.first + s.n) return 0;
+            PagedSeq s;
+            if (seq_of_listed_row(p.c, head / p.c.nkv, s) < 0) return 0;
         }
         return min(kDecRows, p.group - rt * kDecRows);
     };
-    for_share<SPARSE>(p.c, blockIdx.x, kDecBlocks, (NW >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
+    for_share<SPARSE>(p.c, blockIdx.x, kDecBlocks, (kDecWaves >> p.coarse) + kDecOver, work, tiles, rows, body, [&](SegmentCut cut) {
         if (threadIdx.x == 0) part.cuts[blockIdx.x] = cut;
     });
 }
@@ -1304,6 +1333,11 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
     const long long most = SPARSE ? static_cast<long long>(num_selected) * cache->page_size
                                   : static_cast<long long>(batch->max_pages) * cache->page_size;
     const long long segments = row_tiles * cache->num_kv_heads * batch->num_tokens;
+    const long long keys = window > 0 ? std::min<long long>(window, most) : most;
+    if ((keys <= kShortKeys || (segments >= kManySegments && (SPARSE || keys <= 2 * kShortKeys))) && segments <= INT32_MAX) {
+        paged_short_kernel<SPARSE><<<static_cast<unsigned>(segments), 64 * kShortWaves, 0, stream>>>(p);
+        return check_launch(what);
+    }
     while (segments * (((most / kDecKeys + 1) >> p.coarse) + kDecOver) >= (1 << 30)) {
         QE_REQUIRE(most / kDecKeys >> p.coarse > 0, "%s: num_tokens=%d with %d kv heads", what, batch->num_tokens,
                    cache->num_kv_heads);

@@ -73,6 +73,22 @@ def test_single_tokens(qe, form, lens, page, nq, nkv, window):
     _try(qe, form, World(np.random.default_rng(page + nq), lens, page, nq, nkv, joint=nq == 12), window)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("lens,page,nq,nkv,window", SINGLE[:8])
+def test_single_tokens_on_a_wide_table(qe, form, lens, page, nq, nkv, window):
+    """Tables for more keys than there are: the work is divided by the lengths, where narrow ones have a block for each row."""
+    _try(qe, form, World(np.random.default_rng(page + nq), lens, page, nq, nkv, spare=2200 // page, joint=nq == 12), window)
+
+
+@pytest.mark.parametrize("lens", [300, 190, [(2000, 1)] + 200 * [(3, 1)]])
+def test_many_sequences_on_a_wide_table(qe, lens):
+    rng = np.random.default_rng(6)
+    lens = [(int(a), 1) for a in rng.integers(-1, 400, lens)] if isinstance(lens, int) else lens
+    for page in (16, 64):
+        for window in (0, 100):
+            _try(qe, "decode", World(rng, lens, page, 3, 1, spare=2200 // page), window)
+
+
 CHUNKS = [
     ([(0, 2)], 16, 12, 2, 0),
     ([(0, 200)], 64, 12, 2, 0),

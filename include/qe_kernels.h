@@ -550,8 +550,8 @@ typedef struct qe_paged_cache {
  * sequence s, at positions context_len[s], context_len[s] + 1, ...; query_start NULL: row s
  * is the one new token of sequence s (num_tokens = num_seqs).  query_start does not
  * decrease.  num_tokens is the number of rows the buffers hold: rows of no sequence, and
- * those of sequences with a negative context_len, are neither read nor written (a batch
- * padded to a recorded size).  Positions stay below 2^31; at most 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
+ * those of sequences with a negative context_len, are not written, and what they hold does
+ * not matter (a batch padded to a recorded size).  Positions stay below 2^31; at most 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
  * sequences may share pages that neither writes. */
 typedef struct qe_paged_batch {
     const int32_t* block_table; /* [num_seqs][max_pages] */

@@ -48,15 +48,21 @@ struct AppendParams {
     float scale, eps;
 };
 
-__device__ __forceinline__ void load8(const uint16_t* p, const uint16_t* bias, float (&o)[8]) {
-    const f16x8 a = *reinterpret_cast<const f16x8*>(p);
+__device__ __forceinline__ f16x8 eight(const uint16_t* p) { return *reinterpret_cast<const f16x8*>(p); }
+__device__ __forceinline__ void widen(const f16x8& a, float (&o)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(a[e]);
-    if (bias != nullptr) {
-        const f16x8 c = *reinterpret_cast<const f16x8*>(bias);
+}
+// x += b, x *= r * g: where there are some
+__device__ __forceinline__ void add8(bool some, const f16x8& b, float (&x)[8]) {
+    if (!some) return;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] += static_cast<float>(c[e]);
-    }
+    for (int e = 0; e < 8; ++e) x[e] += static_cast<float>(b[e]);
+}
+__device__ __forceinline__ void scale8(bool some, const f16x8& g, float r, float (&x)[8]) {
+    if (!some) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= r * static_cast<float>(g[e]);
 }
 __device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
     f16x8 a;
@@ -67,42 +73,61 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
 
 __global__ __launch_bounds__(256) void qkv_norm_rope_paged_append_kernel(AppendParams p) {
     __shared__ float s_sin[kPgDim / 2], s_cos[kPgDim / 2];
-    const int t = blockIdx.x, j = threadIdx.x & 15;
+    const int t = blockIdx.x, j = threadIdx.x & 15, d = 8 * j, half = p.rot / 2;
     const int head = blockIdx.y * 16 + (threadIdx.x >> 4);
+    const bool there = head < p.nq + p.c.nkv;  // whole rows of 16 lanes
+    const bool is_k = head >= p.nq;
+    const int h = is_k ? head - p.nq : head;
+    const int pd = d < half ? d + half : d - half;  // the partners of a rotation in halves
+    const bool partner = d < p.rot && !p.interleaved;
+    const uint16_t* bias = is_k ? p.kb : p.qb;
+    const uint16_t* norm = is_k ? p.kn : p.qn;
+    // all that a row's place in memory gives is asked for before its place in the batch is known
+    f16x8 x8, y8, v8, bx, by, bv, gx, gy;
+    if (there) {
+        const uint16_t* src = (is_k ? p.k + t * p.kv_stride : p.q + t * p.q_stride) + h * kPgDim;
+        x8 = eight(src + d);
+        if (partner) y8 = eight(src + pd);
+        if (is_k) {
+            v8 = eight(p.v + t * p.kv_stride + h * kPgDim + d);
+            if (p.vb != nullptr) bv = eight(p.vb + h * kPgDim + d);
+        }
+        if (bias != nullptr) {
+            bx = eight(bias + h * kPgDim + d);
+            if (partner) by = eight(bias + h * kPgDim + pd);
+        }
+        if (norm != nullptr) {
+            gx = eight(norm + d);
+            if (partner) gy = eight(norm + pd);
+        }
+    }
+    const double turns = static_cast<int>(threadIdx.x) < half ? p.turns[threadIdx.x] : 0.0;
     const int seq = paged_seq_of_row(p.c, t);
     if (seq < 0) return;
     const PagedSeq s = paged_seq(p.c, seq);
     if (t < s.first || t >= s.first + s.n) return;
     const int pos = s.ctx + t - s.first;
-    const int half = p.rot / 2;
     if (static_cast<int>(threadIdx.x) < half) {
-        const double a = static_cast<double>(pos) * p.turns[threadIdx.x];
+        const double a = static_cast<double>(pos) * turns;
         float sn, cs;
         sincospif(2.0f * static_cast<float>(a - rint(a)), &sn, &cs);
         s_sin[threadIdx.x] = sn * p.scale;
         s_cos[threadIdx.x] = cs * p.scale;
     }
+    const int page = is_k && there ? paged_page(p.c, seq, pos >> p.c.shift) : -1;
     __syncthreads();
-    if (head >= p.nq + p.c.nkv) return;  // whole rows of 16 lanes
-    const bool is_k = head >= p.nq;
-    const int h = is_k ? head - p.nq : head;
-    const uint16_t* src = (is_k ? p.k + t * p.kv_stride : p.q + t * p.q_stride) + h * kPgDim;
-    const uint16_t* bias = is_k ? p.kb : p.qb;
-    if (bias != nullptr) bias += h * kPgDim;
-    const uint16_t* norm = is_k ? p.kn : p.qn;
-    const int d = 8 * j;
+    if (!there) return;
     float x[8];
-    load8(src + d, bias != nullptr ? bias + d : nullptr, x);
+    widen(x8, x);
+    add8(bias != nullptr, bx, x);
     float r = 1.0f;
     if (norm != nullptr) {
         float ss = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
         r = 1.0f / sqrtf(row16_sum(ss) * (1.0f / kPgDim) + p.eps);
-        const f16x8 g = *reinterpret_cast<const f16x8*>(norm + d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= r * static_cast<float>(g[e]);
     }
+    scale8(norm != nullptr, gx, r, x);
     if (d < p.rot) {
         float o[8];
         if (p.interleaved) {
@@ -114,14 +139,10 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_paged_append_kernel(AppendP
             }
         } else {
             const bool low = d < half;
-            const int pd = low ? d + half : d - half;
             float y[8];
-            load8(src + pd, bias != nullptr ? bias + pd : nullptr, y);
-            if (norm != nullptr) {
-                const f16x8 g = *reinterpret_cast<const f16x8*>(norm + pd);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] *= r * static_cast<float>(g[e]);
-            }
+            widen(y8, y);
+            add8(bias != nullptr, by, y);
+            scale8(norm != nullptr, gy, r, y);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int i = (low ? d : pd) + e;
@@ -135,10 +156,10 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_paged_append_kernel(AppendP
         store8(p.q_out + (static_cast<size_t>(t) * p.nq + h) * kPgDim + d, x);
         return;
     }
-    const int page = paged_page(p.c, seq, pos >> p.c.shift);
     if (page < 0) return;
     float w[8];
-    load8(p.v + t * p.kv_stride + h * kPgDim + d, p.vb != nullptr ? p.vb + h * kPgDim + d : nullptr, w);
+    widen(v8, w);
+    add8(p.vb != nullptr, bv, w);
     // an element that fp16 cannot hold poisons the token's K row in place of its V row
     bool fits = true;
 #pragma unroll

@@ -551,7 +551,7 @@ typedef struct qe_paged_cache {
  * is the one new token of sequence s (num_tokens = num_seqs).  query_start does not
  * decrease.  num_tokens is the number of rows the buffers hold: rows of no sequence, and
  * those of sequences with a negative context_len, are not written, and what they hold does
- * not matter (a batch padded to a recorded size).  Positions stay below 2^31; at most 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
+ * not matter (a batch padded to a recorded size).  Positions stay below 2^31; fewer than 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
  * sequences may share pages that neither writes. */
 typedef struct qe_paged_batch {
     const int32_t* block_table; /* [num_seqs][max_pages] */
@@ -607,8 +607,9 @@ int qe_launch_qkv_norm_rope_paged_append(const uint16_t* q, uint16_t* q_out, con
 
 /* Attention on this cache: the row at position p attends to the positions up to p, with
  * window > 0 the last `window` of them, that have a row in the cache; scale 1 / sqrt(128).
- * Scores, softmax sums and outputs in fp32; the softmax weights are rounded to fp16 (2^-11) for
- * the product with V; outputs rounded once to fp16.  row_lse (float [num_tokens][num_q_heads],
+ * Scores, softmax sums and outputs in fp32; for the product with V the softmax weights are
+ * rounded to 2^-22, in chunks of more than 16 rows (tokens times q heads of a kv head) to fp16
+ * (2^-11); outputs rounded once to fp16.  row_lse (float [num_tokens][num_q_heads],
  * NULL = not wanted) receives the natural logarithm of each row's softmax sum.  A row with
  * nothing to attend to gives zeros and -inf; one whose every score is -inf gives NaN and -inf.
  * Rows of a page that nobody attends to may hold anything.  q and attn_out are
@@ -651,7 +652,7 @@ int qe_launch_paged_key_bounds(const qe_paged_cache* cache, const qe_paged_batch
  * last.  A block's score is the largest that its bounds allow a key in it to get from any of the
  * kv head's q heads, in whole steps: with m_h = max |q| and n = rint(127 q / m_h) of q head h (an
  * infinity or NaN: zeros), fp32(step * max_h fp32(m_h * sum_d max(n_d high_d, n_d low_d))); an
- * infinite step comes before every score.  `workspace` (4-byte aligned, the size that the _bytes
+ * infinite step comes before every score.  num_tokens * num_kv_heads below 2^22.  `workspace` (4-byte aligned, the size that the _bytes
  * call gives) is scratch that two launches in flight must not share. */
 int qe_paged_select_workspace_bytes(int num_tokens, int num_kv_heads, int max_pages, size_t* bytes);
 int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,

@@ -409,17 +409,17 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
 //   eight keys of a lane are those of its own eight 16-byte loads (load i: key 4 i + g, dims 8 c .. 8 c + 7):
 //   product j takes element j of each, put together by v_perm, and belongs to dims 8 c + j.
 // So K and V go from memory to registers to the matrix cores with no trip through LDS, and a
-// lane ends with dims 32 g .. 32 g + 31 of head c.  The softmax weights are rounded to fp16 for
-// the product with V (2^-11, as everywhere in this library's matrix-core attention); scores, sums
-// and outputs are fp32.
+// lane ends with dims 32 g .. 32 g + 31 of head c.  The softmax weights go into the product with V
+// as two fp16 numbers each (2^-22): the second product costs nothing beside the loads, and with one (2^-11) the
+// error of a single token's output came to 1.4 to 1.6 times that of fp32 weights.  Scores, sums and outputs are fp32.
 //
 // Bound by memory: K and V are read once, 512 bytes a key and kv head.  The next tile's K is
 // requested as soon as this one's is in the matrix cores, and its V as soon as that is: 16 KB in
-// flight a wave, 128 KB a CU (8 waves with 2 a SIMD; with 4 waves a block and two blocks a CU the
-// merge has twice the parts and everything takes 5% longer).  V goes past the caches: 2% on the
-// long cases, and nothing where other tokens select the same blocks, which keep it.
+// flight a wave, 128 KB a CU.  A block a CU with 8 waves: with two of 4 waves the runs take as long, but
+// have twice the parts, and the merge takes 0.5 to 4 us more.  V goes past the caches (48 sequences 51 us, else 55;
+// 131000 keys 24, else 28), but not where other tokens may have selected the same blocks.
 // 48 sequences of up to 4000 tokens (293 MB): 51 us, 5.7 TB/s, and 5.6 for the merge; one of
-// 131000 (134 MB): 24 and 5.3 us; one of 300: 7 and 5.3, of which 2 are the division of the work.
+// 131000 (134 MB): 24 (5.6 TB/s) and 6.  2.2 us of either are the division of the work.
 constexpr int kDecWaves = 8;     // waves of a block
 constexpr int kDecBlocks = 256;  // of a launch: one a CU
 constexpr int kDecKeys = 32;     // keys of a tile
@@ -592,12 +592,13 @@ __device__ __forceinline__ void token_rows(const PagedView& p, int seq, int h, c
                 for (int r = 0; r < 4; ++r) acc[j][r] *= alpha;
         }
         const float neg = mref == -INFINITY ? 0.0f : -mref;  // masked scores give exp2(-inf) = 0
-        f16x8 pf;
+        f16x8 pf, rest;  // a weight in two parts
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 2][i & 3], kPgScale, neg));
             lsum += w;
             pf[i] = static_cast<_Float16>(w);
+            rest[i] = static_cast<_Float16>(w - static_cast<float>(pf[i]));
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -606,6 +607,7 @@ __device__ __forceinline__ void token_rows(const PagedView& p, int seq, int h, c
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(vf[2 * i + 1][j >> 1], vf[2 * i][j >> 1], take);
             acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf, acc[j], 0, 0, 0);
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), rest, acc[j], 0, 0, 0);
         }
         if (t + 1 < e) request_v(nxt);
         cur = nxt;
@@ -778,8 +780,11 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // other's gaps.  Rows that are few for their sequences (num_tokens * group < 512 num_seqs) take two
 // blocks of 4 waves a CU, with 2 stages and rings of 4 halves: segments of 128 rows, half the waste on short
 // ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 205 us (920
-// TF) before the chip lowers its clock and 215 - 245 after, with 4 waves 275; a mixed batch of 43
-// sequences: 54 us, with 8 waves 76; 17 tokens at 1200: 14 us, with 8 waves 17.
+// TF) before the chip lowers its clock and 215 to 245 after, with 4 waves 234 and 251 to 266; a mixed batch of
+// 43 sequences: 54 us, with 8 waves 64; 17 tokens at 1200: 14.5 us, with 8 waves 15.
+//
+// The weights are rounded to fp16 for the product with V (2^-11, as in this library's other
+// attention of chunks): a second product, as for single tokens, would be half as many MFMAs again.
 //
 // A sequence with up to 16 rows of a kv head (single tokens beside the chunks, drafts) is attended as in
 // the section above, each wave on keys of its own: a tile of 128 rows would be mostly empty.  It counts half
@@ -1334,7 +1339,8 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
                                   : static_cast<long long>(batch->max_pages) * cache->page_size;
     const long long segments = row_tiles * cache->num_kv_heads * batch->num_tokens;
     const long long keys = window > 0 ? std::min<long long>(window, most) : most;
-    if ((keys <= kShortKeys || (segments >= kManySegments && (SPARSE || keys <= 2 * kShortKeys))) && segments <= INT32_MAX) {
+    if ((keys <= kShortKeys || (segments >= kManySegments && (SPARSE || keys <= 2 * kShortKeys))) &&
+        segments < (1 << 24)) {  // (a launch has fewer than 2^32 threads)
         paged_short_kernel<SPARSE><<<static_cast<unsigned>(segments), 64 * kShortWaves, 0, stream>>>(p);
         return check_launch(what);
     }
@@ -1444,7 +1450,7 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
     // Blocks of eight waves read K and V once for 256 rows, those of four waves waste less on sequences of few rows
-    // (2048 rows at 14000: 205 and 232 us; 40 single tokens and three prompts: 68 and 58).
+    // (2048 rows at 14000: 205 and 234 us; 40 single tokens and three prompts: 64 and 54).
     if (static_cast<long long>(batch->num_tokens) * p.group >= 512LL * batch->num_seqs)
         QE_TRY(launch_prefill<8>(p, batch, cache, stream, what));
     else

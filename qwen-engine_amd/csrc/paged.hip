@@ -723,7 +723,7 @@ bool select_workspace(long long num_tokens, long long num_kv_heads, long long ma
 
 extern "C" int qe_paged_select_workspace_bytes(int num_tokens, int num_kv_heads, int max_pages, size_t* bytes) {
     QE_REQUIRE(bytes, "paged_select_workspace_bytes: NULL pointer");
-    QE_REQUIRE(num_tokens >= 0 && num_tokens <= (1 << 24) && num_kv_heads > 0 && num_kv_heads <= 1024 && max_pages > 0 &&
+    QE_REQUIRE(num_tokens >= 0 && num_tokens < (1 << 24) && num_kv_heads > 0 && num_kv_heads <= 1024 && max_pages > 0 &&
                    select_workspace(num_tokens, num_kv_heads, max_pages, bytes),
                "paged_select_workspace_bytes: num_tokens=%d num_kv_heads=%d max_pages=%d", num_tokens, num_kv_heads,
                max_pages);
@@ -756,7 +756,8 @@ extern "C" int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* c
     const long long runs = (tiles + tiles_per_run - 1) / tiles_per_run;
     p.rows_per_run = static_cast<int>(p.rows_per_tile * tiles_per_run);
     size_t bytes = 0;
-    QE_REQUIRE(select_workspace(n, nkv, batch->max_pages, &bytes) && runs * p.chunks <= INT32_MAX && n * nkv <= INT32_MAX,
+    // (a launch has fewer than 2^32 threads)
+    QE_REQUIRE(select_workspace(n, nkv, batch->max_pages, &bytes) && runs * p.chunks < (1 << 24) && n * nkv < (1 << 22),
                "%s: num_tokens=%d max_pages=%d", what, batch->num_tokens, batch->max_pages);
     const size_t pages = static_cast<size_t>(cache->num_pages) * nkv;
     const PagedSpan spans[] = {{selected, 4 * static_cast<size_t>(n) * nkv * num_selected, "selected"},

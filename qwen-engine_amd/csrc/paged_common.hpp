@@ -118,7 +118,7 @@ inline int paged_check(const char* what, const qe_paged_cache* c, const qe_paged
     QE_REQUIRE(aligned(c->k, 16) && aligned(c->v, 16), "%s: the pages must be 16-byte aligned", what);
     QE_REQUIRE(b->num_seqs >= 0 && b->num_tokens >= 0 && b->max_pages > 0, "%s: num_seqs=%d num_tokens=%d max_pages=%d",
                what, b->num_seqs, b->num_tokens, b->max_pages);
-    QE_REQUIRE(b->num_tokens <= (1 << 24) && b->num_seqs <= (1 << 24), "%s: num_tokens=%d num_seqs=%d (at most 2^24)",
+    QE_REQUIRE(b->num_tokens < (1 << 24) && b->num_seqs < (1 << 24), "%s: num_tokens=%d num_seqs=%d (below 2^24)",
                what, b->num_tokens, b->num_seqs);
     QE_REQUIRE(static_cast<long long>(b->max_pages) * c->page_size <= (1LL << 30),
                "%s: max_pages=%d pages of %d tokens (2^30 positions at most)", what, b->max_pages, c->page_size);

@@ -3,6 +3,7 @@ workspace sizes, and the rotary tables."""
 import ctypes
 import math
 import os
+import re
 import shutil
 import subprocess
 
@@ -275,7 +276,7 @@ near(names(), "paged_append")
 assert e[0].grid == (4, 1, 1) and e[0].stream == 0x5000, e
 ok(L.qe_launch_attention_gqa_paged_decode(q, c, t, ws, out, V(0), s, I(12), I(0)))
 near(names(), "paged_decode_kernel", "paged_decode_merge")
-ok(L.qe_launch_attention_gqa_paged_sparse(q, c, t, a, ws, out, V(0), s, I(12), I(8)))
+ok(L.qe_launch_attention_gqa_paged_sparse(q, c, t, a, ws, out, V(0), s, I(12), I(32)))
 near(names(), "paged_decode_kernel", "paged_decode_merge")
 for size in (16, 32, 64, 256):
     c, t = describe(100, True, size)
@@ -287,6 +288,81 @@ ok(L.qe_launch_paged_key_bounds(c, t, a, b, s))
 ok(L.qe_launch_paged_select(q, c, t, a, b, out, ws, s, I(12), I(8), I(1), I(1)))
 near(names(), "paged_key_bounds", "paged_score", "paged_select")
 """)
+
+
+def test_launches_too_large(recorder):
+    """A launch has fewer than 2^32 threads."""
+    launch_recorder.run(recorder, CALLS + """
+L.qe_last_error.restype = ctypes.c_char_p
+def refused(rc, text):
+    assert rc != 0 and text in L.qe_last_error(), L.qe_last_error()
+    assert names() == []
+refused(L.qe_launch_paged_select(q, *describe(tokens=1 << 21), a, b, out, ws, V(0), I(12), I(8), I(1), I(1)), b"num_tokens=2097152")
+refused(L.qe_launch_paged_select(q, *describe(tokens=1 << 20, max_pages=1 << 14), a, b, out, ws, V(0), I(12), I(8), I(1), I(1)), b"max_pages=16384")
+refused(L.qe_launch_paged_key_bounds(*describe(tokens=1 << 24), a, b, V(0)), b"below 2^24")
+""")
+
+
+def test_routes(recorder):
+    """Which kernels take which sizes."""
+    launch_recorder.run(recorder, CALLS + """
+def decode(window=0, q_heads=12, **how):
+    ok(L.qe_launch_attention_gqa_paged_decode(q, *describe(**how), ws, out, V(0), V(0), I(q_heads), I(window)))
+    e = events()
+    return e[0].grid[0], *names()
+def sparse(n, **how):
+    ok(L.qe_launch_attention_gqa_paged_sparse(q, *describe(**how), a, ws, out, V(0), V(0), I(12), I(n)))
+    e = events()
+    return e[0].grid[0], *names()
+def is_short(got, blocks):
+    assert got[0] == blocks and len(got) == 2 and "paged_short" in got[1], got
+def is_shared(got):
+    assert got[0] == 256 and len(got) == 3 and "paged_decode_kernel" in got[1] and "merge" in got[2], got
+is_short(decode(max_pages=16), 8)                          # 1024 keys
+is_shared(decode(max_pages=17))
+is_short(decode(window=1024), 8)
+is_shared(decode(window=1025))
+is_short(decode(max_pages=16, q_heads=34), 16)             # two groups of 16 heads each
+is_shared(decode(max_pages=32, tokens=95))
+is_short(decode(max_pages=32, tokens=96), 192)             # 2048 keys
+is_shared(decode(max_pages=33, tokens=96))
+is_short(sparse(16), 8)
+is_shared(sparse(17))
+is_shared(sparse(500, tokens=95))
+is_short(sparse(500, tokens=96), 192)
+def merge(tokens, **how):
+    return decode(tokens=tokens, **how)[2]
+assert "Li32ELi1024E" in merge(7) and "Li4ELi256E" in merge(8)
+def prefill(tokens, q_heads):
+    ok(L.qe_launch_attention_gqa_paged_prefill(q, *describe(tokens, True), ws, out, V(0), V(0), I(q_heads), I(0)))
+    e = events()
+    return e[0].grid[0], names()[0]
+for tokens, q_heads, waves, few in ((2, 12, 4, 1), (3, 12, 4, 0), (85, 12, 4, 0), (86, 12, 8, 0), (16, 2, 4, 1), (512, 2, 8, 0)):
+    blocks, name = prefill(tokens, q_heads)
+    assert blocks == 2048 // waves and "Li%dELb%d" % (waves, few) in name, (tokens, q_heads, blocks, name)
+def select(max_pages):
+    ok(L.qe_launch_paged_select(q, *describe(max_pages=max_pages), a, b, out, ws, V(0), I(12), I(8), I(1), I(1)))
+    return names()[1]
+for pages, name in ((1, "Li256ELi8E"), (2048, "Li256ELi8E"), (2049, "Li512ELi8E"), (4096, "Li512ELi8E"), (4097, "Li1024ELi16E"),
+                    (16384, "Li1024ELi16E"), (16385, "select_long")):
+    assert name in select(pages), (pages, select(pages))
+""")
+
+
+@pytest.mark.parametrize("kernel", ["paged_prefill_kernel"])
+def test_tiles_read_at_turned_addresses_are_aligned_for_it(kernel, tmp_path):
+    """Its LDS addresses are turned by exclusive or of 16 to 240."""
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not available")
+    root, out = launch_recorder.ROOT, str(tmp_path / "variables.ll")
+    csrc = os.path.join(root, "qwen-engine_amd", "csrc")
+    r = subprocess.run([hipcc, "-std=c++17", "--offload-arch=gfx950", "--offload-device-only", "-S", "-emit-llvm", "-O1", "-Xclang",
+                        "-disable-llvm-passes", f"-I{root}/include", f"-I{csrc}", os.path.join(csrc, "attention_paged.hip"),
+                        "-o", out], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    found = re.findall(rf"^@\S*\d{kernel}\S*4smem = .*addrspace\(3\) global .*align (\d+)", open(out).read(), re.M)
+    assert len(found) == 8 and all(int(a) >= 256 for a in found), found
 
 
 def test_cpp_mirror_compiles():

@@ -418,7 +418,7 @@ __device__ __forceinline__ void merge_parts(void* ws, int blocks, uint16_t* out,
 // flight a wave, 128 KB a CU.  A block a CU with 8 waves: with two of 4 waves the runs take as long, but
 // have twice the parts, and the merge takes 0.5 to 4 us more.  V goes past the caches (48 sequences 51 us, else 55;
 // 131000 keys 24, else 28), but not where other tokens may have selected the same blocks.
-// 48 sequences of up to 4000 tokens (293 MB): 51 us, 5.7 TB/s, and 5.6 for the merge; one of
+// 48 sequences (286000 keys, 293 MB): 51 us, 5.7 TB/s, and 5.6 for the merge; one of
 // 131000 (134 MB): 24 (5.6 TB/s) and 6.  2.2 us of either are the division of the work.
 constexpr int kDecWaves = 8;     // waves of a block
 constexpr int kDecBlocks = 256;  // of a launch: one a CU
@@ -1380,7 +1380,8 @@ int launch_prefill(PrefillParams p, const qe_paged_batch* batch, const qe_paged_
                        : few ? paged_prefill_kernel<false, WAVES, true> : paged_prefill_kernel<false, WAVES, false>;
     kernel<<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
     const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, Shape::blocks) * (Shape::rows / 8);
-    paged_prefill_merge_kernel<WAVES><<<static_cast<unsigned>(std::min(items, 2048LL)), 256, 0, stream>>>(p);
+    // as many blocks as fit the chip at once: each counts the cuts again (mixed batch 12.8 us, with 512 18, with 2048 15)
+    paged_prefill_merge_kernel<WAVES><<<static_cast<unsigned>(std::min(items, 1024LL)), 256, 0, stream>>>(p);
     return QE_OK;
 }
 

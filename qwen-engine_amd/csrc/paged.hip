@@ -185,7 +185,8 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_paged_append_kernel(AppendP
 // NaN has m = inf and bytes of 0.
 //
 // grid (rows, kv heads), 256 threads: a block works where its row is the first of its page or of its
-// sequence; 16 lanes a row of keys, 16 rows at once, up to four rounds of them requested together.
+// sequence; 16 lanes a row of keys, 16 rows at once, up to four rounds of them requested together.  Bound by
+// latency: the row's sequence, its page, the keys, the meeting in LDS behind each other, 3.4 us for one row and 4.7 for 200.
 __global__ __launch_bounds__(256) void paged_key_bounds_kernel(PagedView c, int8_t* bounds, float* step) {
     __shared__ __align__(16) uint16_t s_high[4][kPgDim], s_low[4][kPgDim];
     __shared__ uint32_t s_odd[4];
@@ -292,7 +293,8 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 // registers for the rows of the run that are of one sequence.  Rows are taken as many at a time as 16
 // columns hold; more than 16 q heads take several runs of columns.  The block quantizes q once, 16
 // threads a column (every wave for itself, and the bounds read again for every 16 columns, 200 rows on
-// 1563 blocks took 39 us).
+// 1563 blocks took 39 us; so it is 17.3: vector instructions 72 % of the time, of which the divisions of q take
+// 2.5 us; one row on 2047 blocks 4.5).
 __global__ __launch_bounds__(256) void paged_score_kernel(SelectParams p) {
     __shared__ float s_t[4][16][17];
     __shared__ __align__(16) int8_t s_q[16][2 * kPgDim + 16];  // positive and negative parts of each column (and 16 bytes, for the banks)
@@ -429,7 +431,7 @@ __device__ __forceinline__ bool select_range(const SelectParams& p, int& n) {
 // found by two bits at once, from the highest in which the scores differ, until as many keys as wanted
 // are left above: three counts by ballots, and one barrier, each time.  (A count of digits in LDS, as
 // below, took 12.8 us for the 2048 keys of 131000 positions: scores have few different first digits,
-// so the lanes met at the same counters.)
+// so the lanes met at the same counters.  So it is 8.0, the 400 lists of 1563 keys 10.)
 template <int THREADS, int KEYS>
 __global__ __launch_bounds__(THREADS) void paged_select_kernel(SelectParams p) {
     constexpr int kWaves = THREADS / 64;

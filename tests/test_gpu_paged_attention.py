@@ -165,6 +165,20 @@ def test_missing_pages(qe, form, page):
         assert np.isneginf(lse[3 * n:]).all()  # the window of the last one lies behind the table
 
 
+@pytest.mark.parametrize("n", [40, 200])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_missing_pages_before_many_rows(qe, page, n):
+    """The same for chunks that fill tiles: holes at the first, a middle and the last page of a sequence and of a row."""
+    lens = [(9 * page, n), (0, n), (400, n), (20 * page, n)]
+    last = (400 + n - 1) // page
+    w = World(np.random.default_rng(page + n), lens, page, 6, 2, holes=[(0, 0), (0, 3), (0, 4), (0, 9), (1, 0), (2, 400 // page), (2, last)],
+              pad_rows=2)
+    w.table = np.ascontiguousarray(w.table[:, :max(15, last + 1)])
+    w.max_pages = w.table.shape[1]
+    for window in (0, page + 3, 150):
+        _try(qe, "prefill", w, window)
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_positions_far_behind_the_table(qe, form):
     n = 1 if form == "decode" else 4

@@ -793,6 +793,8 @@ constexpr int kPfKeys = 64;           // keys of a tile: what shares are cut bet
 constexpr int kPfHalf = 32;           // keys of a stage
 constexpr int kPfHalfBytes = kPfHalf * kPgDim * 2;
 constexpr int kPfOver = 4 * kPfKeys;  // what a segment costs beside its keys, in keys
+constexpr int kLeastTiles = 2;        // of a share
+constexpr long long kMergeBlocks = 1024;
 // Blocks of WAVES waves, 32 rows each; a CU holds eight waves.
 template <int WAVES>
 struct PrefillShape {
@@ -1276,7 +1278,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         }
         tile_barrier();  // the tiles are read: the next segment fills them
     };
-    constexpr int kLeastTiles = 2;
     auto rows = [&](const PagedSeq& s, int, int rt) __attribute__((always_inline)) { return min(kRows, s.n * p.group - rt * kRows); };
     for_share<false>(p.c, block, kBlocks, max(1, p.group * kLeastTiles * kPfKeys >> p.coarse), work, tiles, rows, body,
                      [&](SegmentCut cut) {
@@ -1284,11 +1285,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                      });
 }
 
-template <int WAVES>
+template <int WAVES, int GROUPS>
 __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillParams p) {
     typedef PrefillShape<WAVES> Shape;
     static_assert(Shape::blocks <= kMergeCuts, "a cut for each block");
-    merge_parts<Shape::rows, 1, 256>(p.ws, Shape::blocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
+    merge_parts<Shape::rows, GROUPS, 256>(p.ws, Shape::blocks, p.out, p.lse, p.nq, [&](const SegmentCut& c) {
         return RowMap{paged_seq(p.c, c.item).first, c.row_tile * Shape::rows, p.group, c.head * p.group};
     });
 }
@@ -1379,9 +1380,15 @@ int launch_prefill(PrefillParams p, const qe_paged_batch* batch, const qe_paged_
     auto* kernel = one ? few ? paged_prefill_kernel<true, WAVES, true> : paged_prefill_kernel<true, WAVES, false>
                        : few ? paged_prefill_kernel<false, WAVES, true> : paged_prefill_kernel<false, WAVES, false>;
     kernel<<<Shape::blocks, 64 * WAVES, 0, stream>>>(p);
+    // As many blocks as fit the chip at once: each counts the cuts again (mixed batch 12.8 us, with 512 18, with 2048 15).
+    // Where four times as many are no more, and rows may have more parts than a wave asks for at once, four groups of
+    // lanes share a row's (in all, us: 17 tokens at 1200 20.6 and 21.8, 64 at 100000 81 and 95; 200 at 8000, which
+    // are too many, 41.5 and 39.4; 40 at 0 14.3 and 13.7).
     const long long items = std::min<long long>(row_tiles * cache->num_kv_heads, Shape::blocks) * (Shape::rows / 8);
-    // as many blocks as fit the chip at once: each counts the cuts again (mixed batch 12.8 us, with 512 18, with 2048 15)
-    paged_prefill_merge_kernel<WAVES><<<static_cast<unsigned>(std::min(items, 1024LL)), 256, 0, stream>>>(p);
+    if (4 * items <= kMergeBlocks && static_cast<long long>(batch->max_pages) * cache->page_size > 8 * kLeastTiles * kPfKeys)
+        paged_prefill_merge_kernel<WAVES, 4><<<static_cast<unsigned>(4 * items), 256, 0, stream>>>(p);
+    else
+        paged_prefill_merge_kernel<WAVES, 1><<<static_cast<unsigned>(std::min(items, kMergeBlocks)), 256, 0, stream>>>(p);
     return QE_OK;
 }
 

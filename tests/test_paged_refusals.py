@@ -340,6 +340,11 @@ def prefill(tokens, q_heads):
 for tokens, q_heads, waves, few in ((2, 12, 4, 1), (3, 12, 4, 0), (85, 12, 4, 0), (86, 12, 8, 0), (16, 2, 4, 1), (512, 2, 8, 0)):
     blocks, name = prefill(tokens, q_heads)
     assert blocks == 2048 // waves and "Li%dELb%d" % (waves, few) in name, (tokens, q_heads, blocks, name)
+def chunk_merge(tokens, max_pages):
+    ok(L.qe_launch_attention_gqa_paged_prefill(q, *describe(tokens, True, max_pages=max_pages), ws, out, V(0), V(0), I(12), I(0)))
+    return names()[1]
+assert "Li4ELi4E" in chunk_merge(80, 17) and "Li4ELi1E" in chunk_merge(80, 16) and "Li8ELi4E" in chunk_merge(86, 17)
+assert "Li8ELi1E" in chunk_merge(171, 17)
 def select(max_pages):
     ok(L.qe_launch_paged_select(q, *describe(max_pages=max_pages), a, b, out, ws, V(0), I(12), I(8), I(1), I(1)))
     return names()[1]

@@ -779,12 +779,15 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // K and V (128 KB): a segment of 256 rows reads each key once, and the waves drift apart and fill each
 // other's gaps.  Rows that are few for their sequences (num_tokens * group < 512 num_seqs) take two
 // blocks of 4 waves a CU, with 2 stages and rings of 4 halves: segments of 128 rows, half the waste on short
-// ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 205 us (920
-// TF) before the chip lowers its clock and 215 to 245 after, with 4 waves 234 and 251 to 266; a mixed batch of
+// ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 213 us (890
+// TF) before the chip lowers its clock and 220 to 255 after, with 4 waves a tenth more; a mixed batch of
 // 43 sequences: 54 us, with 8 waves 64; 17 tokens at 1200: 14.5 us, with 8 waves 15.
 //
 // The weights are rounded to fp16 for the product with V (2^-11, as in this library's other
 // attention of chunks): a second product, as for single tokens, would be half as many MFMAs again.
+// Outputs are divided by the sum of the rounded weights, so that the roundings of a row's largest ones cancel (a
+// lone key gives its V; the mixed batch's error 2.6e-4 instead of 2.9e-4; 4 % of the long chunk's time); log
+// sums are of the weights themselves.
 //
 // A sequence with up to 16 rows of a kv head (single tokens beside the chunks, drafts) is attended as in
 // the section above, each wave on keys of its own: a tile of 128 rows would be mostly empty.  It counts half
@@ -1053,8 +1056,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         f32x16 acc[4];
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) acc[dt] = f32x16{};
-        float mref = -INFINITY, lsum = 0.0f;
-        bool any = false;  // the row has had a key
+        float mref = -INFINITY, lsum = 0.0f, lround = 0.0f;  // the sums of the weights and of what they are rounded to
+        bool any = false;                                    // the row has had a key
         auto mask = [&](int half, f32x16& sc) __attribute__((always_inline)) {
             if (__builtin_expect(!holes && within(half, bare0, bare_n), 1)) {
                 any = true;
@@ -1079,6 +1082,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                 const float alpha = !grow ? 1.0f : __builtin_amdgcn_exp2f(mref - to);
                 mref = to;
                 lsum *= alpha;
+                lround *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -1094,13 +1098,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
             return mx;
         };
         // weights 2 i and 2 i + 1 of a half's scores, packed
-        auto weights = [&](const f32x16& sc, int i, float neg, float (&ps)[2]) __attribute__((always_inline)) {
+        auto weights = [&](const f32x16& sc, int i, float neg, float (&ps)[3]) __attribute__((always_inline)) {
             const f32x2 e = {__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], kPgScale, neg)),
                              __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], kPgScale, neg))};
             ps[0] += e.x;
             ps[1] += e.y;
-            uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, f16x2));
-            asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]));  // here, not past the mask's branch
+            const f16x2 r = __builtin_convertvector(e, f16x2), ones = {1, 1};
+            ps[2] = __builtin_amdgcn_fdot2(r, ones, ps[2], false);
+            uint32_t w = __builtin_bit_cast(uint32_t, r);
+            asm volatile("" : "+v"(w), "+v"(ps[0]), "+v"(ps[1]), "+v"(ps[2]));  // here, not past the mask's branch
             return w;
         };
         auto times_q = [&](const f16x8& k, int i, f32x16& sc) __attribute__((always_inline)) {
@@ -1130,7 +1136,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         auto stage = [&](int t, int ks, int vs, int then, const Job& job, auto parts, const f32x16& cur, f32x16& nxt, uint32_t (&pc)[8], uint32_t (&pp)[8],
                          float& mx) __attribute__((always_inline)) {
             constexpr int first_part = decltype(parts)::value;
-            float ps[2] = {0.0f, 0.0f}, neg = 0.0f;
+            float ps[3] = {0.0f, 0.0f, 0.0f}, neg = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 times_q(f[i % AHEAD], i, nxt);
@@ -1159,6 +1165,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                 __builtin_amdgcn_sched_barrier(0);
             }
             lsum += ps[0] + ps[1];
+            lround += ps[2];
         };
         // The same where the wave has no half t + 1, or none of the others.
         const int mine = wave_last < key0 ? 0 : min(halves, (wave_last - key0) / kPfHalf + 1);  // its halves
@@ -1177,10 +1184,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
             }
             if (t < mine) {
                 const float neg = mref == -INFINITY ? 0.0f : -mref;
-                float ps[2] = {0.0f, 0.0f};
+                float ps[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) pc[i] = weights(cur, i, neg, ps);
                 lsum += ps[0] + ps[1];
+                lround += ps[2];
             }
         };
         if (it0 < it1) {
@@ -1250,11 +1258,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
             }
         }
         lsum += __shfl_xor(lsum, 32);
+        lround += __shfl_xor(lround, 32);
         const int other_any = __shfl_xor(static_cast<int>(any), 32);  // (asked by all lanes)
         if (any || other_any != 0) mref = fmaxf(mref, kPgLowest);
         if (r < rows) {
             if (slot < 0) {
-                const float inv = row_inverse(mref, lsum);
+                const float inv = row_inverse(mref, lround);
                 const size_t at = static_cast<size_t>(s.first + qi) * p.nq + qh;
                 uint16_t* o = p.out + at * kPgDim;
 #pragma unroll
@@ -1267,13 +1276,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
             } else {
                 const size_t at = static_cast<size_t>(2 * block + slot) * kRows + wave * 32 + fr;
                 if (h == 0) part.ml[at] = make_float2(mref, lsum);
+                const float even = lround > 0.0f ? lsum / lround : 1.0f;  // the merge divides by sums of lsum
                 float* po = part.o + at * kPgDim;
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
                         *reinterpret_cast<float4*>(po + 32 * dt + 8 * g + 4 * h) =
-                            make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+                            make_float4(acc[dt][4 * g] * even, acc[dt][4 * g + 1] * even, acc[dt][4 * g + 2] * even, acc[dt][4 * g + 3] * even);
             }
         }
         tile_barrier();  // the tiles are read: the next segment fills them
@@ -1458,7 +1468,7 @@ extern "C" int qe_launch_attention_gqa_paged_prefill(const uint16_t* q, const qe
     p.group = num_q_heads / cache->num_kv_heads;
     p.window = window;
     // Blocks of eight waves read K and V once for 256 rows, those of four waves waste less on sequences of few rows
-    // (2048 rows at 14000: 205 and 234 us; 40 single tokens and three prompts: 64 and 54).
+    // (2048 rows at 14000: 213 and 234 us; 40 single tokens and three prompts: 64 and 54).
     if (static_cast<long long>(batch->num_tokens) * p.group >= 512LL * batch->num_seqs)
         QE_TRY(launch_prefill<8>(p, batch, cache, stream, what));
     else

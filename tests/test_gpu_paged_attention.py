@@ -265,6 +265,18 @@ def test_the_only_key_scores_minus_infinity(qe, form, nq):
     assert np.isnan(out).all() and np.isneginf(lse).all()
 
 
+@pytest.mark.parametrize("form,lens,nq", [("decode", [(i, 1) for i in range(40)], 12), ("prefill", [(9, 3), (700, 60), (0, 1)], 12),
+                                          ("prefill", [(333, 300)], 12), ("prefill", [(1000, 5)], 1)])
+def test_one_key_gives_its_value(qe, form, lens, nq):
+    """A window of one key: rows of V, bit for bit (a weight and the sum it is divided by are one number, off by 2^-22 at
+    most, and a step of fp16 is 2^-11)."""
+    nkv = 1 if nq == 1 else 2
+    w = World(np.random.default_rng(25), lens, 16, nq, nkv, single=form == "decode")
+    out, lse = attend(qe, form, w, w.queries(2.0), window=1)
+    for row, s, pos in w.tokens():
+        assert np.array_equal(out[row].reshape(nkv, -1, HD), np.repeat(w.v[s][:, pos][:, None], nq // nkv, 1)), (row, s, pos)
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_large_scores_and_rising_ones(qe, form):
     """Weights that underflow, a maximum that comes last, scores of a few hundred."""

@@ -14,11 +14,13 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kPgScale = 1.4426950408889634f * 0.08838834764831845f;  // log2(e) / sqrt(128)
 constexpr float kPgLowest = -3.4e38f;  // the maximum of keys whose every score is -inf: a sum of 0, so NaN
-// A row's reference value (what its scores are lowered by before the exponential) is its
-// running maximum (in chunks rounded down to a whole number), renewed only when that has grown
-// by more than this: weights then stay below 2^9, and their relative precision in fp16 does
-// not change.
-constexpr float kPgLag = 8.0f;
+// A row's reference value (what its scores are lowered by before the exponential) lies kPgRoom below
+// its running maximum (in chunks rounded down to a whole number), and is renewed only when the maximum
+// has grown by more than kPgLag.  So the largest weight is between 2^7 and 2^15, as high as fp16 goes: weights down to
+// 2^-21 of it are normal numbers there and keep their relative precision, smaller ones are off by 2^-32 of it.
+// (Beside weights of 1 those of 2^-16 had 8 bits left and those of 2^-25 none, which a key far above
+// many others, as long texts have it, makes visible: 4 % of the others' sum at 2^-20.6.)
+constexpr float kPgRoom = 7.0f, kPgLag = 8.0f;
 
 // ---- shares of the work ------------------------------------------------------
 // The lengths are on the device, so the division of the work is made there.  A
@@ -581,10 +583,11 @@ __device__ __forceinline__ void token_rows(const PagedView& p, int seq, int h, c
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
         mx = xor32_max(xor16_max(mx)) * kPgScale;
-        const bool grow = mx > mref + kPgLag;
+        const bool grow = mx > mref + (kPgRoom + kPgLag);
         if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float alpha = grow ? __builtin_amdgcn_exp2f(mref - mx) : 1.0f;
-            mref = grow ? mx : mref;
+            const float to = grow ? mx - kPgRoom : mref;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(mref - to) : 1.0f;
+            mref = to;
             lsum *= alpha;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -1076,9 +1079,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         // Reference values are whole numbers (exponents of two), so what was weighed by an old one, the
         // weights pw in wait among it, is scaled without rounding.
         auto renew_ref = [&](float mx, uint32_t (&pw)[8]) __attribute__((always_inline)) {
-            const bool grow = mx > mref + kPgLag;
+            const bool grow = mx > mref + (kPgRoom + kPgLag);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(grow) != 0, 0)) {
-                const float to = grow ? floorf(mx) : mref;
+                const float to = grow ? floorf(mx) - kPgRoom : mref;
                 const float alpha = !grow ? 1.0f : __builtin_amdgcn_exp2f(mref - to);
                 mref = to;
                 lsum *= alpha;

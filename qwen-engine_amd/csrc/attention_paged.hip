@@ -1076,8 +1076,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                 sc[v] = seen ? sc[v] : -INFINITY;
             }
         };
-        // Reference values are whole numbers (exponents of two), so what was weighed by an old one, the
-        // weights pw in wait among it, is scaled without rounding.
+        // Reference values are whole numbers (exponents of two), so what was weighed by an old one, the weights pw in
+        // wait among it, is scaled without rounding (but for weights that end below 2^-21 of the largest).
         auto renew_ref = [&](float mx, uint32_t (&pw)[8]) __attribute__((always_inline)) {
             const bool grow = mx > mref + (kPgRoom + kPgLag);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(grow) != 0, 0)) {
@@ -1090,9 +1090,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
                 for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                     for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
-                const f16x2 a = {static_cast<_Float16>(alpha), static_cast<_Float16>(alpha)};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) pw[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, pw[i]) * a);
+                for (int i = 0; i < 8; ++i) {  // (in fp32: a scale below 2^-24 would be 0 in fp16, a weight times it need not)
+                    const f32x2 w = __builtin_convertvector(__builtin_bit_cast(f16x2, pw[i]), f32x2) * alpha;
+                    pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, f16x2));
+                }
             }
         };
         auto max_of = [&](const f32x16& sc, int v0, int n, float mx) __attribute__((always_inline)) {

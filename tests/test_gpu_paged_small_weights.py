@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from paged_levels import FP16, TWO_FP16, Levels, check, far_below
+from paged_levels import FP16, OCTAVE, TWO_FP16, Levels, check, far_below
 from test_gpu_paged_attention import attend, qe  # noqa: F401 (qe: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +33,21 @@ def test_the_first_key_far_above_30000(qe, form, new, weight, depth):  # noqa: F
     q = w.levels(16)
     out, lse = attend(qe, form, w, q)
     check(out, lse, w.attention_within(q, weight), 300)
+
+
+@pytest.mark.parametrize("form,new,weight", FORMS)
+@pytest.mark.parametrize("copies", [1, 300])
+@pytest.mark.parametrize("depth", [12.1, 18.1, 20.1, 24.1])
+def test_a_key_far_above_the_ones_just_weighed(qe, form, new, weight, copies, depth):  # noqa: F811
+    """Keys 0 to 31 set a reference value, those of 32 to 63 lie as far above it as they may, and key 70 is `depth` octaves
+    above them: what was weighed before counts that much less."""
+    if new == 100 and copies > 1:
+        copies = 40
+    level, value = far_below(300, depth + 7.8, every=300)
+    level[0], value[0] = level[1], value[1]
+    level[32:64] = -depth / (16 * OCTAVE)
+    level[70], value[70] = 0, 0
+    w = Levels(level, value, new=new, copies=copies)
+    q = w.levels(16)
+    out, lse = attend(qe, form, w, q)
+    check(out, lse, w.attention_within(q, weight), copies)

@@ -861,9 +861,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
     const Partials part = partials<kRows>(p.ws, kBlocks);
     constexpr int NP = ONE ? 1 : 2;             // pages of a half tile, at most
 
-    // every tile requested so far is in LDS, for every wave, and what was read before is read
+    // Every tile requested so far is in LDS, for every wave, and what was read before is read: the reads' own
+    // wait too, for nothing else holds the products that need them before the barrier.
     auto tile_barrier = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);

@@ -105,7 +105,9 @@ inline size_t paged_pool_bytes(const qe_paged_cache* c) {
 // Checks of the descriptions and of the heads; fills the kernels' view.
 inline int paged_check(const char* what, const qe_paged_cache* c, const qe_paged_batch* b, PagedView* out) {
     QE_REQUIRE(c && b, "%s: NULL cache or batch", what);
-    QE_REQUIRE(c->k && c->v && b->block_table && b->context_len, "%s: NULL pointer in the cache or the batch", what);
+    // (a batch of no sequences has empty arrays)
+    QE_REQUIRE(c->k && c->v && (b->num_seqs == 0 || (b->block_table && b->context_len)),
+               "%s: NULL pointer in the cache or the batch", what);
     QE_REQUIRE(c->head_dim == kPgDim, "%s: head_dim=%d (only 128 is built)", what, c->head_dim);
     QE_REQUIRE(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128 ||
                    c->page_size == 256,

@@ -548,10 +548,10 @@ def paged_cache(k, v):
         _typed(t, torch.float16, "pages")
         if t.dim() != 4 or t.shape != k.shape:
             raise RuntimeError(f"pages of shapes {tuple(k.shape)} and {tuple(v.shape)}")
-        if t.stride()[1:] != (t.shape[2] * t.shape[3], t.shape[3], 1) or \
-                (t.shape[0] > 1 and (t.stride(0) != k.stride(0) or t.stride(0) < t.shape[1] * t.stride(1))):
+        n, heads, size, dim = t.shape
+        if t.stride()[2:] != (dim, 1) or (heads > 1 and t.stride(1) != size * dim) or \
+                (n > 1 and (t.stride(0) != k.stride(0) or t.stride(0) < heads * size * dim)):
             raise RuntimeError(f"pages of strides {k.stride()} and {v.stride()}")  # (0 would mean behind each other)
-    n, heads, size, dim = k.shape
     stride = k.stride(0) if n > 1 else heads * size * dim
     return _Described(_PagedCache(k.data_ptr(), v.data_ptr(), stride, n, size, heads, dim), k, v)
 

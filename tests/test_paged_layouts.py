@@ -15,3 +15,12 @@ def test_pages_that_lie_over_each_other():
         for k, v in ((one, one), (one, _pages(8, 2, 16, 128)), (_pages(8, 2, 16, 128), one)):
             with pytest.raises(RuntimeError, match="strides"):
                 qe.paged_cache(k, v)
+
+
+def test_one_head_whatever_its_stride():
+    """Pages of one head are the same memory in either order of heads and rows: what stops these is that they are on no GPU."""
+    for one in (_pages(8, 16, 1, 128).transpose(1, 2), _pages(8, 2, 16, 128)[:, 1:], _pages(8, 1, 16, 128)):
+        with pytest.raises(RuntimeError, match="must be on a GPU"):
+            qe.paged_cache(one, one)
+    with pytest.raises(RuntimeError, match="strides"):
+        qe.paged_cache(*[_pages(8, 16, 2, 128).transpose(1, 2)] * 2)

@@ -1340,6 +1340,7 @@ int launch_decode(const char* what, const uint16_t* q, const qe_paged_cache* cac
     QE_TRY(paged_check(what, cache, batch, &p.c));
     QE_TRY(paged_check_heads(what, cache, num_q_heads));
     if (batch->num_tokens == 0 || batch->num_seqs == 0) return QE_OK;
+    QE_REQUIRE(selected || !SPARSE, "%s: NULL pointer", what);
     QE_TRY(check_attention(what, q, cache, batch, attn_out, row_lse, workspace, partials_bytes<kDecRows>(kDecBlocks),
                            selected, num_q_heads, num_selected));
     p.q = q;
@@ -1437,7 +1438,6 @@ extern "C" int qe_launch_attention_gqa_paged_sparse(const uint16_t* q, const qe_
                                                     uint16_t* attn_out, float* row_lse, hipStream_t stream,
                                                     int num_q_heads, int num_selected) {
     const char* what = "attention_gqa_paged_sparse";
-    QE_REQUIRE(selected, "%s: NULL pointer", what);
     QE_REQUIRE(num_selected > 0 && num_selected <= (1 << 20), "%s: num_selected=%d", what, num_selected);
     QE_REQUIRE(!cache || !batch || static_cast<long long>(batch->num_tokens) * cache->num_kv_heads <= (1 << 30),
                "%s: num_tokens=%d", what, batch->num_tokens);

@@ -15,6 +15,13 @@ def test_no_sequences_without_arrays(qe, name):  # noqa: F811
     refusals._says(qe, call(_at(_cache(qe, k=None)), _at(_batch(qe, tokens=0, **empty))), "NULL")
 
 
+@pytest.mark.parametrize("batch", [{"seqs": 0, "tokens": 0}, {"seqs": 4, "tokens": 0, "starts": 4 * P}])
+def test_lists_without_rows(qe, batch):  # noqa: F811
+    """Empty tensors for everything that has rows."""
+    f = qe.lib().qe_launch_attention_gqa_paged_sparse
+    assert f(None, _at(_cache(qe)), _at(_batch(qe, **batch)), None, None, None, None, None, 12, 4) == 0
+
+
 @pytest.mark.gpu
 def test_no_sequences_from_python(qe):  # noqa: F811
     """Tensors without elements have no address."""

@@ -86,3 +86,25 @@ def far_below(n, depth, every=32, seed=0):
     value = np.random.default_rng(seed).uniform(10000, 30000, (n, HD)).astype(np.float16)
     value[::every] = 0
     return level, value
+
+
+def odd_weights(count):
+    """First elements of q for which a key of level -1 has a weight that is far from any fp16 number (a quarter of a step and
+    more), beside one of level 0."""
+    q = np.arange(64, 3000) / 64.0
+    w = 128.0 * np.exp2(-q * OCTAVE)
+    off = np.abs(w.astype(np.float16).astype(np.float64) - w) / w
+    found = q[off > 2.0 ** -12]
+    return found[np.linspace(0, found.size - 1, count).astype(int)].astype(np.float16)
+
+
+def cancelling(n, q0):
+    """Levels 0 and -1 in turns, and values with which a head's outputs are nearly 0 in dims of its own: there an error that
+    all weights of level -1 have in common is not hidden by the output's rounding."""
+    level = np.where(np.arange(n) % 2, -1, 0).astype(np.float16)
+    value = np.ones((n, HD))
+    for d in range(HD):
+        w = np.exp2(-float(q0[d % len(q0)]) * OCTAVE)
+        value[level == 0, d] = -1000.0 * np.float16(w)
+        value[level != 0, d] = 1000.0
+    return level, value.astype(np.float16)

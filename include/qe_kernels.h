@@ -551,8 +551,9 @@ typedef struct qe_paged_cache {
  * is the one new token of sequence s (num_tokens = num_seqs).  query_start does not
  * decrease.  num_tokens is the number of rows the buffers hold: rows of no sequence, and
  * those of sequences with a negative context_len, are not written, and what they hold does
- * not matter (a batch padded to a recorded size).  Positions stay below 2^31; fewer than 2^24 rows and sequences.  Each entry point says which rows of a cache it writes; two
- * sequences may share pages that neither writes. */
+ * not matter (a batch padded to a recorded size).  A batch of no sequences may have NULL
+ * arrays.  Positions stay below 2^31; fewer than 2^24 rows and sequences.  Each entry point
+ * says which rows of a cache it writes; two sequences may share pages that neither writes. */
 typedef struct qe_paged_batch {
     const int32_t* block_table; /* [num_seqs][max_pages] */
     const int32_t* query_start; /* [num_seqs + 1] or NULL */
@@ -577,7 +578,8 @@ typedef struct qe_rope {
  *   QE_ROPE_LINEAR  f_i / factor, factor 1;
  *   QE_ROPE_RAMP    (1 - r_i) f_i + r_i f_i / factor, where r_i goes evenly from 0 to 1 between
  *                   the pair (rounded down) that turns high_turns times within L and the one
- *                   (rounded up) that turns low_turns times; 0.1 ln(factor) + 1;
+ *                   (rounded up) that turns low_turns times, both kept within 0 and
+ *                   rotary_dim - 1; 0.1 ln(factor) + 1;
  *   QE_ROPE_BANDS   the same with r_i = (high_turns - L f_i) / (high_turns - low_turns) within
  *                   [0, 1]: evenly in the number of turns; factor 1.
  * factor >= 1, 0 < low_turns < high_turns (usual: 1 and 32, or 1 and 4).  Host only. */
@@ -616,9 +618,10 @@ int qe_launch_qkv_norm_rope_paged_append(const uint16_t* q, uint16_t* q_out, con
  * [num_tokens][num_q_heads][128], at most 64 q heads for each kv head; q and `workspace`
  * 16-byte, attn_out 8-byte aligned.  `workspace` is scratch of the size that the _bytes call
  * gives (for any batch on any cache), which two launches in flight must not share.  What is
- * written shares memory with nothing (refused).  The work is divided evenly over the chip by
- * what block_table, query_start and context_len say: a row's bits depend on them, for the
- * whole batch, and on nothing else. */
+ * written shares memory with nothing (refused).  The work is divided over the chip by what
+ * query_start and context_len say, and in one of a few ways by sizes (num_seqs, num_tokens,
+ * max_pages, page_size, heads, window, num_selected): a row's bits depend on those, for the whole
+ * batch, beside what it attends to, and on nothing else. */
 
 /* One token of each sequence (query_start NULL): the counterpart of
  * qe_launch_attention_gqa_flash_decode. */
@@ -646,14 +649,16 @@ int qe_launch_paged_key_bounds(const qe_paged_cache* cache, const qe_paged_batch
                                float* bound_steps, hipStream_t stream);
 
 /* For each row and kv head the blocks (of page_size positions) worth attending to, of those
- * up to the row's own that have a page: the first `sinks`, the last `recent` and, of the rest,
- * those with the highest scores (equal scores: the lower block), num_selected in all; selected
+ * up to the row's own that have a page: those below `sinks`, those among the last `recent` up to
+ * the row's own and, of the rest, those with the highest scores (equal scores: the lower block),
+ * num_selected in all; selected
  * (int32 [num_tokens][num_kv_heads][num_selected]) receives them in ascending order, -1 behind the
  * last.  A block's score is the largest that its bounds allow a key in it to get from any of the
  * kv head's q heads, in whole steps: with m_h = max |q| and n = rint(127 q / m_h) of q head h (an
  * infinity or NaN: zeros), fp32(step * max_h fp32(m_h * sum_d max(n_d high_d, n_d low_d))); an
- * infinite step comes before every score.  num_tokens * num_kv_heads below 2^22.  `workspace` (4-byte aligned, the size that the _bytes
- * call gives) is scratch that two launches in flight must not share. */
+ * infinite step comes before every score.  num_tokens * num_kv_heads below 2^22.  `workspace`
+ * (4-byte aligned, the size that the _bytes call gives) is scratch that two launches in flight
+ * must not share. */
 int qe_paged_select_workspace_bytes(int num_tokens, int num_kv_heads, int max_pages, size_t* bytes);
 int qe_launch_paged_select(const uint16_t* q, const qe_paged_cache* cache, const qe_paged_batch* batch,
                            const int8_t* bounds, const float* bound_steps, int32_t* selected, void* workspace,

@@ -33,7 +33,7 @@ constexpr float kPgRoom = 7.0f, kPgLag = 8.0f;
 // at most two cut segments: the one that its share begins in (slot 0) and the one
 // that it ends in (slot 1).  Tile t of a segment of n tiles and weight w belongs to the
 // place t * w / n of its stretch; the bits of a row depend on the lengths of the whole
-// batch, through where the cuts fall, and on nothing else.
+// batch and on the launch's sizes, through where the cuts fall, and on nothing else.
 //
 // Where there are few segments for the blocks (at most one for four), every segment is
 // given whole shares, so that no block has two: a second one costs as much again as a
@@ -782,9 +782,13 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 // K and V (128 KB): a segment of 256 rows reads each key once, and the waves drift apart and fill each
 // other's gaps.  Rows that are few for their sequences (num_tokens * group < 512 num_seqs) take two
 // blocks of 4 waves a CU, with 2 stages and rings of 4 halves: segments of 128 rows, half the waste on short
-// ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 213 us (890
-// TF) before the chip lowers its clock and 220 to 255 after, with 4 waves a tenth more; a mixed batch of
-// 43 sequences: 54 us, with 8 waves 64; 17 tokens at 1200: 14.5 us, with 8 waves 15.
+// ones, and one block starts while the other works.  2048 tokens at 14000, 12 heads over 2: 214 to 220 us (880
+// TF) before the chip lowers its clock and 225 to 269 after, with 4 waves a tenth more; a mixed batch of
+// 43 sequences: 56 to 60 us, with 8 waves a fifth more; 17 tokens at 1200: 14.9 us, with 8 waves 15.
+//
+// All eight forms take every vector register of a wave or nearly; those with FEW spill 14 to 17 of them, offsets of the
+// fill by rows: it reloads each before its load, and the wait for that is a wait for all loads before.  So halves
+// with rows that no one may see (at every sequence's start and end) cost several latencies, not one.
 //
 // The weights are rounded to fp16 for the product with V (2^-11, as in this library's other
 // attention of chunks): a second product, as for single tokens, would be half as many MFMAs again.
@@ -794,7 +798,8 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(DecodeParam
 //
 // A sequence with up to 16 rows of a kv head (single tokens beside the chunks, drafts) is attended as in
 // the section above, each wave on keys of its own: a tile of 128 rows would be mostly empty.  It counts half
-// on the line (59 us for the mixed batch where such rows fill tiles, 54 so; 66 where they count whole, 67 where a quarter).
+// on the line (when it was chosen, the mixed batch: 54 us so, 59 where such rows fill tiles; 66 where they count whole, 67
+// where a quarter).
 constexpr int kPfKeys = 64;           // keys of a tile: what shares are cut between
 constexpr int kPfHalf = 32;           // keys of a stage
 constexpr int kPfHalfBytes = kPfHalf * kPgDim * 2;
@@ -989,7 +994,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_prefill_kernel(PrefillPar
         auto entry_of = [&](int half) __attribute__((always_inline)) {
             return (key0 + kPfHalf * min(half, halves - 1)) >> p.c.shift;
         };
-        bool holes = false;  // some of the run's pages among them are missing
+        bool holes = false;  // some of the run's tiles' entries among them are no page (also behind the last key, where none is needed)
         auto request_entries = [&](int entry) __attribute__((always_inline)) {
             next_base = entry;
             next_l = p.c.table[static_cast<size_t>(seq) * p.c.max_pages + min(entry + lane, p.c.max_pages - 1)];

@@ -610,8 +610,9 @@ int qe_launch_qkv_norm_rope_paged_append(const uint16_t* q, uint16_t* q_out, con
 /* Attention on this cache: the row at position p attends to the positions up to p, with
  * window > 0 the last `window` of them, that have a row in the cache; scale 1 / sqrt(128).
  * Scores, softmax sums and outputs in fp32; for the product with V the softmax weights are
- * rounded to 2^-22 of themselves, in chunks of more than 16 rows (tokens times q heads of a kv head)
- * to 2^-11 (fp16), but no finer than 2^-31 of the row's largest; outputs rounded once to fp16.  row_lse (float [num_tokens][num_q_heads],
+ * rounded to 2^-22 of themselves, in chunks of more than 16 rows (tokens times q heads of a kv head;
+ * a batch of one sequence counts num_tokens, padding too) to 2^-11 (fp16), but no finer than 2^-31
+ * of the row's largest; outputs rounded once to fp16.  row_lse (float [num_tokens][num_q_heads],
  * NULL = not wanted) receives the natural logarithm of each row's softmax sum.  A row with
  * nothing to attend to gives zeros and -inf; one whose every score is -inf gives NaN and -inf.
  * Rows of a page that nobody attends to may hold anything.  q and attn_out are

@@ -19,3 +19,16 @@ def test_weights(qe, form, new, weight, n, page, copies):  # noqa: F811
     q = w.levels(np.tile(q0, 2))
     out, lse = attend(qe, form, w, q)
     check(out, lse, w.attention_within(q, weight), copies)
+
+
+@pytest.mark.parametrize("copies,pad,weight", [(1, 0, TWO_FP16), (1, 3, FP16), (2, 3, TWO_FP16)])
+def test_weights_in_a_padded_batch(qe, copies, pad, weight):  # noqa: F811
+    """Two tokens and 12 rows of a kv head each: a lone sequence counts the rows behind it, several do not."""
+    q0 = odd_weights(6)
+    w = Levels(*cancelling(700, q0), new=2, copies=copies)
+    q = np.pad(w.levels(np.tile(q0, 2)), ((0, pad), (0, 0), (0, 0)))
+    w.rows += pad
+    out, lse = attend(qe, "prefill", w, q)
+    live = 2 * copies
+    assert np.all(out[live:] == -7) and np.all(lse[live:] == -7)
+    check(out[:live], lse[:live], w.attention_within(q, weight), copies)
